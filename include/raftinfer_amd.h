@@ -232,8 +232,8 @@ int raftinfer_amd_online_attention_prefill_kernel_only(
     void *kv_cache, size_t kv_cache_bytes, raftinfer_amd_attention_shape shape,
     int activation_dtype, uint8_t cache_dtype, uint8_t cache_layout, void *stream);
 /* Device capacity-guard counter (replaces the reference merge kernel's trap,
- * qwen35_online_attention.cu:714-717); also counts batched-decode sequences
- * whose length is 0 or above the maximum context.  Synchronizes the device. */
+ * qwen35_online_attention.cu:714-717); also counts batched-decode and compact
+ * decode sequences whose length is 0 or above the maximum context.  Synchronizes the device. */
 int raftinfer_amd_consume_capacity_errors(uint32_t *out);
 
 /* ---- decode graphs (include/raftinfer_amd/hip_graph_decode.hpp) ---- */
@@ -295,6 +295,49 @@ int raftinfer_amd_gated_delta_core(const void *q, const void *k, const void *v, 
                                    void *output, void *workspace, size_t workspace_bytes,
                                    raftinfer_amd_delta_core_shape shape, int chunked,
                                    void *stream);
+
+/* ---- compact KV cache (include/raftinfer_amd/qwen35_compact_cache.hpp) ---- */
+/* Additive: 8-bit blocks, sliding window with sinks, key weights, eviction. */
+enum { RAFTINFER_AMD_CACHE_FP8_E4M3 = 2 }; /* compact caches only; or RAFTINFER_AMD_CACHE_BF16 */
+typedef struct raftinfer_amd_compact_shape {
+  size_t tokens, sequences, query_heads, kv_heads, head_dim, max_context_tokens, past_tokens,
+      cache_stride_bytes, window_tokens, sink_tokens, observed_tokens;
+} raftinfer_amd_compact_shape;
+typedef struct raftinfer_amd_evict_shape {
+  size_t kv_heads, head_dim, context_tokens, max_context_tokens, keep_tokens,
+      out_max_context_tokens, sink_tokens, recent_tokens;
+} raftinfer_amd_evict_shape;
+int raftinfer_amd_compact_cache_bytes(raftinfer_amd_compact_shape shape, uint8_t cache_dtype,
+                                      size_t *out);
+int raftinfer_amd_compact_decode_workspace_bytes(raftinfer_amd_compact_shape shape, size_t *out);
+int raftinfer_amd_compact_prefill_workspace_bytes(raftinfer_amd_compact_shape shape, size_t *out);
+int raftinfer_amd_compact_evict_workspace_bytes(raftinfer_amd_evict_shape shape, size_t *out);
+int raftinfer_amd_compact_cache_append(const void *key, const void *value, void *kv_cache,
+                                       size_t kv_cache_bytes, const uint32_t *context_lengths,
+                                       raftinfer_amd_compact_shape shape, int activation_dtype,
+                                       uint8_t cache_dtype, uint8_t cache_layout, void *stream);
+int raftinfer_amd_compact_attention_prefill(const void *query, const void *key, const void *value,
+                                            const void *gate, void *output, void *kv_cache,
+                                            size_t kv_cache_bytes, float *key_weights,
+                                            void *workspace, size_t workspace_bytes,
+                                            raftinfer_amd_compact_shape shape,
+                                            int activation_dtype, uint8_t cache_dtype,
+                                            uint8_t cache_layout, void *stream);
+int raftinfer_amd_compact_attention_decode(const void *query, const void *key, const void *value,
+                                           const void *gate, void *output, void *kv_cache,
+                                           size_t kv_cache_bytes, const uint32_t *context_lengths,
+                                           float *key_weights, void *workspace,
+                                           size_t workspace_bytes,
+                                           raftinfer_amd_compact_shape shape,
+                                           int activation_dtype, uint8_t cache_dtype,
+                                           uint8_t cache_layout, void *stream);
+int raftinfer_amd_compact_cache_evict(const void *kv_cache, size_t kv_cache_bytes,
+                                      const float *key_weights, void *out_cache,
+                                      size_t out_cache_bytes, float *out_weights,
+                                      int32_t *kept_indices, void *workspace,
+                                      size_t workspace_bytes, raftinfer_amd_evict_shape shape,
+                                      uint8_t cache_dtype, uint8_t out_cache_dtype,
+                                      uint8_t cache_layout, void *stream);
 
 /* ---- attention producers ---- */
 /* qwen35_primitives.cuh:63-67 (qwen35_qk_norm_rope; device_position may be null). */

@@ -58,6 +58,19 @@ class BatchedDecodeShape(ctypes.Structure):
                 ("single_block_max_tokens", _sz)]
 
 
+class CompactShape(ctypes.Structure):
+    _fields_ = [("tokens", _sz), ("sequences", _sz), ("query_heads", _sz), ("kv_heads", _sz),
+                ("head_dim", _sz), ("max_context_tokens", _sz), ("past_tokens", _sz),
+                ("cache_stride_bytes", _sz), ("window_tokens", _sz), ("sink_tokens", _sz),
+                ("observed_tokens", _sz)]
+
+
+class EvictShape(ctypes.Structure):
+    _fields_ = [("kv_heads", _sz), ("head_dim", _sz), ("context_tokens", _sz),
+                ("max_context_tokens", _sz), ("keep_tokens", _sz), ("out_max_context_tokens", _sz),
+                ("sink_tokens", _sz), ("recent_tokens", _sz)]
+
+
 class DeltaCoreShape(ctypes.Structure):
     _fields_ = [("tokens", _sz), ("key_heads", _sz), ("value_heads", _sz), ("key_dim", _sz),
                 ("value_dim", _sz)]
@@ -135,6 +148,18 @@ SIGNATURES = {
     "raftinfer_amd_gated_delta_core_workspace_bytes": ([DeltaCoreShape, _PSZ], _I),
     "raftinfer_amd_gated_delta_core":
         ([_vp, _vp, _vp, _PF, _PF, _F, _PF, _vp, _vp, _sz, DeltaCoreShape, _I, _vp], _I),
+    "raftinfer_amd_compact_cache_bytes": ([CompactShape, _u8, _PSZ], _I),
+    "raftinfer_amd_compact_decode_workspace_bytes": ([CompactShape, _PSZ], _I),
+    "raftinfer_amd_compact_prefill_workspace_bytes": ([CompactShape, _PSZ], _I),
+    "raftinfer_amd_compact_evict_workspace_bytes": ([EvictShape, _PSZ], _I),
+    "raftinfer_amd_compact_cache_append":
+        ([_vp] * 3 + [_sz, _vp, CompactShape, _I, _u8, _u8, _vp], _I),
+    "raftinfer_amd_compact_attention_prefill":
+        ([_vp] * 6 + [_sz, _vp, _vp, _sz, CompactShape, _I, _u8, _u8, _vp], _I),
+    "raftinfer_amd_compact_attention_decode":
+        ([_vp] * 6 + [_sz, _vp, _vp, _vp, _sz, CompactShape, _I, _u8, _u8, _vp], _I),
+    "raftinfer_amd_compact_cache_evict":
+        ([_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _sz, EvictShape, _u8, _u8, _u8, _vp], _I),
     "raftinfer_amd_qk_norm_rope":
         ([_vp, _vp, _vp, QkNormRopeShape, _F, _I, _I, _vp, _vp], _I),
     "raftinfer_amd_split_full_query_gate": ([_vp, _vp, _vp, _sz, _sz, _sz, _I, _vp], _I),

@@ -6,6 +6,7 @@
 // cpp/kernels/qwen35_online_attention.cu:27-196 and :1071-1328.  Device work is
 // this build's own: one workgroup per (KV head, partition) serves the four
 // query heads of the GQA group, so each K/V byte is read from HBM once.
+#include "compact_cache.hpp"
 #include "decode_mfma.hpp"
 #include "decode_scan.hpp"
 #include "norm_rope.hpp"
@@ -1232,7 +1233,7 @@ std::uint32_t qwen35_online_attention_consume_capacity_errors() {
                "reading the capacity error counter failed");
   require<Err>(hipMemcpyToSymbol(HIP_SYMBOL(g_capacity_errors), &zero, sizeof zero) == hipSuccess,
                "clearing the capacity error counter failed");
-  return value;
+  return value + compact_take_capacity_errors();
 }
 
 // ------------------------------------------------------ batched decode

@@ -5,6 +5,7 @@
 #include "raftinfer_amd.h"
 
 #include "raftinfer_amd/hip_graph_decode.hpp"
+#include "raftinfer_amd/qwen35_compact_cache.hpp"
 #include "raftinfer_amd/qwen35_delta.hpp"
 #include "raftinfer_amd/qwen35_online_attention.hpp"
 #include "raftinfer_amd/qwen35_primitives.hpp"
@@ -72,6 +73,15 @@ Qwen35FusedNormRope to_norm(raftinfer_amd_fused_norm_rope n) {
   return {n.query_norm_weight, n.key_norm_weight, static_cast<RaftInferDataType>(n.weight_dtype),
           n.rotary_dim, n.rope_base, n.epsilon};
 }
+Qwen35CompactShape to_compact(raftinfer_amd_compact_shape s) {
+  return {s.tokens,      s.sequences,          s.query_heads,   s.kv_heads,    s.head_dim,       s.max_context_tokens,
+          s.past_tokens, s.cache_stride_bytes, s.window_tokens, s.sink_tokens, s.observed_tokens};
+}
+Qwen35EvictShape to_evict(raftinfer_amd_evict_shape s) {
+  return {s.kv_heads,    s.head_dim,               s.context_tokens, s.max_context_tokens,
+          s.keep_tokens, s.out_max_context_tokens, s.sink_tokens,    s.recent_tokens};
+}
+Qwen35CompactCacheDType to_compact_dtype(uint8_t d) { return static_cast<Qwen35CompactCacheDType>(d); }
 
 } // namespace
 
@@ -430,6 +440,70 @@ int raftinfer_amd_split_query_gate_norm_rope(const void *query_gate, const void 
         {s.tokens, s.heads, s.head_dim, s.rotary_dim, s.position_offset, s.rope_base}, epsilon,
         static_cast<RaftInferDataType>(dtype), static_cast<RaftInferDataType>(weight_dtype),
         to_stream(stream), device_position);
+  });
+}
+
+int raftinfer_amd_compact_cache_bytes(raftinfer_amd_compact_shape shape, uint8_t cache_dtype, size_t *out) {
+  return guarded([&] {
+    out_ref(out) = qwen35_compact_cache_bytes(to_compact(shape), to_compact_dtype(cache_dtype));
+  });
+}
+
+int raftinfer_amd_compact_decode_workspace_bytes(raftinfer_amd_compact_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_compact_decode_workspace_bytes(to_compact(shape)); });
+}
+
+int raftinfer_amd_compact_prefill_workspace_bytes(raftinfer_amd_compact_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_compact_prefill_workspace_bytes(to_compact(shape)); });
+}
+
+int raftinfer_amd_compact_evict_workspace_bytes(raftinfer_amd_evict_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_compact_evict_workspace_bytes(to_evict(shape)); });
+}
+
+int raftinfer_amd_compact_cache_append(const void *key, const void *value, void *cache, size_t cache_bytes,
+                                       const uint32_t *lengths, raftinfer_amd_compact_shape shape, int act,
+                                       uint8_t cache_dtype, uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_compact_cache_append(key, value, cache, cache_bytes, lengths, to_compact(shape), to_dtype(act),
+                                to_compact_dtype(cache_dtype), static_cast<Qwen35KvCacheLayout>(cache_layout),
+                                to_stream(stream));
+  });
+}
+
+int raftinfer_amd_compact_attention_prefill(const void *q, const void *k, const void *v, const void *g, void *o,
+                                            void *cache, size_t cache_bytes, float *key_weights, void *ws,
+                                            size_t ws_bytes, raftinfer_amd_compact_shape shape, int act,
+                                            uint8_t cache_dtype, uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_compact_attention_prefill(q, k, v, g, o, cache, cache_bytes, key_weights, ws, ws_bytes, to_compact(shape),
+                                     to_dtype(act), to_compact_dtype(cache_dtype),
+                                     static_cast<Qwen35KvCacheLayout>(cache_layout), to_stream(stream));
+  });
+}
+
+int raftinfer_amd_compact_attention_decode(const void *q, const void *k, const void *v, const void *g, void *o,
+                                           void *cache, size_t cache_bytes, const uint32_t *lengths,
+                                           float *key_weights, void *ws, size_t ws_bytes,
+                                           raftinfer_amd_compact_shape shape, int act, uint8_t cache_dtype,
+                                           uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_compact_attention_decode(q, k, v, g, o, cache, cache_bytes, lengths, key_weights, ws, ws_bytes,
+                                    to_compact(shape), to_dtype(act), to_compact_dtype(cache_dtype),
+                                    static_cast<Qwen35KvCacheLayout>(cache_layout), to_stream(stream));
+  });
+}
+
+int raftinfer_amd_compact_cache_evict(const void *cache, size_t cache_bytes, const float *key_weights,
+                                      void *out_cache, size_t out_cache_bytes, float *out_weights,
+                                      int32_t *kept_indices, void *ws, size_t ws_bytes,
+                                      raftinfer_amd_evict_shape shape, uint8_t cache_dtype, uint8_t out_cache_dtype,
+                                      uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_compact_cache_evict(cache, cache_bytes, key_weights, out_cache, out_cache_bytes, out_weights, kept_indices,
+                               ws, ws_bytes, to_evict(shape), to_compact_dtype(cache_dtype),
+                               to_compact_dtype(out_cache_dtype), static_cast<Qwen35KvCacheLayout>(cache_layout),
+                               to_stream(stream));
   });
 }
 

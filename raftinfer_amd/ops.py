@@ -16,8 +16,8 @@ import ctypes
 from dataclasses import dataclass
 
 from . import _lib
-from ._lib import (AttentionPolicy, AttentionShape, BatchedDecodeShape, DecodeLayout, DecodePlan,
-                   DeltaCoreShape, DeltaPolicy, DeltaShape, RaftInferError)
+from ._lib import (AttentionPolicy, AttentionShape, BatchedDecodeShape, CompactShape, DecodeLayout,
+                   DecodePlan, DeltaCoreShape, DeltaPolicy, DeltaShape, EvictShape, RaftInferError)
 
 # cpp/execution/qwen35_execution_policy.hpp:7-27 and cpp/include/raftinfer/tensor.h:10-15
 MATERIALIZED, ONLINE_TILED = 0, 1
@@ -349,6 +349,141 @@ def consume_capacity_errors() -> int:
     out = ctypes.c_uint32()
     _call(Qwen35PrimitiveError, _lib.load().raftinfer_amd_consume_capacity_errors(ctypes.byref(out)))
     return out.value
+
+
+# ------------------------------------------------------ compact KV cache
+# include/raftinfer_amd/qwen35_compact_cache.hpp
+CACHE_FP8_E4M3 = 2  # compact caches only (or CACHE_BF16)
+
+
+@dataclass(frozen=True)
+class Qwen35CompactShape:
+    tokens: int
+    sequences: int
+    query_heads: int
+    kv_heads: int
+    head_dim: int
+    max_context_tokens: int
+    past_tokens: int
+    cache_stride_bytes: int = 0
+    window_tokens: int = 0
+    sink_tokens: int = 0
+    observed_tokens: int = 0
+
+    def c(self) -> CompactShape:
+        return CompactShape(self.tokens, self.sequences, self.query_heads, self.kv_heads, self.head_dim,
+                            self.max_context_tokens, self.past_tokens, self.cache_stride_bytes,
+                            self.window_tokens, self.sink_tokens, self.observed_tokens)
+
+
+@dataclass(frozen=True)
+class Qwen35EvictShape:
+    kv_heads: int
+    head_dim: int
+    context_tokens: int
+    max_context_tokens: int
+    keep_tokens: int
+    out_max_context_tokens: int
+    sink_tokens: int = 0
+    recent_tokens: int = 0
+
+    def c(self) -> EvictShape:
+        return EvictShape(self.kv_heads, self.head_dim, self.context_tokens, self.max_context_tokens,
+                          self.keep_tokens, self.out_max_context_tokens, self.sink_tokens,
+                          self.recent_tokens)
+
+
+def _raw(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream_of(stream, tensor) -> int:
+    """The stream's handle; None: the current stream of the tensor's device."""
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(tensor.device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _checked(status: int) -> None:
+    if status != 0:
+        _call(Qwen35PrimitiveError, status)
+
+
+def qwen35_compact_cache_bytes(shape: Qwen35CompactShape, cache_dtype: int) -> int:
+    """Bytes of one sequence's cache."""
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_compact_cache_bytes(shape.c(), cache_dtype, ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_compact_decode_workspace_bytes(shape: Qwen35CompactShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_compact_decode_workspace_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_compact_prefill_workspace_bytes(shape: Qwen35CompactShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_compact_prefill_workspace_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_compact_evict_workspace_bytes(shape: Qwen35EvictShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_compact_evict_workspace_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_compact_cache_append(key, value, kv_cache, shape: Qwen35CompactShape, activation_dtype: int,
+                                cache_dtype: int, cache_layout: int, context_lengths=None, stream=None,
+                                kv_cache_bytes=None) -> None:
+    """Stores shape.tokens rows of every sequence (8-bit caches: codes and scales)."""
+    _checked(_lib.load().raftinfer_amd_compact_cache_append(
+        _raw(key), _raw(value), _raw(kv_cache),
+        _nbytes(kv_cache) if kv_cache_bytes is None else kv_cache_bytes, _raw(context_lengths),
+        shape.c(), activation_dtype, cache_dtype, cache_layout, _stream_of(stream, key)))
+
+
+def qwen35_compact_attention_prefill(query, key, value, gate, output, kv_cache,
+                                     shape: Qwen35CompactShape, activation_dtype: int,
+                                     cache_dtype: int, cache_layout: int, workspace=None,
+                                     key_weights=None, stream=None, kv_cache_bytes=None,
+                                     workspace_bytes=None) -> None:
+    """Stores the prompt's rows and attends over the cache, within the shape's window."""
+    _checked(_lib.load().raftinfer_amd_compact_attention_prefill(
+        _raw(query), _raw(key), _raw(value), _raw(gate), _raw(output), _raw(kv_cache),
+        _nbytes(kv_cache) if kv_cache_bytes is None else kv_cache_bytes, _raw(key_weights),
+        _raw(workspace), _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        activation_dtype, cache_dtype, cache_layout, _stream_of(stream, query)))
+
+
+def qwen35_compact_attention_decode(query, key, value, gate, output, kv_cache,
+                                    shape: Qwen35CompactShape, activation_dtype: int, cache_dtype: int,
+                                    cache_layout: int, workspace, context_lengths=None,
+                                    key_weights=None, stream=None, kv_cache_bytes=None,
+                                    workspace_bytes=None) -> None:
+    """One new token of each sequence; context_lengths (int32/uint32, on the device) include it."""
+    _checked(_lib.load().raftinfer_amd_compact_attention_decode(
+        _raw(query), _raw(key), _raw(value), _raw(gate), _raw(output), _raw(kv_cache),
+        _nbytes(kv_cache) if kv_cache_bytes is None else kv_cache_bytes, _raw(context_lengths),
+        _raw(key_weights), _raw(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        activation_dtype, cache_dtype, cache_layout, _stream_of(stream, query)))
+
+
+def qwen35_compact_cache_evict(kv_cache, key_weights, out_cache, out_weights, kept_indices,
+                               shape: Qwen35EvictShape, cache_dtype: int, out_cache_dtype: int,
+                               cache_layout: int, workspace=None, stream=None, kv_cache_bytes=None,
+                               out_cache_bytes=None, workspace_bytes=None) -> None:
+    """The sinks, the recent entries and those with the largest weights, to out_cache."""
+    _checked(_lib.load().raftinfer_amd_compact_cache_evict(
+        _raw(kv_cache), _nbytes(kv_cache) if kv_cache_bytes is None else kv_cache_bytes,
+        _raw(key_weights), _raw(out_cache),
+        _nbytes(out_cache) if out_cache_bytes is None else out_cache_bytes, _raw(out_weights),
+        _raw(kept_indices), _raw(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(), cache_dtype,
+        out_cache_dtype, cache_layout, _stream_of(stream, kv_cache)))
 
 
 def qwen35_gated_delta(input, conv_weight, recurrent_a, dt_bias, output_norm_weight, output,
