@@ -65,7 +65,7 @@ struct SeenTiles {
 // Whether a token at position p sees key j.
 __host__ __device__ __forceinline__ bool compact_sees(std::uint32_t j, std::uint32_t p, std::uint32_t window,
                                                       std::uint32_t sinks) {
-  return j <= p && (window == 0 || j < sinks || p - j < window);
+  return (j <= p) & ((window == 0) | (j < sinks) | (p - j < window)); // (no branches)
 }
 
 // ------------------------------------------------------- e4m3 and scales

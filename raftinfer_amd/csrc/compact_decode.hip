@@ -10,46 +10,104 @@ namespace {
 using prefill::fexp2;
 using prefill::lds_tr16;
 
-constexpr int kDecodeWaves = 4;
-constexpr int kDecodeThreads = kDecodeWaves * kWave;
-// Workgroups that a call aims at: two per CU, twice.
-constexpr std::uint32_t kDecodeTarget = 1024;
+constexpr int kMergeThreads = 512;
+constexpr int kMergeWaves = kMergeThreads / kWave;
 
 __device__ unsigned int g_compact_capacity_errors = 0;
 
 // Partials of a call, one per (query head, partition): max and sum (exp2 domain),
-// and the unnormalised output; with key weights also every score and each
-// head's final max and 1 / sum.
+// and the unnormalised output; with key weights also every score.
 struct DecodeScratch {
-  float *m, *l, *o, *scores, *final;
-  std::uint32_t tiles, parts, score_stride;
+  float *m, *l, *o, *scores;
+  std::uint32_t tiles, parts, score_stride; // parts: rows of m, l, o per head
 };
 
 __device__ __forceinline__ std::uint32_t context_of(const CompactArgs &a, std::uint32_t seq) {
   return a.lengths == nullptr ? a.past + 1 : a.lengths[seq];
 }
 
-struct DecodeShared {
+template <int WAVES> struct DecodeShared {
   union {
-    bf16_bits v[kDecodeWaves][kCompactBlock * kHeadDim]; // 16-byte chunk c of row r at c ^ (r & 7)
-    float acc[kDecodeWaves][kCompactMaxGroup][kHeadDim];
+    bf16_bits v[WAVES][kCompactBlock * kHeadDim]; // 16-byte chunk c of row r at c ^ 2 (r & 7)
+    // (the pad puts the 16 heads of a store on banks of their own)
+    float acc[WAVES][kCompactMaxGroup][kHeadDim + 4];
   };
-  float m[kDecodeWaves][kCompactMaxGroup];
-  float l[kDecodeWaves][kCompactMaxGroup];
+  float m[WAVES][kCompactMaxGroup];
+  float l[WAVES][kCompactMaxGroup];
+  alignas(16) unsigned char fresh[2][2 * kHeadDim]; // the new token's K and V rows, as stored
 };
 
+__device__ __forceinline__ int v_chunk(int r, int c) { return (c ^ (2 * (r & 7))) << 3; } // in elements
+__device__ __forceinline__ float max_finite_bf16x8(u32x4 w, float m) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const std::uint32_t u = w[e];
+    const float a = fabsf(bf16_lo(u)), b = fabsf(bf16_hi(u));
+    m = fmaxf(m, is_finite_f32(a) ? a : 0.f);
+    m = fmaxf(m, is_finite_f32(b) ? b : 0.f);
+  }
+  return m;
+}
+__device__ __forceinline__ float finite_or_nan(float x) { return is_finite_f32(x) ? x : __builtin_nanf(""); }
+// Sixteen bf16 values as codes of scale 1 / inv.
+__device__ __forceinline__ u32x4 bf16x16_to_fp8(u32x4 lo, u32x4 hi, float inv) {
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const std::uint32_t x = e < 2 ? lo[2 * e] : hi[2 * e - 4], y = e < 2 ? lo[2 * e + 1] : hi[2 * e - 3];
+    r[e] = pack_fp8x4(finite_or_nan(bf16_lo(x)) * inv, finite_or_nan(bf16_hi(x)) * inv,
+                      finite_or_nan(bf16_lo(y)) * inv, finite_or_nan(bf16_hi(y)) * inv);
+  }
+  return r;
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(x)), lane)));
+}
+__device__ __forceinline__ u32x4 rescale_fp8x16(u32x4 w, float ratio) {
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const floatx4 f = fp8x4_to_f32(w[e]);
+    r[e] = pack_fp8x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+  }
+  return r;
+}
+
 // A workgroup takes one partition (sc.tiles 32-key tiles) of one KV head and
-// sequence; its waves take every fourth tile.  Both products run on
+// sequence; wave w takes its steps w, w + WAVES, ..  Both products run on
 // v_mfma_f32_16x16x32_bf16 with the query heads of the group as the 16 columns
-// (those past the group are zero): S = K q^T with K rows as loaded, O^T = V^T P^T
+// (those past the group repeat the last): S = K q^T with K rows as loaded, O^T = V^T P^T
 // with V transposed by the LDS read.  Codes become bf16 without loss; the block's
 // K scale multiplies the scores, its V scale the probabilities.
-template <bool Fp8, bool Weigh>
-__global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(CompactArgs a, DecodeScratch sc) {
-  __shared__ DecodeShared sh;
-  const std::uint32_t part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+//
+// The kernel is bound by its cache reads, so a wave (32 8-bit or 16 bf16 rows a
+// step) asks for rows a step ahead: K(t + 1) goes out when S(t) is formed, V(t + 1)
+// when V(t) is in LDS.
+//
+// The step that holds the new token's position covers its scale block, so its wave also
+// stores the row: it raises the block's scale where the row needs that, rounds the
+// block's other codes again in its registers, and attends over what it writes.
+template <bool Fp8, bool Weigh, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel(CompactArgs a, DecodeScratch sc) {
+  __shared__ DecodeShared<WAVES> sh;
+  // Workgroups go to the 8 XCDs in turn.  All units' first partitions lie first (short
+  // contexts have no others), and a partition's units are rotated by its number, so
+  // that a unit's partitions and the partitions of one number are spread over the XCDs.
+  const std::uint32_t units = a.kv_heads * a.sequences;
+  const std::uint32_t part = blockIdx.x / units;
+  const std::uint32_t unit_id = (blockIdx.x % units + part) % units;
+  const std::uint32_t kvh = unit_id % a.kv_heads, seq = unit_id / a.kv_heads;
+  const bool last = gridDim.x == units; // one partition each: no merge follows
   const std::uint32_t n = context_of(a, seq);
-  if (n == 0 || n > a.max_ctx) return;
+  if (n == 0 || n > a.max_ctx) {
+    // no valid context: NaN rows, counted once (here only if no merge follows)
+    if (last) {
+      if (kvh == 0 && threadIdx.x == 0) atomicAdd(&g_compact_capacity_errors, 1u);
+      bf16_bits *out = a.output + (static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.group * kHeadDim;
+      for (std::uint32_t i = threadIdx.x; i < a.group * kHeadDim; i += WAVES * kWave) out[i] = 0x7FC0;
+    }
+    return;
+  }
   const std::uint32_t p = n - 1;
   const SeenTiles seen(p, p, a.window, a.sinks);
   const std::uint32_t begin = part * sc.tiles;
@@ -60,28 +118,119 @@ __global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(Compa
   const int col = lane & 15; // MFMA column (query head) and A row
   const int kq = lane >> 4;  // k-quarter
   const CompactHead<Fp8> c(a.cache + seq * a.cache_stride, kvh, a.kv_heads, a.max_ctx, a.head_major);
-  constexpr int kPieces = Fp8 ? 4 : 8; // 16-byte pieces of a K row that a lane loads
+  const std::size_t unit = static_cast<std::size_t>(seq) * a.kv_heads + kvh;
+  constexpr int kStep = Fp8 ? 32 : 16;     // keys per step (8 KiB of K and of V)
+  constexpr int kSteps = kCompactBlock / kStep;
+  constexpr int kRB = kStep / 16;          // blocks of 16 K rows
+  constexpr int kPieces = Fp8 ? 4 : 8;     // 16-byte pieces of a K row that a lane loads
+  constexpr int kRowLanes = Fp8 ? 16 : 32; // V: lanes that take one row
+  constexpr int kVRows = 64 / kRowLanes;
+  constexpr int kVLoads = kStep / kVRows;
+  const auto first_key = [&](std::uint32_t it) {
+    return seen.tile(it / kSteps) * kCompactBlock + kStep * (it % kSteps);
+  };
 
-  // q of column `col`, in the dims that this lane's K pieces hold.
+  // Scales come by vector loads: a scalar load counts with the LDS reads, whose next
+  // wait would wait for it.
+  int lane0;
+  asm volatile("v_mov_b32 %0, 0" : "=v"(lane0));
+  u32x4 kr[kRB][kPieces];
+  u32x4 vr[kVLoads];
+  float ks = 1.0f, vs = 1.0f; // scales of the rows in kr, vr
+  const auto load_k = [&](std::uint32_t j0) {
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      std::uint32_t j = j0 + 16 * rb + col;
+      j = j < n ? j : n - 1;
+      const auto *row = reinterpret_cast<const unsigned char *>(c.k + static_cast<std::size_t>(j) * c.row) + 16 * kq;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        kr[rb][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + 64 * i));
+    }
+    if constexpr (Fp8) ks = c.ks[j0 / kCompactBlock + lane0];
+  };
+  const auto load_v = [&](std::uint32_t j0) {
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i) {
+      std::uint32_t j = j0 + kVRows * i + lane / kRowLanes;
+      j = j < n ? j : n - 1;
+      const auto *row = reinterpret_cast<const unsigned char *>(c.v + static_cast<std::size_t>(j) * c.row);
+      vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + 16 * (lane % kRowLanes)));
+    }
+    if constexpr (Fp8) vs = c.vs[j0 / kCompactBlock + lane0];
+  };
+  std::uint32_t it = begin * kSteps + wave;
+  // The last step with a key is the one that holds the new token's row.
+  const std::uint32_t newest_step = (seen.total - 1) * kSteps + p % kCompactBlock / kStep;
+  const std::uint32_t it_end = end * kSteps <= newest_step ? end * kSteps : newest_step + 1;
+  // The new token's rows, for the wave whose step holds them: lanes 0 .. 15 have K, 16 ..
+  // 31 V, 16 dims each.
+  const bool owner = newest_step + 1 == it_end && (newest_step - begin * kSteps) % WAVES == static_cast<std::uint32_t>(wave);
+  const int plane = (lane >> 4) & 1, piece = lane & 15;
+  u32x4 row_new[2];
+  [[maybe_unused]] float scale_old = 0.f;
+  if (owner) {
+    const u32x4 *x = reinterpret_cast<const u32x4 *>((plane ? a.value : a.key) + unit * kHeadDim + 16 * piece);
+    row_new[0] = x[0];
+    row_new[1] = x[1];
+    if constexpr (Fp8) scale_old = ((plane ? c.vs : c.ks) + p / kCompactBlock)[0];
+  }
+  // q of column `col`, in the dims that this lane's K pieces hold.  (Loaded before the
+  // cache rows: a wait for it is then one for nothing younger.)
   bf16x8 qb[8];
   {
-    const bf16_bits *q = a.query + ((static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.group + col) * kHeadDim;
+    const bf16_bits *q = a.query + (unit * a.group + (col < static_cast<int>(a.group) ? col : a.group - 1)) * kHeadDim;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int dim = Fp8 ? 64 * (i >> 1) + 16 * kq + 8 * (i & 1) : 32 * i + 8 * kq;
-      u32x4 w{0u, 0u, 0u, 0u};
-      if (col < static_cast<int>(a.group)) w = *reinterpret_cast<const u32x4 *>(q + dim);
-      qb[i] = __builtin_bit_cast(bf16x8, w);
+      qb[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(q + dim));
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
+  // (a wave without a step loads the first one's rows: the same reason)
+  load_k(first_key(it < it_end ? it : begin * kSteps));
+  load_v(first_key(it < it_end ? it : begin * kSteps));
+
+  // The new token's rows into the cache, and into LDS for the step.  grow: what the block's other codes are multiplied by, 0 where
+  // its scale stays.
+  [[maybe_unused]] float grow_k = 0.f, grow_v = 0.f, new_ks = 1.0f, new_vs = 1.0f;
+  if (owner) {
+    const u32x4 lo = row_new[0], hi = row_new[1];
+    unsigned char *dst = reinterpret_cast<unsigned char *>((plane ? c.v : c.k) + static_cast<std::size_t>(p) * c.row);
+    if constexpr (Fp8) {
+      float *scale = (plane ? c.vs : c.ks) + p / kCompactBlock;
+      const float before = p % kCompactBlock != 0 ? scale_old : 0.f;
+      const float amax = row16_max(max_finite_bf16x8(hi, max_finite_bf16x8(lo, 0.f)));
+      const float after = fmaxf(before, compact_scale(amax));
+      const float inv = compact_inverse(after);
+      const u32x4 codes = bf16x16_to_fp8(lo, hi, inv);
+      const float grow = before != 0.f && after != before ? before * inv : 0.f;
+      if (lane < 32) {
+        *reinterpret_cast<u32x4 *>(dst + 16 * piece) = codes;
+        *reinterpret_cast<u32x4 *>(&sh.fresh[plane][16 * piece]) = codes;
+        if (piece == 0) *scale = after;
+      }
+      new_ks = lane_value(after, 0);
+      new_vs = lane_value(after, 16);
+      grow_k = lane_value(grow, 0);
+      grow_v = lane_value(grow, 16);
+    } else if (lane < 32) {
+      reinterpret_cast<u32x4 *>(dst + 32 * piece)[0] = lo;
+      reinterpret_cast<u32x4 *>(dst + 32 * piece)[1] = hi;
+      *reinterpret_cast<u32x4 *>(&sh.fresh[plane][32 * piece]) = lo;
+      *reinterpret_cast<u32x4 *>(&sh.fresh[plane][32 * piece + 16]) = hi;
+    }
+    wave_lds_order();
+  }
+
   // Transposed V reads: lane r of a 16-lane group supplies 4 dims of key row r / 4
   // and receives its dim of 4 keys.
-  const bf16_bits *vt[4];
+  const bf16_bits *vt[8];
   {
     const int row = 4 * kq + (col >> 2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      vt[j] = &sh.v[wave][row * kHeadDim + (((2 * j + ((col >> 1) & 1)) ^ (row & 7)) << 3) + 4 * (col & 1)];
+    for (int j = 0; j < 8; ++j)
+      vt[j] = &sh.v[wave][row * kHeadDim + v_chunk(row, 2 * j + ((col >> 1) & 1)) + 4 * (col & 1)];
   }
 
   floatx4 acc[16];
@@ -89,44 +238,44 @@ __global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(Compa
   for (int db = 0; db < 16; ++db) acc[db] = floatx4{};
   float m_run = -FLT_MAX, l_run = 0.f;
 
-  for (std::uint32_t it = begin + wave; it < end; it += kDecodeWaves) {
-    const std::uint32_t tile = seen.tile(it);
-    const std::uint32_t j0 = tile * kCompactBlock;
-    const bool whole = j0 + kCompactBlock <= n &&
-                       (a.window == 0 || p - j0 < a.window || j0 + kCompactBlock <= a.sinks); // every key is seen
-    u32x4 kr[2][kPieces];
+  // One step; kMore: it is not the wave's last.  (Two copies, and no condition on the
+  // loads: with one, the waits for K and V would allow for the other's absence.)
+  const auto step = [&]<bool kMore>() __attribute__((always_inline)) {
+    const std::uint32_t j0 = first_key(it);
+    const bool newest = !kMore && owner;
+    const std::uint32_t r_new = p % kStep;
+    const bool whole = j0 + kStep <= n &&
+                       (a.window == 0 || p - j0 < a.window || j0 + kStep <= a.sinks); // every key is seen
+    if (newest) {
+      if constexpr (Fp8) {
+        if (grow_k != 0.f) {
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
-      std::uint32_t j = j0 + 16 * rb + col;
-      j = j < n ? j : n - 1;
-      const auto *row = c.k + static_cast<std::size_t>(j) * c.row;
+          for (int rb = 0; rb < kRB; ++rb) {
+            if (16 * rb + col >= static_cast<int>(r_new)) continue;
+            unsigned char *dst = c.k + static_cast<std::size_t>(j0 + 16 * rb + col) * c.row + 16 * kq;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        kr[rb][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(
-            reinterpret_cast<const unsigned char *>(row) + 64 * i + 16 * kq));
-    }
-    // V: 16 lanes (Fp8) or 32 take one row.
-    constexpr int kVLoads = Fp8 ? 8 : 16;
-    constexpr int kRowLanes = Fp8 ? 16 : 32;
-    u32x4 vr[kVLoads];
+            for (int i = 0; i < kPieces; ++i) {
+              kr[rb][i] = rescale_fp8x16(kr[rb][i], grow_k);
+              *reinterpret_cast<u32x4 *>(dst + 64 * i) = kr[rb][i];
+            }
+          }
+        }
+        ks = new_ks;
+      }
 #pragma unroll
-    for (int i = 0; i < kVLoads; ++i) {
-      const std::uint32_t j = j0 + (64 / kRowLanes) * i + lane / kRowLanes;
-      const auto *row = c.v + static_cast<std::size_t>(j < n ? j : n - 1) * c.row;
-      vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(
-          reinterpret_cast<const unsigned char *>(row) + 16 * (lane % kRowLanes)));
-    }
-    float k_scale = kLog2e / 16.0f, v_scale = 1.0f;
-    if constexpr (Fp8) {
-      k_scale *= c.ks[tile];
-      v_scale = c.vs[tile];
+      for (int rb = 0; rb < kRB; ++rb)
+        if (16 * rb + col == static_cast<int>(r_new)) {
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) kr[rb][i] = *reinterpret_cast<const u32x4 *>(&sh.fresh[0][64 * i + 16 * kq]);
+        }
     }
 
     // Scores of keys j0 + 16 rb + 4 kq + i for head `col`.
-    float s[2][4];
+    const float k_scale = ks * (kLog2e / 16.0f);
+    float s[kRB][4];
     float mx = -INFINITY;
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
+    for (int rb = 0; rb < kRB; ++rb) {
       floatx4 d{};
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
@@ -141,17 +290,26 @@ __global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(Compa
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[rb][i] = d[i] * k_scale;
-        if (!whole && !compact_sees(j0 + 16 * rb + 4 * kq + i, p, a.window, a.sinks)) s[rb][i] = -INFINITY;
-        mx = fmaxf(mx, s[rb][i]);
-      }
+      for (int i = 0; i < 4; ++i) s[rb][i] = d[i] * k_scale;
     }
+    if (!whole) {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[rb][i] = compact_sees(j0 + 16 * rb + 4 * kq + i, p, a.window, a.sinks) ? s[rb][i] : -INFINITY;
+    }
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rb][i]);
+    if constexpr (kMore) load_k(first_key(it + WAVES));
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (Weigh) {
       if (col < static_cast<int>(a.group)) {
-        float *row = sc.scores + ((static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.group + col) * sc.score_stride;
+        float *row = sc.scores + (unit * a.group + col) * sc.score_stride;
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb)
+        for (int rb = 0; rb < kRB; ++rb)
           *reinterpret_cast<floatx4 *>(row + j0 + 16 * rb + 4 * kq) = floatx4{s[rb][0], s[rb][1], s[rb][2], s[rb][3]};
       }
     }
@@ -164,49 +322,85 @@ __global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(Compa
       for (int db = 0; db < 16; ++db) acc[db] *= f;
       m_run = m_new;
     }
-    u32x4 pw;
+    if (newest) {
+      if constexpr (Fp8) {
+        if (grow_v != 0.f) {
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
+          for (int i = 0; i < kVLoads; ++i) {
+            const std::uint32_t row = kVRows * i + lane / kRowLanes;
+            if (row >= r_new) continue;
+            vr[i] = rescale_fp8x16(vr[i], grow_v);
+            *reinterpret_cast<u32x4 *>(c.v + static_cast<std::size_t>(j0 + row) * c.row + 16 * (lane % kRowLanes)) = vr[i];
+          }
+        }
+        vs = new_vs;
+      }
+      const u32x4 fresh = *reinterpret_cast<const u32x4 *>(&sh.fresh[1][16 * (lane % kRowLanes)]);
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i)
+        if (kVRows * i + lane / kRowLanes == static_cast<int>(r_new)) vr[i] = fresh;
+    }
+    std::uint32_t pw[2 * kRB];
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         e[i] = fexp2(s[rb][i] - m_run);
         l_run += e[i];
-        e[i] *= v_scale;
+        e[i] *= vs;
       }
       pw[2 * rb] = pack_bf16x2(e[0], e[1]);
       pw[2 * rb + 1] = pack_bf16x2(e[2], e[3]);
     }
-    const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
-
     // V rows into LDS as bf16; a key that is not seen gives a row of zeros (its
     // probability is 0, and 0 times what an unused row holds may be NaN).
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i) {
+        const std::uint32_t keep = compact_sees(j0 + kVRows * i + lane / kRowLanes, p, a.window, a.sinks) ? ~0u : 0u;
+        vr[i] &= u32x4{keep, keep, keep, keep};
+      }
+    }
     wave_lds_order();
 #pragma unroll
     for (int i = 0; i < kVLoads; ++i) {
-      const int r = (64 / kRowLanes) * i + lane / kRowLanes;
+      const int r = kVRows * i + lane / kRowLanes;
       const int piece = lane % kRowLanes;
-      u32x4 w = vr[i];
-      if (!whole && !compact_sees(j0 + r, p, a.window, a.sinks)) w = u32x4{0u, 0u, 0u, 0u};
+      const u32x4 w = vr[i];
       bf16_bits *row = sh.v[wave] + r * kHeadDim;
       if constexpr (Fp8) {
-        *reinterpret_cast<u32x4 *>(row + (((2 * piece) ^ (r & 7)) << 3)) = fp8x8_to_bf16(w[0], w[1]);
-        *reinterpret_cast<u32x4 *>(row + (((2 * piece + 1) ^ (r & 7)) << 3)) = fp8x8_to_bf16(w[2], w[3]);
+        // the upper 8 lanes of a row store their second chunk first: 16 banks, not 8 twice
+        const u32x4 x = fp8x8_to_bf16(w[0], w[1]), y = fp8x8_to_bf16(w[2], w[3]);
+        const bool up = piece >= 8;
+        *reinterpret_cast<u32x4 *>(row + v_chunk(r, 2 * piece + up)) = up ? y : x;
+        *reinterpret_cast<u32x4 *>(row + v_chunk(r, 2 * piece + !up)) = up ? x : y;
       } else {
-        *reinterpret_cast<u32x4 *>(row + ((piece ^ (r & 7)) << 3)) = w;
+        *reinterpret_cast<u32x4 *>(row + v_chunk(r, piece)) = w;
       }
     }
+    if constexpr (kMore) load_v(first_key(it + WAVES));
+    __builtin_amdgcn_sched_barrier(0);
     wave_lds_order();
     // k-slot (kq, e) of the product <-> key 16 (e / 4) + 4 kq + e % 4, the order
     // in which the scores lie.
 #pragma unroll
     for (int db = 0; db < 16; ++db) {
-      const bf16_bits *v0 = vt[db & 3] + 64 * (db >> 2);
-      const u32x2 lo = lds_tr16(v0), hi = lds_tr16(v0 + 16 * kHeadDim);
-      acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}), pb, acc[db], 0, 0, 0);
+      const bf16_bits *v0 = vt[db & 7] + 128 * (db >> 3);
+      const u32x2 lo = lds_tr16(v0);
+      if constexpr (kRB == 2) {
+        const u32x2 hi = lds_tr16(v0 + 16 * kHeadDim);
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
+            __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
+      } else {
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+            __builtin_bit_cast(prefill::short4v, lo), __builtin_bit_cast(prefill::short4v, u32x2{pw[0], pw[1]}), acc[db], 0, 0, 0);
+      }
     }
-  }
+  };
+  for (; it + WAVES < it_end; it += WAVES) step.template operator()<true>();
+  if (it < it_end) step.template operator()<false>();
 
   // Join the waves.  l: the four lanes of a column hold partial sums.
   const float l_tot = sum_xor32(sum_xor16(l_run));
@@ -215,92 +409,144 @@ __global__ __launch_bounds__(kDecodeThreads, 2) void compact_decode_kernel(Compa
     sh.m[wave][lane] = m_run;
     sh.l[wave][lane] = l_tot;
   }
+  if (col < static_cast<int>(a.group)) {
 #pragma unroll
-  for (int db = 0; db < 16; ++db) *reinterpret_cast<floatx4 *>(&sh.acc[wave][col][16 * db + 4 * kq]) = acc[db];
+    for (int db = 0; db < 16; ++db) *reinterpret_cast<floatx4 *>(&sh.acc[wave][col][16 * db + 4 * kq]) = acc[db];
+  }
   __syncthreads();
-  const int d = threadIdx.x;
-  for (std::uint32_t h = 0; h < a.group; ++h) {
+  for (std::uint32_t i = threadIdx.x; i < a.group * kHeadDim; i += WAVES * kWave) {
+    const std::uint32_t h = i / kHeadDim, d = i % kHeadDim;
     float m = -FLT_MAX, l = 0.f, o = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) m = fmaxf(m, sh.m[w][h]);
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, sh.m[w][h]);
 #pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float f = fexp2(sh.m[w][h] - m);
       l = fmaf(sh.l[w][h], f, l);
       o = fmaf(sh.acc[w][h][d], f, o);
     }
-    const std::size_t at = ((static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.group + h) * sc.parts + part;
+    if (last) {
+      const std::size_t at = unit * a.group * kHeadDim + i;
+      a.output[at] = f32_to_bf16(o / l * sigmoid_gate(bf16_to_f32(a.gate[at])));
+      continue;
+    }
+    const std::size_t at = (unit * a.group + h) * sc.parts + part;
     sc.o[at * kHeadDim + d] = o;
     if (d == 0) {
       sc.m[at] = m;
       sc.l[at] = l;
     }
   }
+  if constexpr (Weigh) {
+    if (!last) return;
+    for (std::uint32_t i = threadIdx.x; i < seen.total * kCompactBlock; i += WAVES * kWave) {
+      const std::uint32_t j = seen.tile(i / kCompactBlock) * kCompactBlock + i % kCompactBlock;
+      if (!compact_sees(j, p, a.window, a.sinks)) continue;
+      float w = 0.f;
+      for (std::uint32_t h = 0; h < a.group; ++h) {
+        float m = -FLT_MAX, l = 0.f;
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) m = fmaxf(m, sh.m[x][h]);
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) l = fmaf(sh.l[x][h], fexp2(sh.m[x][h] - m), l);
+        w += fexp2(sc.scores[(unit * a.group + h) * sc.score_stride + j] - m) * (1.0f / l);
+      }
+      a.weights[unit * a.max_ctx + j] += w;
+    }
+  }
 }
 
-// One workgroup per (query head, sequence): wave w takes partials w, w + 4, ..,
-// a lane four dims.
-__global__ __launch_bounds__(kDecodeThreads) void compact_merge_kernel(CompactArgs a, DecodeScratch sc) {
-  __shared__ float o_of[kDecodeWaves][kHeadDim], m_of[kDecodeWaves], l_of[kDecodeWaves];
-  const std::uint32_t head = blockIdx.x, seq = blockIdx.y;
-  const std::uint32_t heads = a.kv_heads * a.group;
-  const std::uint32_t n = context_of(a, seq);
-  const std::size_t row = static_cast<std::size_t>(seq) * heads + head;
-  if (n == 0 || n > a.max_ctx) {
-    if (head == 0 && threadIdx.x == 0) atomicAdd(&g_compact_capacity_errors, 1u);
-    a.output[row * kHeadDim + threadIdx.x] = f32_to_bf16(__builtin_nanf(""));
-    return;
-  }
-  const std::uint32_t active = (SeenTiles(n - 1, n - 1, a.window, a.sinks).total + sc.tiles - 1) / sc.tiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float m = -FLT_MAX, l = 0.f;
-  floatx4 o{};
-  for (std::uint32_t i = wave; i < active; i += kDecodeWaves) {
-    const std::size_t at = row * sc.parts + i;
-    const float mi = sc.m[at];
+// Max and 1 / sum over a head's partials, by one wave.
+__device__ __forceinline__ void final_of(const DecodeScratch &sc, std::size_t row, std::uint32_t active, float &m, float &inv) {
+  const int lane = threadIdx.x & 63;
+  float l = 0.f;
+  m = -FLT_MAX;
+  for (std::uint32_t i = lane; i < active; i += 64) {
+    const float mi = sc.m[row * sc.parts + i], li = sc.l[row * sc.parts + i];
     const float m_new = fmaxf(m, mi);
-    const float f = fexp2(m - m_new), g = fexp2(mi - m_new);
-    o = o * f + *reinterpret_cast<const floatx4 *>(sc.o + at * kHeadDim + 4 * lane) * g;
-    l = l * f + sc.l[at] * g;
+    l = l * fexp2(m - m_new) + li * fexp2(mi - m_new);
     m = m_new;
   }
-  *reinterpret_cast<floatx4 *>(&o_of[wave][4 * lane]) = o;
-  if (lane == 0) {
-    m_of[wave] = m;
-    l_of[wave] = l;
-  }
-  __syncthreads();
-  m = fmaxf(fmaxf(m_of[0], m_of[1]), fmaxf(m_of[2], m_of[3]));
-  float sum = 0.f, out = 0.f;
-#pragma unroll
-  for (int w = 0; w < kDecodeWaves; ++w) {
-    const float f = fexp2(m_of[w] - m);
-    sum = fmaf(l_of[w], f, sum);
-    out = fmaf(o_of[w][threadIdx.x], f, out);
-  }
-  const std::size_t at = row * kHeadDim + threadIdx.x;
-  a.output[at] = f32_to_bf16(out / sum * sigmoid_gate(bf16_to_f32(a.gate[at])));
-  if (a.weights != nullptr && threadIdx.x == 0) {
-    sc.final[2 * row] = m;
-    sc.final[2 * row + 1] = 1.0f / sum;
-  }
+  const float m_all = wave_max(m);
+  inv = 1.0f / wave_sum(l * fexp2(m - m_all));
+  m = m_all;
 }
 
-// weights[kvh][j] += the group's probabilities of key j; a thread per seen key.
-__global__ __launch_bounds__(kDecodeThreads) void compact_weigh_kernel(CompactArgs a, DecodeScratch sc) {
-  const std::uint32_t kvh = blockIdx.y, seq = blockIdx.z;
+// Blocks x < query heads join a head's partials: wave w takes partials w, w + 8, ..
+// in batches of 8, whose loads go out before the partials' maxima are known; a lane
+// has four dims.  The blocks behind them (key weights) add the group's probabilities
+// to 512 seen keys of one KV head each.
+__global__ __launch_bounds__(kMergeThreads) void compact_merge_kernel(CompactArgs a, DecodeScratch sc) {
+  __shared__ float o_of[kMergeWaves][kHeadDim], m_of[kCompactMaxGroup], l_of[kCompactMaxGroup];
+  const std::uint32_t seq = blockIdx.y;
+  const std::uint32_t heads = a.kv_heads * a.group;
   const std::uint32_t n = context_of(a, seq);
-  if (n == 0 || n > a.max_ctx) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool valid = n != 0 && n <= a.max_ctx;
+  if (blockIdx.x < heads) {
+    const std::uint32_t head = blockIdx.x;
+    const std::size_t row = static_cast<std::size_t>(seq) * heads + head;
+    if (!valid) {
+      if (head == 0 && threadIdx.x == 0) atomicAdd(&g_compact_capacity_errors, 1u);
+      if (threadIdx.x < kHeadDim) a.output[row * kHeadDim + threadIdx.x] = 0x7FC0;
+      return;
+    }
+    const float gate = threadIdx.x < kHeadDim ? bf16_to_f32(a.gate[row * kHeadDim + threadIdx.x]) : 0.f;
+    const std::uint32_t active = (SeenTiles(n - 1, n - 1, a.window, a.sinks).total + sc.tiles - 1) / sc.tiles;
+    constexpr int kBatch = 8;
+    floatx4 x[kBatch];
+    float mx[kBatch];
+    const auto load = [&](std::uint32_t i0) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const std::uint32_t i = i0 + kMergeWaves * b < active ? i0 + kMergeWaves * b : active - 1;
+        x[b] = *reinterpret_cast<const floatx4 *>(sc.o + (row * sc.parts + i) * kHeadDim + 4 * lane);
+        mx[b] = sc.m[row * sc.parts + i];
+      }
+    };
+    load(wave);
+    float m, inv;
+    final_of(sc, row, active, m, inv);
+    floatx4 o{};
+    for (std::uint32_t i0 = wave; i0 < active; i0 += kMergeWaves * kBatch) {
+      if (i0 != static_cast<std::uint32_t>(wave)) load(i0);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (i0 + kMergeWaves * b < active) o += x[b] * fexp2(mx[b] - m);
+    }
+    *reinterpret_cast<floatx4 *>(&o_of[wave][4 * lane]) = o;
+    __syncthreads();
+    if (threadIdx.x >= kHeadDim) return;
+    float out = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMergeWaves; ++w) out += o_of[w][threadIdx.x];
+    a.output[row * kHeadDim + threadIdx.x] = f32_to_bf16(out * inv * sigmoid_gate(gate));
+    return;
+  }
+  if (!valid) return;
   const SeenTiles seen(n - 1, n - 1, a.window, a.sinks);
-  const std::uint32_t it = (blockIdx.x * kDecodeThreads + threadIdx.x) / kCompactBlock;
-  if (it >= seen.total) return;
-  const std::uint32_t j = seen.tile(it) * kCompactBlock + threadIdx.x % kCompactBlock;
+  const std::uint32_t chunk = (blockIdx.x - heads) / a.kv_heads, kvh = (blockIdx.x - heads) % a.kv_heads;
+  if (chunk * kMergeThreads >= seen.total * kCompactBlock) return; // (uniform)
+  const std::uint32_t active = (seen.total + sc.tiles - 1) / sc.tiles;
+  const std::size_t unit = static_cast<std::size_t>(seq) * a.kv_heads + kvh;
+  for (std::uint32_t h = wave; h < a.group; h += kMergeWaves) {
+    float m, inv;
+    final_of(sc, unit * a.group + h, active, m, inv);
+    if (lane == 0) {
+      m_of[h] = m;
+      l_of[h] = inv;
+    }
+  }
+  __syncthreads();
+  const std::uint32_t i = chunk * kMergeThreads + threadIdx.x;
+  if (i >= seen.total * kCompactBlock) return;
+  const std::uint32_t j = seen.tile(i / kCompactBlock) * kCompactBlock + i % kCompactBlock;
   if (!compact_sees(j, n - 1, a.window, a.sinks)) return;
-  const std::size_t row = (static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.group;
   float w = 0.f;
   for (std::uint32_t h = 0; h < a.group; ++h)
-    w += fexp2(sc.scores[(row + h) * sc.score_stride + j] - sc.final[2 * (row + h)]) * sc.final[2 * (row + h) + 1];
-  a.weights[(static_cast<std::size_t>(seq) * a.kv_heads + kvh) * a.max_ctx + j] += w;
+    w += fexp2(sc.scores[(unit * a.group + h) * sc.score_stride + j] - m_of[h]) * l_of[h];
+  a.weights[unit * a.max_ctx + j] += w;
 }
 
 std::uint32_t most_tiles(const CompactArgs &a, std::uint32_t n) {
@@ -312,19 +558,23 @@ std::uint32_t most_tiles(const CompactArgs &a, std::uint32_t n) {
   return some < all ? static_cast<std::uint32_t>(some) : all;
 }
 
-// At most this many partitions for any context up to max_ctx.
-std::uint32_t most_parts(const CompactArgs &a) {
+// Waves per workgroup, and the partitions that a context of `tiles` tiles is cut into.
+constexpr std::uint32_t kAlone = 16; // tiles that one workgroup takes alone, without a merge
+int decode_waves(const CompactArgs &a) { return a.lengths != nullptr ? 4 : 8; }
+std::uint32_t part_count(const CompactArgs &a, std::uint32_t tiles) {
+  if (tiles <= kAlone) return 1;
   const std::uint32_t units = a.sequences * a.kv_heads;
-  const std::uint32_t target = units >= kDecodeTarget ? 1 : kDecodeTarget / units;
-  const std::uint32_t few = (most_tiles(a, a.max_ctx) + kDecodeWaves - 1) / kDecodeWaves;
-  return few < target ? few : target;
+  const std::uint32_t waves = static_cast<std::uint32_t>(decode_waves(a));
+  const std::uint32_t slots = a.lengths != nullptr ? 4096 : 256;
+  const std::uint32_t want = units >= slots ? 1 : slots / units;
+  const std::uint32_t most = (tiles + waves - 1) / waves;
+  return want < most ? want : most;
 }
 
 std::size_t round16(std::size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-DecodeScratch scratch_of(const CompactArgs &a, void *workspace, std::size_t *bytes) {
+DecodeScratch scratch_of(const CompactArgs &a, std::size_t parts, void *workspace, std::size_t *bytes) {
   const std::size_t heads = static_cast<std::size_t>(a.sequences) * a.kv_heads * a.group;
-  const std::size_t parts = most_parts(a);
   DecodeScratch sc{};
   sc.parts = static_cast<std::uint32_t>(parts);
   sc.score_stride = (a.max_ctx + kCompactBlock - 1) / kCompactBlock * kCompactBlock;
@@ -335,48 +585,59 @@ DecodeScratch scratch_of(const CompactArgs &a, void *workspace, std::size_t *byt
     at += round16(floats * sizeof(float));
     return q;
   };
-  sc.o = take(heads * parts * kHeadDim);
-  sc.m = take(heads * parts);
-  sc.l = take(heads * parts);
-  if (a.observed != 0) {
-    sc.scores = take(heads * sc.score_stride);
-    sc.final = take(heads * 2);
+  if (a.observed != 0) sc.scores = take(heads * sc.score_stride);
+  if (parts > 1) {
+    sc.o = take(heads * parts * kHeadDim);
+    sc.m = take(heads * parts);
+    sc.l = take(heads * parts);
   }
   if (bytes != nullptr) *bytes = at;
   return sc;
 }
 
-template <bool Fp8> void launch_decode(const CompactArgs &a, const DecodeScratch &sc, std::uint32_t parts, hipStream_t stream) {
-  const dim3 grid{parts, a.kv_heads, a.sequences};
-  if (a.weights != nullptr)
-    compact_decode_kernel<Fp8, true><<<grid, kDecodeThreads, 0, stream>>>(a, sc);
+template <bool Fp8, bool Weigh>
+void launch_decode(const CompactArgs &a, const DecodeScratch &sc, std::uint32_t parts, hipStream_t stream) {
+  const unsigned grid = parts * a.kv_heads * a.sequences;
+  if (decode_waves(a) == 8)
+    compact_decode_kernel<Fp8, Weigh, 8><<<grid, 8 * kWave, 0, stream>>>(a, sc);
   else
-    compact_decode_kernel<Fp8, false><<<grid, kDecodeThreads, 0, stream>>>(a, sc);
+    compact_decode_kernel<Fp8, Weigh, 4><<<grid, 4 * kWave, 0, stream>>>(a, sc);
 }
 
 } // namespace
 
 std::size_t compact_decode_workspace(const CompactArgs &a) {
+  // With lengths or without, and for every length: both part counts grow with the tiles.
+  const std::uint32_t tiles = most_tiles(a, a.max_ctx);
+  CompactArgs with = a, without = a;
+  const std::uint32_t some = 1;
+  with.lengths = &some; // (not read)
+  without.lengths = nullptr;
+  const std::uint32_t x = part_count(with, tiles), y = part_count(without, tiles);
   std::size_t bytes = 0;
-  (void)scratch_of(a, nullptr, &bytes);
+  (void)scratch_of(a, x > y ? x : y, nullptr, &bytes);
   return bytes;
 }
 
 void compact_decode(const CompactArgs &a, bool fp8, void *workspace, hipStream_t stream) {
-  compact_append(a, fp8, stream);
-  DecodeScratch sc = scratch_of(a, workspace, nullptr);
-  const std::uint32_t longest = a.lengths == nullptr ? a.past + 1 : a.max_ctx;
   const std::uint32_t total = a.lengths == nullptr ? SeenTiles(a.past, a.past, a.window, a.sinks).total
-                                                   : most_tiles(a, longest);
-  sc.tiles = (total + sc.parts - 1) / sc.parts;
-  if (sc.tiles < kDecodeWaves) sc.tiles = kDecodeWaves;
-  const std::uint32_t parts = (total + sc.tiles - 1) / sc.tiles;
-  if (fp8) launch_decode<true>(a, sc, parts, stream);
-  else launch_decode<false>(a, sc, parts, stream);
-  compact_merge_kernel<<<dim3{a.kv_heads * a.group, a.sequences}, kDecodeThreads, 0, stream>>>(a, sc);
-  if (a.weights != nullptr)
-    compact_weigh_kernel<<<dim3{(total * kCompactBlock + kDecodeThreads - 1) / kDecodeThreads, a.kv_heads, a.sequences},
-                           kDecodeThreads, 0, stream>>>(a, sc);
+                                                   : most_tiles(a, a.max_ctx);
+  std::uint32_t parts = part_count(a, total);
+  DecodeScratch sc = scratch_of(a, parts, workspace, nullptr);
+  sc.tiles = (total + parts - 1) / parts;
+  if (parts > 1) { // the same number of tiles for every wave
+    const std::uint32_t waves = static_cast<std::uint32_t>(decode_waves(a));
+    sc.tiles = (sc.tiles + waves - 1) / waves * waves;
+  }
+  parts = (total + sc.tiles - 1) / sc.tiles;
+  const bool weigh = a.weights != nullptr;
+  if (fp8 && weigh) launch_decode<true, true>(a, sc, parts, stream);
+  else if (fp8) launch_decode<true, false>(a, sc, parts, stream);
+  else if (weigh) launch_decode<false, true>(a, sc, parts, stream);
+  else launch_decode<false, false>(a, sc, parts, stream);
+  if (parts == 1) return;
+  const std::uint32_t chunks = weigh ? (total * kCompactBlock + kMergeThreads - 1) / kMergeThreads : 0;
+  compact_merge_kernel<<<dim3{a.kv_heads * (a.group + chunks), a.sequences}, kMergeThreads, 0, stream>>>(a, sc);
 }
 
 std::uint32_t compact_take_capacity_errors() {
