@@ -127,7 +127,12 @@ namespace {
 using namespace raftinfer::amd;
 using Err = Qwen35PrimitiveError;
 
-constexpr std::size_t kMaxPositions = 0x7FFFFFFF; // positions and columns are 32-bit in the kernels
+// Positions, rows and columns are 32-bit in the kernels, and a grid holds fewer than
+// 2^32 threads in x and 2^16 workgroups in y and z.
+constexpr std::size_t kMaxPositions = std::size_t{1} << 28;
+constexpr std::size_t kMaxHeadPositions = std::size_t{1} << 31; // over all KV heads
+constexpr std::size_t kMaxQueryRows = std::size_t{1} << 26;
+constexpr std::size_t kMaxUnits = std::size_t{1} << 17; // sequences times KV heads
 constexpr std::size_t kMaxGrid = 65535;
 
 std::size_t cache_bytes_of(std::size_t positions, std::size_t kv_heads, Qwen35CompactCacheDType dtype) {
@@ -147,6 +152,11 @@ std::size_t cache_bytes_of(std::size_t positions, std::size_t kv_heads, Qwen35Co
 void validate_heads(std::size_t kv_heads, std::size_t head_dim) {
   require<Err>(kv_heads > 0 && kv_heads <= kMaxGrid / 2, "compact cache kv_heads must be 1 to 32767");
   require<Err>(head_dim == kHeadDim, "compact cache head_dim must be 256");
+}
+
+void validate_positions(std::size_t positions, std::size_t kv_heads) {
+  require<Err>(positions > 0 && positions <= kMaxPositions && positions <= kMaxHeadPositions / kv_heads,
+               "compact attention max_context_tokens must be 1 to 2^28, 2^31 over all KV heads");
 }
 
 void validate_layout(Qwen35KvCacheLayout layout) {
@@ -183,12 +193,12 @@ void validate_shape(const Qwen35CompactShape &s, bool lengths_given) {
   validate_heads(s.kv_heads, s.head_dim);
   require<Err>(s.tokens > 0, "compact attention tokens must be positive");
   require<Err>(s.sequences > 0 && s.sequences <= kMaxGrid, "compact attention sequences must be 1 to 65535");
-  require<Err>(s.max_context_tokens > 0 && s.max_context_tokens <= kMaxPositions,
-               "compact attention max_context_tokens must be 1 to 2^31 - 1");
+  validate_positions(s.max_context_tokens, s.kv_heads);
+  require<Err>(s.sequences <= kMaxUnits / s.kv_heads, "compact attention has too many sequences and KV heads");
   require<Err>(s.query_heads > 0 && s.query_heads % s.kv_heads == 0 &&
                    s.query_heads / s.kv_heads <= kCompactMaxGroup,
                "compact attention query_heads must be 1 to 16 per KV head");
-  require<Err>(s.tokens <= kMaxPositions / s.query_heads, "compact attention has too many query rows");
+  require<Err>(s.tokens <= kMaxQueryRows / s.query_heads, "compact attention has too many query rows");
   if (!lengths_given)
     require<Err>(s.tokens <= s.max_context_tokens && s.past_tokens <= s.max_context_tokens - s.tokens,
                  "compact attention context exceeds cache capacity");
@@ -264,8 +274,7 @@ void validate_call(const void *q, const void *k, const void *v, const void *g, c
 
 std::size_t qwen35_compact_cache_bytes(Qwen35CompactShape shape, Qwen35CompactCacheDType dtype) {
   validate_heads(shape.kv_heads, shape.head_dim);
-  require<Err>(shape.max_context_tokens > 0 && shape.max_context_tokens <= kMaxPositions,
-               "compact attention max_context_tokens must be 1 to 2^31 - 1");
+  validate_positions(shape.max_context_tokens, shape.kv_heads);
   return cache_bytes_of(shape.max_context_tokens, shape.kv_heads, dtype);
 }
 
@@ -349,8 +358,8 @@ namespace {
 CompactEvictArgs evict_args(const Qwen35EvictShape &s) {
   validate_heads(s.kv_heads, s.head_dim);
   require<Err>(s.context_tokens > 0, "compact eviction context_tokens must be positive");
-  require<Err>(s.max_context_tokens <= kMaxPositions && s.out_max_context_tokens <= kMaxPositions,
-               "compact attention max_context_tokens must be 1 to 2^31 - 1");
+  validate_positions(s.max_context_tokens, s.kv_heads);
+  validate_positions(s.out_max_context_tokens, s.kv_heads);
   require<Err>(s.context_tokens <= s.max_context_tokens, "compact eviction context exceeds cache capacity");
   require<Err>(s.keep_tokens > 0 && s.keep_tokens <= s.context_tokens,
                "compact eviction keep_tokens must be 1 to context_tokens");

@@ -109,11 +109,6 @@ __device__ __forceinline__ bool is_finite_f32(float x) {
 // ---------------------------------------------------------- launches
 void compact_append(const CompactArgs &a, bool fp8, hipStream_t stream);
 
-// How a decode call is split: partitions of `tiles` 32-key tiles, at most `parts`.
-struct CompactDecodePlan {
-  std::uint32_t tiles, parts;
-};
-CompactDecodePlan compact_decode_plan(const CompactArgs &a);
 std::size_t compact_decode_workspace(const CompactArgs &a);
 void compact_decode(const CompactArgs &a, bool fp8, void *workspace, hipStream_t stream);
 

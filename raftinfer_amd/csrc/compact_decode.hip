@@ -558,17 +558,36 @@ std::uint32_t most_tiles(const CompactArgs &a, std::uint32_t n) {
   return some < all ? static_cast<std::uint32_t>(some) : all;
 }
 
-// Waves per workgroup, and the partitions that a context of `tiles` tiles is cut into.
-constexpr std::uint32_t kAlone = 16; // tiles that one workgroup takes alone, without a merge
-int decode_waves(const CompactArgs &a) { return a.lengths != nullptr ? 4 : 8; }
-std::uint32_t part_count(const CompactArgs &a, std::uint32_t tiles) {
-  if (tiles <= kAlone) return 1;
-  const std::uint32_t units = a.sequences * a.kv_heads;
-  const std::uint32_t waves = static_cast<std::uint32_t>(decode_waves(a));
-  const std::uint32_t slots = a.lengths != nullptr ? 4096 : 256;
-  const std::uint32_t want = units >= slots ? 1 : slots / units;
-  const std::uint32_t most = (tiles + waves - 1) / waves;
-  return want < most ? want : most;
+// How a call is split whose contexts have up to `total` tiles.  Short contexts: one
+// workgroup of 8 waves per unit and no merge (201 tokens: 9.4 us; cut in two with a
+// merge 14.5 against 14.4 in a graph, and a launch more).  Else partitions of 4 to 32
+// tiles such that about 512 workgroups of 4 waves run at once, two per CU: 16 sequences
+// behind a window of 4096, partitions of 4 / 8 / 16 / 32 tiles 62 / 59 / 55 / 63 us;
+// finer than 32 tiles where there are more (32 ragged sequences, 32 / 64: 214 / 218 us),
+// and at most 64 partitions, which the merge takes in one batch (16000 tokens, 125 / 63
+// partitions: 20.0 / 18.0 us).  Where that leaves at most one workgroup per CU, it gets
+// 8 waves (60001 tokens: 33.5 against 35.0 us).
+constexpr std::uint32_t kAlone = 16;
+constexpr std::uint32_t kMostParts = 64;
+struct DecodeSplit {
+  int waves;
+  std::uint32_t tiles, parts;
+};
+DecodeSplit split_of(const CompactArgs &a, std::uint32_t total) {
+  if (total <= kAlone) return {8, kAlone, 1};
+  const std::uint64_t units = static_cast<std::uint64_t>(a.sequences) * a.kv_heads;
+  const std::uint64_t even = (total * units / 512 + 2) / 4 * 4;
+  std::uint32_t tiles = even < 4 ? 4 : even > 32 ? 32 : static_cast<std::uint32_t>(even);
+  const std::uint32_t least = ((total + kMostParts - 1) / kMostParts + 3) / 4 * 4;
+  if (tiles < least) tiles = least;
+  const std::uint32_t parts = (total + tiles - 1) / tiles;
+  if (parts * units > 256 || tiles < 32) return {4, tiles, parts};
+  return {8, (tiles + 7) / 8 * 8, (total + (tiles + 7) / 8 * 8 - 1) / ((tiles + 7) / 8 * 8)};
+}
+// The most partitions that any context of at most `total` tiles is cut into.
+std::uint32_t most_parts(std::uint32_t total) {
+  if (total <= kAlone) return 1;
+  return (total + 3) / 4 < kMostParts ? (total + 3) / 4 : kMostParts;
 }
 
 std::size_t round16(std::size_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -596,9 +615,9 @@ DecodeScratch scratch_of(const CompactArgs &a, std::size_t parts, void *workspac
 }
 
 template <bool Fp8, bool Weigh>
-void launch_decode(const CompactArgs &a, const DecodeScratch &sc, std::uint32_t parts, hipStream_t stream) {
-  const unsigned grid = parts * a.kv_heads * a.sequences;
-  if (decode_waves(a) == 8)
+void launch_decode(const CompactArgs &a, const DecodeScratch &sc, const DecodeSplit &split, hipStream_t stream) {
+  const unsigned grid = split.parts * a.kv_heads * a.sequences;
+  if (split.waves == 8)
     compact_decode_kernel<Fp8, Weigh, 8><<<grid, 8 * kWave, 0, stream>>>(a, sc);
   else
     compact_decode_kernel<Fp8, Weigh, 4><<<grid, 4 * kWave, 0, stream>>>(a, sc);
@@ -607,35 +626,23 @@ void launch_decode(const CompactArgs &a, const DecodeScratch &sc, std::uint32_t 
 } // namespace
 
 std::size_t compact_decode_workspace(const CompactArgs &a) {
-  // With lengths or without, and for every length: both part counts grow with the tiles.
-  const std::uint32_t tiles = most_tiles(a, a.max_ctx);
-  CompactArgs with = a, without = a;
-  const std::uint32_t some = 1;
-  with.lengths = &some; // (not read)
-  without.lengths = nullptr;
-  const std::uint32_t x = part_count(with, tiles), y = part_count(without, tiles);
   std::size_t bytes = 0;
-  (void)scratch_of(a, x > y ? x : y, nullptr, &bytes);
+  (void)scratch_of(a, most_parts(most_tiles(a, a.max_ctx)), nullptr, &bytes);
   return bytes;
 }
 
 void compact_decode(const CompactArgs &a, bool fp8, void *workspace, hipStream_t stream) {
   const std::uint32_t total = a.lengths == nullptr ? SeenTiles(a.past, a.past, a.window, a.sinks).total
                                                    : most_tiles(a, a.max_ctx);
-  std::uint32_t parts = part_count(a, total);
-  DecodeScratch sc = scratch_of(a, parts, workspace, nullptr);
-  sc.tiles = (total + parts - 1) / parts;
-  if (parts > 1) { // the same number of tiles for every wave
-    const std::uint32_t waves = static_cast<std::uint32_t>(decode_waves(a));
-    sc.tiles = (sc.tiles + waves - 1) / waves * waves;
-  }
-  parts = (total + sc.tiles - 1) / sc.tiles;
+  const DecodeSplit split = split_of(a, total);
+  DecodeScratch sc = scratch_of(a, split.parts, workspace, nullptr);
+  sc.tiles = split.tiles;
   const bool weigh = a.weights != nullptr;
-  if (fp8 && weigh) launch_decode<true, true>(a, sc, parts, stream);
-  else if (fp8) launch_decode<true, false>(a, sc, parts, stream);
-  else if (weigh) launch_decode<false, true>(a, sc, parts, stream);
-  else launch_decode<false, false>(a, sc, parts, stream);
-  if (parts == 1) return;
+  if (fp8 && weigh) launch_decode<true, true>(a, sc, split, stream);
+  else if (fp8) launch_decode<true, false>(a, sc, split, stream);
+  else if (weigh) launch_decode<false, true>(a, sc, split, stream);
+  else launch_decode<false, false>(a, sc, split, stream);
+  if (split.parts == 1) return;
   const std::uint32_t chunks = weigh ? (total * kCompactBlock + kMergeThreads - 1) / kMergeThreads : 0;
   compact_merge_kernel<<<dim3{a.kv_heads * (a.group + chunks), a.sequences}, kMergeThreads, 0, stream>>>(a, sc);
 }

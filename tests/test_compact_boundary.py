@@ -45,7 +45,8 @@ def test_sizes():
     ({"head_dim": 128}, "head_dim must be 256"), ({"kv_heads": 0}, "kv_heads"), ({"query_heads": 0}, "query_heads"),
     ({"query_heads": 6}, "query_heads"), ({"query_heads": 68}, "query_heads"), ({"tokens": 0}, "tokens must be positive"),
     ({"sequences": 0}, "sequences"), ({"sequences": 65536}, "sequences"), ({"max_context_tokens": 0}, "max_context_tokens"),
-    ({"max_context_tokens": 2 ** 31}, "max_context_tokens"), ({"past_tokens": 4096}, "exceeds cache capacity"),
+    ({"max_context_tokens": 2 ** 28 + 1}, "max_context_tokens"), ({"kv_heads": 4096, "query_heads": 4096, "max_context_tokens": 2 ** 20}, "max_context_tokens"),
+    ({"kv_heads": 1024, "query_heads": 1024, "sequences": 129}, "too many sequences"), ({"past_tokens": 4096}, "exceeds cache capacity"),
     ({"past_tokens": 2 ** 64 - 1}, "exceeds cache capacity"), ({"observed_tokens": 2}, "observes more"),
     ({"tokens": 2}, "one token"), ({"observed_tokens": 1}, "key_weights go with")])
 def test_decode_refuses_shapes(change, message):
