@@ -10,14 +10,14 @@ namespace {
 
 using prefill::fexp2;
 using prefill::kLazyRescale;
-using prefill::lds_b128;
-using prefill::lds_tr16;
 
-constexpr int kPWaves = 4;
+constexpr int kPWaves = 8;
 constexpr int kPThreads = kPWaves * kWave;
+constexpr int kSmallWaves = 4; // the merge and the key weights
+constexpr int kSmallThreads = kSmallWaves * kWave;
 constexpr int kPCols = 32 * kPWaves; // columns (token, head of the group) per workgroup
 constexpr int kTileElems = kCompactBlock * kHeadDim;
-constexpr std::uint32_t kPrefillTarget = 512; // workgroups that a call aims at: two per CU
+constexpr std::uint32_t kPrefillTarget = 256; // workgroups that a call aims at: one per CU
 
 // Partials of a split call, [split][kv_head][column], and the final max (exp2
 // domain) and 1 / sum of each column for the key weights.
@@ -26,25 +26,87 @@ struct PrefillScratch {
   std::uint32_t splits, cols; // cols: rounded up to whole workgroups
 };
 
-struct PrefillShared {
-  bf16_bits k[2][kTileElems]; // 16-byte chunk c of row r at c ^ (r & 7)
-  bf16_bits v[2][kTileElems];
-  std::uint32_t odd[2]; // the tile in slot i has infinite or NaN values
+// 16-byte chunk c of row r of a bf16 tile lies at c ^ row_key(r): the 16 rows of a
+// ds_read_b128 pass and the 4 rows x 64 bytes of a ds_read_b64_tr_b16 pass share no bank.
+__device__ __forceinline__ int row_key(int r) { return 4 * (r & 3) + ((r >> 2) & 3); }
+__device__ __forceinline__ int tile_at(int r, int c) { return r * kHeadDim + ((c ^ row_key(r)) << 3); } // in elements
+
+template <bool Fp8> struct PrefillShared {
+  static constexpr int kSlots = Fp8 ? 2 : 3;
+  bf16_bits k[kSlots][kTileElems];
+  bf16_bits v[kSlots][kTileElems];
+  unsigned char raw[Fp8 ? 3 : 1][Fp8 ? 2 * kTileElems : 16]; // K codes, then V codes, rows of 256 bytes
+  float scale[3][kWave];                                     // K scale, V scale of a tile, in turn
+  std::uint32_t odd; // some masked tile had infinite or NaN values
 };
 
-__device__ __forceinline__ int tile_at(int r, int c) { return r * kHeadDim + ((c ^ (r & 7)) << 3); }
-
-__device__ __forceinline__ std::uint32_t odd_bits(std::uint32_t w) {
-  return ((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u) ? 1u : 0u;
+// Whether some column of tokens p_lo .. p_hi does not see some key of the tile at j0.
+__device__ __forceinline__ bool tile_masked(std::uint32_t j0, std::uint32_t p_lo, std::uint32_t p_hi, std::uint32_t window,
+                                            std::uint32_t sinks) {
+  return j0 + kCompactBlock - 1 > p_lo || (window != 0 && j0 + kCompactBlock > sinks && p_hi - j0 >= window);
 }
 
-// A workgroup takes 128 columns (column = token * group + head) of one KV head and a
+// Adds the infinite and NaN values of the masked tiles to the accumulators of the
+// columns that see their keys (a positive probability times such a value is the
+// value).  Register 4 x + e of o[nb] is dim 32 nb + 8 x + 4 kh + e of the lane's column.
+template <bool Fp8>
+__device__ __forceinline__ void add_odd_values(const CompactHead<Fp8> &c, const SeenTiles &seen, std::uint32_t begin,
+                                               std::uint32_t end, std::uint32_t p_lo, std::uint32_t p_hi, std::uint32_t pos,
+                                               std::uint32_t window, std::uint32_t sinks, std::uint32_t n_keys, int kh,
+                                               floatx16 (&o)[8]) {
+#pragma unroll 1
+  for (std::uint32_t it = begin; it < end; ++it) {
+    const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
+    if (!tile_masked(j0, p_lo, p_hi, window, sinks)) continue;
+#pragma unroll 1
+    for (std::uint32_t j = j0; j < j0 + kCompactBlock && j < n_keys; ++j) {
+      if (!compact_sees(j, pos, window, sinks)) continue;
+      const auto *row = c.v + static_cast<std::size_t>(j) * c.row + 4 * kh;
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          floatx4 v;
+          if constexpr (Fp8) {
+            v = fp8x4_to_f32(*reinterpret_cast<const std::uint32_t *>(row + 32 * nb + 8 * x));
+          } else {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(row + 32 * nb + 8 * x);
+            v = floatx4{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nb][4 * x + e] += is_finite_f32(v[e]) ? 0.f : v[e];
+        }
+    }
+  }
+}
+__device__ __forceinline__ u32x4 fp8x8_to_bf16_scaled(std::uint32_t lo, std::uint32_t hi, float scale) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const pair b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const pair c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const pair d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return u32x4{__builtin_bit_cast(std::uint32_t, a), __builtin_bit_cast(std::uint32_t, b),
+               __builtin_bit_cast(std::uint32_t, c), __builtin_bit_cast(std::uint32_t, d)};
+}
+__device__ __forceinline__ bf16x8 lds_operand(unsigned addr) {
+  return __builtin_bit_cast(bf16x8, *(const __attribute__((address_space(3))) u32x4 *)(std::uintptr_t)(addr));
+}
+__device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((prefill::lds_short4v *)(std::uintptr_t)(addr)));
+}
+
+// A workgroup takes 256 columns (column = token * group + head) of one KV head and a
 // contiguous range of the 32-key tiles that they see; a wave takes 32 columns.  The
-// tiles pass through two LDS slots, as bf16, shared by the waves.  S^T = K Q^T and
-// O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, Q and O in registers.
+// tiles lie in LDS as bf16, shared by the waves, and arrive by LDS-direct loads: bf16
+// tiles in place, two tiles ahead, 8-bit tiles as codes, three tiles ahead, which the
+// waves turn into bf16 times the block's scale (exact: 4 significant bits, a power of
+// two) a tile ahead.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, Q and
+// O in registers, two waves per SIMD: one's softmax runs beside the other's products.
 template <bool Fp8, bool Split>
-__global__ __launch_bounds__(kPThreads, 2) void compact_prefill_kernel(CompactArgs a, PrefillScratch sc) {
-  __shared__ PrefillShared sh;
+__global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void compact_prefill_kernel(
+    CompactArgs a, PrefillScratch sc) {
+  __shared__ __attribute__((aligned(1024))) PrefillShared<Fp8> sh;
+  constexpr int kSlots = PrefillShared<Fp8>::kSlots;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kh = lane >> 5;
@@ -64,205 +126,192 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_kernel(CompactAr
   const std::uint32_t col_in = col < all_cols ? col : all_cols - 1; // columns past the last repeat it
   const std::uint32_t tok = col_in / a.group;
   const std::uint32_t pos = a.past + tok;
-  const std::size_t io_row =
-      (static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col_in - tok * a.group);
+  const auto io_row = [&] { return (static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col_in - tok * a.group); };
 
   bf16x8 q[16];
   {
-    const bf16_bits *src = a.query + io_row * kHeadDim + 8 * kh;
+    const bf16_bits *src = a.query + io_row() * kHeadDim + 8 * kh;
 #pragma unroll
     for (int s = 0; s < 16; ++s) q[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(src + 16 * s));
   }
-  if (tid < 2) sh.odd[tid] = 0;
+  if (tid == 0) sh.odd = 0;
 
-  // Staging: rows past the last key repeat it (their scores are masked).
-  constexpr int kStage = Fp8 ? 4 : 1;
-  [[maybe_unused]] u32x4 st[kStage];
-  const auto load_tile = [&](std::uint32_t it, int slot) {
+  // Loads of tile `it` (its kLoads per wave): rows past the last key repeat it (their
+  // scores are masked).
+  constexpr int kLoads = Fp8 ? 3 : 4;
+  const std::uint32_t row_bytes = static_cast<std::uint32_t>(c.row * sizeof(typename CompactHead<Fp8>::T));
+  const auto load_tile = [&](std::uint32_t it) {
     const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
     const std::uint32_t last = n_keys - 1 - j0; // >= 0: the tile has a key
+    const auto *kb = c.k + static_cast<std::size_t>(j0) * c.row, *vb = c.v + static_cast<std::size_t>(j0) * c.row;
     if constexpr (Fp8) {
+      // a load instruction moves 4 rows of K or V: 8 + 8, one each per wave
+      const std::uint32_t r = 4 * wave + (lane >> 4);
+      const std::uint32_t voff = (r < last ? r : last) * row_bytes + 16u * (lane & 15);
+      const unsigned to = lds_address(sh.raw[(it - begin) % 3]) + 1024u * wave;
+      load_lds_b128(kb, voff, to);
+      load_lds_b128(vb, voff, to + kTileElems);
+      // every wave loads the scales, each the same ones: K's in even lanes, V's in odd ones
+      load_lds_b32(c.ks + j0 / kCompactBlock,
+                   lane & 1 ? static_cast<std::uint32_t>(reinterpret_cast<const unsigned char *>(c.vs) - reinterpret_cast<const unsigned char *>(c.ks)) : 0u,
+                   lds_address(sh.scale[(it - begin) % 3]));
+    } else {
+      const int slot = (it - begin) % kSlots;
+      const unsigned lk = lds_address(sh.k[slot]), lv = lds_address(sh.v[slot]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        std::uint32_t r = 16 * i + (tid >> 4);
-        r = r < last ? r : last;
-        const std::size_t off = static_cast<std::size_t>(j0 + r) * c.row + 16 * (tid & 15);
-        st[2 * i] = *reinterpret_cast<const u32x4 *>(c.k + off);
-        st[2 * i + 1] = *reinterpret_cast<const u32x4 *>(c.v + off);
-      }
-    } else {
-      const unsigned lk = lds_address(sh.k[slot]), lv = lds_address(sh.v[slot]);
-      const bf16_bits *kb = c.k + static_cast<std::size_t>(j0) * c.row, *vb = c.v + static_cast<std::size_t>(j0) * c.row;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int inst = 4 * wave + i;
+        const int inst = 2 * wave + i; // rows 2 inst, 2 inst + 1
         const int r = 2 * inst + kh;
-        const std::uint32_t rr = static_cast<std::uint32_t>(r) < last ? r : last;
-        const std::uint32_t voff = rr * static_cast<std::uint32_t>(c.row * 2) + 16u * (n32 ^ (r & 7));
+        const std::uint32_t voff = (static_cast<std::uint32_t>(r) < last ? r : last) * row_bytes + 16u * (n32 ^ row_key(r));
         load_lds_b128(kb, voff, lk + 1024u * inst);
         load_lds_b128(vb, voff, lv + 1024u * inst);
       }
     }
   };
-  const auto store_tile = [&](int slot) {
+  // 8-bit tiles: codes of tile `it` to bf16; thread -> 16 dims of a row of K and of V.
+  const auto convert = [&](std::uint32_t it) {
     if constexpr (Fp8) {
+      const int slot = (it - begin) & 1, from = (it - begin) % 3;
+      const int r = tid >> 4, piece = tid & 15;
+      const float ks = sh.scale[from][0], vs = sh.scale[from][1];
+      const bool up = piece >= 8; // the upper lanes store their second chunk first: no bank twice
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 16 * i + (tid >> 4), piece = tid & 15;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          *reinterpret_cast<u32x4 *>(sh.k[slot] + tile_at(r, 2 * piece + h)) = fp8x8_to_bf16(st[2 * i][2 * h], st[2 * i][2 * h + 1]);
-          *reinterpret_cast<u32x4 *>(sh.v[slot] + tile_at(r, 2 * piece + h)) = fp8x8_to_bf16(st[2 * i + 1][2 * h], st[2 * i + 1][2 * h + 1]);
-        }
+      for (int plane = 0; plane < 2; ++plane) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(sh.raw[from] + plane * kTileElems + r * kHeadDim + 16 * piece);
+        const float scale = plane ? vs : ks;
+        const u32x4 x = fp8x8_to_bf16_scaled(w[0], w[1], scale), y = fp8x8_to_bf16_scaled(w[2], w[3], scale);
+        bf16_bits *tile = plane ? sh.v[slot] : sh.k[slot];
+        *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + up)) = up ? y : x;
+        *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + !up)) = up ? x : y;
       }
-    } else {
-      wait_vm<0>();
     }
   };
 
   // Operand addresses: K row n32, chunk 2 s + kh; V by transposed reads, where lane r
   // of a 16-lane group supplies 4 dims of key row r / 4 and receives its dim of 4 keys.
-  int k_at[4], v_at[2];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) k_at[j] = tile_at(n32, 2 * j + kh);
-  {
-    const int g = lane >> 4, r = lane & 15;
-    const int row = 4 * kh + (r >> 2);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int d = 32 * j + 16 * (g & 1) + 4 * (r & 3);
-      v_at[j] = tile_at(row, d >> 3) + (d & 7);
-    }
-  }
+  // (Chunk numbers differ from a lane's first by an exclusive-or, or by 16.)
+  const unsigned k_lane = 2 * tile_at(n32, kh);
+  const int v_row = 4 * kh + ((lane & 15) >> 2);
+  const unsigned v_lane = 2 * (tile_at(v_row, 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 4 * (lane & 1));
 
   floatx16 o[8];
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) o[nb] = floatx16{};
   float m_run = -FLT_MAX, l_run = 0.f;
 
+  constexpr std::uint32_t kAhead = Fp8 ? 3 : 2; // a tile's loads go out so many tiles ahead
   if (begin < end) {
-    load_tile(begin, 0);
-    store_tile(0);
+    load_tile(begin);
+    for (std::uint32_t i = 1; i < kAhead; ++i)
+      if (begin + i < end) load_tile(begin + i);
+    wait_vm<0>();
+    if constexpr (Fp8) {
+      __syncthreads();
+      convert(begin);
+    }
   }
   __syncthreads();
+  // The waits for q belong here: left to the first use in the loop, they would be made on
+  // every tile, for the tiles' loads too.
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(q[i]));
+  // At the top of tile it: it is in LDS as bf16 (8 bit: it + 1 as codes), and the loads
+  // of the tile behind it are on the way.
   for (std::uint32_t it = begin; it < end; ++it) {
-    const int slot = (it - begin) & 1;
+    const int slot = Fp8 ? (it - begin) & 1 : (it - begin) % kSlots;
     const std::uint32_t tile = seen.tile(it);
     const std::uint32_t j0 = tile * kCompactBlock;
-    const bool more = it + 1 < end;
-    if (more) load_tile(it + 1, slot ^ 1);
-    float k_scale = kLog2e / 16.0f;
-    [[maybe_unused]] float v_scale = 1.0f;
-    if constexpr (Fp8) {
-      k_scale *= c.ks[tile];
-      v_scale = c.vs[tile];
-    }
-    const bf16_bits *kt = sh.k[slot], *vt = sh.v[slot];
+    const bool ahead = it + kAhead < end;
+    if (ahead) load_tile(it + kAhead);
     // Some column does not see some key of the tile (the same for every wave).
-    const bool masked = j0 + kCompactBlock - 1 > p_lo ||
-                        (a.window != 0 && j0 + kCompactBlock > a.sinks && p_hi - j0 >= a.window);
-    bool odd = false;
+    const bool masked = tile_masked(j0, p_lo, p_hi, a.window, a.sinks);
     if (masked) {
-      // A masked key has probability 0, and 0 times an infinite or NaN value is not
-      // 0: such a tile takes another path, key by key.
+      // A masked key has probability 0, and 0 times an infinite or NaN value is not 0:
+      // such values are taken out of the tile here and added behind the loop, to the
+      // columns that see their keys.
       std::uint32_t bad = 0;
+      u32x4 *mine = reinterpret_cast<u32x4 *>(sh.v[slot] + 16 * tid);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(vt + 8 * (tid + kPThreads * i));
-        bad |= odd_bits(w[0]) | odd_bits(w[1]) | odd_bits(w[2]) | odd_bits(w[3]);
+      for (int i = 0; i < 2; ++i) {
+        u32x4 w = mine[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const std::uint32_t x = w[e];
+          const std::uint32_t fine = ((x & 0x7F80u) != 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) != 0x7F800000u ? 0xFFFF0000u : 0u);
+          bad |= ~fine;
+          w[e] = x & fine;
+        }
+        if (bad != 0) mine[i] = w;
       }
-      if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane == 0) sh.odd[slot] = tile + 1;
+      if (bad != 0) sh.odd = 1;
       __syncthreads();
-      odd = sh.odd[slot] == tile + 1;
     }
 
+    // Operands are read four products ahead.
+    bf16x8 op[4];
+    const unsigned k_base = lds_address(sh.k[slot]) + k_lane, v_base = lds_address(sh.v[slot]) + v_lane;
+    const auto read_k = [&](int i) { return lds_operand((k_base ^ (32u * (i >> 1))) + 256u * (i & 1)); }; // k-step i / 2 + 8 (i % 2)
+    const auto read_v = [&](int i) { // key step i / 8, dims block i % 8
+      // rows 8 apart have keys that differ in bit 1
+      const unsigned at = (v_base ^ (64u * (i & 3))) + 256u * ((i >> 2) & 1) + 8192u * (i >> 3);
+      const u32x2 lo = lds_tr_operand(at), hi = lds_tr_operand((at ^ 32u) + 4096u);
+      return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) op[i] = read_k(i);
     floatx16 s = floatx16{};
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      bf16x8 ka[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ka[j] = lds_b128(kt + k_at[j] + 64 * b);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[j], q[4 * b + j], s, 0, 0, 0);
+    for (int i = 0; i < 16; ++i) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q[(i >> 1) + 8 * (i & 1)], s, 0, 0, 0);
+      op[i & 3] = i + 4 < 16 ? read_k(i + 4) : read_v(i + 4 - 16);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (Fp8 && it + 1 < end) convert(it + 1);
     // Register i holds key j0 + 8 (i / 4) + 4 kh + i % 4 of this lane's column.
-    float mx = -INFINITY;
+    constexpr float kScale = kLog2e / 16.0f;
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const std::uint32_t j = j0 + 8 * (i >> 2) + 4 * kh + (i & 3);
-        s[i] = compact_sees(j, pos, a.window, a.sinks) ? s[i] * k_scale : -INFINITY;
-        mx = fmaxf(mx, s[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] *= k_scale;
-        mx = fmaxf(mx, s[i]);
+        s[i] = compact_sees(j, pos, a.window, a.sinks) ? s[i] : -INFINITY;
       }
     }
-    mx = max_xor32(mx);
+    float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+    mx = max_xor32(mx) * kScale;
     // The accumulators are scaled only where a max grows by more than 2^8, which
     // the probabilities can exceed 1 by.
     const bool grow = mx > m_run + kLazyRescale;
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-      const float m_new = grow ? mx : m_run;
       const float f = grow ? fexp2(m_run - mx) : 1.0f;
       l_run *= f;
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) o[nb] *= f;
-      m_run = m_new;
+      m_run = grow ? mx : m_run;
     }
-    float p[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[i] = fexp2(s[i] - m_run);
-      l_run += p[i];
-      if constexpr (Fp8) p[i] *= v_scale;
+      s[i] = fexp2(fmaf(s[i], kScale, -m_run));
+      l_run += s[i];
     }
-    if (!odd) {
-      // k-slot (kb, kh, e) <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of p.
+    // k-slot (kb, kh, e) <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of s.
+    bf16x8 pb[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const u32x4 w{pack_bf16x2(p[8 * kb], p[8 * kb + 1]), pack_bf16x2(p[8 * kb + 2], p[8 * kb + 3]),
-                      pack_bf16x2(p[8 * kb + 4], p[8 * kb + 5]), pack_bf16x2(p[8 * kb + 6], p[8 * kb + 7])};
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, w);
+    for (int kb = 0; kb < 2; ++kb)
+      pb[kb] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(s[8 * kb], s[8 * kb + 1]), pack_bf16x2(s[8 * kb + 2], s[8 * kb + 3]),
+                                                pack_bf16x2(s[8 * kb + 4], s[8 * kb + 5]), pack_bf16x2(s[8 * kb + 6], s[8 * kb + 7])});
 #pragma unroll
-        for (int nb = 0; nb < 8; ++nb) {
-          const bf16_bits *v0 = vt + v_at[nb & 1] + 64 * (nb >> 1) + 16 * kb * kHeadDim;
-          const u32x2 lo = lds_tr16(v0), hi = lds_tr16(v0 + 8 * kHeadDim);
-          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
-                                                          pb, o[nb], 0, 0, 0);
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int r = 0; r < kCompactBlock; ++r) {
-        // p of key r: register 4 (r / 8) + r % 4 of the column's lane with kh = r / 4 % 2
-        float pr = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pr = i == 4 * (r >> 3) + (r & 3) ? p[i] : pr;
-        pr = __shfl(pr, n32 + 32 * ((r >> 2) & 1));
-        const bool sees = compact_sees(j0 + r, pos, a.window, a.sinks);
-#pragma unroll
-        for (int nb = 0; nb < 8; ++nb) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int d = 32 * nb + 8 * x + 4 * kh;
-            const u32x2 w = *reinterpret_cast<const u32x2 *>(vt + tile_at(r, d >> 3) + (d & 7));
-            const float v0 = bf16_lo(w[0]), v1 = bf16_hi(w[0]), v2 = bf16_lo(w[1]), v3 = bf16_hi(w[1]);
-            o[nb][4 * x] += sees ? pr * v0 : 0.f;
-            o[nb][4 * x + 1] += sees ? pr * v1 : 0.f;
-            o[nb][4 * x + 2] += sees ? pr * v2 : 0.f;
-            o[nb][4 * x + 3] += sees ? pr * v3 : 0.f;
-          }
-        }
-      }
+    for (int i = 0; i < 16; ++i) {
+      o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], pb[i >> 3], o[i & 7], 0, 0, 0);
+      if (i + 4 < 16) op[i & 3] = read_v(i + 4);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (more) store_tile(slot ^ 1);
+    if (ahead) wait_vm<kLoads>(); else wait_vm<0>(); // all loads but those of this iteration have landed
     __syncthreads();
   }
 
+  if (sh.odd != 0) add_odd_values<Fp8>(c, seen, begin, end, p_lo, p_hi, pos, a.window, a.sinks, n_keys, kh, o);
   const float l = sum_xor32(l_run);
   if constexpr (Split) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + kvh) * sc.cols + col;
@@ -286,7 +335,7 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_kernel(CompactAr
       sc.final[2 * at] = m_run;
       sc.final[2 * at + 1] = inv;
     }
-    const std::size_t base = io_row * kHeadDim + 4 * kh;
+    const std::size_t base = io_row() * kHeadDim + 4 * kh;
 #pragma unroll
     for (int nb = 0; nb < 8; ++nb)
 #pragma unroll
@@ -303,8 +352,8 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_kernel(CompactAr
 }
 
 // Joins a split call: a wave per column, a lane four dims.
-__global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(CompactArgs a, PrefillScratch sc) {
-  const std::uint32_t col = blockIdx.x * kPWaves + (threadIdx.x >> 6);
+__global__ __launch_bounds__(kSmallThreads) void compact_prefill_merge_kernel(CompactArgs a, PrefillScratch sc) {
+  const std::uint32_t col = blockIdx.x * kSmallWaves + (threadIdx.x >> 6);
   const std::uint32_t kvh = blockIdx.y;
   const int lane = threadIdx.x & 63;
   if (col >= a.tokens * a.group) return;
@@ -341,8 +390,8 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
 // probabilities again from the columns' final max and sum.  The owner sums them, so
 // nothing is added twice or in a changing order.
 template <bool Fp8>
-__global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
-  __shared__ float sum[kPWaves][kCompactBlock];
+__global__ __launch_bounds__(kSmallThreads, 2) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
+  __shared__ float sum[kSmallWaves][kCompactBlock];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, kh = lane >> 5;
@@ -371,7 +420,7 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = 0.f;
   const std::uint32_t all_cols = a.tokens * a.group;
-  for (std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave; c0 < all_cols; c0 += 32 * kPWaves) {
+  for (std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave; c0 < all_cols; c0 += 32 * kSmallWaves) {
     const bool real = c0 + n32 < all_cols;
     const std::uint32_t col = real ? c0 + n32 : all_cols - 1;
     const std::uint32_t tok = col / a.group, pos = a.past + tok;
@@ -442,13 +491,13 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   const dim3 grid{col_blocks(a) * a.kv_heads, splits};
   if (splits > 1) {
     compact_prefill_kernel<Fp8, true><<<grid, kPThreads, 0, stream>>>(a, sc);
-    compact_prefill_merge_kernel<<<dim3{(a.tokens * a.group + kPWaves - 1) / kPWaves, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
+    compact_prefill_merge_kernel<<<dim3{(a.tokens * a.group + kSmallWaves - 1) / kSmallWaves, a.kv_heads}, kSmallThreads, 0, stream>>>(a, sc);
   } else {
     compact_prefill_kernel<Fp8, false><<<grid, kPThreads, 0, stream>>>(a, sc);
   }
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
-    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
+    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kSmallThreads, 0, stream>>>(a, sc);
   }
 }
 
