@@ -263,10 +263,16 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q[(i >> 1) + 8 * (i & 1)], s, 0, 0, 0);
-      op[i & 3] = i + 4 < 16 ? read_k(i + 4) : read_v(i + 4 - 16);
+      if (i + 4 < 16) op[i & 3] = read_k(i + 4);
+      else if (!Fp8) op[i & 3] = read_v(i + 4 - 16);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (Fp8 && it + 1 < end) convert(it + 1);
+    if constexpr (Fp8) {
+      if (it + 1 < end) convert(it + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) op[i] = read_v(i);
+    }
     // Register i holds key j0 + 8 (i / 4) + 4 kh + i % 4 of this lane's column.
     constexpr float kScale = kLog2e / 16.0f;
     if (masked) {
