@@ -11,13 +11,11 @@ namespace {
 using prefill::fexp2;
 using prefill::kLazyRescale;
 
-constexpr int kPWaves = 8;
+constexpr int kPWaves = 4;
 constexpr int kPThreads = kPWaves * kWave;
-constexpr int kSmallWaves = 4; // the merge and the key weights
-constexpr int kSmallThreads = kSmallWaves * kWave;
 constexpr int kPCols = 32 * kPWaves; // columns (token, head of the group) per workgroup
 constexpr int kTileElems = kCompactBlock * kHeadDim;
-constexpr std::uint32_t kPrefillTarget = 256; // workgroups that a call aims at: one per CU
+constexpr std::uint32_t kPrefillTarget = 512; // workgroups that a call aims at: two per CU
 
 // Partials of a split call, [split][kv_head][column], and the final max (exp2
 // domain) and 1 / sum of each column for the key weights.
@@ -31,13 +29,12 @@ struct PrefillScratch {
 __device__ __forceinline__ int row_key(int r) { return 4 * (r & 3) + ((r >> 2) & 3); }
 __device__ __forceinline__ int tile_at(int r, int c) { return r * kHeadDim + ((c ^ row_key(r)) << 3); } // in elements
 
+// 64 or 80 KiB: two workgroups per CU.
 template <bool Fp8> struct PrefillShared {
-  static constexpr int kSlots = Fp8 ? 2 : 3;
-  bf16_bits k[kSlots][kTileElems];
-  bf16_bits v[kSlots][kTileElems];
-  unsigned char raw[Fp8 ? 3 : 1][Fp8 ? 2 * kTileElems : 16]; // K codes, then V codes, rows of 256 bytes
-  float scale[3][kWave];                                     // K scale, V scale of a tile, in turn
-  std::uint32_t odd; // some masked tile had infinite or NaN values
+  bf16_bits k[2][kTileElems];
+  bf16_bits v[2][kTileElems];
+  // 8 bit: a tile's K codes, then V codes, rows of 256 bytes
+  unsigned char raw[Fp8 ? 2 * kTileElems : 16];
 };
 
 // Whether some column of tokens p_lo .. p_hi does not see some key of the tile at j0.
@@ -95,18 +92,18 @@ __device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((prefill::lds_short4v *)(std::uintptr_t)(addr)));
 }
 
-// A workgroup takes 256 columns (column = token * group + head) of one KV head and a
+// A workgroup takes 128 columns (column = token * group + head) of one KV head and a
 // contiguous range of the 32-key tiles that they see; a wave takes 32 columns.  The
-// tiles lie in LDS as bf16, shared by the waves, and arrive by LDS-direct loads: bf16
-// tiles in place, two tiles ahead, 8-bit tiles as codes, three tiles ahead, which the
-// waves turn into bf16 times the block's scale (exact: 4 significant bits, a power of
-// two) a tile ahead.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, Q and
-// O in registers, two waves per SIMD: one's softmax runs beside the other's products.
+// tiles lie in two LDS slots as bf16, shared by the waves, and are asked for by
+// LDS-direct loads a tile ahead: bf16 tiles in place, 8-bit tiles as codes, which each
+// wave turns into bf16 times the block's scale (exact: 4 significant bits, a power of
+// two) for the rows that it loaded.  S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_32x32x16_bf16, Q and O in registers.  Two workgroups share a CU, so that
+// one's softmax runs beside the other's products.
 template <bool Fp8, bool Split>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void compact_prefill_kernel(
     CompactArgs a, PrefillScratch sc) {
   __shared__ __attribute__((aligned(1024))) PrefillShared<Fp8> sh;
-  constexpr int kSlots = PrefillShared<Fp8>::kSlots;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kh = lane >> 5;
@@ -122,65 +119,81 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   const std::uint32_t end = Split ? static_cast<std::uint32_t>(static_cast<std::uint64_t>(seen.total) * (blockIdx.y + 1) / sc.splits) : seen.total;
   const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
 
-  const std::uint32_t col = col0 + 32 * wave + n32;
-  const std::uint32_t col_in = col < all_cols ? col : all_cols - 1; // columns past the last repeat it
-  const std::uint32_t tok = col_in / a.group;
-  const std::uint32_t pos = a.past + tok;
-  const auto io_row = [&] { return (static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col_in - tok * a.group); };
+  // This lane's column; those past the last repeat it.  (Formed anew where it is used:
+  // the loop over the tiles needs every register.)
+  const auto late_lane = [&] {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  const auto column = [&] { return col0 + 32 * wave + (late_lane() & 31); };
+  const auto token_of = [&](std::uint32_t col) { return (col < all_cols ? col : all_cols - 1) / a.group; };
+  const auto io_row = [&](std::uint32_t col) {
+    const std::uint32_t in = col < all_cols ? col : all_cols - 1, tok = in / a.group;
+    return (static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (in - tok * a.group);
+  };
 
   bf16x8 q[16];
   {
-    const bf16_bits *src = a.query + io_row() * kHeadDim + 8 * kh;
+    const bf16_bits *src = a.query + io_row(column()) * kHeadDim + 8 * kh;
 #pragma unroll
     for (int s = 0; s < 16; ++s) q[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(src + 16 * s));
   }
-  if (tid == 0) sh.odd = 0;
+  std::uint64_t odd = 0; // lanes that took infinite or NaN values out of a masked tile
 
-  // Loads of tile `it` (its kLoads per wave): rows past the last key repeat it (their
-  // scores are masked).
-  constexpr int kLoads = Fp8 ? 3 : 4;
+  // Loads of tile `it`: rows past the last key repeat it (their scores are masked).
   const std::uint32_t row_bytes = static_cast<std::uint32_t>(c.row * sizeof(typename CompactHead<Fp8>::T));
+  [[maybe_unused]] float ks = 1.0f, vs = 1.0f; // of the tile whose codes are loaded
   const auto load_tile = [&](std::uint32_t it) {
     const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
     const std::uint32_t last = n_keys - 1 - j0; // >= 0: the tile has a key
     const auto *kb = c.k + static_cast<std::size_t>(j0) * c.row, *vb = c.v + static_cast<std::size_t>(j0) * c.row;
+    const int l = late_lane();
     if constexpr (Fp8) {
-      // a load instruction moves 4 rows of K or V: 8 + 8, one each per wave
-      const std::uint32_t r = 4 * wave + (lane >> 4);
-      const std::uint32_t voff = (r < last ? r : last) * row_bytes + 16u * (lane & 15);
-      const unsigned to = lds_address(sh.raw[(it - begin) % 3]) + 1024u * wave;
-      load_lds_b128(kb, voff, to);
-      load_lds_b128(vb, voff, to + kTileElems);
-      // every wave loads the scales, each the same ones: K's in even lanes, V's in odd ones
-      load_lds_b32(c.ks + j0 / kCompactBlock,
-                   lane & 1 ? static_cast<std::uint32_t>(reinterpret_cast<const unsigned char *>(c.vs) - reinterpret_cast<const unsigned char *>(c.ks)) : 0u,
-                   lds_address(sh.scale[(it - begin) % 3]));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { // 4 rows an instruction
+        const std::uint32_t r = 8 * wave + 4 * i + (l >> 4);
+        const std::uint32_t voff = (r < last ? r : last) * row_bytes + 16u * (l & 15);
+        const unsigned to = lds_address(sh.raw) + 1024u * (2 * wave + i);
+        load_lds_b128(kb, voff, to);
+        load_lds_b128(vb, voff, to + kTileElems);
+      }
     } else {
-      const int slot = (it - begin) % kSlots;
+      const int slot = (it - begin) & 1;
       const unsigned lk = lds_address(sh.k[slot]), lv = lds_address(sh.v[slot]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int inst = 2 * wave + i; // rows 2 inst, 2 inst + 1
-        const int r = 2 * inst + kh;
-        const std::uint32_t voff = (static_cast<std::uint32_t>(r) < last ? r : last) * row_bytes + 16u * (n32 ^ row_key(r));
+      for (int i = 0; i < 4; ++i) {
+        const int inst = 4 * wave + i; // rows 2 inst, 2 inst + 1
+        const int r = 2 * inst + (l >> 5);
+        const std::uint32_t voff = (static_cast<std::uint32_t>(r) < last ? r : last) * row_bytes + 16u * ((l & 31) ^ row_key(r));
         load_lds_b128(kb, voff, lk + 1024u * inst);
         load_lds_b128(vb, voff, lv + 1024u * inst);
       }
     }
   };
-  // 8-bit tiles: codes of tile `it` to bf16; thread -> 16 dims of a row of K and of V.
-  const auto convert = [&](std::uint32_t it) {
+  const auto load_scales = [&](std::uint32_t it) {
     if constexpr (Fp8) {
-      const int slot = (it - begin) & 1, from = (it - begin) % 3;
-      const int r = tid >> 4, piece = tid & 15;
-      const float ks = sh.scale[from][0], vs = sh.scale[from][1];
+      const std::uint32_t at = seen.tile(it) + (late_lane() >> 6); // (+ 0: vector loads, see the decode kernel)
+      ks = c.ks[at];
+      vs = c.vs[at];
+    }
+  };
+  // The loads of tile `it` have landed; 8 bit: the codes that this wave loaded become
+  // bf16 (lane -> 16 dims of a row).
+  const auto finish_tile = [&](std::uint32_t it) {
+    wait_vm<0>();
+    if constexpr (Fp8) {
+      const int slot = (it - begin) & 1;
+      const int l = late_lane();
+      const int piece = l & 15;
       const bool up = piece >= 8; // the upper lanes store their second chunk first: no bank twice
 #pragma unroll
-      for (int plane = 0; plane < 2; ++plane) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(sh.raw[from] + plane * kTileElems + r * kHeadDim + 16 * piece);
-        const float scale = plane ? vs : ks;
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * wave + 4 * (i & 1) + (l >> 4);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(sh.raw + (i >> 1) * kTileElems + r * kHeadDim + 16 * piece);
+        const float scale = i >> 1 ? vs : ks;
         const u32x4 x = fp8x8_to_bf16_scaled(w[0], w[1], scale), y = fp8x8_to_bf16_scaled(w[2], w[3], scale);
-        bf16_bits *tile = plane ? sh.v[slot] : sh.k[slot];
+        bf16_bits *tile = i >> 1 ? sh.v[slot] : sh.k[slot];
         *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + up)) = up ? y : x;
         *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + !up)) = up ? x : y;
       }
@@ -199,41 +212,32 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   for (int nb = 0; nb < 8; ++nb) o[nb] = floatx16{};
   float m_run = -FLT_MAX, l_run = 0.f;
 
-  constexpr std::uint32_t kAhead = Fp8 ? 3 : 2; // a tile's loads go out so many tiles ahead
   if (begin < end) {
     load_tile(begin);
-    for (std::uint32_t i = 1; i < kAhead; ++i)
-      if (begin + i < end) load_tile(begin + i);
-    wait_vm<0>();
-    if constexpr (Fp8) {
-      __syncthreads();
-      convert(begin);
-    }
+    load_scales(begin);
+    finish_tile(begin);
   }
   __syncthreads();
   // The waits for q belong here: left to the first use in the loop, they would be made on
   // every tile, for the tiles' loads too.
 #pragma unroll
   for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(q[i]));
-  // At the top of tile it: it is in LDS as bf16 (8 bit: it + 1 as codes), and the loads
-  // of the tile behind it are on the way.
   for (std::uint32_t it = begin; it < end; ++it) {
-    const int slot = Fp8 ? (it - begin) & 1 : (it - begin) % kSlots;
-    const std::uint32_t tile = seen.tile(it);
-    const std::uint32_t j0 = tile * kCompactBlock;
-    const bool ahead = it + kAhead < end;
-    if (ahead) load_tile(it + kAhead);
+    const int slot = (it - begin) & 1;
+    const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
+    const bool more = it + 1 < end;
+    if (more) load_tile(it + 1);
     // Some column does not see some key of the tile (the same for every wave).
     const bool masked = tile_masked(j0, p_lo, p_hi, a.window, a.sinks);
     if (masked) {
       // A masked key has probability 0, and 0 times an infinite or NaN value is not 0:
       // such values are taken out of the tile here and added behind the loop, to the
       // columns that see their keys.
-      std::uint32_t bad = 0;
-      u32x4 *mine = reinterpret_cast<u32x4 *>(sh.v[slot] + 16 * tid);
+      u32x4 *mine = reinterpret_cast<u32x4 *>(sh.v[slot] + 8 * (64 * wave + late_lane()));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        u32x4 w = mine[i];
+      for (int i = 0; i < 4; ++i) {
+        u32x4 w = mine[kPThreads * i];
+        std::uint32_t bad = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const std::uint32_t x = w[e];
@@ -241,9 +245,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
           bad |= ~fine;
           w[e] = x & fine;
         }
-        if (bad != 0) mine[i] = w;
+        if (bad != 0) mine[kPThreads * i] = w;
+        odd |= __builtin_amdgcn_ballot_w64(bad != 0);
       }
-      if (bad != 0) sh.odd = 1;
       __syncthreads();
     }
 
@@ -263,22 +267,17 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q[(i >> 1) + 8 * (i & 1)], s, 0, 0, 0);
-      if (i + 4 < 16) op[i & 3] = read_k(i + 4);
-      else if (!Fp8) op[i & 3] = read_v(i + 4 - 16);
+      op[i & 3] = i + 4 < 16 ? read_k(i + 4) : read_v(i + 4 - 16);
       __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (Fp8) {
-      if (it + 1 < end) convert(it + 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) op[i] = read_v(i);
     }
     // Register i holds key j0 + 8 (i / 4) + 4 kh + i % 4 of this lane's column.
     constexpr float kScale = kLog2e / 16.0f;
     if (masked) {
+      const int late = late_lane();
+      const std::uint32_t pos = a.past + token_of(col0 + 32 * wave + (late & 31));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const std::uint32_t j = j0 + 8 * (i >> 2) + 4 * kh + (i & 3);
+        const std::uint32_t j = j0 + 8 * (i >> 2) + 4 * (late >> 5) + (i & 3);
         s[i] = compact_sees(j, pos, a.window, a.sinks) ? s[i] : -INFINITY;
       }
     }
@@ -301,6 +300,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       s[i] = fexp2(fmaf(s[i], kScale, -m_run));
       l_run += s[i];
     }
+    if (more) load_scales(it + 1);
     // k-slot (kb, kh, e) <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of s.
     bf16x8 pb[2];
 #pragma unroll
@@ -313,11 +313,16 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       if (i + 4 < 16) op[i & 3] = read_v(i + 4);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (ahead) wait_vm<kLoads>(); else wait_vm<0>(); // all loads but those of this iteration have landed
+    if (more) finish_tile(it + 1);
     __syncthreads();
   }
 
-  if (sh.odd != 0) add_odd_values<Fp8>(c, seen, begin, end, p_lo, p_hi, pos, a.window, a.sinks, n_keys, kh, o);
+  const std::uint32_t col = column();
+  // (the tiles' LDS is free)
+  auto *odd_of = reinterpret_cast<std::uint32_t *>(&sh);
+  if (lane == 0) odd_of[wave] = odd != 0;
+  __syncthreads();
+  if ((odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3]) != 0) add_odd_values<Fp8>(c, seen, begin, end, p_lo, p_hi, a.past + token_of(col), a.window, a.sinks, n_keys, kh, o);
   const float l = sum_xor32(l_run);
   if constexpr (Split) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + kvh) * sc.cols + col;
@@ -341,54 +346,85 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       sc.final[2 * at] = m_run;
       sc.final[2 * at + 1] = inv;
     }
-    const std::size_t base = io_row() * kHeadDim + 4 * kh;
+    const std::size_t base = io_row(col) * kHeadDim + 4 * kh;
+    u32x2 g[32]; // (every load before the first store, which it might alias)
 #pragma unroll
-    for (int nb = 0; nb < 8; ++nb)
+    for (int i = 0; i < 32; ++i) g[i] = *reinterpret_cast<const u32x2 *>(a.gate + base + 8 * i);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const std::size_t at = base + 32 * nb + 8 * x;
-        const u32x2 g = *reinterpret_cast<const u32x2 *>(a.gate + at);
-        const float r0 = o[nb][4 * x] * inv * sigmoid_gate(bf16_lo(g[0]));
-        const float r1 = o[nb][4 * x + 1] * inv * sigmoid_gate(bf16_hi(g[0]));
-        const float r2 = o[nb][4 * x + 2] * inv * sigmoid_gate(bf16_lo(g[1]));
-        const float r3 = o[nb][4 * x + 3] * inv * sigmoid_gate(bf16_hi(g[1]));
-        *reinterpret_cast<u32x2 *>(a.output + at) = u32x2{pack_bf16x2(r0, r1), pack_bf16x2(r2, r3)};
-      }
+    for (int i = 0; i < 32; ++i) {
+      const int nb = i >> 2, x = 4 * (i & 3);
+      const float r0 = o[nb][x] * inv * sigmoid_gate(bf16_lo(g[i][0])), r1 = o[nb][x + 1] * inv * sigmoid_gate(bf16_hi(g[i][0]));
+      const float r2 = o[nb][x + 2] * inv * sigmoid_gate(bf16_lo(g[i][1])), r3 = o[nb][x + 3] * inv * sigmoid_gate(bf16_hi(g[i][1]));
+      *reinterpret_cast<u32x2 *>(a.output + base + 8 * i) = u32x2{pack_bf16x2(r0, r1), pack_bf16x2(r2, r3)};
+    }
   }
 }
 
-// Joins a split call: a wave per column, a lane four dims.
-__global__ __launch_bounds__(kSmallThreads) void compact_prefill_merge_kernel(CompactArgs a, PrefillScratch sc) {
-  const std::uint32_t col = blockIdx.x * kSmallWaves + (threadIdx.x >> 6);
-  const std::uint32_t kvh = blockIdx.y;
+// Joins a split call: W waves per column take its splits in turn, eight loads of a
+// partial row at a time in flight, a lane four dims.
+template <int W>
+__global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(CompactArgs a, PrefillScratch sc) {
+  __shared__ float o_of[kPWaves][kHeadDim];
   const int lane = threadIdx.x & 63;
-  if (col >= a.tokens * a.group) return;
-  float m = -FLT_MAX;
-  for (std::uint32_t s = 0; s < sc.splits; ++s)
-    m = fmaxf(m, sc.m[(static_cast<std::size_t>(s) * a.kv_heads + kvh) * sc.cols + col]);
-  float l = 0.f;
-  floatx4 o{};
-  for (std::uint32_t s = 0; s < sc.splits; ++s) {
-    const std::size_t at = (static_cast<std::size_t>(s) * a.kv_heads + kvh) * sc.cols + col;
-    const float ls = sc.l[at], ms = sc.m[at];
-    if (ls == 0.f && ms == -FLT_MAX) continue; // the split holds no key that the column sees
-    const float f = fexp2(ms - m);
-    l = fmaf(ls, f, l);
-    o += *reinterpret_cast<const floatx4 *>(sc.o + at * kHeadDim + 4 * lane) * f;
-  }
-  const float inv = 1.0f / l;
-  if (a.weights != nullptr && lane == 0) {
-    const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col;
-    sc.final[2 * at] = m;
-    sc.final[2 * at + 1] = inv;
-  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const std::uint32_t all_cols = a.tokens * a.group;
+  const std::uint32_t col_of = blockIdx.x * (kPWaves / W) + wave / W;
+  const std::uint32_t col = col_of < all_cols ? col_of : all_cols - 1;
+  const std::uint32_t kvh = blockIdx.y;
+  const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * sc.cols; // between splits
+  const std::size_t at0 = static_cast<std::size_t>(kvh) * sc.cols + col;
   const std::uint32_t tok = col / a.group;
-  const std::size_t at =
+  const std::size_t out_at =
       ((static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col - tok * a.group)) * kHeadDim + 4 * lane;
-  const u32x2 g = *reinterpret_cast<const u32x2 *>(a.gate + at);
+  const u32x2 g = *reinterpret_cast<const u32x2 *>(a.gate + out_at);
+  constexpr int kBatch = 8;
+  floatx4 x[kBatch];
+  const auto load = [&](std::uint32_t s0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const std::uint32_t s = s0 + W * b < sc.splits ? s0 + W * b : sc.splits - 1;
+      x[b] = *reinterpret_cast<const floatx4 *>(sc.o + (at0 + s * stride) * kHeadDim + 4 * lane);
+    }
+  };
+  const std::uint32_t first = W == 1 ? 0 : wave % W;
+  load(first);
+  // max and sum over the splits; those without a key that the column sees have l = 0
+  float m = -FLT_MAX, l = 0.f;
+  for (std::uint32_t s = lane; s < sc.splits; s += 64) {
+    const float ms = sc.m[at0 + s * stride], ls = sc.l[at0 + s * stride];
+    const float m_new = fmaxf(m, ms);
+    l = l * fexp2(m - m_new) + ls * fexp2(ms - m_new);
+    m = m_new;
+  }
+  const float m_all = wave_max(m);
+  const float inv = 1.0f / wave_sum(l * fexp2(m - m_all));
+  floatx4 o{};
+  for (std::uint32_t s0 = first; s0 < sc.splits; s0 += W * kBatch) {
+    if (s0 != first) load(s0);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const std::uint32_t s = s0 + W * b;
+      if (s >= sc.splits) break;
+      const float ms = sc.m[at0 + s * stride];
+      if (ms == -FLT_MAX && sc.l[at0 + s * stride] == 0.f) continue; // nothing was summed
+      o += x[b] * fexp2(ms - m_all);
+    }
+  }
+  if constexpr (W > 1) {
+    *reinterpret_cast<floatx4 *>(&o_of[wave][4 * lane]) = o;
+    __syncthreads();
+    if (wave % W != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) o += *reinterpret_cast<const floatx4 *>(&o_of[wave + w][4 * lane]);
+  }
+  if (col_of >= all_cols) return;
+  if (a.weights != nullptr && lane == 0) {
+    sc.final[2 * at0] = m_all;
+    sc.final[2 * at0 + 1] = inv;
+  }
   const float r0 = o[0] * inv * sigmoid_gate(bf16_lo(g[0])), r1 = o[1] * inv * sigmoid_gate(bf16_hi(g[0]));
   const float r2 = o[2] * inv * sigmoid_gate(bf16_lo(g[1])), r3 = o[3] * inv * sigmoid_gate(bf16_hi(g[1]));
-  *reinterpret_cast<u32x2 *>(a.output + at) = u32x2{pack_bf16x2(r0, r1), pack_bf16x2(r2, r3)};
+  *reinterpret_cast<u32x2 *>(a.output + out_at) = u32x2{pack_bf16x2(r0, r1), pack_bf16x2(r2, r3)};
 }
 
 // Key weights of the last `observed` tokens: a workgroup owns a 32-key tile of one KV
@@ -396,8 +432,8 @@ __global__ __launch_bounds__(kSmallThreads) void compact_prefill_merge_kernel(Co
 // probabilities again from the columns' final max and sum.  The owner sums them, so
 // nothing is added twice or in a changing order.
 template <bool Fp8>
-__global__ __launch_bounds__(kSmallThreads, 2) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
-  __shared__ float sum[kSmallWaves][kCompactBlock];
+__global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
+  __shared__ float sum[kPWaves][kCompactBlock];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, kh = lane >> 5;
@@ -426,7 +462,7 @@ __global__ __launch_bounds__(kSmallThreads, 2) void compact_prefill_weigh_kernel
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = 0.f;
   const std::uint32_t all_cols = a.tokens * a.group;
-  for (std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave; c0 < all_cols; c0 += 32 * kSmallWaves) {
+  for (std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave; c0 < all_cols; c0 += 32 * kPWaves) {
     const bool real = c0 + n32 < all_cols;
     const std::uint32_t col = real ? c0 + n32 : all_cols - 1;
     const std::uint32_t tok = col / a.group, pos = a.past + tok;
@@ -497,13 +533,17 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   const dim3 grid{col_blocks(a) * a.kv_heads, splits};
   if (splits > 1) {
     compact_prefill_kernel<Fp8, true><<<grid, kPThreads, 0, stream>>>(a, sc);
-    compact_prefill_merge_kernel<<<dim3{(a.tokens * a.group + kSmallWaves - 1) / kSmallWaves, a.kv_heads}, kSmallThreads, 0, stream>>>(a, sc);
+    const std::uint32_t cols = a.tokens * a.group;
+    if (splits > 8)
+      compact_prefill_merge_kernel<kPWaves><<<dim3{cols, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
+    else
+      compact_prefill_merge_kernel<1><<<dim3{(cols + kPWaves - 1) / kPWaves, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
   } else {
     compact_prefill_kernel<Fp8, false><<<grid, kPThreads, 0, stream>>>(a, sc);
   }
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
-    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kSmallThreads, 0, stream>>>(a, sc);
+    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
   }
 }
 
