@@ -37,6 +37,19 @@ template <bool Fp8> struct PrefillShared {
   unsigned char raw[Fp8 ? 2 * kTileElems : 16];
 };
 
+// Sets the infinite and NaN values among eight bf16 to 0; whether there were any.
+__device__ __forceinline__ bool without_odd(u32x4 &w) {
+  std::uint32_t bad = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const std::uint32_t x = w[e];
+    const std::uint32_t fine = ((x & 0x7F80u) != 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) != 0x7F800000u ? 0xFFFF0000u : 0u);
+    bad |= ~fine;
+    w[e] = x & fine;
+  }
+  return bad != 0;
+}
+
 // Whether some column of tokens p_lo .. p_hi does not see some key of the tile at j0.
 __device__ __forceinline__ bool tile_masked(std::uint32_t j0, std::uint32_t p_lo, std::uint32_t p_hi, std::uint32_t window,
                                             std::uint32_t sinks) {
@@ -98,9 +111,10 @@ __device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
 // LDS-direct loads a tile ahead: bf16 tiles in place, 8-bit tiles as codes, which each
 // wave turns into bf16 times the block's scale (exact: 4 significant bits, a power of
 // two) for the rows that it loaded.  S^T = K Q^T and O^T = V^T P^T on
-// v_mfma_f32_32x32x16_bf16, Q and O in registers.  Two workgroups share a CU, so that
-// one's softmax runs beside the other's products.
-template <bool Fp8, bool Split>
+// v_mfma_f32_32x32x16_bf16, Q and O in registers.  A tile's softmax, one barrier, then
+// its product with V and the next tile's scores in turn: two workgroups share a CU, so
+// that one's softmax runs beside the other's products.
+template <bool Fp8, bool Split, bool Weigh>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void compact_prefill_kernel(
     CompactArgs a, PrefillScratch sc) {
   __shared__ __attribute__((aligned(1024))) PrefillShared<Fp8> sh;
@@ -139,63 +153,66 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
     for (int s = 0; s < 16; ++s) q[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(src + 16 * s));
   }
-  std::uint64_t odd = 0; // lanes that took infinite or NaN values out of a masked tile
 
-  // Loads of tile `it`: rows past the last key repeat it (their scores are masked).
+  // Loads of tile `it`'s K or V (a wave loads rows 8 wave .. + 7): rows past the last
+  // key repeat it (their scores are masked).  In a whole tile the instructions' offsets
+  // are the lane's, an exclusive-or (the rows' keys differ in bits of their own) and a
+  // scalar.
   const std::uint32_t row_bytes = static_cast<std::uint32_t>(c.row * sizeof(typename CompactHead<Fp8>::T));
-  [[maybe_unused]] float ks = 1.0f, vs = 1.0f; // of the tile whose codes are loaded
-  const auto load_tile = [&](std::uint32_t it) {
+  const auto load_tile = [&](std::uint32_t it, bool is_v) {
     const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
     const std::uint32_t last = n_keys - 1 - j0; // >= 0: the tile has a key
-    const auto *kb = c.k + static_cast<std::size_t>(j0) * c.row, *vb = c.v + static_cast<std::size_t>(j0) * c.row;
+    const auto *tile = reinterpret_cast<const unsigned char *>((is_v ? c.v : c.k) + static_cast<std::size_t>(j0) * c.row);
+    const int l = late_lane();
+    constexpr int kInst = Fp8 ? 2 : 4, kRows = 8 / kInst; // rows an instruction
+    const unsigned to = Fp8 ? lds_address(sh.raw) + (is_v ? kTileElems : 0) + 2048u * wave
+                            : lds_address(is_v ? sh.v[(it - begin) & 1] : sh.k[(it - begin) & 1]) + 4096u * wave;
+    const std::uint32_t in = l / (64 / kRows), chunk = l % (64 / kRows); // row and 16-byte chunk of instruction 0
+    if (last >= kCompactBlock - 1) {
+      const std::uint32_t off = in * row_bytes + 16u * (Fp8 ? chunk : chunk ^ row_key(8 * wave + in));
+#pragma unroll
+      for (int i = 0; i < kInst; ++i)
+        load_lds_b128(tile + (8u * wave + kRows * i) * row_bytes, Fp8 ? off : off ^ (16u * (8 * (i & 1) + (i >> 1))), to + 1024u * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kInst; ++i) {
+        const std::uint32_t r = 8 * wave + kRows * i + in;
+        load_lds_b128(tile, (r < last ? r : last) * row_bytes + 16u * (Fp8 ? chunk : chunk ^ row_key(r)), to + 1024u * i);
+      }
+    }
+  };
+  // This wave's rows of tile `it`'s K or V have landed (the caller waits): 8-bit codes
+  // become bf16 times the block's scale.  A masked key has
+  // probability 0, and 0 times an infinite or NaN value is not 0: in V tiles that some
+  // column does not see whole, such values are taken out here and added behind the
+  // loop, to the columns that see their keys.
+  std::uint64_t odd = 0; // lanes that took values out
+  const auto finish_tile = [&](std::uint32_t it, bool is_v, [[maybe_unused]] float scale) {
+    const int slot = (it - begin) & 1;
+    const bool clean = is_v && tile_masked(seen.tile(it) * kCompactBlock, p_lo, p_hi, a.window, a.sinks);
+    bf16_bits *tile = is_v ? sh.v[slot] : sh.k[slot];
     const int l = late_lane();
     if constexpr (Fp8) {
+      // lane -> 8 dims (one bf16 chunk) of rows 2 i + lane / 32
+      u32x2 raw[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) { // 4 rows an instruction
-        const std::uint32_t r = 8 * wave + 4 * i + (l >> 4);
-        const std::uint32_t voff = (r < last ? r : last) * row_bytes + 16u * (l & 15);
-        const unsigned to = lds_address(sh.raw) + 1024u * (2 * wave + i);
-        load_lds_b128(kb, voff, to);
-        load_lds_b128(vb, voff, to + kTileElems);
-      }
-    } else {
-      const int slot = (it - begin) & 1;
-      const unsigned lk = lds_address(sh.k[slot]), lv = lds_address(sh.v[slot]);
+      for (int i = 0; i < 4; ++i)
+        raw[i] = *reinterpret_cast<const u32x2 *>(sh.raw + (is_v ? kTileElems : 0) + (8 * wave + 2 * i) * kHeadDim + 8 * l);
+      const int at = (l & 31) ^ row_key(8 * wave + (l >> 5));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int inst = 4 * wave + i; // rows 2 inst, 2 inst + 1
-        const int r = 2 * inst + (l >> 5);
-        const std::uint32_t voff = (static_cast<std::uint32_t>(r) < last ? r : last) * row_bytes + 16u * ((l & 31) ^ row_key(r));
-        load_lds_b128(kb, voff, lk + 1024u * inst);
-        load_lds_b128(vb, voff, lv + 1024u * inst);
+        u32x4 x = fp8x8_to_bf16_scaled(raw[i][0], raw[i][1], scale);
+        if (clean) odd |= __builtin_amdgcn_ballot_w64(without_odd(x));
+        *reinterpret_cast<u32x4 *>(tile + (8 * wave + 2 * i + (l >> 5)) * kHeadDim + 8 * (at ^ (8 * (i & 1) + (i >> 1)))) = x;
       }
-    }
-  };
-  const auto load_scales = [&](std::uint32_t it) {
-    if constexpr (Fp8) {
-      const std::uint32_t at = seen.tile(it) + (late_lane() >> 6); // (+ 0: vector loads, see the decode kernel)
-      ks = c.ks[at];
-      vs = c.vs[at];
-    }
-  };
-  // The loads of tile `it` have landed; 8 bit: the codes that this wave loaded become
-  // bf16 (lane -> 16 dims of a row).
-  const auto finish_tile = [&](std::uint32_t it) {
-    wait_vm<0>();
-    if constexpr (Fp8) {
-      const int slot = (it - begin) & 1;
-      const int l = late_lane();
-      const int piece = l & 15;
-      const bool up = piece >= 8; // the upper lanes store their second chunk first: no bank twice
+    } else if (clean) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 8 * wave + 4 * (i & 1) + (l >> 4);
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(sh.raw + (i >> 1) * kTileElems + r * kHeadDim + 16 * piece);
-        const float scale = i >> 1 ? vs : ks;
-        const u32x4 x = fp8x8_to_bf16_scaled(w[0], w[1], scale), y = fp8x8_to_bf16_scaled(w[2], w[3], scale);
-        bf16_bits *tile = i >> 1 ? sh.v[slot] : sh.k[slot];
-        *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + up)) = up ? y : x;
-        *reinterpret_cast<u32x4 *>(tile + tile_at(r, 2 * piece + !up)) = up ? x : y;
+        u32x4 *mine = reinterpret_cast<u32x4 *>(tile + 2048 * wave + 512 * i + 8 * l);
+        u32x4 w = *mine;
+        const bool bad = without_odd(w);
+        if (bad) *mine = w;
+        odd |= __builtin_amdgcn_ballot_w64(bad);
       }
     }
   };
@@ -212,73 +229,54 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   for (int nb = 0; nb < 8; ++nb) o[nb] = floatx16{};
   float m_run = -FLT_MAX, l_run = 0.f;
 
-  if (begin < end) {
-    load_tile(begin);
-    load_scales(begin);
-    finish_tile(begin);
-  }
-  __syncthreads();
-  // The waits for q belong here: left to the first use in the loop, they would be made on
-  // every tile, for the tiles' loads too.
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(q[i]));
-  for (std::uint32_t it = begin; it < end; ++it) {
-    const int slot = (it - begin) & 1;
-    const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
-    const bool more = it + 1 < end;
-    if (more) load_tile(it + 1);
-    // Some column does not see some key of the tile (the same for every wave).
-    const bool masked = tile_masked(j0, p_lo, p_hi, a.window, a.sinks);
-    if (masked) {
-      // A masked key has probability 0, and 0 times an infinite or NaN value is not 0:
-      // such values are taken out of the tile here and added behind the loop, to the
-      // columns that see their keys.
-      u32x4 *mine = reinterpret_cast<u32x4 *>(sh.v[slot] + 8 * (64 * wave + late_lane()));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x4 w = mine[kPThreads * i];
-        std::uint32_t bad = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const std::uint32_t x = w[e];
-          const std::uint32_t fine = ((x & 0x7F80u) != 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) != 0x7F800000u ? 0xFFFF0000u : 0u);
-          bad |= ~fine;
-          w[e] = x & fine;
-        }
-        if (bad != 0) mine[kPThreads * i] = w;
-        odd |= __builtin_amdgcn_ballot_w64(bad != 0);
-      }
-      __syncthreads();
-    }
+  const auto scale_of = [&](const float *scales, std::uint32_t it) {
+    if constexpr (Fp8) return scales[seen.tile(it)]; // (a scalar load: no LDS reads are under way then)
+    return 1.0f;
+  };
+  const auto k_addr = [&](std::uint32_t it) { return lds_address(sh.k[(it - begin) & 1]) + k_lane; };
+  const auto read_k = [&](unsigned base, int i) { return lds_operand((base ^ (32u * (i >> 1))) + 256u * (i & 1)); }; // k-step i / 2 + 8 (i % 2)
+  const auto read_v = [&](unsigned base, int i) { // key step i / 8, dims block i % 8
+    // rows 8 apart have keys that differ in bit 1
+    const unsigned at = 256u * ((i >> 2) & 1) + 8192u * (i >> 3);
+    const u32x2 lo = lds_tr_operand((base ^ (64u * (i & 3))) + at), hi = lds_tr_operand((base ^ (64u * (i & 3) + 32u)) + (at + 4096u));
+    return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+  };
+  const auto q_of = [&](int i) -> const bf16x8 & { return q[(i >> 1) + 8 * (i & 1)]; };
 
-    // Operands are read four products ahead.
-    bf16x8 op[4];
-    const unsigned k_base = lds_address(sh.k[slot]) + k_lane, v_base = lds_address(sh.v[slot]) + v_lane;
-    const auto read_k = [&](int i) { return lds_operand((k_base ^ (32u * (i >> 1))) + 256u * (i & 1)); }; // k-step i / 2 + 8 (i % 2)
-    const auto read_v = [&](int i) { // key step i / 8, dims block i % 8
-      // rows 8 apart have keys that differ in bit 1
-      const unsigned at = (v_base ^ (64u * (i & 3))) + 256u * ((i >> 2) & 1) + 8192u * (i >> 3);
-      const u32x2 lo = lds_tr_operand(at), hi = lds_tr_operand((at ^ 32u) + 4096u);
-      return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-    };
+  floatx16 s = floatx16{}; // scores of tile it: register i has key 8 (i / 4) + 4 kh + i % 4
+  if (begin < end) {
+    load_tile(begin, false);
+    const float ks = scale_of(c.ks, begin);
+    wait_vm<0>();
+    finish_tile(begin, false, ks);
+    __syncthreads();
+    load_tile(begin, true);
+    if (begin + 1 < end) load_tile(begin + 1, false);
+    // The waits for q belong here: left to the first use in the loop, they would be made on
+    // every tile, for the tiles' loads too.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) op[i] = read_k(i);
-    floatx16 s = floatx16{};
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(q[i]));
+    const unsigned base = k_addr(begin);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q[(i >> 1) + 8 * (i & 1)], s, 0, 0, 0);
-      op[i & 3] = i + 4 < 16 ? read_k(i + 4) : read_v(i + 4 - 16);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // Register i holds key j0 + 8 (i / 4) + 4 kh + i % 4 of this lane's column.
+    for (int i = 0; i < 16; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k(base, i), q_of(i), s, 0, 0, 0);
+  }
+  // One tile; kMore: it is not the last.
+  const auto step = [&]<bool kMore>(std::uint32_t it) __attribute__((always_inline)) {
+    const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
+    [[maybe_unused]] const float vs = scale_of(c.vs, it), ks = kMore ? scale_of(c.ks, it + 1) : 1.0f;
     constexpr float kScale = kLog2e / 16.0f;
-    if (masked) {
+    if (tile_masked(j0, p_lo, p_hi, a.window, a.sinks)) { // some column does not see some key
       const int late = late_lane();
       const std::uint32_t pos = a.past + token_of(col0 + 32 * wave + (late & 31));
+      const std::uint32_t j_lane = j0 + 4 * (late >> 5);
+      if (a.window == 0) {
+        const int lim = static_cast<int>(pos) - static_cast<int>(j_lane);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const std::uint32_t j = j0 + 8 * (i >> 2) + 4 * (late >> 5) + (i & 3);
-        s[i] = compact_sees(j, pos, a.window, a.sinks) ? s[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) <= lim ? s[i] : -INFINITY;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[i] = compact_sees(j_lane + 8 * (i >> 2) + (i & 3), pos, a.window, a.sinks) ? s[i] : -INFINITY;
       }
     }
     float mx = fmaxf(s[0], s[1]);
@@ -295,27 +293,59 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       for (int nb = 0; nb < 8; ++nb) o[nb] *= f;
       m_run = grow ? mx : m_run;
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = fexp2(fmaf(s[i], kScale, -m_run));
-      l_run += s[i];
-    }
-    if (more) load_scales(it + 1);
-    // k-slot (kb, kh, e) <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of s.
+    // k-slot (kb, kh, e) of V^T P^T <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of s.
     bf16x8 pb[2];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-      pb[kb] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(s[8 * kb], s[8 * kb + 1]), pack_bf16x2(s[8 * kb + 2], s[8 * kb + 3]),
-                                                pack_bf16x2(s[8 * kb + 4], s[8 * kb + 5]), pack_bf16x2(s[8 * kb + 6], s[8 * kb + 7])});
+    for (int kb = 0; kb < 2; ++kb) {
+      u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], pb[i >> 3], o[i & 7], 0, 0, 0);
-      if (i + 4 < 16) op[i & 3] = read_v(i + 4);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = fexp2(fmaf(s[8 * kb + 2 * e], kScale, -m_run)), p1 = fexp2(fmaf(s[8 * kb + 2 * e + 1], kScale, -m_run));
+        const std::uint32_t pair = pack_bf16x2(p0, p1);
+        w[e] = pair;
+        // The sum is that of the rounded probabilities, with which the output is a convex
+        // combination of the V rows; key weights need the exact one.
+        if constexpr (Weigh) l_run += p0 + p1; else l_run = dot2_bf16(pair, 0x3F803F80u, l_run);
+      }
+      pb[kb] = __builtin_bit_cast(bf16x8, w);
     }
-    if (more) finish_tile(it + 1);
-    __syncthreads();
+    // V(it) and K(it + 1), asked for a tile ago
+    wait_vm<0>();
+    finish_tile(it, true, vs);
+    if constexpr (Fp8 && kMore) finish_tile(it + 1, false, ks);
+    __syncthreads(); // ... of every wave; and no wave reads V(it - 1) or K(it) any more
+    const unsigned v_base = lds_address(sh.v[(it - begin) & 1]) + v_lane;
+    if constexpr (kMore) {
+      load_tile(it + 1, true);
+      if (it + 2 < end) load_tile(it + 2, false);
+      // O += V(it) P(it) and S(it + 1) in turn: the second is a chain of dependent products.
+      const unsigned k_base = k_addr(it + 1);
+      bf16x8 vo[2], ko[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ko[i] = read_k(k_base, i);
+        vo[i] = read_v(v_base, i);
+      }
+      s = floatx16{};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[i & 1], q_of(i), s, 0, 0, 0);
+        if (i + 2 < 16) ko[i & 1] = read_k(k_base, i + 2);
+        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vo[i & 1], pb[i >> 3], o[i & 7], 0, 0, 0);
+        if (i + 2 < 16) vo[i & 1] = read_v(v_base, i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(v_base, i), pb[i >> 3], o[i & 7], 0, 0, 0);
+    }
+  };
+  if (begin < end) {
+    for (std::uint32_t it = begin; it + 1 < end; ++it) step.template operator()<true>(it);
+    step.template operator()<false>(end - 1);
   }
+  __syncthreads();
 
   const std::uint32_t col = column();
   // (the tiles' LDS is free)
@@ -531,15 +561,21 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   const std::uint32_t splits = split_count(a, SeenTiles(first, last, a.window, a.sinks).total);
   const PrefillScratch sc = scratch_of(a, splits, workspace, nullptr);
   const dim3 grid{col_blocks(a) * a.kv_heads, splits};
+  const auto launch = [&](auto split) {
+    if (a.weights != nullptr)
+      compact_prefill_kernel<Fp8, split, true><<<grid, kPThreads, 0, stream>>>(a, sc);
+    else
+      compact_prefill_kernel<Fp8, split, false><<<grid, kPThreads, 0, stream>>>(a, sc);
+  };
   if (splits > 1) {
-    compact_prefill_kernel<Fp8, true><<<grid, kPThreads, 0, stream>>>(a, sc);
+    launch(std::true_type{});
     const std::uint32_t cols = a.tokens * a.group;
     if (splits > 8)
       compact_prefill_merge_kernel<kPWaves><<<dim3{cols, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
     else
       compact_prefill_merge_kernel<1><<<dim3{(cols + kPWaves - 1) / kPWaves, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
   } else {
-    compact_prefill_kernel<Fp8, false><<<grid, kPThreads, 0, stream>>>(a, sc);
+    launch(std::false_type{});
   }
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
