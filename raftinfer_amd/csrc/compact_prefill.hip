@@ -318,21 +318,22 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     if constexpr (kMore) {
       load_tile(it + 1, true);
       if (it + 2 < end) load_tile(it + 2, false);
-      // O += V(it) P(it) and S(it + 1) in turn: the second is a chain of dependent products.
+      // O += V(it) P(it), then S(it + 1); operands are read four products ahead.
       const unsigned k_base = k_addr(it + 1);
-      bf16x8 vo[2], ko[2];
+      bf16x8 op[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ko[i] = read_k(k_base, i);
-        vo[i] = read_v(v_base, i);
+      for (int i = 0; i < 4; ++i) op[i] = read_v(v_base, i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], pb[i >> 3], o[i & 7], 0, 0, 0);
+        op[i & 3] = i + 4 < 16 ? read_v(v_base, i + 4) : read_k(k_base, i + 4 - 16);
+        __builtin_amdgcn_sched_barrier(0);
       }
       s = floatx16{};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[i & 1], q_of(i), s, 0, 0, 0);
-        if (i + 2 < 16) ko[i & 1] = read_k(k_base, i + 2);
-        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vo[i & 1], pb[i >> 3], o[i & 7], 0, 0, 0);
-        if (i + 2 < 16) vo[i & 1] = read_v(v_base, i + 2);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q_of(i), s, 0, 0, 0);
+        if (i + 4 < 16) op[i & 3] = read_k(k_base, i + 4);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
