@@ -350,7 +350,8 @@ def weights_of(r, hkv, n):
 
 @pytest.mark.parametrize("dtype,out_dtype,layout", [(BF16, BF16, 1), (BF16, FP8, 1), (FP8, FP8, 1), (FP8, FP8, 0), (BF16, BF16, 0)])
 @pytest.mark.parametrize("n,keep,sinks,recent,spare", [(1, 1, 0, 0, 0), (64, 64, 3, 5, 0), (100, 33, 0, 0, 40), (100, 1, 1, 0, 3),
-                                                       (333, 100, 4, 96, 0), (333, 101, 4, 96, 1), (1500, 700, 4, 64, 5)])
+                                                       (333, 100, 4, 96, 0), (333, 101, 4, 96, 1), (1500, 700, 4, 64, 5), (4096, 1000, 0, 1, 0),
+                                                       (4097, 4000, 5, 0, 0), (17000, 33, 1, 1, 0)])
 def test_evict(gpu, dtype, out_dtype, layout, n, keep, sinks, recent, spare):
     r = rng(110 + n)
     hkv = 3
@@ -377,6 +378,26 @@ def test_evict(gpu, dtype, out_dtype, layout, n, keep, sinks, recent, spare):
             out.ref[:, h, :keep] = held[:, h, idx]
     out.check("new cache")
     c.check("old cache")
+
+
+@pytest.mark.parametrize("n,keep", [(16384, 200), (16385, 107), (65536, 9000), (65537, 65000), (150001, 40000)])
+@pytest.mark.parametrize("few", [False, True])
+def test_evict_selection_of_long_caches(gpu, n, keep, few):
+    # the choice alone (rows of one head): spread weights, or a handful of different ones
+    r = rng(125)
+    w = weights_of(r, 2, n) if not few else r.integers(0, 4, (2, n)).astype(np.float32)
+    buf = torch.zeros(ops.qwen35_compact_cache_bytes(ops.Qwen35CompactShape(1, 1, 2, 2, D, n, 0), FP8), device="cuda", dtype=torch.uint8)
+    out = torch.zeros(ops.qwen35_compact_cache_bytes(ops.Qwen35CompactShape(1, 1, 2, 2, D, keep, 0), FP8), device="cuda", dtype=torch.uint8)
+    out_w, kept = torch.empty(2, keep, device="cuda"), torch.empty(2, keep, device="cuda", dtype=torch.int32)
+    shape = ops.Qwen35EvictShape(2, D, n, n, keep, keep, 7, 100)
+    ws = torch.full((ops.qwen35_compact_evict_workspace_bytes(shape),), 0xFF, device="cuda", dtype=torch.uint8)
+    ops.qwen35_compact_cache_evict(buf, dev(w, torch.float32), out, out_w, kept, shape, FP8, FP8, 1, ws)
+    for h in range(2):
+        rank = w[h].astype(np.float64)
+        rank[:7] = rank[n - 100:] = np.inf
+        want = np.sort(np.argsort(-rank, kind="stable")[:keep])
+        assert np.array_equal(kept[h].cpu().numpy(), want)
+        assert np.array_equal(host(out_w[h]), w[h][want])
 
 
 def test_evict_order_of_odd_weights(gpu):
