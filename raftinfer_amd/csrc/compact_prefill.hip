@@ -246,12 +246,12 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   floatx16 s = floatx16{}; // scores of tile it: register i has key 8 (i / 4) + 4 kh + i % 4
   if (begin < end) {
     load_tile(begin, false);
+    load_tile(begin, true);
     const float ks = scale_of(c.ks, begin);
     wait_vm<0>();
     finish_tile(begin, false, ks);
-    __syncthreads();
-    load_tile(begin, true);
     if (begin + 1 < end) load_tile(begin + 1, false);
+    __syncthreads();
     // The waits for q belong here: left to the first use in the loop, they would be made on
     // every tile, for the tiles' loads too.
 #pragma unroll
@@ -318,22 +318,23 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     if constexpr (kMore) {
       load_tile(it + 1, true);
       if (it + 2 < end) load_tile(it + 2, false);
-      // O += V(it) P(it), then S(it + 1); operands are read four products ahead.
+      // O += V(it) P(it), then S(it + 1); operands are read kRing products ahead.
       const unsigned k_base = k_addr(it + 1);
-      bf16x8 op[4];
+      constexpr int kRing = 6;
+      bf16x8 op[kRing];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) op[i] = read_v(v_base, i);
+      for (int i = 0; i < kRing; ++i) op[i] = read_v(v_base, i);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], pb[i >> 3], o[i & 7], 0, 0, 0);
-        op[i & 3] = i + 4 < 16 ? read_v(v_base, i + 4) : read_k(k_base, i + 4 - 16);
+        o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % kRing], pb[i >> 3], o[i & 7], 0, 0, 0);
+        op[i % kRing] = i + kRing < 16 ? read_v(v_base, i + kRing) : read_k(k_base, i + kRing - 16);
         __builtin_amdgcn_sched_barrier(0);
       }
       s = floatx16{};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i & 3], q_of(i), s, 0, 0, 0);
-        if (i + 4 < 16) op[i & 3] = read_k(k_base, i + 4);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[(i + 16) % kRing], q_of(i), s, 0, 0, 0);
+        if (i + kRing < 16) op[(i + 16) % kRing] = read_k(k_base, i + kRing);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
