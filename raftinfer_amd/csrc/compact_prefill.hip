@@ -15,7 +15,7 @@ constexpr int kPWaves = 4;
 constexpr int kPThreads = kPWaves * kWave;
 constexpr int kPCols = 32 * kPWaves; // columns (token, head of the group) per workgroup
 constexpr int kTileElems = kCompactBlock * kHeadDim;
-constexpr std::uint32_t kPrefillTarget = 512; // workgroups that a call aims at: two per CU
+constexpr std::uint32_t kPrefillCus = 256;
 
 // Partials of a split call, [split][kv_head][column], and the final max (exp2
 // domain) and 1 / sum of each column for the key weights.
@@ -525,12 +525,20 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
 
 std::uint32_t col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kPCols - 1) / kPCols; }
 
-// Key splits of a call whose widest column block sees `tiles` tiles.
+// Key splits of a call whose widest column block sees `tiles` tiles: two workgroups per
+// CU where each still has 16 tiles, else one per CU, of at least four tiles.  Two per CU
+// overlap softmax and products but leave twice the partial rows to be joined.  Measured
+// (2 KV heads, 8 query heads each; one against two per CU): 500 tokens behind 2000
+// (10 tiles at two) 58.1 against 61.8 us, behind 4000 (18) 79.1 against 77.5, behind
+// 16000 (64) 208 against 174; 1000 tokens (8) 48.8 against 55.6, 1500 (23) 77.2 against
+// 71.3.  Four tiles against eight: 2 tokens behind 2000 26.5 against 31.5 us, 500 tokens
+// 36.0 against 38.5.  (Grows with `tiles`: the workspace is sized at the largest.)
 std::uint32_t split_count(const CompactArgs &a, std::uint32_t tiles) {
   const std::uint64_t groups = static_cast<std::uint64_t>(col_blocks(a)) * a.kv_heads;
-  std::uint64_t splits = groups >= kPrefillTarget ? 1 : kPrefillTarget / groups;
-  if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4; // at least four tiles each
-  return static_cast<std::uint32_t>(splits);
+  const std::uint64_t wanted = groups * tiles >= 2 * kPrefillCus * 16 ? 2 * kPrefillCus : kPrefillCus;
+  const std::uint64_t splits = groups >= wanted ? 1 : wanted / groups;
+  const std::uint64_t most = (static_cast<std::uint64_t>(tiles) + 3) / 4;
+  return static_cast<std::uint32_t>(splits < most ? splits : most);
 }
 
 PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t splits, void *workspace, std::size_t *bytes) {
