@@ -56,36 +56,34 @@ __device__ __forceinline__ bool tile_masked(std::uint32_t j0, std::uint32_t p_lo
   return j0 + kCompactBlock - 1 > p_lo || (window != 0 && j0 + kCompactBlock > sinks && p_hi - j0 >= window);
 }
 
-// Adds the infinite and NaN values of the masked tiles to the accumulators of the
-// columns that see their keys (a positive probability times such a value is the
-// value).  Register 4 x + e of o[nb] is dim 32 nb + 8 x + 4 kh + e of the lane's column.
-template <bool Fp8>
+// Adds the infinite and NaN values of the masked tiles among begin, begin + stride, ..
+// to the accumulators of a column that sees their keys (a positive probability times
+// such a value is the value).  The lane has kQuads quads of its column's dims: quad i is
+// dims 4 k + 256 / kQuads * i + 0 .. 3, and add(4 i + e, x) adds to one.
+template <bool Fp8, int kQuads, class Add>
 __device__ __forceinline__ void add_odd_values(const CompactHead<Fp8> &c, const SeenTiles &seen, std::uint32_t begin,
-                                               std::uint32_t end, std::uint32_t p_lo, std::uint32_t p_hi, std::uint32_t pos,
-                                               std::uint32_t window, std::uint32_t sinks, std::uint32_t n_keys, int kh,
-                                               floatx16 (&o)[8]) {
+                                               std::uint32_t end, std::uint32_t stride, std::uint32_t p_lo, std::uint32_t p_hi,
+                                               std::uint32_t pos, const CompactArgs &a, int k, Add add) {
 #pragma unroll 1
-  for (std::uint32_t it = begin; it < end; ++it) {
+  for (std::uint32_t it = begin; it < end; it += stride) {
     const std::uint32_t j0 = seen.tile(it) * kCompactBlock;
-    if (!tile_masked(j0, p_lo, p_hi, window, sinks)) continue;
+    if (!tile_masked(j0, p_lo, p_hi, a.window, a.sinks)) continue;
 #pragma unroll 1
-    for (std::uint32_t j = j0; j < j0 + kCompactBlock && j < n_keys; ++j) {
-      if (!compact_sees(j, pos, window, sinks)) continue;
-      const auto *row = c.v + static_cast<std::size_t>(j) * c.row + 4 * kh;
+    for (std::uint32_t j = j0; j < j0 + kCompactBlock && j <= p_hi; ++j) {
+      if (!compact_sees(j, pos, a.window, a.sinks)) continue;
+      const auto *row = c.v + static_cast<std::size_t>(j) * c.row + 4 * k;
 #pragma unroll
-      for (int nb = 0; nb < 8; ++nb)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          floatx4 v;
-          if constexpr (Fp8) {
-            v = fp8x4_to_f32(*reinterpret_cast<const std::uint32_t *>(row + 32 * nb + 8 * x));
-          } else {
-            const u32x2 w = *reinterpret_cast<const u32x2 *>(row + 32 * nb + 8 * x);
-            v = floatx4{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nb][4 * x + e] += is_finite_f32(v[e]) ? 0.f : v[e];
+      for (int i = 0; i < kQuads; ++i) {
+        floatx4 v;
+        if constexpr (Fp8) {
+          v = fp8x4_to_f32(*reinterpret_cast<const std::uint32_t *>(row + kHeadDim / kQuads * i));
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2 *>(row + kHeadDim / kQuads * i);
+          v = floatx4{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add(4 * i + e, is_finite_f32(v[e]) ? 0.f : v[e]);
+      }
     }
   }
 }
@@ -100,6 +98,11 @@ __device__ __forceinline__ u32x4 fp8x8_to_bf16_scaled(std::uint32_t lo, std::uin
 }
 __device__ __forceinline__ bf16x8 lds_operand(unsigned addr) {
   return __builtin_bit_cast(bf16x8, *(const __attribute__((address_space(3))) u32x4 *)(std::uintptr_t)(addr));
+}
+// Of 16 lanes, lane r supplies 8 bytes of row r / 2 and receives its byte of 8 rows.
+__device__ __forceinline__ u32x2 lds_tr8_operand(unsigned addr) {
+  typedef int pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) pair *)(std::uintptr_t)(addr)));
 }
 __device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((prefill::lds_short4v *)(std::uintptr_t)(addr)));
@@ -354,7 +357,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   auto *odd_of = reinterpret_cast<std::uint32_t *>(&sh);
   if (lane == 0) odd_of[wave] = odd != 0;
   __syncthreads();
-  if ((odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3]) != 0) add_odd_values<Fp8>(c, seen, begin, end, p_lo, p_hi, a.past + token_of(col), a.window, a.sinks, n_keys, kh, o);
+  if ((odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3]) != 0)
+    add_odd_values<Fp8, 32>(c, seen, begin, end, 1, p_lo, p_hi, a.past + token_of(col), a, kh,
+                            [&](int i, float x) __attribute__((always_inline)) { o[i >> 4][i & 15] += x; });
   const float l = sum_xor32(l_run);
   if constexpr (Split) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + kvh) * sc.cols + col;
@@ -389,6 +394,382 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       const float r2 = o[nb][x + 2] * inv * sigmoid_gate(bf16_lo(g[i][1])), r3 = o[nb][x + 3] * inv * sigmoid_gate(bf16_hi(g[i][1]));
       *reinterpret_cast<u32x2 *>(a.output + base + 8 * i) = u32x2{pack_bf16x2(r0, r1), pack_bf16x2(r2, r3)};
     }
+  }
+}
+
+// The same for calls with too few columns to fill the chip by 128: a workgroup takes 32
+// columns of one KV head, its waves take every fourth tile of the range by themselves and
+// are joined in LDS.  Products on v_mfma_f32_16x16x32_bf16 with two blocks of 16 columns.
+// K and V rows lie in LDS as they are in the cache (8-bit operands become bf16 behind the
+// read; the block's scales go on the scores and the probabilities), asked for by
+// LDS-direct loads of the wave's own kStages tiles ahead.
+constexpr int kKCols = 32;
+struct KeysShared {
+  union {
+    unsigned char rows[kPWaves][4 * kTileElems]; // [stage][K, V], 16-byte chunks as keys_at
+    // (the pad puts the 16 columns of a store on banks of their own)
+    float acc[kPWaves][kKCols][kHeadDim + 4];
+  };
+  alignas(1024) bf16_bits gate[kPWaves][kKCols / kPWaves][kHeadDim];
+  float m[kPWaves][kKCols], l[kPWaves][kKCols];
+};
+// What a row's number is exclusive-ored to its 16-byte chunks' places with (linear in the
+// bits of r): a pass of the K reads takes one chunk of 16 rows, of the V reads
+// 16 bytes of the 16 rows 4 k + 0 .. 3, 16 + 4 k + 0 .. 3 of two k (8 bit) or 32 of 8 rows.
+template <bool Fp8> __device__ __forceinline__ constexpr std::uint32_t keys_at(std::uint32_t r, bool is_v) {
+  if (!is_v) return r & 15;
+  return Fp8 ? (r & 3) | (r >> 4 & 1) << 2 | (r >> 2 & 1) << 3 : 2 * (r & 7);
+}
+template <bool Fp8, bool Split>
+__global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
+    CompactArgs a, PrefillScratch sc) {
+  __shared__ __attribute__((aligned(1024))) KeysShared sh;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col16 = lane & 15, kq = lane >> 4;
+  // grid (kv_heads, column blocks, splits)
+  const std::uint32_t kvh = blockIdx.x;
+  const std::uint32_t all_cols = a.tokens * a.group;
+  const std::uint32_t col0 = (gridDim.y - 1 - blockIdx.y) * kKCols; // longest first
+  const std::uint32_t last_x = all_cols - col0 < kKCols ? all_cols - col0 - 1 : kKCols - 1;
+  // Column col0 + x (x < 32; those past the last repeat it) is head in_first + x - token_in(x)
+  // * group of token first + token_in(x).  The quotient of n <= 46 and group <= 16 is
+  // n (1024 / group + 1) >> 10, as 16 n < 1024.
+  const std::uint32_t first = col0 / a.group, in_first = col0 - first * a.group, over = 1024 / a.group + 1;
+  const auto token_in = [&](std::uint32_t x) { return ((x < last_x ? x : last_x) + in_first) * over >> 10; };
+  const std::uint32_t p_lo = a.past + first, p_hi = p_lo + token_in(last_x);
+  // First element of the column's row of query, gate and output, from `row0`.  (The launch
+  // has at most 2^14 KV heads and a workgroup 47 rows between its tokens: 32 bits hold it.)
+  const std::size_t row0 = (static_cast<std::size_t>(first) * a.kv_heads + kvh) * a.group * kHeadDim;
+  const auto row_at = [&](std::uint32_t x) {
+    const std::uint32_t tok = token_in(x);
+    return (tok * (a.kv_heads - 1) * a.group + in_first + (x < last_x ? x : last_x)) * kHeadDim;
+  };
+  const SeenTiles seen(p_lo, p_hi, a.window, a.sinks);
+  std::uint32_t begin = 0, end = seen.total;
+  if constexpr (Split) {
+    const std::uint32_t each = seen.total / sc.splits, more = seen.total - each * sc.splits;
+    begin = blockIdx.z * each + (blockIdx.z < more ? blockIdx.z : more);
+    end = begin + each + (blockIdx.z < more);
+    if (begin == end) { // nothing to sum
+      if (threadIdx.x < kKCols) {
+        const std::size_t at = (static_cast<std::size_t>(blockIdx.z) * a.kv_heads + kvh) * sc.cols + col0 + threadIdx.x;
+        sc.m[at] = -FLT_MAX;
+        sc.l[at] = 0.f;
+      }
+      return;
+    }
+  }
+  const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
+
+  // Steps: the wave's tiles.  LDS-direct loads of one plane of step t: rows past the last
+  // key repeat it (their scores are masked).
+  const std::uint32_t steps = begin + wave < end ? (end - begin - wave + kPWaves - 1) / kPWaves : 0;
+  const auto tile_of = [&](std::uint32_t t) { return seen.tile(begin + wave + kPWaves * t); };
+  constexpr int kStages = Fp8 ? 2 : 1;
+  constexpr int kRowBytes = Fp8 ? 256 : 512, kRows = 1024 / kRowBytes; // rows of an instruction
+  constexpr int kLoads = kCompactBlock / kRows;
+  const std::uint32_t row_bytes = static_cast<std::uint32_t>(c.row * sizeof(typename CompactHead<Fp8>::T));
+  const unsigned rows_at = lds_address(sh.rows[wave]);
+  const auto plane_at = [&](std::uint32_t t, bool is_v) {
+    return rows_at + kRowBytes * kCompactBlock * (2 * (t % kStages) + is_v);
+  };
+  const std::uint32_t in_row = lane / (64 / kRows), chunk = lane % (64 / kRows);
+  const std::uint32_t off_k = in_row * row_bytes + 16 * (chunk ^ keys_at<Fp8>(in_row, false));
+  const std::uint32_t off_v = in_row * row_bytes + 16 * (chunk ^ keys_at<Fp8>(in_row, true));
+  const auto load = [&](std::uint32_t t, bool is_v) __attribute__((always_inline)) {
+    const std::uint32_t j0 = tile_of(t) * kCompactBlock, last = p_hi - j0; // >= 0: the tile has a key
+    const auto *tile = reinterpret_cast<const unsigned char *>((is_v ? c.v : c.k) + static_cast<std::size_t>(j0) * c.row);
+    const unsigned to = plane_at(t, is_v);
+    if (last >= kCompactBlock - 1) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_lds_b128(tile + kRows * i * row_bytes, (is_v ? off_v : off_k) ^ (16 * keys_at<Fp8>(kRows * i, is_v)), to + 1024 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const std::uint32_t r = kRows * i + in_row;
+        load_lds_b128(tile, (r < last ? r : last) * row_bytes + 16 * (chunk ^ keys_at<Fp8>(r, is_v)), to + 1024 * i);
+      }
+    }
+  };
+  // Lane l: scales of step t0 + l.
+  float ks_of = 1.0f, vs_of = 1.0f;
+  const auto load_scales = [&](std::uint32_t t0) {
+    if constexpr (Fp8) {
+      const std::uint32_t t = t0 + lane < steps ? t0 + lane : steps - 1;
+      ks_of = c.ks[tile_of(t)];
+      vs_of = c.vs[tile_of(t)];
+    }
+  };
+  const auto lane_value = [](float x, std::uint32_t l) {
+    return __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(x)), l)));
+  };
+
+  // q of the lane's two columns, in the dims that its K operands hold.
+  bf16x8 qb[2][8];
+  std::uint32_t pos[2];
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) {
+    pos[cb] = p_lo + token_in(16 * cb + col16);
+    const bf16_bits *q = a.query + row0 + row_at(16 * cb + col16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int dim = Fp8 ? 64 * (i >> 1) + 16 * kq + 8 * (i & 1) : 32 * i + 8 * kq;
+      qb[cb][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(q + dim));
+    }
+  }
+  if (steps != 0) {
+    load_scales(0);
+    load(0, false);
+    load(0, true);
+    if (kStages == 2 && steps > 1) {
+      load(1, false);
+      load(1, true);
+    }
+  }
+  // The wave writes columns 4 i + wave: their gates, two at a time.
+  if constexpr (!Split) {
+#pragma unroll
+    for (int i = 0; i < kKCols / kPWaves; i += 2)
+      load_lds_b128(a.gate + row0, 2 * row_at(kPWaves * (i + (lane >> 5)) + wave) + 16 * (lane & 31), lds_address(sh.gate[wave][i]));
+  }
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(qb[cb][i]));
+  asm volatile("" : "+v"(ks_of), "+v"(vs_of));
+
+  // K operands: row 16 rb + col16, chunk 4 i + kq.  V operands by transposed reads, k-slot
+  // (kq, e) of the product <-> key 16 (e / 4) + 4 kq + e % 4, the order of the scores.
+  const unsigned k_lane = kRowBytes * col16 + 16 * (kq ^ keys_at<Fp8>(col16, false));
+  const std::uint32_t v_row = Fp8 ? 16 * (col16 >> 3) + 4 * kq + (col16 >> 1 & 3) : 4 * kq + (col16 >> 2);
+  const unsigned v_lane = kRowBytes * v_row + (16 * ((Fp8 ? 0 : col16 >> 1 & 1) ^ keys_at<Fp8>(v_row, true)) + 8 * (col16 & 1));
+
+  floatx4 acc[2][16]; // [column block][16 dims]: dims 16 db + 4 kq + e of the lane's column
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+    for (int db = 0; db < 16; ++db) acc[cb][db] = floatx4{};
+  float m_run[2] = {-FLT_MAX, -FLT_MAX}, l_run[2] = {0.f, 0.f};
+  std::uint64_t odd = 0; // lanes that took infinite or NaN values out of a masked tile
+
+#pragma unroll 1
+  for (std::uint32_t t = 0; t < steps; ++t) {
+    if (Fp8 && t % 64 == 0 && t != 0) {
+      load_scales(t);
+      asm volatile("" : "+v"(ks_of), "+v"(vs_of)); // (waited for here, not on every step)
+    }
+    const float k_scale = (Fp8 ? lane_value(ks_of, t % 64) : 1.0f) * (kLog2e / 16.0f);
+    const float v_scale = Fp8 ? lane_value(vs_of, t % 64) : 1.0f;
+    const std::uint32_t j0 = tile_of(t) * kCompactBlock;
+    const bool masked = tile_masked(j0, p_lo, p_hi, a.window, a.sinks);
+    // K(t): what may be under way behind it is V(t), K(t + 1), V(t + 1) (and the gates)
+    if (kStages == 2 && t + 1 < steps) wait_vm<3 * kLoads>(); else wait_vm<kLoads>();
+    floatx4 s[2][2]; // [column block][row block]: keys j0 + 16 rb + 4 kq + i
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) s[cb][rb] = floatx4{};
+    const unsigned k_base = plane_at(t, false) + k_lane;
+#pragma unroll
+    for (int i = 0; i < kRowBytes / 64; ++i) {
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const bf16x8 w = lds_operand((k_base ^ (64u * i)) + 16 * kRowBytes * rb);
+        if constexpr (Fp8) {
+          const u32x4 x = __builtin_bit_cast(u32x4, w);
+          const bf16x8 lo = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(x[0], x[1])), hi = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(x[2], x[3]));
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qb[cb][2 * i], s[cb][rb], 0, 0, 0);
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qb[cb][2 * i + 1], s[cb][rb], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, qb[cb][i], s[cb][rb], 0, 0, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    wait_lgkm0(); // the reads are done: their place is free
+    if (t + kStages < steps) load(t + kStages, false);
+    if (masked) {
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[cb][rb][i] = compact_sees(j0 + 16 * rb + 4 * kq + i, pos[cb], a.window, a.sinks) ? s[cb][rb][i] : -INFINITY;
+    }
+    // The accumulators are scaled only where a max grows by more than 2^8, which the
+    // probabilities can exceed 1 by.
+    float mx[2];
+    bool grow = false;
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      float x = fmaxf(s[cb][0][0], s[cb][1][0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) x = fmaxf(fmaxf(x, s[cb][0][i]), s[cb][1][i]);
+      mx[cb] = max_xor32(max_xor16(x)) * k_scale;
+      grow |= mx[cb] > m_run[cb] + kLazyRescale;
+    }
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        const float m_new = fmaxf(m_run[cb], mx[cb]), f = fexp2(m_run[cb] - m_new);
+        l_run[cb] *= f;
+#pragma unroll
+        for (int db = 0; db < 16; ++db) {
+          // (in accumulation registers but for here: moved out and in on every tile otherwise)
+          floatx4 x = acc[cb][db];
+          asm volatile("" : "+v"(x));
+          x *= f;
+          asm volatile("" : "+v"(x));
+          acc[cb][db] = x;
+        }
+        m_run[cb] = m_new;
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+      for (int db = 0; db < 16; ++db) asm volatile("" : "+a"(acc[cb][db]));
+    u32x4 pw[2];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = fexp2(fmaf(s[cb][rb][i], k_scale, -m_run[cb]));
+          l_run[cb] += e[i];
+          e[i] *= v_scale;
+        }
+        pw[cb][2 * rb] = pack_bf16x2(e[0], e[1]);
+        pw[cb][2 * rb + 1] = pack_bf16x2(e[2], e[3]);
+      }
+    // V(t): behind it K(t + 1) and, of two stages, V(t + 1) and K(t + 2)
+    if (kStages == 2 && t + 2 < steps) wait_vm<3 * kLoads>();
+    else if (t + 1 < steps) wait_vm<kStages * kLoads>();
+    else wait_vm<0>();
+    const unsigned v_plane = plane_at(t, true);
+    if (masked) {
+      // A masked key has probability 0, and 0 times an infinite or NaN value is not 0: such
+      // values are taken out here and added behind the loop, to the columns that see them.
+      // (A value is odd if its exponent's, or its code's, bits are all set.)
+      constexpr std::uint32_t kOnes = Fp8 ? 0x7F7F7F7Fu : 0x7F807F80u, kOne = Fp8 ? 0x01010101u : 0x00800080u;
+      std::uint32_t carry = 0;
+#pragma unroll 4
+      for (int i = 0; i < kLoads; ++i) {
+        const u32x4 w = __builtin_bit_cast(u32x4, lds_operand(v_plane + 1024 * i + 16 * lane));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) carry |= (w[e] & kOnes) + kOne;
+      }
+      const std::uint64_t bad = __builtin_amdgcn_ballot_w64((carry & 0x80808080u & ~kOnes) != 0);
+      if (bad != 0) {
+        odd |= bad;
+#pragma unroll 1
+        for (int i = 0; i < kLoads; ++i) {
+          const unsigned at = v_plane + 1024 * i + 16 * lane;
+          u32x4 w = __builtin_bit_cast(u32x4, lds_operand(at));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const std::uint32_t top = ((w[e] & kOnes) + kOne) & 0x80808080u & ~kOnes;
+            // all bits of the values whose top bit is set
+            w[e] &= ~(Fp8 ? (top >> 7) * 0xFFu : (top >> 15) * 0xFFFFu);
+          }
+          *(__attribute__((address_space(3))) u32x4 *)(std::uintptr_t)(at) = w;
+        }
+      }
+      wave_lds_order();
+    }
+    const unsigned v_base = v_plane + v_lane;
+#pragma unroll
+    for (int db = 0; db < 16; ++db) {
+      bf16x8 v;
+      if constexpr (Fp8) {
+        const u32x2 w = lds_tr8_operand(v_base ^ (16u * db));
+        v = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1]));
+      } else {
+        const u32x2 lo = lds_tr_operand(v_base ^ (32u * db)), hi = lds_tr_operand((v_base ^ (32u * db)) + 16 * kRowBytes);
+        v = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+      }
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+        acc[cb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pw[cb]), acc[cb][db], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    wait_lgkm0();
+    if (t + kStages < steps) load(t + kStages, true);
+  }
+  if (odd != 0) {
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb)
+      add_odd_values<Fp8, 16>(c, seen, begin + wave, end, kPWaves, p_lo, p_hi, pos[cb], a, kq,
+                              [&](int i, float x) __attribute__((always_inline)) { acc[cb][i >> 2][i & 3] += x; });
+  }
+
+  // Join the waves: a wave takes every fourth column, a lane four dims.
+  wait_vm<0>();
+  __syncthreads();
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) {
+    const float l = sum_xor32(sum_xor16(l_run[cb]));
+    if (kq == 0) {
+      sh.m[wave][16 * cb + col16] = m_run[cb];
+      sh.l[wave][16 * cb + col16] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < 16; ++db) *reinterpret_cast<floatx4 *>(&sh.acc[wave][16 * cb + col16][16 * db + 4 * kq]) = acc[cb][db];
+  }
+  __syncthreads();
+  // Lane x, and x + 32: the waves' shares of column x.
+  float m = -FLT_MAX, l = 0.f, share[kPWaves];
+#pragma unroll
+  for (int w = 0; w < kPWaves; ++w) m = fmaxf(m, sh.m[w][lane & 31]);
+#pragma unroll
+  for (int w = 0; w < kPWaves; ++w) {
+    share[w] = fexp2(sh.m[w][lane & 31] - m);
+    l = fmaf(sh.l[w][lane & 31], share[w], l);
+  }
+  if constexpr (Split) {
+    const std::size_t at = (static_cast<std::size_t>(blockIdx.z) * a.kv_heads + kvh) * sc.cols + col0;
+    if (threadIdx.x < kKCols) {
+      sc.m[at + lane] = m;
+      sc.l[at + lane] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kKCols / kPWaves; ++i) {
+      const int x = kPWaves * i + wave;
+      floatx4 o{};
+#pragma unroll
+      for (int w = 0; w < kPWaves; ++w) o += *reinterpret_cast<const floatx4 *>(&sh.acc[w][x][4 * lane]) * lane_value(share[w], x);
+      *reinterpret_cast<floatx4 *>(sc.o + (at + x) * kHeadDim + 4 * lane) = o;
+    }
+  } else {
+    const float inv = 1.0f / l;
+    if (a.weights != nullptr && threadIdx.x <= last_x) {
+      const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col0 + lane;
+      sc.final[2 * at] = m;
+      sc.final[2 * at + 1] = inv;
+    }
+    u32x2 out[kKCols / kPWaves];
+#pragma unroll
+    for (int i = 0; i < kKCols / kPWaves; ++i) {
+      const int x = kPWaves * i + wave;
+      floatx4 o{};
+#pragma unroll
+      for (int w = 0; w < kPWaves; ++w) o += *reinterpret_cast<const floatx4 *>(&sh.acc[w][x][4 * lane]) * lane_value(share[w] * inv, x);
+      const u32x2 g = *reinterpret_cast<const u32x2 *>(&sh.gate[wave][i][4 * lane]);
+      out[i] = u32x2{pack_bf16x2(o[0] * sigmoid_gate(bf16_lo(g[0])), o[1] * sigmoid_gate(bf16_hi(g[0]))),
+                     pack_bf16x2(o[2] * sigmoid_gate(bf16_lo(g[1])), o[3] * sigmoid_gate(bf16_hi(g[1])))};
+    }
+#pragma unroll
+    for (int i = 0; i < kKCols / kPWaves; ++i)
+      if (kPWaves * i + wave <= static_cast<int>(last_x))
+        *reinterpret_cast<u32x2 *>(a.output + row0 + row_at(kPWaves * i + wave) + 4 * lane) = out[i];
   }
 }
 
@@ -524,21 +905,45 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
 }
 
 std::uint32_t col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kPCols - 1) / kPCols; }
+std::uint32_t key_col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kKCols - 1) / kKCols; }
 
-// Key splits of a call whose widest column block sees `tiles` tiles: two workgroups per
-// CU where each still has 16 tiles, else one per CU, of at least four tiles.  Two per CU
-// overlap softmax and products but leave twice the partial rows to be joined.  Measured
-// (2 KV heads, 8 query heads each; one against two per CU): 500 tokens behind 2000
-// (10 tiles at two) 58.1 against 61.8 us, behind 4000 (18) 79.1 against 77.5, behind
-// 16000 (64) 208 against 174; 1000 tokens (8) 48.8 against 55.6, 1500 (23) 77.2 against
-// 71.3.  Four tiles against eight: 2 tokens behind 2000 26.5 against 31.5 us, 500 tokens
-// 36.0 against 38.5.  (Grows with `tiles`: the workspace is sized at the largest.)
-std::uint32_t split_count(const CompactArgs &a, std::uint32_t tiles) {
+// How a call is run whose column blocks see `fewest` (the first) to `tiles` (the last) tiles.
+// All figures: 2 KV heads of 8 query heads, 8 bit (bf16), store and merge included.
+//
+// Little work: waves that split the tiles, in splits of at least 16 tiles until every CU has
+// a workgroup.  The measure is (32 columns, tile) per CU, up to 40 of 8 bit or 32 of bf16,
+// with the first block's tiles for three quarters: without splits the shared tiles below wait
+// for their longest block, which a prompt without a past has few like.  Against those: 500
+// tokens 26.9 us for 35.8, 128 tokens 19.0 (20.1) for 26.6 (26.2), 10 behind 100 18.9 (19.7)
+// for 22.0 (21.1), 2 behind 30000 33.5 (44.6) for 48.3 (54.5), 1400 tokens (30 per CU) 67.3
+// (70.1) for 82.6 (73.3), 500 behind 1000 (35) 41.7 (42.8) for 47.1 (45.1), 1000 behind a
+// window of 500 (35) 47.6 (50.3) for 46.0 (44.7); but 300 behind a window of 2048 (41) 52.3
+// for 47.3, 64 behind 30000 (117) 79.9 (90.1) for 77.8 (75.8), 500 behind 16000 (490) 241
+// (253) for 178 (165).  Splits of 8, 16 and 32 tiles: 2 behind 30000 34.1 / 33.5 / 36.5 us,
+// 64 behind 4000 31.2 / 31.5 / 37.1.
+//
+// Else two workgroups of 128 columns per CU where each still has 16 tiles, or one per CU, of
+// at least four tiles.  Two overlap softmax and products but leave twice the partial rows
+// to be joined (one against two: 500 behind 2000, 10 tiles at two, 58.1 against 61.8 us,
+// behind 4000, 18 tiles, 79.1 against 77.5, behind 16000, 64 tiles, 208 against 174).
+//
+// (The splits grow with `tiles` in both, the second has no fewer, and neither fewer tiles
+// nor 8 bit choose it where more or bf16 do not: the workspace is sized for bf16 and the
+// most tiles.)
+struct PrefillSplit {
+  bool by_keys;         // compact_prefill_keys_kernel
+  std::uint32_t splits; // ranges of the tiles
+};
+PrefillSplit split_of(const CompactArgs &a, bool fp8, std::uint32_t fewest, std::uint32_t tiles) {
+  const std::uint64_t small = static_cast<std::uint64_t>(key_col_blocks(a)) * a.kv_heads;
   const std::uint64_t groups = static_cast<std::uint64_t>(col_blocks(a)) * a.kv_heads;
+  const auto at_least = [&](std::uint64_t splits, std::uint32_t each) {
+    const std::uint64_t most = (static_cast<std::uint64_t>(tiles) + each - 1) / each;
+    return static_cast<std::uint32_t>(splits < 1 ? 1 : splits < most ? splits : most);
+  };
+  if (small * (3 * static_cast<std::uint64_t>(fewest) + tiles) <= 4 * kPrefillCus * (fp8 ? 40u : 32u)) return {true, at_least(kPrefillCus / small, 16)};
   const std::uint64_t wanted = groups * tiles >= 2 * kPrefillCus * 16 ? 2 * kPrefillCus : kPrefillCus;
-  const std::uint64_t splits = groups >= wanted ? 1 : wanted / groups;
-  const std::uint64_t most = (static_cast<std::uint64_t>(tiles) + 3) / 4;
-  return static_cast<std::uint32_t>(splits < most ? splits : most);
+  return {false, at_least(wanted / groups, 4)};
 }
 
 PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t splits, void *workspace, std::size_t *bytes) {
@@ -568,11 +973,15 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   // a column block's tiles: at most those of the last block's span ending at the last key
   const std::uint32_t span = (kPCols + a.group - 1) / a.group + 1;
   const std::uint32_t first = a.tokens > span ? last - span + 1 : a.past;
-  const std::uint32_t splits = split_count(a, SeenTiles(first, last, a.window, a.sinks).total);
+  const std::uint32_t tiles = SeenTiles(first, last, a.window, a.sinks).total;
+  const std::uint32_t fewest = SeenTiles(a.past, a.past, a.window, a.sinks).total;
+  const auto [by_keys, splits] = split_of(a, Fp8, fewest < tiles ? fewest : tiles, tiles);
   const PrefillScratch sc = scratch_of(a, splits, workspace, nullptr);
-  const dim3 grid{col_blocks(a) * a.kv_heads, splits};
-  const auto launch = [&](auto split) {
-    if (a.weights != nullptr)
+  const dim3 grid{col_blocks(a) * a.kv_heads, splits}, keys_grid{a.kv_heads, key_col_blocks(a), splits};
+  const auto launch = [&, by_keys = by_keys](auto split) {
+    if (by_keys)
+      compact_prefill_keys_kernel<Fp8, split><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
+    else if (a.weights != nullptr)
       compact_prefill_kernel<Fp8, split, true><<<grid, kPThreads, 0, stream>>>(a, sc);
     else
       compact_prefill_kernel<Fp8, split, false><<<grid, kPThreads, 0, stream>>>(a, sc);
@@ -597,7 +1006,8 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
 
 std::size_t compact_prefill_workspace(const CompactArgs &a) {
   std::size_t bytes = 0;
-  (void)scratch_of(a, split_count(a, (a.max_ctx + kCompactBlock - 1) / kCompactBlock), nullptr, &bytes);
+  const std::uint32_t most = (a.max_ctx + kCompactBlock - 1) / kCompactBlock;
+  (void)scratch_of(a, split_of(a, false, most, most).splits, nullptr, &bytes);
   return bytes;
 }
 

@@ -305,6 +305,81 @@ def test_prefill_many_tokens(gpu):
     near_weights(host(w), 0.0, want, rel.max() + 2.0 ** -20, "weights")
 
 
+def some_tokens(t):
+    return sorted({0, 1, 7, 8, 9, 15, 16, 31, 32, 33, t // 2, t - 3, t - 2, t - 1} & set(range(t)))
+
+
+# Enough columns and keys that workgroups of 128 columns share the tiles: whole, and split over the keys.
+WIDE = [(16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40), (7, 13, 501, 300, 0, 0), (7, 13, 503, 800, 400, 3),
+        (2, 16, 130, 3001, 0, 0), (2, 16, 131, 4000, 3000, 70), (1, 16, 300, 5000, 4999, 1), (1, 3, 900, 4000, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype,layout", [(BF16, 1), (FP8, 1), (BF16, 0), (FP8, 0)])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", WIDE)
+def test_prefill_wide(gpu, dtype, layout, hkv, group, t, past, window, sinks):
+    r = rng(92 + t)
+    heads, n, observed = hkv * group, past + t, 3
+    c = filled(r, dtype, layout, hkv, n + 5, past)
+    k, v, q, g = rows(r, t, hkv), rows(r, t, hkv), bf16(normal(r, t, heads, D)), bf16(normal(r, t, heads, D))
+    shape = c.shape(t, heads, past, window_tokens=window, sink_tokens=sinks, observed_tokens=observed)
+    ws = torch.full((ops.qwen35_compact_prefill_workspace_bytes(shape),), 0xFF, device="cuda", dtype=torch.uint8)
+    w = torch.zeros(hkv, n + 5, device="cuda")
+    out, again = (torch.empty(t, heads, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    args = dev(q), dev(k), dev(v), dev(g)
+    ops.qwen35_compact_attention_prefill(*args, out, c.buf, shape, ops.DTYPE_BF16, dtype, layout, ws, key_weights=w)
+    c.want_store(past, k, v)
+    got = host(out)
+    assert np.isfinite(got).all()
+    for i in some_tokens(t):
+        m = past + i + 1
+        want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], c.held(m), past + i, window, sinks)
+        near(got[i:i + 1], want, bound, f"token {i}")
+    want, rel = np.zeros((hkv, n)), 0.0
+    for i in range(t - observed, t):
+        _, _, ww, e = ref.attention(q[i:i + 1], g[i:i + 1], c.held(past + i + 1), past + i, window, sinks, 1)
+        want[:, :past + i + 1] += ww
+        rel = max(rel, e.max())
+    near_weights(host(w)[:, :n], 0.0, want, rel + 2.0 ** -20, "weights")
+    # without the weights, and over the same rows once more: the same bits
+    plain = c.shape(t, heads, past, window_tokens=window, sink_tokens=sinks)
+    small = torch.full((ops.qwen35_compact_prefill_workspace_bytes(plain),), 0xFF, device="cuda", dtype=torch.uint8)
+    for o in (out, again):
+        ops.qwen35_compact_attention_prefill(*args, o, c.buf, plain, ops.DTYPE_BF16, dtype, layout, small)
+    assert torch.equal(out, again)
+    for i in some_tokens(t):
+        m = past + i + 1
+        want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], c.held(m), past + i, window, sinks)
+        near(host(out)[i:i + 1], want, bound, f"token {i} without weights")
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", [(16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40),
+                                                           (2, 16, 131, 4000, 3000, 70)])
+def test_bad_values_among_wide_columns(gpu, what, hkv, group, t, past, window, sinks):
+    r = rng(93)
+    heads, n = hkv * group, past + t
+    k, v = rows(r, n, hkv), rows(r, n, hkv)
+    q, g = bf16(normal(r, t, heads, D)), bf16(normal(r, t, heads, D))
+    bad = [n - 20, past + t // 2] + ([past - window + 10] if window else [])   # seen by some tokens each
+    v[bad] = what
+    c = Cache(r, BF16, 1, hkv, n)
+    c.store(0, k[:past], v[:past])
+    shape = c.shape(t, heads, past, window_tokens=window, sink_tokens=sinks)
+    out = torch.empty(t, heads, D, device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(ops.qwen35_compact_prefill_workspace_bytes(shape), device="cuda", dtype=torch.uint8)
+    ops.qwen35_compact_attention_prefill(dev(q), dev(k[past:]), dev(v[past:]), dev(g), out, c.buf, shape, ops.DTYPE_BF16,
+                                         BF16, 1, ws)
+    held, got = np.stack([k.transpose(1, 0, 2), v.transpose(1, 0, 2)]).astype(np.float64), host(out)
+    for i in sorted(set(some_tokens(t)) | {t - 21, t - 20, t - 19, t // 2 - 1, t // 2 + 1}):
+        ok = ref.sees(past + i, window, sinks, n)
+        if ok[bad].any():
+            assert not np.isfinite(got[i]).any(), i
+        else:
+            held_i = np.where(ok[None, None, :, None], held, 0)
+            want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], held_i, past + i, window, sinks)
+            near(got[i:i + 1], want, bound, f"token {i}")
+
+
 # ------------------------------------------------------------------ values that reach no one
 
 @pytest.mark.parametrize("t,past,window,sinks", [(40, 100, 0, 0), (40, 100, 30, 0), (40, 100, 30, 40), (1, 100, 30, 40)])
