@@ -3,6 +3,7 @@
 #include "compact_cache.hpp"
 #include "prefill_tile.hpp"
 
+#include <algorithm>
 #include <cfloat>
 
 namespace raftinfer::amd {
@@ -21,7 +22,22 @@ constexpr std::uint32_t kPrefillCus = 256;
 // domain) and 1 / sum of each column for the key weights.
 struct PrefillScratch {
   float *m, *l, *o, *final;
-  std::uint32_t splits, cols; // cols: rounded up to whole workgroups
+  std::uint32_t cols;         // columns of a KV head, rounded up to whole workgroups
+  std::uint32_t block;        // columns of a workgroup
+  std::uint32_t tiles, most;  // of a column block's ranges: tiles of one, ranges
+};
+
+// A column block's ranges: of about equal length, and of `tiles` tiles unless those were
+// more than `most`.
+struct TileRanges {
+  std::uint32_t count, each, more; // the first `more` have a tile above `each`
+  __device__ __forceinline__ TileRanges(const PrefillScratch &sc, std::uint32_t total) {
+    count = (total + sc.tiles - 1) / sc.tiles;
+    count = count < sc.most ? count : sc.most;
+    each = total / count;
+    more = total - each * count;
+  }
+  __device__ __forceinline__ std::uint32_t begin(std::uint32_t i) const { return i * each + (i < more ? i : more); }
 };
 
 // 16-byte chunk c of row r of a bf16 tile lies at c ^ row_key(r): the 16 rows of a
@@ -132,8 +148,15 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   const std::uint32_t p_lo = a.past + col0 / a.group, p_hi = a.past + (col_end - 1) / a.group;
   const std::uint32_t n_keys = p_hi + 1;
   const SeenTiles seen(p_lo, p_hi, a.window, a.sinks);
-  const std::uint32_t begin = Split ? static_cast<std::uint32_t>(static_cast<std::uint64_t>(seen.total) * blockIdx.y / sc.splits) : 0;
-  const std::uint32_t end = Split ? static_cast<std::uint32_t>(static_cast<std::uint64_t>(seen.total) * (blockIdx.y + 1) / sc.splits) : seen.total;
+  std::uint32_t begin = 0, end = seen.total;
+  bool part = false; // of several
+  if constexpr (Split) {
+    const TileRanges ranges(sc, seen.total);
+    if (blockIdx.y >= ranges.count) return; // (uniform)
+    begin = ranges.begin(blockIdx.y);
+    end = ranges.begin(blockIdx.y + 1);
+    part = ranges.count > 1;
+  }
   const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
 
   // This lane's column; those past the last repeat it.  (Formed anew where it is used:
@@ -247,7 +270,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   const auto q_of = [&](int i) -> const bf16x8 & { return q[(i >> 1) + 8 * (i & 1)]; };
 
   floatx16 s = floatx16{}; // scores of tile it: register i has key 8 (i / 4) + 4 kh + i % 4
-  if (begin < end) {
+  {
     load_tile(begin, false);
     load_tile(begin, true);
     const float ks = scale_of(c.ks, begin);
@@ -346,10 +369,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         o[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(v_base, i), pb[i >> 3], o[i & 7], 0, 0, 0);
     }
   };
-  if (begin < end) {
-    for (std::uint32_t it = begin; it + 1 < end; ++it) step.template operator()<true>(it);
-    step.template operator()<false>(end - 1);
-  }
+  for (std::uint32_t it = begin; it + 1 < end; ++it) step.template operator()<true>(it);
+  step.template operator()<false>(end - 1);
   __syncthreads();
 
   const std::uint32_t col = column();
@@ -361,13 +382,12 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     add_odd_values<Fp8, 32>(c, seen, begin, end, 1, p_lo, p_hi, a.past + token_of(col), a, kh,
                             [&](int i, float x) __attribute__((always_inline)) { o[i >> 4][i & 15] += x; });
   const float l = sum_xor32(l_run);
-  if constexpr (Split) {
+  if (Split && part) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + kvh) * sc.cols + col;
     if (kh == 0) {
       sc.m[at] = m_run;
       sc.l[at] = l;
     }
-    if (begin == end) return;
     float *dst = sc.o + at * kHeadDim + 4 * kh;
 #pragma unroll
     for (int nb = 0; nb < 8; ++nb)
@@ -447,18 +467,13 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
   };
   const SeenTiles seen(p_lo, p_hi, a.window, a.sinks);
   std::uint32_t begin = 0, end = seen.total;
+  bool part = false; // of several
   if constexpr (Split) {
-    const std::uint32_t each = seen.total / sc.splits, more = seen.total - each * sc.splits;
-    begin = blockIdx.z * each + (blockIdx.z < more ? blockIdx.z : more);
-    end = begin + each + (blockIdx.z < more);
-    if (begin == end) { // nothing to sum
-      if (threadIdx.x < kKCols) {
-        const std::size_t at = (static_cast<std::size_t>(blockIdx.z) * a.kv_heads + kvh) * sc.cols + col0 + threadIdx.x;
-        sc.m[at] = -FLT_MAX;
-        sc.l[at] = 0.f;
-      }
-      return;
-    }
+    const TileRanges ranges(sc, seen.total);
+    if (blockIdx.z >= ranges.count) return; // (uniform)
+    begin = ranges.begin(blockIdx.z);
+    end = ranges.begin(blockIdx.z + 1);
+    part = ranges.count > 1;
   }
   const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
 
@@ -529,7 +544,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     }
   }
   // The wave writes columns 4 i + wave: their gates, two at a time.
-  if constexpr (!Split) {
+  if (!part) {
 #pragma unroll
     for (int i = 0; i < kKCols / kPWaves; i += 2)
       load_lds_b128(a.gate + row0, 2 * row_at(kPWaves * (i + (lane >> 5)) + wave) + 16 * (lane & 31), lds_address(sh.gate[wave][i]));
@@ -734,7 +749,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     share[w] = fexp2(sh.m[w][lane & 31] - m);
     l = fmaf(sh.l[w][lane & 31], share[w], l);
   }
-  if constexpr (Split) {
+  if (Split && part) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.z) * a.kv_heads + kvh) * sc.cols + col0;
     if (threadIdx.x < kKCols) {
       sc.m[at + lane] = m;
@@ -773,8 +788,8 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
   }
 }
 
-// Joins a split call: W waves per column take its splits in turn, eight loads of a
-// partial row at a time in flight, a lane four dims.
+// Joins the ranges of the columns that have several: W waves per column take them in
+// turn, eight loads of a partial row at a time in flight, a lane four dims.
 template <int W>
 __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(CompactArgs a, PrefillScratch sc) {
   __shared__ float o_of[kPWaves][kHeadDim];
@@ -784,6 +799,10 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
   const std::uint32_t col_of = blockIdx.x * (kPWaves / W) + wave / W;
   const std::uint32_t col = col_of < all_cols ? col_of : all_cols - 1;
   const std::uint32_t kvh = blockIdx.y;
+  const std::uint32_t first = col - col % sc.block, last = first + sc.block < all_cols ? first + sc.block - 1 : all_cols - 1;
+  const std::uint32_t splits =
+      TileRanges(sc, SeenTiles(a.past + first / a.group, a.past + last / a.group, a.window, a.sinks).total).count;
+  if (splits == 1) return; // (for W > 1 the whole workgroup)
   const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * sc.cols; // between splits
   const std::size_t at0 = static_cast<std::size_t>(kvh) * sc.cols + col;
   const std::uint32_t tok = col / a.group;
@@ -795,15 +814,15 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
   const auto load = [&](std::uint32_t s0) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const std::uint32_t s = s0 + W * b < sc.splits ? s0 + W * b : sc.splits - 1;
+      const std::uint32_t s = s0 + W * b < splits ? s0 + W * b : splits - 1;
       x[b] = *reinterpret_cast<const floatx4 *>(sc.o + (at0 + s * stride) * kHeadDim + 4 * lane);
     }
   };
-  const std::uint32_t first = W == 1 ? 0 : wave % W;
-  load(first);
+  const std::uint32_t s_first = W == 1 ? 0 : wave % W;
+  load(s_first);
   // max and sum over the splits; those without a key that the column sees have l = 0
   float m = -FLT_MAX, l = 0.f;
-  for (std::uint32_t s = lane; s < sc.splits; s += 64) {
+  for (std::uint32_t s = lane; s < splits; s += 64) {
     const float ms = sc.m[at0 + s * stride], ls = sc.l[at0 + s * stride];
     const float m_new = fmaxf(m, ms);
     l = l * fexp2(m - m_new) + ls * fexp2(ms - m_new);
@@ -812,12 +831,12 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
   const float m_all = wave_max(m);
   const float inv = 1.0f / wave_sum(l * fexp2(m - m_all));
   floatx4 o{};
-  for (std::uint32_t s0 = first; s0 < sc.splits; s0 += W * kBatch) {
-    if (s0 != first) load(s0);
+  for (std::uint32_t s0 = s_first; s0 < splits; s0 += W * kBatch) {
+    if (s0 != s_first) load(s0);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const std::uint32_t s = s0 + W * b;
-      if (s >= sc.splits) break;
+      if (s >= splits) break;
       const float ms = sc.m[at0 + s * stride];
       if (ms == -FLT_MAX && sc.l[at0 + s * stride] == 0.f) continue; // nothing was summed
       o += x[b] * fexp2(ms - m_all);
@@ -931,24 +950,42 @@ std::uint32_t key_col_blocks(const CompactArgs &a) { return (a.tokens * a.group 
 // nor 8 bit choose it where more or bf16 do not: the workspace is sized for bf16 and the
 // most tiles.)
 struct PrefillSplit {
-  bool by_keys;         // compact_prefill_keys_kernel
-  std::uint32_t splits; // ranges of the tiles
+  bool by_keys;        // compact_prefill_keys_kernel
+  std::uint32_t count; // ranges of the longest column block
+  std::uint32_t tiles; // of a range
 };
-PrefillSplit split_of(const CompactArgs &a, bool fp8, std::uint32_t fewest, std::uint32_t tiles) {
-  const std::uint64_t small = static_cast<std::uint64_t>(key_col_blocks(a)) * a.kv_heads;
-  const std::uint64_t groups = static_cast<std::uint64_t>(col_blocks(a)) * a.kv_heads;
-  const auto at_least = [&](std::uint64_t splits, std::uint32_t each) {
-    const std::uint64_t most = (static_cast<std::uint64_t>(tiles) + each - 1) / each;
-    return static_cast<std::uint32_t>(splits < 1 ? 1 : splits < most ? splits : most);
+PrefillSplit split_of(const CompactArgs &a, bool fp8, std::uint32_t past) {
+  const std::uint32_t last = past + a.tokens - 1;
+  // about the tiles of the last block, which has the most
+  const std::uint32_t span = (kPCols + a.group - 1) / a.group + 1;
+  const std::uint32_t tiles = SeenTiles(a.tokens > span ? last - span + 1 : past, last, a.window, a.sinks).total;
+  const std::uint32_t fewest = std::min(SeenTiles(past, past, a.window, a.sinks).total, tiles);
+  // in the mean: they grow over the tokens that see the first key
+  const std::uint64_t reach = static_cast<std::uint64_t>(a.window) + a.sinks;
+  const std::uint64_t growing = a.window == 0 ? a.tokens : std::min<std::uint64_t>(reach > past ? reach - past : 0, a.tokens);
+  const double mean = tiles - 0.5 * (tiles - fewest) * static_cast<double>(growing) / a.tokens;
+  const double small = static_cast<double>(key_col_blocks(a)) * a.kv_heads * mean; // (32 columns, tile)
+  const double wide = static_cast<double>(col_blocks(a)) * a.kv_heads * mean;
+  const auto ranges = [&](bool by_keys, double work, double workgroups, std::uint32_t least) {
+    const double wanted = std::max(1.0, workgroups * tiles / work); // of the longest block
+    const std::uint32_t most = (tiles + least - 1) / least;
+    const auto n = wanted < most ? static_cast<std::uint32_t>(wanted) : most;
+    return PrefillSplit{by_keys, n, (tiles + n - 1) / n};
   };
-  if (small * (3 * static_cast<std::uint64_t>(fewest) + tiles) <= 4 * kPrefillCus * (fp8 ? 40u : 32u)) return {true, at_least(kPrefillCus / small, 16)};
-  const std::uint64_t wanted = groups * tiles >= 2 * kPrefillCus * 16 ? 2 * kPrefillCus : kPrefillCus;
-  return {false, at_least(wanted / groups, 4)};
+  if (small <= kPrefillCus * (fp8 ? 40.0 : 32.0)) return ranges(true, small, kPrefillCus, 16);
+  return ranges(false, wide, wide >= 2 * kPrefillCus * 16.0 ? 2 * kPrefillCus : kPrefillCus, 4);
+}
+// The ranges that the workspace holds: what a prompt's start or its end in a full cache
+// takes, whichever type it has.  (A call between them that would take more takes these.)
+std::uint32_t most_ranges(const CompactArgs &a) {
+  std::uint32_t most = 1;
+  for (const std::uint32_t past : {0u, a.max_ctx - a.tokens})
+    for (const bool fp8 : {false, true}) most = std::max(most, split_of(a, fp8, past).count);
+  return most;
 }
 
-PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t splits, void *workspace, std::size_t *bytes) {
+PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t ranges, void *workspace, std::size_t *bytes) {
   PrefillScratch sc{};
-  sc.splits = splits;
   sc.cols = col_blocks(a) * kPCols;
   auto *p = static_cast<unsigned char *>(workspace);
   std::size_t at = 0;
@@ -959,43 +996,42 @@ PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t splits, void *work
   };
   const std::size_t cols = static_cast<std::size_t>(sc.cols) * a.kv_heads;
   if (a.observed != 0) sc.final = take(2 * cols);
-  if (splits > 1) {
-    sc.m = take(splits * cols);
-    sc.l = take(splits * cols);
-    sc.o = take(splits * cols * kHeadDim);
+  if (ranges > 1) {
+    sc.m = take(ranges * cols);
+    sc.l = take(ranges * cols);
+    sc.o = take(ranges * cols * kHeadDim);
   }
   if (bytes != nullptr) *bytes = at;
   return sc;
 }
 
 template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, hipStream_t stream) {
-  const std::uint32_t last = a.past + a.tokens - 1;
-  // a column block's tiles: at most those of the last block's span ending at the last key
-  const std::uint32_t span = (kPCols + a.group - 1) / a.group + 1;
-  const std::uint32_t first = a.tokens > span ? last - span + 1 : a.past;
-  const std::uint32_t tiles = SeenTiles(first, last, a.window, a.sinks).total;
-  const std::uint32_t fewest = SeenTiles(a.past, a.past, a.window, a.sinks).total;
-  const auto [by_keys, splits] = split_of(a, Fp8, fewest < tiles ? fewest : tiles, tiles);
-  const PrefillScratch sc = scratch_of(a, splits, workspace, nullptr);
-  const dim3 grid{col_blocks(a) * a.kv_heads, splits}, keys_grid{a.kv_heads, key_col_blocks(a), splits};
-  const auto launch = [&, by_keys = by_keys](auto split) {
-    if (by_keys)
-      compact_prefill_keys_kernel<Fp8, split><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
+  PrefillSplit split = split_of(a, Fp8, a.past);
+  split.count = std::min(split.count, most_ranges(a));
+  PrefillScratch sc = scratch_of(a, split.count, workspace, nullptr);
+  sc.block = split.by_keys ? kKCols : kPCols;
+  sc.tiles = split.tiles;
+  sc.most = split.count;
+  const dim3 grid{col_blocks(a) * a.kv_heads, split.count}, keys_grid{a.kv_heads, key_col_blocks(a), split.count};
+  const auto launch = [&](auto several) {
+    if (split.by_keys)
+      compact_prefill_keys_kernel<Fp8, several><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
     else if (a.weights != nullptr)
-      compact_prefill_kernel<Fp8, split, true><<<grid, kPThreads, 0, stream>>>(a, sc);
+      compact_prefill_kernel<Fp8, several, true><<<grid, kPThreads, 0, stream>>>(a, sc);
     else
-      compact_prefill_kernel<Fp8, split, false><<<grid, kPThreads, 0, stream>>>(a, sc);
+      compact_prefill_kernel<Fp8, several, false><<<grid, kPThreads, 0, stream>>>(a, sc);
   };
-  if (splits > 1) {
+  if (split.count > 1) {
     launch(std::true_type{});
     const std::uint32_t cols = a.tokens * a.group;
-    if (splits > 8)
+    if (split.count > 8)
       compact_prefill_merge_kernel<kPWaves><<<dim3{cols, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
     else
       compact_prefill_merge_kernel<1><<<dim3{(cols + kPWaves - 1) / kPWaves, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
   } else {
     launch(std::false_type{});
   }
+  const std::uint32_t last = a.past + a.tokens - 1;
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
     compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
@@ -1006,8 +1042,7 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
 
 std::size_t compact_prefill_workspace(const CompactArgs &a) {
   std::size_t bytes = 0;
-  const std::uint32_t most = (a.max_ctx + kCompactBlock - 1) / kCompactBlock;
-  (void)scratch_of(a, split_of(a, false, most, most).splits, nullptr, &bytes);
+  (void)scratch_of(a, most_ranges(a), nullptr, &bytes);
   return bytes;
 }
 
