@@ -926,29 +926,25 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
 std::uint32_t col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kPCols - 1) / kPCols; }
 std::uint32_t key_col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kKCols - 1) / kKCols; }
 
-// How a call is run whose column blocks see `fewest` (the first) to `tiles` (the last) tiles.
-// All figures: 2 KV heads of 8 query heads, 8 bit (bf16), store and merge included.
+// How a call is run.  All figures: 4 KV heads of 4 query heads, 8 bit (bf16), store and
+// merge included.
 //
-// Little work: waves that split the tiles, in splits of at least 16 tiles until every CU has
-// a workgroup.  The measure is (32 columns, tile) per CU, up to 40 of 8 bit or 32 of bf16,
-// with the first block's tiles for three quarters: without splits the shared tiles below wait
-// for their longest block, which a prompt without a past has few like.  Against those: 500
-// tokens 26.9 us for 35.8, 128 tokens 19.0 (20.1) for 26.6 (26.2), 10 behind 100 18.9 (19.7)
-// for 22.0 (21.1), 2 behind 30000 33.5 (44.6) for 48.3 (54.5), 1400 tokens (30 per CU) 67.3
-// (70.1) for 82.6 (73.3), 500 behind 1000 (35) 41.7 (42.8) for 47.1 (45.1), 1000 behind a
-// window of 500 (35) 47.6 (50.3) for 46.0 (44.7); but 300 behind a window of 2048 (41) 52.3
-// for 47.3, 64 behind 30000 (117) 79.9 (90.1) for 77.8 (75.8), 500 behind 16000 (490) 241
-// (253) for 178 (165).  Splits of 8, 16 and 32 tiles: 2 behind 30000 34.1 / 33.5 / 36.5 us,
-// 64 behind 4000 31.2 / 31.5 / 37.1.
+// Little work: waves that split the tiles, in ranges of at least 16 tiles until every CU has
+// a workgroup.  The measure is (32 columns, tile) per CU, up to 40 of 8 bit or 32 of bf16.
+// Against tiles shared by 128 columns: 500 tokens 26.9 us (27.8) for 36.9 (36.1), 128 tokens
+// 19.0 (20.1) for 26.6 (26.2), 10 behind 100 18.9 (19.7) for 22.0 (21.1), 2 behind 30000 33.5
+// (44.6) for 48.3 (54.5), 1000 tokens (32 per CU) 43.4 (45.6) for 54.2 (52.0), 500 behind
+// 1000 (40) 41.1 (42.4) for 47.7 (45.0); 1000 behind a window of 500 (35) 47.3 (49.7) for
+// 47.3 (46.3), 300 behind a window of 2048 (41) 51.8 for 48.3, 1200 tokens (45) 57.8 (60.6)
+// for 59.6 (56.6), 500 behind 4000 (130) 82.1 (85.5) for 77.3 (75.2).  Ranges of 8, 16 and 32
+// tiles: 2 behind 30000 34.1 / 33.5 / 36.5 us, 64 behind 4000 31.2 / 31.5 / 37.1.
 //
-// Else two workgroups of 128 columns per CU where each still has 16 tiles, or one per CU, of
-// at least four tiles.  Two overlap softmax and products but leave twice the partial rows
+// Else two workgroups of 128 columns per CU where each has 16 tiles in the mean, or one per
+// CU, of at least four tiles.  Two overlap softmax and products but leave more partial rows
 // to be joined (one against two: 500 behind 2000, 10 tiles at two, 58.1 against 61.8 us,
-// behind 4000, 18 tiles, 79.1 against 77.5, behind 16000, 64 tiles, 208 against 174).
-//
-// (The splits grow with `tiles` in both, the second has no fewer, and neither fewer tiles
-// nor 8 bit choose it where more or bf16 do not: the workspace is sized for bf16 and the
-// most tiles.)
+// behind 4000, 18 tiles, 79.1 against 77.5, 3000 tokens 164 (145) against 137 (131)).  A
+// column block is cut into as many ranges as its own tiles need: a prompt's first ones into
+// one, which is not joined (1400 tokens 67.3 us, all blocks cut alike 82.6).
 struct PrefillSplit {
   bool by_keys;        // compact_prefill_keys_kernel
   std::uint32_t count; // ranges of the longest column block

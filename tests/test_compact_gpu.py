@@ -309,9 +309,11 @@ def some_tokens(t):
     return sorted({0, 1, 7, 8, 9, 15, 16, 31, 32, 33, t // 2, t - 3, t - 2, t - 1} & set(range(t)))
 
 
-# Enough columns and keys that workgroups of 128 columns share the tiles: whole, and split over the keys.
+# Enough columns and keys that workgroups of 128 columns share the tiles, whole and split over the keys; the last
+# three, of 128 and of 32 columns, split the later tokens' keys only.
 WIDE = [(16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40), (7, 13, 501, 300, 0, 0), (7, 13, 503, 800, 400, 3),
-        (2, 16, 130, 3001, 0, 0), (2, 16, 131, 4000, 3000, 70), (1, 16, 300, 5000, 4999, 1), (1, 3, 900, 4000, 0, 0)]
+        (2, 16, 130, 3001, 0, 0), (2, 16, 131, 4000, 3000, 70), (1, 16, 300, 5000, 4999, 1), (1, 3, 900, 4000, 0, 0),
+        (4, 4, 1400, 0, 0, 0), (1, 1, 1200, 0, 0, 0), (1, 2, 700, 5, 600, 3)]
 
 
 @pytest.mark.parametrize("dtype,layout", [(BF16, 1), (FP8, 1), (BF16, 0), (FP8, 0)])
