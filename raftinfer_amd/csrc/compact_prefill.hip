@@ -587,21 +587,44 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb) s[cb][rb] = floatx4{};
     const unsigned k_base = plane_at(t, false) + k_lane;
+    const auto read_k = [&](int i) { return lds_operand((k_base ^ (64u * (i >> 1))) + 16 * kRowBytes * (i & 1)); };
+    // (operands are read kRing products ahead: left to the compiler, one, and each waits)
+    constexpr int kRing = 8;
+    // 8-bit operands are converted between the products of the one before.
+    const auto pair_of = [](std::uint32_t w, bool hi) {
+      typedef __bf16 pair __attribute__((ext_vector_type(2)));
+      const pair x = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+      return __builtin_bit_cast(std::uint32_t, x);
+    };
+    {
+      bf16x8 op[kRing];
 #pragma unroll
-    for (int i = 0; i < kRowBytes / 64; ++i) {
+      for (int i = 0; i < kRing; ++i) op[i] = read_k(i);
+      if constexpr (Fp8) {
+        // operand n: half n & 1 of read n / 2
+        const auto code = [&](int n, int w) { return __builtin_bit_cast(u32x4, op[n >> 1])[2 * (n & 1) + w]; };
+        u32x4 now{pair_of(code(0, 0), false), pair_of(code(0, 0), true), pair_of(code(0, 1), false), pair_of(code(0, 1), true)}, next = now;
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        const bf16x8 w = lds_operand((k_base ^ (64u * i)) + 16 * kRowBytes * rb);
-        if constexpr (Fp8) {
-          const u32x4 x = __builtin_bit_cast(u32x4, w);
-          const bf16x8 lo = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(x[0], x[1])), hi = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(x[2], x[3]));
+        for (int n = 0; n < kRowBytes / 16; ++n) {
+          const int rb = n >> 1 & 1, qi = 2 * (n >> 2) + (n & 1);
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qb[cb][2 * i], s[cb][rb], 0, 0, 0);
+          for (int cb = 0; cb < 2; ++cb) {
+            s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now), qb[cb][qi], s[cb][rb], 0, 0, 0);
+            if (n + 1 < kRowBytes / 16) {
+              next[2 * cb] = pair_of(code(n + 1, cb), false);
+              next[2 * cb + 1] = pair_of(code(n + 1, cb), true);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          now = next;
+        }
+      } else {
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qb[cb][2 * i + 1], s[cb][rb], 0, 0, 0);
-        } else {
+        for (int i = 0; i < kRowBytes / 32; ++i) {
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb) s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, qb[cb][i], s[cb][rb], 0, 0, 0);
+          for (int cb = 0; cb < 2; ++cb) s[cb][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op[i % kRing], qb[cb][i >> 1], s[cb][i & 1], 0, 0, 0);
+          if (i + kRing < kRowBytes / 32) op[i % kRing] = read_k(i + kRing);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -701,19 +724,35 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
       wave_lds_order();
     }
     const unsigned v_base = v_plane + v_lane;
-#pragma unroll
-    for (int db = 0; db < 16; ++db) {
-      bf16x8 v;
+    const auto read_v = [&](int db) {
       if constexpr (Fp8) {
-        const u32x2 w = lds_tr8_operand(v_base ^ (16u * db));
-        v = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1]));
+        return lds_tr8_operand(v_base ^ (16u * db));
       } else {
         const u32x2 lo = lds_tr_operand(v_base ^ (32u * db)), hi = lds_tr_operand((v_base ^ (32u * db)) + 16 * kRowBytes);
-        v = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
+    };
+    std::conditional_t<Fp8, u32x2, u32x4> op[kRing];
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb)
-        acc[cb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pw[cb]), acc[cb][db], 0, 0, 0);
+    for (int db = 0; db < kRing; ++db) op[db] = read_v(db);
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 now;
+    if constexpr (Fp8) now = u32x4{pair_of(op[0][0], false), pair_of(op[0][0], true), pair_of(op[0][1], false), pair_of(op[0][1], true)};
+#pragma unroll
+    for (int db = 0; db < 16; ++db) {
+      if constexpr (!Fp8) now = op[db % kRing];
+      u32x4 next = now;
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        acc[cb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now), __builtin_bit_cast(bf16x8, pw[cb]), acc[cb][db], 0, 0, 0);
+        if (Fp8 && db + 1 < 16) {
+          next[2 * cb] = pair_of(op[(db + 1) % kRing][cb], false);
+          next[2 * cb + 1] = pair_of(op[(db + 1) % kRing][cb], true);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (db + kRing < 16) op[db % kRing] = read_v(db + kRing);
+      now = next;
     }
     __builtin_amdgcn_sched_barrier(0);
     wait_lgkm0();
