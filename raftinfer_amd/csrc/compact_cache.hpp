@@ -106,6 +106,21 @@ __device__ __forceinline__ bool is_finite_f32(float x) {
   return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
 }
 
+// ------------------------------------------------- operands out of LDS
+__device__ __forceinline__ bf16x8 lds_operand(unsigned addr) {
+  return __builtin_bit_cast(bf16x8, *(const __attribute__((address_space(3))) u32x4 *)(std::uintptr_t)(addr));
+}
+// Transposed: of 16 lanes, lane r supplies 8 bytes of row r / 4 (bf16) and receives its
+// element of 4 rows, or of row r / 2 (codes) and receives its code of 8 rows.
+__device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
+  typedef short quad __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) quad *)(std::uintptr_t)(addr)));
+}
+__device__ __forceinline__ u32x2 lds_tr8_operand(unsigned addr) {
+  typedef int pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) pair *)(std::uintptr_t)(addr)));
+}
+
 // ---------------------------------------------------------- launches
 void compact_append(const CompactArgs &a, bool fp8, hipStream_t stream);
 

@@ -8,7 +8,6 @@ namespace raftinfer::amd {
 namespace {
 
 using prefill::fexp2;
-using prefill::lds_tr16;
 
 constexpr int kMergeThreads = 512;
 constexpr int kMergeWaves = kMergeThreads / kWave;
@@ -28,7 +27,9 @@ __device__ __forceinline__ std::uint32_t context_of(const CompactArgs &a, std::u
 
 template <int WAVES> struct DecodeShared {
   union {
-    bf16_bits v[WAVES][kCompactBlock * kHeadDim]; // 16-byte chunk c of row r at c ^ 2 (r & 7)
+    // V rows as cached (a step of 8-bit or bf16 rows takes 8 KiB), 16-byte chunk c of row r at
+    // c ^ v_key(r)
+    alignas(1024) unsigned char v[WAVES][8192];
     // (the pad puts the 16 heads of a store on banks of their own)
     float acc[WAVES][kCompactMaxGroup][kHeadDim + 4];
   };
@@ -37,7 +38,11 @@ template <int WAVES> struct DecodeShared {
   alignas(16) unsigned char fresh[2][2 * kHeadDim]; // the new token's K and V rows, as stored
 };
 
-__device__ __forceinline__ int v_chunk(int r, int c) { return (c ^ (2 * (r & 7))) << 3; } // in elements
+// (a pass of the transposed reads takes 16 bytes of the 16 rows 4 k + 0 .. 3, 16 + 4 k + 0 .. 3
+// of two k, or of bf16 32 bytes of 8 rows: no two on one bank)
+template <bool Fp8> __device__ __forceinline__ std::uint32_t v_key(std::uint32_t r) {
+  return Fp8 ? (r & 3) | (r >> 4 & 1) << 2 | (r >> 2 & 1) << 3 : 2 * (r & 7);
+}
 __device__ __forceinline__ float max_finite_bf16x8(u32x4 w, float m) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -77,7 +82,7 @@ __device__ __forceinline__ u32x4 rescale_fp8x16(u32x4 w, float ratio) {
 // sequence; wave w takes its steps w, w + WAVES, ..  Both products run on
 // v_mfma_f32_16x16x32_bf16 with the query heads of the group as the 16 columns
 // (those past the group repeat the last): S = K q^T with K rows as loaded, O^T = V^T P^T
-// with V transposed by the LDS read.  Codes become bf16 without loss; the block's
+// with V transposed by the LDS read.  Codes become bf16 behind the reads, without loss; the block's
 // K scale multiplies the scores, its V scale the probabilities.
 //
 // The kernel is bound by its cache reads, so a wave (32 8-bit or 16 bf16 rows a
@@ -223,15 +228,14 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
     wave_lds_order();
   }
 
-  // Transposed V reads: lane r of a 16-lane group supplies 4 dims of key row r / 4
-  // and receives its dim of 4 keys.
-  const bf16_bits *vt[8];
-  {
-    const int row = 4 * kq + (col >> 2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      vt[j] = &sh.v[wave][row * kHeadDim + v_chunk(row, 2 * j + ((col >> 1) & 1)) + 4 * (col & 1)];
-  }
+  // Transposed V reads: of 16 lanes, lane r supplies 8 bytes (8 or 4 dims) of key row r / 2 or
+  // r / 4 of the group's and receives its dim of all of them.
+  constexpr int kVBytes = Fp8 ? 256 : 512;
+  const std::uint32_t v_row = Fp8 ? 16 * (col >> 3) + 4 * kq + (col >> 1 & 3) : 4 * kq + (col >> 2);
+  const unsigned v_read = lds_address(sh.v[wave]) + kVBytes * v_row +
+                          (16 * ((Fp8 ? 0 : col >> 1 & 1) ^ v_key<Fp8>(v_row)) + 8 * (col & 1));
+  const std::uint32_t v_put_row = lane / kRowLanes; // of the first load: row kVRows i + v_put_row for load i
+  const unsigned v_put = kVBytes * v_put_row + 16 * ((lane % kRowLanes) ^ v_key<Fp8>(v_put_row));
 
   floatx4 acc[16];
 #pragma unroll
@@ -364,39 +368,33 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
     }
     wave_lds_order();
 #pragma unroll
-    for (int i = 0; i < kVLoads; ++i) {
-      const int r = kVRows * i + lane / kRowLanes;
-      const int piece = lane % kRowLanes;
-      const u32x4 w = vr[i];
-      bf16_bits *row = sh.v[wave] + r * kHeadDim;
-      if constexpr (Fp8) {
-        // the upper 8 lanes of a row store their second chunk first: 16 banks, not 8 twice
-        const u32x4 x = fp8x8_to_bf16(w[0], w[1]), y = fp8x8_to_bf16(w[2], w[3]);
-        const bool up = piece >= 8;
-        *reinterpret_cast<u32x4 *>(row + v_chunk(r, 2 * piece + up)) = up ? y : x;
-        *reinterpret_cast<u32x4 *>(row + v_chunk(r, 2 * piece + !up)) = up ? x : y;
-      } else {
-        *reinterpret_cast<u32x4 *>(row + v_chunk(r, piece)) = w;
-      }
-    }
+    for (int i = 0; i < kVLoads; ++i) // (v_key is linear in the bits of the row)
+      *reinterpret_cast<u32x4 *>(&sh.v[wave][(v_put ^ (16 * v_key<Fp8>(kVRows * i))) + kVBytes * kVRows * i]) = vr[i];
     if constexpr (kMore) load_v(first_key(it + WAVES));
     __builtin_amdgcn_sched_barrier(0);
     wave_lds_order();
     // k-slot (kq, e) of the product <-> key 16 (e / 4) + 4 kq + e % 4, the order
-    // in which the scores lie.
+    // in which the scores lie.  Operands are read kRing products ahead.
+    constexpr int kRing = 8;
+    const auto read_v = [&](int db) {
+      if constexpr (Fp8) return lds_tr8_operand(v_read ^ (16u * db));
+      else return lds_tr_operand(v_read ^ (32u * db));
+    };
+    u32x2 op[kRing];
+#pragma unroll
+    for (int db = 0; db < kRing; ++db) op[db] = read_v(db);
 #pragma unroll
     for (int db = 0; db < 16; ++db) {
-      const bf16_bits *v0 = vt[db & 7] + 128 * (db >> 3);
-      const u32x2 lo = lds_tr16(v0);
-      if constexpr (kRB == 2) {
-        const u32x2 hi = lds_tr16(v0 + 16 * kHeadDim);
-        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
-            __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
+      const u32x2 w = op[db % kRing];
+      if constexpr (Fp8) {
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1])),
+                                                          __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
       } else {
         acc[db] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
-            __builtin_bit_cast(prefill::short4v, lo), __builtin_bit_cast(prefill::short4v, u32x2{pw[0], pw[1]}), acc[db], 0, 0, 0);
+            __builtin_bit_cast(prefill::short4v, w), __builtin_bit_cast(prefill::short4v, u32x2{pw[0], pw[1]}), acc[db], 0, 0, 0);
       }
+      if (db + kRing < 16) op[db % kRing] = read_v(db + kRing);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   for (; it + WAVES < it_end; it += WAVES) step.template operator()<true>();

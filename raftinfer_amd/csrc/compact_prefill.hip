@@ -112,17 +112,6 @@ __device__ __forceinline__ u32x4 fp8x8_to_bf16_scaled(std::uint32_t lo, std::uin
   return u32x4{__builtin_bit_cast(std::uint32_t, a), __builtin_bit_cast(std::uint32_t, b),
                __builtin_bit_cast(std::uint32_t, c), __builtin_bit_cast(std::uint32_t, d)};
 }
-__device__ __forceinline__ bf16x8 lds_operand(unsigned addr) {
-  return __builtin_bit_cast(bf16x8, *(const __attribute__((address_space(3))) u32x4 *)(std::uintptr_t)(addr));
-}
-// Of 16 lanes, lane r supplies 8 bytes of row r / 2 and receives its byte of 8 rows.
-__device__ __forceinline__ u32x2 lds_tr8_operand(unsigned addr) {
-  typedef int pair __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) pair *)(std::uintptr_t)(addr)));
-}
-__device__ __forceinline__ u32x2 lds_tr_operand(unsigned addr) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((prefill::lds_short4v *)(std::uintptr_t)(addr)));
-}
 
 // A workgroup takes 128 columns (column = token * group + head) of one KV head and a
 // contiguous range of the 32-key tiles that they see; a wave takes 32 columns.  The
