@@ -148,9 +148,11 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
       std::uint32_t j = j0 + 16 * rb + col;
       j = j < n ? j : n - 1;
       const auto *row = reinterpret_cast<const unsigned char *>(c.k + static_cast<std::size_t>(j) * c.row) + 16 * kq;
+      // (Not non-temporal, as V: a load takes half of each line, and the other half came from
+      // memory again.  Batch of 32 218 -> 203 us, 60001 tokens 33.4 -> 30.2 in a graph; V so
+      // too 216 and 34.4.)
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        kr[rb][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + 64 * i));
+      for (int i = 0; i < kPieces; ++i) kr[rb][i] = *reinterpret_cast<const u32x4 *>(row + 64 * i);
     }
     if constexpr (Fp8) ks = c.ks[j0 / kCompactBlock + lane0];
   };
@@ -557,14 +559,14 @@ std::uint32_t most_tiles(const CompactArgs &a, std::uint32_t n) {
 }
 
 // How a call is split whose contexts have up to `total` tiles.  Short contexts: one
-// workgroup of 8 waves per unit and no merge (201 tokens: 9.4 us; cut in two with a
+// workgroup of 8 waves per unit and no merge (201 tokens: 8.9 us; cut in two with a
 // merge 14.5 against 14.4 in a graph, and a launch more).  Else partitions of 4 to 32
-// tiles such that about 512 workgroups of 4 waves run at once, two per CU: 16 sequences
-// behind a window of 4096, partitions of 4 / 8 / 16 / 32 tiles 62 / 59 / 55 / 63 us;
-// finer than 32 tiles where there are more (32 ragged sequences, 32 / 64: 214 / 218 us),
-// and at most 64 partitions, which the merge takes in one batch (16000 tokens, 125 / 63
-// partitions: 20.0 / 18.0 us).  Where that leaves at most one workgroup per CU, it gets
-// 8 waves (60001 tokens: 33.5 against 35.0 us).
+// tiles such that about 256 workgroups of 4 waves run, one or two per CU (in a graph: 16
+// sequences behind a window of 4096 in 32 / 24 / 16 tiles 52.2 / 57.2 / 53.9 us, 4 of 8192
+// with key weights 27.7 / 32.7 / 28.4); no longer where there are more (32 ragged sequences,
+// 32 / 64 tiles: 203 / 210 us), and at most 64 partitions, which the merge takes in one
+// batch (60001 tokens, 64 / 128: 30.3 / 31.0 us, 16000 tokens 17.1 / 18.8).  Where that leaves
+// at most one workgroup per CU, it gets 8 waves (60001 tokens: 33.5 against 35.0 us).
 constexpr std::uint32_t kAlone = 16;
 constexpr std::uint32_t kMostParts = 64;
 struct DecodeSplit {
@@ -574,7 +576,7 @@ struct DecodeSplit {
 DecodeSplit split_of(const CompactArgs &a, std::uint32_t total) {
   if (total <= kAlone) return {8, kAlone, 1};
   const std::uint64_t units = static_cast<std::uint64_t>(a.sequences) * a.kv_heads;
-  const std::uint64_t even = (total * units / 512 + 2) / 4 * 4;
+  const std::uint64_t even = (total * units / 256 + 2) / 4 * 4;
   std::uint32_t tiles = even < 4 ? 4 : even > 32 ? 32 : static_cast<std::uint32_t>(even);
   const std::uint32_t least = ((total + kMostParts - 1) / kMostParts + 3) / 4 * 4;
   if (tiles < least) tiles = least;
