@@ -888,12 +888,13 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
 }
 
 // Key weights of the last `observed` tokens: a workgroup owns a 32-key tile of one KV
-// head, its waves take every fourth block of 32 observed columns and form the
+// head, its 8 waves take every eighth block of 32 observed columns and form the
 // probabilities again from the columns' final max and sum.  The owner sums them, so
 // nothing is added twice or in a changing order.
+constexpr int kWeighWaves = 8;
 template <bool Fp8>
-__global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
-  __shared__ float sum[kPWaves][kCompactBlock];
+__global__ __launch_bounds__(kWeighWaves *kWave, 1) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
+  __shared__ float sum[kWeighWaves][kCompactBlock];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, kh = lane >> 5;
@@ -904,7 +905,23 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
   const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
   float k_scale = kLog2e / 16.0f;
   if constexpr (Fp8) k_scale *= c.ks[tile];
-  bf16x8 k[16];
+  const std::uint32_t all_cols = a.tokens * a.group;
+  std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave;
+  bf16x8 k[16], q[16];
+  float m = 0.f, inv = 0.f;
+  std::uint32_t pos = 0;
+  const auto load = [&] { // a block's columns: those past the last repeat it
+    const std::uint32_t col = c0 + n32 < all_cols ? c0 + n32 : all_cols - 1, tok = col / a.group;
+    pos = a.past + tok;
+    const bf16_bits *src =
+        a.query + ((static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col - tok * a.group)) * kHeadDim + 8 * kh;
+#pragma unroll
+    for (int b = 0; b < 16; ++b) q[b] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(src + 16 * b));
+    const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col;
+    m = sc.final[2 * at];
+    inv = sc.final[2 * at + 1];
+  };
+  if (c0 < all_cols) load();
   {
     const std::uint32_t j = j0 + n32 <= last ? j0 + n32 : last;
     const auto *row = c.k + static_cast<std::size_t>(j) * c.row + 8 * kh;
@@ -921,24 +938,22 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
   float w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = 0.f;
-  const std::uint32_t all_cols = a.tokens * a.group;
-  for (std::uint32_t c0 = (a.tokens - a.observed) * a.group + 32 * wave; c0 < all_cols; c0 += 32 * kPWaves) {
+  for (; c0 < all_cols;) {
     const bool real = c0 + n32 < all_cols;
-    const std::uint32_t col = real ? c0 + n32 : all_cols - 1;
-    const std::uint32_t tok = col / a.group, pos = a.past + tok;
-    const bf16_bits *q =
-        a.query + ((static_cast<std::size_t>(tok) * a.kv_heads + kvh) * a.group + (col - tok * a.group)) * kHeadDim + 8 * kh;
-    floatx16 s = floatx16{};
+    floatx16 s = floatx16{}, s1 = floatx16{}; // (two chains)
 #pragma unroll
-    for (int b = 0; b < 16; ++b)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b], __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(q + 16 * b)), s, 0, 0, 0);
-    const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col;
-    const float m = sc.final[2 * at], inv = sc.final[2 * at + 1];
+    for (int b = 0; b < 16; b += 2) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b], q[b], s, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b + 1], q[b + 1], s1, 0, 0, 0);
+    }
+    s += s1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const std::uint32_t j = j0 + 8 * (i >> 2) + 4 * kh + (i & 3);
       w[i] += real && compact_sees(j, pos, a.window, a.sinks) ? fexp2(s[i] * k_scale - m) * inv : 0.f;
     }
+    c0 += 32 * kWeighWaves;
+    if (c0 < all_cols) load();
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -946,9 +961,12 @@ __global__ __launch_bounds__(kPThreads, 2) void compact_prefill_weigh_kernel(Com
     if (n32 == 0) sum[wave][8 * (i >> 2) + 4 * kh + (i & 3)] = w[i];
   }
   __syncthreads();
-  if (threadIdx.x < kCompactBlock && j0 + threadIdx.x <= last)
-    a.weights[static_cast<std::size_t>(kvh) * a.max_ctx + j0 + threadIdx.x] +=
-        (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
+  if (threadIdx.x < kCompactBlock && j0 + threadIdx.x <= last) {
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWeighWaves; ++i) all += sum[i][threadIdx.x];
+    a.weights[static_cast<std::size_t>(kvh) * a.max_ctx + j0 + threadIdx.x] += all;
+  }
 }
 
 std::uint32_t col_blocks(const CompactArgs &a) { return (a.tokens * a.group + kPCols - 1) / kPCols; }
@@ -1058,7 +1076,7 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   const std::uint32_t last = a.past + a.tokens - 1;
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
-    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kPThreads, 0, stream>>>(a, sc);
+    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kWeighWaves * kWave, 0, stream>>>(a, sc);
   }
 }
 
