@@ -79,17 +79,25 @@ __device__ __forceinline__ void clear_histogram(SelectShared &sh) {
 // Ranks of entries first + 1024 i + thread; 0, which no weight has, for those that the
 // weights do not decide (sinks, recent ones, behind the last).
 template <int R>
-__device__ __forceinline__ void load_ranks(const CompactEvictArgs &a, const Wanted &wanted, std::uint32_t first, std::uint32_t (&r)[R]) {
+__device__ __forceinline__ void load_weights(const CompactEvictArgs &a, std::uint32_t first, float (&x)[R]) {
   const float *w = a.weights + static_cast<std::size_t>(blockIdx.x) * a.max_ctx;
-  float x[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const std::uint32_t at = first + i * kSelectThreads + threadIdx.x;
     x[i] = w[at < a.context ? at : a.context - 1];
   }
+}
+template <int R>
+__device__ __forceinline__ void ranks_of(const Wanted &wanted, std::uint32_t first, const float (&x)[R], std::uint32_t (&r)[R]) {
 #pragma unroll
   for (int i = 0; i < R; ++i)
     r[i] = first + i * kSelectThreads + threadIdx.x - wanted.lo < wanted.hi - wanted.lo ? rank_of(x[i]) : 0u;
+}
+template <int R>
+__device__ __forceinline__ void load_ranks(const CompactEvictArgs &a, const Wanted &wanted, std::uint32_t first, std::uint32_t (&r)[R]) {
+  float x[R];
+  load_weights<R>(a, first, x);
+  ranks_of<R>(wanted, first, x, r);
 }
 // Writes the kept ones of those entries in ascending order: counts per row of 1024
 // entries and wave, one prefix sum, and a lane's place from its wave's masks.
@@ -195,8 +203,8 @@ __global__ __launch_bounds__(kSelectThreads) void compact_count_kernel(CompactEv
 __global__ __launch_bounds__(kSelectThreads) void compact_narrow_kernel(CompactEvictArgs a, SelectScratch sc) {
   __shared__ SelectShared sh;
   const Wanted wanted(a);
-  std::uint32_t r[kSegR];
-  load_ranks<kSegR>(a, wanted, blockIdx.y * kSegment, r);
+  float x[kSegR];
+  load_weights<kSegR>(a, blockIdx.y * kSegment, x);
   const std::size_t seg = static_cast<std::size_t>(blockIdx.x) * gridDim.y + blockIdx.y;
   std::uint32_t digit = 2048; // no entry is wanted: all of them are smaller
   if (wanted.need != 0) {
@@ -210,6 +218,8 @@ __global__ __launch_bounds__(kSelectThreads) void compact_narrow_kernel(CompactE
     }
     digit = pick_digit(sh, h1, h0, need);
   }
+  std::uint32_t r[kSegR];
+  ranks_of<kSegR>(wanted, blockIdx.y * kSegment, x, r);
   std::uint32_t larger = 0, shared = 0;
 #pragma unroll
   for (int i = 0; i < kSegR; ++i) {
@@ -236,11 +246,20 @@ __global__ __launch_bounds__(kSelectThreads) void compact_write_kernel(CompactEv
   std::uint32_t r[kSegR];
   load_ranks<kSegR>(a, wanted, blockIdx.y * kSegment, r);
   const std::size_t seg0 = static_cast<std::size_t>(blockIdx.x) * gridDim.y;
-  // f(rank, segment) over the ranks that share the threshold's first digit
+  // f(rank, segment) over the ranks that share the threshold's first digit, a wave those of
+  // every 16th segment, four loads at a time under way
   const auto each = [&](auto f) {
     for (std::uint32_t s = threadIdx.x >> 6; s < gridDim.y; s += kSelectThreads / 64) {
       const std::uint32_t n = sc.shared[seg0 + s];
-      for (std::uint32_t i = threadIdx.x & 63; i < n; i += 64) f(sc.ranks[(seg0 + s) * kSegment + i], s);
+      const std::uint32_t *ranks = sc.ranks + (seg0 + s) * kSegment;
+      for (std::uint32_t i = threadIdx.x & 63; i < n; i += 4 * 64) {
+        std::uint32_t r4[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) r4[b] = ranks[i + 64 * b < n ? i + 64 * b : i];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (i + 64 * b < n) f(r4[b], s);
+      }
     }
   };
   // Kept for sure after the first digit: in all segments before this one, and in all (which
