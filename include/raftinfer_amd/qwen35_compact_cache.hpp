@@ -7,7 +7,9 @@
 //
 // Validation failures throw Qwen35PrimitiveError before any launch.  Nothing
 // allocates, creates streams or synchronizes; every call may be captured into a
-// graph.  Calls that run at the same time need a workspace each.
+// graph.  Calls that run at the same time need a workspace each.  What a call
+// writes (outputs, cache, key weights, workspace) overlaps none of its other
+// arguments.
 //
 // Cache of one sequence: bf16, the layout of the online attention's bf16 cache
 // ([K plane | V plane], [kv_head][max_context_tokens][256] head-major or
@@ -59,7 +61,7 @@ struct Qwen35CompactShape {
 struct Qwen35EvictShape {
   std::size_t kv_heads;
   std::size_t head_dim; // 256
-  std::size_t context_tokens;
+  std::size_t context_tokens; // at most 65535 * 4096
   std::size_t max_context_tokens;
   std::size_t keep_tokens;
   std::size_t out_max_context_tokens;
@@ -117,7 +119,7 @@ void qwen35_compact_attention_decode(const void *query, const void *key, const v
 // [kv_heads][out_max_context_tokens], 0 behind them), and their indices to
 // kept_indices (int32 [kv_heads][keep_tokens]).  key_weights: float
 // [kv_heads][max_context_tokens].  A bf16 cache may go to an 8-bit one; 8-bit
-// blocks get the scales that their new rows need.  The outputs overlap no input.
+// blocks get the scales that their new rows need.
 void qwen35_compact_cache_evict(const void *kv_cache, std::size_t kv_cache_bytes,
                                 const float *key_weights, void *out_cache, std::size_t out_cache_bytes,
                                 float *out_weights, std::int32_t *kept_indices, void *workspace,

@@ -3,6 +3,8 @@
 #include "compact_cache.hpp"
 #include "raftinfer_amd/qwen35_compact_cache.hpp"
 
+#include <initializer_list>
+
 namespace raftinfer::amd {
 namespace {
 
@@ -134,6 +136,7 @@ constexpr std::size_t kMaxHeadPositions = std::size_t{1} << 31; // over all KV h
 constexpr std::size_t kMaxQueryRows = std::size_t{1} << 26;
 constexpr std::size_t kMaxUnits = std::size_t{1} << 17; // sequences times KV heads
 constexpr std::size_t kMaxGrid = 65535;
+constexpr std::size_t kMaxEvictContext = kMaxGrid * 4096; // segments of the selection
 
 std::size_t cache_bytes_of(std::size_t positions, std::size_t kv_heads, Qwen35CompactCacheDType dtype) {
   const char *overflow = "compact cache byte size overflow";
@@ -205,7 +208,33 @@ void validate_shape(const Qwen35CompactShape &s, bool lengths_given) {
   require<Err>(s.observed_tokens <= s.tokens, "compact attention observes more tokens than the call has");
 }
 
-void validate_cache(const Qwen35CompactShape &s, Qwen35CompactCacheDType dtype, const void *cache,
+struct Bytes {
+  const void *at;
+  std::size_t count;
+};
+// What a call writes overlaps neither what it reads nor what else it writes.
+void validate_apart(std::initializer_list<Bytes> written, std::initializer_list<Bytes> read, const char *message) {
+  const auto apart = [](const Bytes &a, const Bytes &b) {
+    const auto x = reinterpret_cast<std::uintptr_t>(a.at), y = reinterpret_cast<std::uintptr_t>(b.at);
+    return x <= y ? a.count <= y - x : b.count <= x - y;
+  };
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    for (auto other = w + 1; other != written.end(); ++other) require<Err>(apart(*w, *other), message);
+    for (const Bytes &r : read) require<Err>(apart(*w, r), message);
+  }
+}
+// Checked last: everything else about the call is valid.
+void validate_overlap(const Qwen35CompactShape &s, const void *q, const void *k, const void *v, const void *g,
+                      const void *output, const void *cache, std::size_t cache_bytes, const float *weights,
+                      const void *workspace, std::size_t workspace_bytes) {
+  const std::size_t tokens = s.sequences * s.tokens;
+  const std::size_t heads = tokens * s.query_heads * kHeadDim * 2, rows = tokens * s.kv_heads * kHeadDim * 2;
+  const std::size_t weight_bytes = weights != nullptr ? s.sequences * s.kv_heads * s.max_context_tokens * sizeof(float) : 0;
+  validate_apart({{output, heads}, {cache, cache_bytes}, {weights, weight_bytes}, {workspace, workspace_bytes}},
+                 {{q, heads}, {k, rows}, {v, rows}, {g, heads}}, "compact attention outputs overlap other arguments");
+}
+
+std::size_t validate_cache(const Qwen35CompactShape &s, Qwen35CompactCacheDType dtype, const void *cache,
                     std::size_t bytes) {
   const std::size_t one = cache_bytes_of(s.max_context_tokens, s.kv_heads, dtype);
   require<Err>(cache != nullptr, "compact cache pointer is null");
@@ -218,6 +247,7 @@ void validate_cache(const Qwen35CompactShape &s, Qwen35CompactCacheDType dtype, 
                             one, "compact cache byte size overflow");
   }
   require<Err>(bytes >= need, "compact cache is too small");
+  return need;
 }
 
 CompactArgs to_args(const Qwen35CompactShape &s) {
@@ -303,8 +333,10 @@ void qwen35_compact_cache_append(const void *key, const void *value, void *kv_ca
   validate_shape(shape, context_lengths != nullptr);
   require<Err>(context_lengths == nullptr || shape.tokens == 1, "compact append with lengths stores one token per sequence");
   validate_layout(layout);
-  validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
+  const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
   require<Err>(aligned16(key) && aligned16(value), "compact attention inputs and output must be 16-byte aligned");
+  const std::size_t rows = shape.sequences * shape.tokens * shape.kv_heads * kHeadDim * 2;
+  validate_apart({{kv_cache, used}}, {{key, rows}, {value, rows}}, "compact cache overlaps the rows to be stored");
   CompactArgs a = to_args(shape);
   fill_pointers(a, nullptr, key, value, nullptr, nullptr, kv_cache, layout);
   a.lengths = context_lengths;
@@ -323,7 +355,8 @@ void qwen35_compact_attention_prefill(const void *query, const void *key, const 
   const std::size_t need = qwen35_compact_prefill_workspace_bytes(shape);
   validate_call(query, key, value, gate, output, key_weights, workspace, workspace_bytes, need, shape, act, layout,
                 stream);
-  validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
+  const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
+  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, key_weights, workspace, need);
   CompactArgs a = to_args(shape);
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;
@@ -343,7 +376,8 @@ void qwen35_compact_attention_decode(const void *query, const void *key, const v
   const std::size_t need = qwen35_compact_decode_workspace_bytes(shape);
   validate_call(query, key, value, gate, output, key_weights, workspace, workspace_bytes, need, shape, act, layout,
                 stream);
-  validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
+  const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
+  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, key_weights, workspace, need);
   CompactArgs a = to_args(shape);
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;
@@ -361,6 +395,7 @@ CompactEvictArgs evict_args(const Qwen35EvictShape &s) {
   validate_positions(s.max_context_tokens, s.kv_heads);
   validate_positions(s.out_max_context_tokens, s.kv_heads);
   require<Err>(s.context_tokens <= s.max_context_tokens, "compact eviction context exceeds cache capacity");
+  require<Err>(s.context_tokens <= kMaxEvictContext, "compact eviction context_tokens must be at most 65535 * 4096");
   require<Err>(s.keep_tokens > 0 && s.keep_tokens <= s.context_tokens,
                "compact eviction keep_tokens must be 1 to context_tokens");
   require<Err>(s.keep_tokens <= s.out_max_context_tokens, "compact eviction keeps more than the new cache holds");
@@ -408,6 +443,14 @@ void qwen35_compact_cache_evict(const void *kv_cache, std::size_t kv_cache_bytes
   require<Err>(need == 0 || workspace != nullptr, "compact attention workspace is null");
   require<Err>(workspace_bytes >= need, "compact attention workspace is too small");
   require<Err>(aligned16(workspace), "compact attention workspace must be 16-byte aligned");
+  const std::size_t in_bytes = cache_bytes_of(shape.max_context_tokens, shape.kv_heads, cache_dtype);
+  const std::size_t out_bytes = cache_bytes_of(shape.out_max_context_tokens, shape.kv_heads, out_cache_dtype);
+  validate_apart({{out_cache, out_bytes},
+                  {out_weights, shape.kv_heads * shape.out_max_context_tokens * sizeof(float)},
+                  {kept_indices, shape.kv_heads * shape.keep_tokens * sizeof(std::int32_t)},
+                  {workspace, need}},
+                 {{kv_cache, in_bytes}, {key_weights, shape.kv_heads * shape.max_context_tokens * sizeof(float)}},
+                 "compact eviction outputs overlap other arguments");
   a.cache = static_cast<const unsigned char *>(kv_cache);
   a.weights = key_weights;
   a.out_cache = static_cast<unsigned char *>(out_cache);

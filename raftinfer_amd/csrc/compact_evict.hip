@@ -179,6 +179,7 @@ __global__ __launch_bounds__(kSelectThreads) void compact_select_kernel(CompactE
 // which workgroups run.
 constexpr int kSegR = 4;
 constexpr std::uint32_t kSegment = kSegR * kSelectThreads;
+static_assert(kSegment == 4096); // (the entry point allows 65535 of them)
 struct SelectScratch {
   std::uint32_t *hist;    // [kv_head][segment][2048]
   std::uint32_t *larger;  // [kv_head][segment]: entries kept for sure after the first digit

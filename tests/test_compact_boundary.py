@@ -150,3 +150,59 @@ def test_evict_refuses_pointers_and_types():
                         ({"stream": 0}, "stream is null"), ({"kv_cache_bytes": 10}, "too small"), ({"out_cache_bytes": 10}, "too small")]:
         with pytest.raises(ops.Qwen35PrimitiveError, match=message):
             go(**kw)
+
+
+def places(sizes, overlap=None):
+    """Stand-ins for the arguments, one behind the other; overlap (i, j, by): i starts `by` bytes before the end of j."""
+    at, t = 1 << 32, []
+    for n in sizes:
+        t.append(FakeTensor(n, at))
+        at += (n + 255) // 256 * 256
+    if overlap:
+        i, j, by = overlap
+        t[i] = FakeTensor(sizes[i], t[j].data_ptr() + sizes[j] - by)
+    return t
+
+
+@pytest.mark.parametrize("call", ["decode", "prefill"])
+@pytest.mark.parametrize("written", [4, 5, 6, 7])   # output, cache, workspace, key weights
+def test_attention_refuses_overlap(call, written):
+    shape = dataclasses.replace(MODEL, observed_tokens=1)
+    need = getattr(ops, f"qwen35_compact_{call}_workspace_bytes")(shape)
+    assert need > 0
+    head, row = 16 * 512, 4 * 512
+    sizes = [head, row, row, head, head, ops.qwen35_compact_cache_bytes(shape, FP8), need, 4 * 4096 * 4]
+    for other in set(range(8)) - {written}:
+        t = places(sizes, (written, other, 16))
+        with pytest.raises(ops.Qwen35PrimitiveError, match="outputs overlap other arguments"):
+            getattr(ops, f"qwen35_compact_attention_{call}")(*t[:6], shape, ops.DTYPE_BF16, FP8, 1, t[6], key_weights=t[7],
+                                                             stream=0x1234)
+
+
+def test_append_refuses_overlap():
+    row, cache = 4 * 512, ops.qwen35_compact_cache_bytes(MODEL, FP8)
+    for other in (0, 1):
+        t = places([row, row, cache], (2, other, 16))
+        with pytest.raises(ops.Qwen35PrimitiveError, match="overlaps the rows"):
+            ops.qwen35_compact_cache_append(*t, MODEL, ops.DTYPE_BF16, FP8, 1, stream=0x1234)
+
+
+@pytest.mark.parametrize("written", [2, 3, 4, 5])   # cache, weights, indices, workspace
+def test_evict_refuses_overlap(written):
+    shape = E(4, 256, 30000, 40000, 1000, 1200)
+    need = ops.qwen35_compact_evict_workspace_bytes(shape)
+    assert need > 0
+    big, small = (S(1, 1, 4, 4, 256, n, 0) for n in (40000, 1200))
+    sizes = [ops.qwen35_compact_cache_bytes(big, BF16), 4 * 40000 * 4, ops.qwen35_compact_cache_bytes(small, FP8), 4 * 1200 * 4,
+             4 * 1000 * 4, need]
+    for other in set(range(6)) - {written}:
+        t = places(sizes, (written, other, 16))
+        with pytest.raises(ops.Qwen35PrimitiveError, match="outputs overlap other arguments"):
+            ops.qwen35_compact_cache_evict(*t[:5], shape, BF16, FP8, 1, t[5], stream=0x1234)
+
+
+def test_evict_refuses_too_many_segments():
+    shape = E(1, 256, 65535 * 4096 + 1, 2 ** 28, 10, 10)
+    with pytest.raises(ops.Qwen35PrimitiveError, match="at most 65535"):
+        ops.qwen35_compact_evict_workspace_bytes(shape)
+    assert ops.qwen35_compact_evict_workspace_bytes(dataclasses.replace(shape, context_tokens=65535 * 4096)) > 0
