@@ -382,6 +382,86 @@ def test_bad_values_among_wide_columns(gpu, what, hkv, group, t, past, window, s
             near(got[i:i + 1], want, bound, f"token {i}")
 
 
+@pytest.mark.parametrize("dtype,layout", [(BF16, 0), (FP8, 1), (FP8, 0)])
+def test_many_heads(gpu, dtype, layout):
+    r = rng(94)
+    c = filled(r, dtype, layout, 1000, 80, 33)
+    run_prefill(c, r, 2000, 5, 33, observed=2)
+    run_decode(c, r, 2000, 38, weights=True)
+    run_decode(c, r, 3000, 39, window=20, sinks=3)
+
+
+@pytest.mark.parametrize("dtype,layout,past", [(FP8, 1, 200), (FP8, 0, 200), (BF16, 1, 200), (BF16, 0, 500)])
+def test_rows_behind_4_gib(gpu, dtype, layout, past):
+    """The last positions of a cache whose planes pass 2^32 bytes, against a small cache: a window hides the rest."""
+    r = rng(95)
+    hkv, heads, cap, small = 4, 16, 1 << 22, 1024
+    base = cap - small
+    c = Cache(r, dtype, layout, hkv, small)
+    shape = lambda t, p, **kw: ops.Qwen35CompactShape(t, 1, heads, hkv, D, cap, base + p, window_tokens=64, **kw)
+    big = torch.empty(ops.qwen35_compact_cache_bytes(shape(1, 0), dtype), device="cuda", dtype=torch.uint8)
+    assert big.numel() > 1 << 32
+    k, v = rows(r, past, hkv), rows(r, past, hkv)
+    ops.qwen35_compact_cache_append(dev(k), dev(v), big, shape(past, 0), ops.DTYPE_BF16, dtype, layout)
+    c.want_store(0, k, v)
+
+    def check(t, p, call, size):
+        k, v, q, g = rows(r, t, hkv), rows(r, t, hkv), bf16(normal(r, t, heads, D)), bf16(normal(r, t, heads, D))
+        sh = shape(t, p)
+        ws = torch.empty(size(sh), device="cuda", dtype=torch.uint8)
+        out = torch.empty(t, heads, D, device="cuda", dtype=torch.bfloat16)
+        call(dev(q), dev(k), dev(v), dev(g), out, big, sh, ops.DTYPE_BF16, dtype, layout, ws)
+        c.want_store(p, k, v)
+        want, bound, _, _ = ref.attention(q, g, c.held(p + t), p, 64)
+        near(host(out), want, bound, f"{t} behind {p}")
+
+    check(70, past, ops.qwen35_compact_attention_prefill, ops.qwen35_compact_prefill_workspace_bytes)
+    check(1, past + 70, ops.qwen35_compact_attention_decode, ops.qwen35_compact_decode_workspace_bytes)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("t,past,hkv,group", [(130, 3001, 2, 16), (20, 3001, 2, 8), (300, 0, 4, 4)])
+def test_prefill_in_a_graph(gpu, dtype, t, past, hkv, group):
+    """Captured once and replayed with eager calls of other inputs between, on the same workspace in turn."""
+    r = rng(96)
+    heads = hkv * group
+    c = filled(r, dtype, 1, hkv, past + t, past)
+    shape = c.shape(t, heads, past, observed_tokens=2)
+    ws = torch.empty(ops.qwen35_compact_prefill_workspace_bytes(shape), device="cuda", dtype=torch.uint8)
+    weights = torch.zeros(hkv, past + t, device="cuda")
+    inputs = [[dev(normal(r, t, m, D)) for m in (heads, hkv, hkv, heads)] for _ in range(3)]
+    held = [x.clone() for x in inputs[0]]
+    start = c.buf.clone()
+
+    def go(x, out, stream=None):
+        ops.qwen35_compact_attention_prefill(*x, out, c.buf, shape, ops.DTYPE_BF16, dtype, 1, ws, key_weights=weights,
+                                             stream=stream)
+
+    want = []
+    for x in inputs:
+        c.buf.copy_(start)
+        weights.zero_()
+        out = torch.empty(t, heads, D, device="cuda", dtype=torch.bfloat16)
+        go(x, out)
+        want.append((out, c.buf.clone(), weights.clone()))
+    out = torch.empty_like(want[0][0])
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        go(held, out, stream)
+    for i in (0, 2, 1, 2):
+        go(inputs[(i + 1) % 3], torch.empty_like(out))
+        for dst, src in zip(held, inputs[i]):
+            dst.copy_(src)
+        c.buf.copy_(start)
+        weights.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip((out, c.buf, weights), want[i]):
+            assert torch.equal(got, w), i
+
+
 # ------------------------------------------------------------------ values that reach no one
 
 @pytest.mark.parametrize("t,past,window,sinks", [(40, 100, 0, 0), (40, 100, 30, 0), (40, 100, 30, 40), (1, 100, 30, 40)])
