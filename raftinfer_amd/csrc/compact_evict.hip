@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kSelectThreads) void compact_select_kernel(CompactE
 // one and the ranks of those that share it (few, unless many weights are alike).  In the
 // third every segment finds the rest of the threshold from all of these, and writes its
 // kept entries behind those of the segments before it.  No count depends on the order in
-// which workgroups run.  60001 entries of 4 heads: 3.3 + 7.7 + 9.9 us, the latency of dependent
+// which workgroups run.  60001 entries of 4 heads: 3.5 + 6.8 + 9.4 us, the latency of dependent
 // loads and barriers (the weights are 1 MB).
 constexpr int kSegR = 4;
 constexpr std::uint32_t kSegment = kSegR * kSelectThreads;
@@ -213,11 +213,16 @@ __global__ __launch_bounds__(kSelectThreads) void compact_narrow_kernel(CompactE
   if (wanted.need != 0) {
     const std::uint32_t *hist = sc.hist + static_cast<std::size_t>(blockIdx.x) * gridDim.y * 2048 + 2046 - 2 * threadIdx.x;
     std::uint32_t h0 = 0, h1 = 0, need = wanted.need;
-#pragma unroll 8
-    for (std::uint32_t s = 0; s < gridDim.y; ++s) {
-      const u32x2 h = *reinterpret_cast<const u32x2 *>(hist + static_cast<std::size_t>(s) * 2048);
-      h0 += h[0];
-      h1 += h[1];
+    for (std::uint32_t s0 = 0; s0 < gridDim.y; s0 += 16) { // (sixteen loads under way: they come from other XCDs' workgroups)
+      u32x2 h[16];
+#pragma unroll
+      for (std::uint32_t b = 0; b < 16; ++b)
+        h[b] = *reinterpret_cast<const u32x2 *>(hist + static_cast<std::size_t>(s0 + b < gridDim.y ? s0 + b : s0) * 2048);
+#pragma unroll
+      for (std::uint32_t b = 0; b < 16; ++b) {
+        h0 += s0 + b < gridDim.y ? h[b][0] : 0u;
+        h1 += s0 + b < gridDim.y ? h[b][1] : 0u;
+      }
     }
     digit = pick_digit(sh, h1, h0, need);
   }
@@ -246,19 +251,30 @@ __global__ __launch_bounds__(kSelectThreads) void compact_write_kernel(CompactEv
   __shared__ SelectShared sh;
   __shared__ std::uint32_t sure_of[kSegR * kSelectThreads / 64], equal_of[kSegR * kSelectThreads / 64];
   const Wanted wanted(a);
-  std::uint32_t r[kSegR];
-  load_ranks<kSegR>(a, wanted, blockIdx.y * kSegment, r);
+  float x[kSegR];
+  load_weights<kSegR>(a, blockIdx.y * kSegment, x);
   const std::size_t seg0 = static_cast<std::size_t>(blockIdx.x) * gridDim.y;
   // f(rank, segment) over the ranks that share the threshold's first digit, a wave those of
-  // every 16th segment, four loads at a time under way
+  // every 16th segment, four loads at a time under way.  The first four, and how many its
+  // first segment has, are asked for here with all else.
+  const std::uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const std::size_t first_seg = seg0 + (wave < gridDim.y ? wave : 0);
+  const std::uint32_t first_n = sc.shared[first_seg];
+  std::uint32_t first_ranks[4]; // (what lies behind the last of those is not used)
+#pragma unroll
+  for (int b = 0; b < 4; ++b) first_ranks[b] = sc.ranks[first_seg * kSegment + lane + 64 * b];
   const auto each = [&](auto f) {
-    for (std::uint32_t s = threadIdx.x >> 6; s < gridDim.y; s += kSelectThreads / 64) {
-      const std::uint32_t n = sc.shared[seg0 + s];
+    for (std::uint32_t s = wave; s < gridDim.y; s += kSelectThreads / 64) {
+      const std::uint32_t n = s == wave ? first_n : sc.shared[seg0 + s];
       const std::uint32_t *ranks = sc.ranks + (seg0 + s) * kSegment;
-      for (std::uint32_t i = threadIdx.x & 63; i < n; i += 4 * 64) {
+      for (std::uint32_t i = lane; i < n; i += 4 * 64) {
         std::uint32_t r4[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) r4[b] = ranks[i + 64 * b < n ? i + 64 * b : i];
+        for (int b = 0; b < 4; ++b) r4[b] = first_ranks[b];
+        if (s != wave || i != lane) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) r4[b] = ranks[i + 64 * b < n ? i + 64 * b : i];
+        }
 #pragma unroll
         for (int b = 0; b < 4; ++b)
           if (i + 64 * b < n) f(r4[b], s);
@@ -273,6 +289,8 @@ __global__ __launch_bounds__(kSelectThreads) void compact_write_kernel(CompactEv
     all += n;
     mine += s < blockIdx.y ? n : 0u;
   }
+  std::uint32_t r[kSegR];
+  ranks_of<kSegR>(wanted, blockIdx.y * kSegment, x, r);
   std::uint32_t larger_before, larger_all;
   (void)block_prefix(mine, sh.waves, larger_before);
   (void)block_prefix(all, sh.waves, larger_all);
