@@ -19,6 +19,7 @@ struct CompactArgs {
   float *weights;
   std::uint32_t tokens, sequences, kv_heads, group, max_ctx, past, window, sinks, observed;
   bool head_major;
+  bool store_inside; // prefill of bf16: the attention kernel stores the rows, and reads the new ones from key / value
 };
 
 // One KV head of one sequence's cache.
@@ -128,7 +129,7 @@ std::size_t compact_decode_workspace(const CompactArgs &a);
 void compact_decode(const CompactArgs &a, bool fp8, void *workspace, hipStream_t stream);
 
 std::size_t compact_prefill_workspace(const CompactArgs &a);
-void compact_prefill(const CompactArgs &a, bool fp8, void *workspace, hipStream_t stream);
+void compact_prefill(CompactArgs a, bool fp8, void *workspace, hipStream_t stream);
 
 struct CompactEvictArgs {
   const unsigned char *cache;

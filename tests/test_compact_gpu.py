@@ -310,10 +310,10 @@ def some_tokens(t):
 
 
 # Enough columns and keys that workgroups of 128 columns share the tiles, whole and split over the keys; the last
-# three, of 128 and of 32 columns, split the later tokens' keys only.
+# three of them, of 128 and of 32 columns, split the later tokens' keys only.
 WIDE = [(16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40), (7, 13, 501, 300, 0, 0), (7, 13, 503, 800, 400, 3),
         (2, 16, 130, 3001, 0, 0), (2, 16, 131, 4000, 3000, 70), (1, 16, 300, 5000, 4999, 1), (1, 3, 900, 4000, 0, 0),
-        (4, 4, 1400, 0, 0, 0), (1, 1, 1200, 0, 0, 0), (1, 2, 700, 5, 600, 3)]
+        (2, 5, 700, 640, 0, 0), (4, 4, 1400, 0, 0, 0), (1, 1, 1200, 0, 0, 0), (1, 2, 700, 5, 600, 3)]
 
 
 @pytest.mark.parametrize("dtype,layout", [(BF16, 1), (FP8, 1), (BF16, 0), (FP8, 0)])
@@ -356,7 +356,7 @@ def test_prefill_wide(gpu, dtype, layout, hkv, group, t, past, window, sinks):
 
 @pytest.mark.parametrize("what", [np.nan, np.inf])
 @pytest.mark.parametrize("hkv,group,t,past,window,sinks", [(16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40),
-                                                           (2, 16, 131, 4000, 3000, 70)])
+                                                           (2, 16, 131, 4000, 3000, 70), (16, 16, 130, 608, 0, 0)])
 def test_bad_values_among_wide_columns(gpu, what, hkv, group, t, past, window, sinks):
     r = rng(93)
     heads, n = hkv * group, past + t
@@ -464,7 +464,8 @@ def test_prefill_in_a_graph(gpu, dtype, t, past, hkv, group):
 
 # ------------------------------------------------------------------ values that reach no one
 
-@pytest.mark.parametrize("t,past,window,sinks", [(40, 100, 0, 0), (40, 100, 30, 0), (40, 100, 30, 40), (1, 100, 30, 40)])
+@pytest.mark.parametrize("t,past,window,sinks", [(40, 100, 0, 0), (40, 100, 30, 0), (40, 100, 30, 40), (1, 100, 30, 40),
+                                                 (40, 96, 0, 0), (40, 96, 30, 40)])
 @pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
 def test_bad_values_reach_only_the_tokens_that_see_them(gpu, t, past, window, sinks, what):
     # rows of infinite or NaN values in K (100 + 20) and V (one in the window's edge, one in the new tokens)
