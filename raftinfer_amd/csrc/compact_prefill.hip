@@ -165,7 +165,7 @@ __device__ __forceinline__ u32x4 fp8x8_to_bf16_scaled(std::uint32_t lo, std::uin
 // that one's softmax runs beside the other's products.
 //
 // 500 tokens of 16 heads behind 30001, 8 bit: 285 us, 870 TFLOP/s; 6001 behind a window of
-// 1024, bf16: 146 us.  A wave's tile takes 4300 clocks, 1024 of them of matrix time (two
+// 1024, bf16, with the store: 155 us.  A wave's tile takes 4300 clocks, 1024 of them of matrix time (two
 // waves a SIMD, 50% busy): softmax 450, conversion 1000, barrier 200, products 2300; no
 // waits for loads, no bank conflicts.  One workgroup of 256 columns per CU took 174 us for
 // the window, 64 columns a wave do not fit its registers.
