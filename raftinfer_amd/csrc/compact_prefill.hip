@@ -19,9 +19,11 @@ constexpr int kTileElems = kCompactBlock * kHeadDim;
 constexpr std::uint32_t kPrefillCus = 256;
 
 // Partials of a split call, [split][kv_head][column], and the final max (exp2
-// domain) and 1 / sum of each column for the key weights.
+// domain) and 1 / sum of each column for the key weights.  An output is divided by the sum
+// of the probabilities as they were rounded to bf16 for the product with V (l), so that it is
+// an average of the V rows; the key weights by the sum of the exact ones (lw).
 struct PrefillScratch {
-  float *m, *l, *o, *final;
+  float *m, *l, *lw, *o, *final;
   std::uint32_t cols;         // columns of a KV head, rounded up to whole workgroups
   std::uint32_t block;        // columns of a workgroup
   std::uint32_t tiles, most;  // of a column block's ranges: tiles of one, ranges
@@ -296,6 +298,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb) o[nb] = floatx16{};
   float m_run = -FLT_MAX, l_run = 0.f;
+  [[maybe_unused]] float lw_run = 0.f;
 
   const auto scale_of = [&](const float *scales, std::uint32_t it) {
     if constexpr (Fp8) return scales[seen.tile(it)]; // (a scalar load: no LDS reads are under way then)
@@ -360,6 +363,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
       const float f = grow ? fexp2(m_run - mx) : 1.0f;
       l_run *= f;
+      if constexpr (Weigh) lw_run *= f;
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) o[nb] *= f;
       m_run = grow ? mx : m_run;
@@ -374,9 +378,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         const float p0 = fexp2(fmaf(s[8 * kb + 2 * e], kScale, -m_run)), p1 = fexp2(fmaf(s[8 * kb + 2 * e + 1], kScale, -m_run));
         const std::uint32_t pair = pack_bf16x2(p0, p1);
         w[e] = pair;
-        // The sum is that of the rounded probabilities, with which the output is a convex
-        // combination of the V rows; key weights need the exact one.
-        if constexpr (Weigh) l_run += p0 + p1; else l_run = dot2_bf16(pair, 0x3F803F80u, l_run);
+        l_run = dot2_bf16(pair, 0x3F803F80u, l_run); // (1, 1)
+        if constexpr (Weigh) lw_run += p0 + p1;
       }
       pb[kb] = __builtin_bit_cast(bf16x8, w);
     }
@@ -427,11 +430,13 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     add_odd_values<Fp8, 32>(c, seen, begin, end, 1, p_lo, p_hi, a.past + token_of(col), a, kvh, kh,
                             [&](int i, float x) __attribute__((always_inline)) { o[i >> 4][i & 15] += x; });
   const float l = sum_xor32(l_run);
+  [[maybe_unused]] const float lw = Weigh ? sum_xor32(lw_run) : 0.f;
   if (Split && part) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + kvh) * sc.cols + col;
     if (kh == 0) {
       sc.m[at] = m_run;
       sc.l[at] = l;
+      if constexpr (Weigh) sc.lw[at] = lw;
     }
     float *dst = sc.o + at * kHeadDim + 4 * kh;
 #pragma unroll
@@ -443,10 +448,10 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   } else {
     if (col >= all_cols) return;
     const float inv = 1.0f / l;
-    if (a.weights != nullptr && kh == 0) {
+    if (Weigh && kh == 0) {
       const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col;
       sc.final[2 * at] = m_run;
-      sc.final[2 * at + 1] = inv;
+      sc.final[2 * at + 1] = 1.0f / lw;
     }
     const std::size_t base = io_row(col) * kHeadDim + 4 * kh;
     u32x2 g[32]; // (every load before the first store, which it might alias)
@@ -846,6 +851,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     if (threadIdx.x < kKCols) {
       sc.m[at + lane] = m;
       sc.l[at + lane] = l;
+      if (a.weights != nullptr) sc.lw[at + lane] = l;
     }
 #pragma unroll
     for (int i = 0; i < kKCols / kPWaves; ++i) {
@@ -915,11 +921,13 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
   const std::uint32_t s_first = W == 1 ? 0 : wave % W;
   load(s_first);
   // max and sum over the splits; those without a key that the column sees have l = 0
-  float m = -FLT_MAX, l = 0.f;
+  float m = -FLT_MAX, l = 0.f, lw = 0.f;
   for (std::uint32_t s = lane; s < splits; s += 64) {
     const float ms = sc.m[at0 + s * stride], ls = sc.l[at0 + s * stride];
-    const float m_new = fmaxf(m, ms);
-    l = l * fexp2(m - m_new) + ls * fexp2(ms - m_new);
+    const float lws = a.weights != nullptr ? sc.lw[at0 + s * stride] : 0.f;
+    const float m_new = fmaxf(m, ms), f = fexp2(m - m_new), fs = fexp2(ms - m_new);
+    l = l * f + ls * fs;
+    lw = lw * f + lws * fs;
     m = m_new;
   }
   const float m_all = wave_max(m);
@@ -944,9 +952,12 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
     for (int w = 1; w < W; ++w) o += *reinterpret_cast<const floatx4 *>(&o_of[wave + w][4 * lane]);
   }
   if (col_of >= all_cols) return;
-  if (a.weights != nullptr && lane == 0) {
-    sc.final[2 * at0] = m_all;
-    sc.final[2 * at0 + 1] = inv;
+  if (a.weights != nullptr) {
+    const float all = wave_sum(lw * fexp2(m - m_all));
+    if (lane == 0) {
+      sc.final[2 * at0] = m_all;
+      sc.final[2 * at0 + 1] = 1.0f / all;
+    }
   }
   const float r0 = o[0] * inv * sigmoid_gate(bf16_lo(g[0])), r1 = o[1] * inv * sigmoid_gate(bf16_hi(g[0]));
   const float r2 = o[2] * inv * sigmoid_gate(bf16_lo(g[1])), r3 = o[3] * inv * sigmoid_gate(bf16_hi(g[1]));
@@ -1108,6 +1119,7 @@ PrefillScratch scratch_of(const CompactArgs &a, std::uint32_t ranges, void *work
   if (ranges > 1) {
     sc.m = take(ranges * cols);
     sc.l = take(ranges * cols);
+    if (a.observed != 0) sc.lw = take(ranges * cols);
     sc.o = take(ranges * cols * kHeadDim);
   }
   if (bytes != nullptr) *bytes = at;

@@ -1,0 +1,84 @@
+"""The compact KV cache at values where roundings show: the weights that the values are averaged with sum to what the
+average is divided by, and key weights change no output."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import bf16, normal, rng
+from raftinfer_amd import ops
+from test_compact_gpu import BF16, D, FP8, WIDE, Cache, dev, filled, host, rows
+
+pytestmark = pytest.mark.gpu
+
+# (KV heads, group, tokens, past, window, sinks): many columns, keys whole and in ranges
+SHAPES = [WIDE[i] for i in (0, 1, 4, 7)]
+
+
+def prefill(c, x, t, heads, past, window=0, sinks=0, observed=0):
+    shape = c.shape(t, heads, past, window_tokens=window, sink_tokens=sinks, observed_tokens=observed)
+    ws = torch.full((ops.qwen35_compact_prefill_workspace_bytes(shape),), 0xFF, device="cuda", dtype=torch.uint8)
+    out = torch.empty(t, heads, D, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(c.hkv, c.cap, device="cuda") if observed else None
+    ops.qwen35_compact_attention_prefill(*x, out, c.buf, shape, ops.DTYPE_BF16, c.dtype, c.layout, ws, key_weights=w)
+    return out, w
+
+
+# ------------------------------------------------------------------ an average of equal values is that value
+
+ALIKE = 1.875  # a bf16 and an e4m3 number; its neighbours in bf16 are 2^-7 away
+
+
+def alike(hkv, n):
+    """Keys of score 0 and, 15 of 16, of a score whose probability is 0.9 of half a bf16 step above 1/2 of that (so
+    bf16 rounds it down by 2^-8.2 of itself), and the same value at every key.  The score is the sum of the key's first four dims
+    / 16, e4m3 numbers of a block's scale 2^-5."""
+    rest = -16 * np.log(0.5 * (1 + 0.9 * 2.0 ** -8))
+    k = np.zeros((n, hkv, D), np.float32)
+    at = np.arange(n) % 16 != 0
+    for i in range(4):
+        digit = 0.0 if rest == 0 else 2.0 ** (max(np.floor(np.log2(abs(rest))), -11) - 3)
+        part = np.round(rest / digit) * digit
+        k[at, :, i] = -part
+        rest -= part
+    assert abs(rest) < 2.0 ** -12
+    return k, np.full((n, hkv, D), ALIKE, np.float32)
+
+
+def queries(t, heads):
+    q = np.zeros((t, heads, D), np.float32)
+    q[..., :4] = 1
+    return dev(q), dev(np.full((t, heads, D), 200, np.float32))  # a gate that is 1 in f32
+
+
+# The sums take n steps of 2^-24 each and the quotient two more: 2^-11.6 of the value at 5000 keys, where 2^-8.9 of
+# it is half a step of the result.  So every output is the value itself.
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("observed", [0, 1])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", SHAPES)
+def test_prefill_of_equal_values(gpu, dtype, observed, hkv, group, t, past, window, sinks):
+    k, v = alike(hkv, past + t)
+    c = Cache(rng(1), dtype, 1, hkv, past + t)
+    if past:
+        c.store(0, k[:past], v[:past])
+    q, g = queries(t, hkv * group)
+    out, w = prefill(c, (q, dev(k[past:]), dev(v[past:]), g), t, hkv * group, past, window, sinks, observed)
+    assert (host(out) == ALIKE).all()
+    if observed:  # probabilities that sum to 1 a head
+        total = host(w).astype(np.float64).sum(1)
+        assert np.abs(total / group - 1).max() < (past + t + 64) * 2.0 ** -23
+
+
+# ------------------------------------------------------------------ key weights change no output
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", SHAPES)
+def test_prefill_with_weights_gives_the_same_output(gpu, dtype, hkv, group, t, past, window, sinks):
+    r = rng(3)
+    heads = hkv * group
+    c = filled(r, dtype, 1, hkv, past + t, past)
+    x = dev(normal(r, t, heads, D)), dev(rows(r, t, hkv)), dev(rows(r, t, hkv)), dev(normal(r, t, heads, D))
+    start = c.buf.clone()
+    plain, _ = prefill(c, x, t, heads, past, window, sinks)
+    c.buf.copy_(start)
+    weighed, _ = prefill(c, x, t, heads, past, window, sinks, observed=min(t, 3))
+    assert torch.equal(plain, weighed)
