@@ -471,7 +471,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 // columns of one KV head, its waves take every fourth tile of the range by themselves and
 // are joined in LDS.  Products on v_mfma_f32_16x16x32_bf16 with two blocks of 16 columns.
 // K and V rows lie in LDS as they are in the cache (8-bit operands become bf16 behind the
-// read; the block's scales go on the scores and the probabilities), asked for by
+// read; the block's scales go on the scores and on V's operands), asked for by
 // LDS-direct loads of the wave's own kStages tiles ahead.
 //
 // 500 tokens of 16 heads, 8 bit: 17.3 us for 2.1 GFLOP, of which 3.4 until q and the first
@@ -486,7 +486,7 @@ struct KeysShared {
     float acc[kPWaves][kKCols][kHeadDim + 4];
   };
   alignas(1024) bf16_bits gate[kPWaves][kKCols / kPWaves][kHeadDim];
-  float m[kPWaves][kKCols], l[kPWaves][kKCols];
+  float m[kPWaves][kKCols], l[kPWaves][kKCols], lw[kPWaves][kKCols];
 };
 // What a row's number is exclusive-ored to its 16-byte chunks' places with (linear in the
 // bits of r): a pass of the K reads takes one chunk of 16 rows, of the V reads
@@ -495,7 +495,7 @@ template <bool Fp8> __device__ __forceinline__ constexpr std::uint32_t keys_at(s
   if (!is_v) return r & 15;
   return Fp8 ? (r & 3) | (r >> 4 & 1) << 2 | (r >> 2 & 1) << 3 : 2 * (r & 7);
 }
-template <bool Fp8, bool Split>
+template <bool Fp8, bool Split, bool Weigh>
 __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     CompactArgs a, PrefillScratch sc) {
   __shared__ __attribute__((aligned(1024))) KeysShared sh;
@@ -625,6 +625,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
 #pragma unroll
     for (int db = 0; db < 16; ++db) acc[cb][db] = floatx4{};
   float m_run[2] = {-FLT_MAX, -FLT_MAX}, l_run[2] = {0.f, 0.f};
+  [[maybe_unused]] float lw_run[2] = {0.f, 0.f};
   std::uint64_t odd = 0; // lanes that took infinite or NaN values out of a masked tile
 
 #pragma unroll 1
@@ -649,9 +650,9 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     // (operands are read kRing products ahead: left to the compiler, one, and each waits)
     constexpr int kRing = 8;
     // 8-bit operands are converted between the products of the one before.
-    const auto pair_of = [](std::uint32_t w, bool hi) {
+    const auto pair_of = [](std::uint32_t w, bool hi, float scale) {
       typedef __bf16 pair __attribute__((ext_vector_type(2)));
-      const pair x = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+      const pair x = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
       return __builtin_bit_cast(std::uint32_t, x);
     };
     {
@@ -661,7 +662,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
       if constexpr (Fp8) {
         // operand n: half n & 1 of read n / 2
         const auto code = [&](int n, int w) { return __builtin_bit_cast(u32x4, op[n >> 1])[2 * (n & 1) + w]; };
-        u32x4 now{pair_of(code(0, 0), false), pair_of(code(0, 0), true), pair_of(code(0, 1), false), pair_of(code(0, 1), true)}, next = now;
+        u32x4 now{pair_of(code(0, 0), false, 1.0f), pair_of(code(0, 0), true, 1.0f), pair_of(code(0, 1), false, 1.0f), pair_of(code(0, 1), true, 1.0f)}, next = now;
 #pragma unroll
         for (int n = 0; n < kRowBytes / 16; ++n) {
           const int rb = n >> 1 & 1, qi = 2 * (n >> 2) + (n & 1);
@@ -669,8 +670,8 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
           for (int cb = 0; cb < 2; ++cb) {
             s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now), qb[cb][qi], s[cb][rb], 0, 0, 0);
             if (n + 1 < kRowBytes / 16) {
-              next[2 * cb] = pair_of(code(n + 1, cb), false);
-              next[2 * cb + 1] = pair_of(code(n + 1, cb), true);
+              next[2 * cb] = pair_of(code(n + 1, cb), false, 1.0f);
+              next[2 * cb + 1] = pair_of(code(n + 1, cb), true, 1.0f);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -715,6 +716,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
       for (int cb = 0; cb < 2; ++cb) {
         const float m_new = fmaxf(m_run[cb], mx[cb]), f = fexp2(m_run[cb] - m_new);
         l_run[cb] *= f;
+        if constexpr (Weigh) lw_run[cb] *= f;
 #pragma unroll
         for (int db = 0; db < 16; ++db) {
           // (in accumulation registers but for here: moved out and in on every tile otherwise)
@@ -740,11 +742,13 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e[i] = fexp2(fmaf(s[cb][rb][i], k_scale, -m_run[cb]));
-          l_run[cb] += e[i];
-          e[i] *= v_scale;
+          if constexpr (Weigh) lw_run[cb] += e[i];
         }
-        pw[cb][2 * rb] = pack_bf16x2(e[0], e[1]);
-        pw[cb][2 * rb + 1] = pack_bf16x2(e[2], e[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pw[cb][2 * rb + i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+          l_run[cb] = dot2_bf16(pw[cb][2 * rb + i], 0x3F803F80u, l_run[cb]); // (1, 1)
+        }
       }
     // V(t): behind it K(t + 1) and, of two stages, V(t + 1) and K(t + 2)
     if (kStages == 2 && t + 2 < steps) wait_vm<3 * kLoads>();
@@ -795,7 +799,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     for (int db = 0; db < kRing; ++db) op[db] = read_v(db);
     __builtin_amdgcn_sched_barrier(0);
     u32x4 now;
-    if constexpr (Fp8) now = u32x4{pair_of(op[0][0], false), pair_of(op[0][0], true), pair_of(op[0][1], false), pair_of(op[0][1], true)};
+    if constexpr (Fp8) now = u32x4{pair_of(op[0][0], false, v_scale), pair_of(op[0][0], true, v_scale), pair_of(op[0][1], false, v_scale), pair_of(op[0][1], true, v_scale)};
 #pragma unroll
     for (int db = 0; db < 16; ++db) {
       if constexpr (!Fp8) now = op[db % kRing];
@@ -804,8 +808,8 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
       for (int cb = 0; cb < 2; ++cb) {
         acc[cb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now), __builtin_bit_cast(bf16x8, pw[cb]), acc[cb][db], 0, 0, 0);
         if (Fp8 && db + 1 < 16) {
-          next[2 * cb] = pair_of(op[(db + 1) % kRing][cb], false);
-          next[2 * cb + 1] = pair_of(op[(db + 1) % kRing][cb], true);
+          next[2 * cb] = pair_of(op[(db + 1) % kRing][cb], false, v_scale);
+          next[2 * cb + 1] = pair_of(op[(db + 1) % kRing][cb], true, v_scale);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -829,9 +833,11 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
 #pragma unroll
   for (int cb = 0; cb < 2; ++cb) {
     const float l = sum_xor32(sum_xor16(l_run[cb]));
+    [[maybe_unused]] const float lw = Weigh ? sum_xor32(sum_xor16(lw_run[cb])) : 0.f;
     if (kq == 0) {
       sh.m[wave][16 * cb + col16] = m_run[cb];
       sh.l[wave][16 * cb + col16] = l;
+      if constexpr (Weigh) sh.lw[wave][16 * cb + col16] = lw;
     }
 #pragma unroll
     for (int db = 0; db < 16; ++db) *reinterpret_cast<floatx4 *>(&sh.acc[wave][16 * cb + col16][16 * db + 4 * kq]) = acc[cb][db];
@@ -839,19 +845,21 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
   __syncthreads();
   // Lane x, and x + 32: the waves' shares of column x.
   float m = -FLT_MAX, l = 0.f, share[kPWaves];
+  [[maybe_unused]] float lw = 0.f;
 #pragma unroll
   for (int w = 0; w < kPWaves; ++w) m = fmaxf(m, sh.m[w][lane & 31]);
 #pragma unroll
   for (int w = 0; w < kPWaves; ++w) {
     share[w] = fexp2(sh.m[w][lane & 31] - m);
     l = fmaf(sh.l[w][lane & 31], share[w], l);
+    if constexpr (Weigh) lw = fmaf(sh.lw[w][lane & 31], share[w], lw);
   }
   if (Split && part) {
     const std::size_t at = (static_cast<std::size_t>(blockIdx.z) * a.kv_heads + kvh) * sc.cols + col0;
     if (threadIdx.x < kKCols) {
       sc.m[at + lane] = m;
       sc.l[at + lane] = l;
-      if (a.weights != nullptr) sc.lw[at + lane] = l;
+      if constexpr (Weigh) sc.lw[at + lane] = lw;
     }
 #pragma unroll
     for (int i = 0; i < kKCols / kPWaves; ++i) {
@@ -863,10 +871,10 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
     }
   } else {
     const float inv = 1.0f / l;
-    if (a.weights != nullptr && threadIdx.x <= last_x) {
+    if (Weigh && threadIdx.x <= last_x) {
       const std::size_t at = static_cast<std::size_t>(kvh) * sc.cols + col0 + lane;
       sc.final[2 * at] = m;
-      sc.final[2 * at + 1] = inv;
+      sc.final[2 * at + 1] = 1.0f / lw;
     }
     u32x2 out[kKCols / kPWaves];
 #pragma unroll
@@ -1135,8 +1143,10 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   sc.most = split.count;
   const dim3 grid{col_blocks(a) * a.kv_heads, split.count}, keys_grid{a.kv_heads, key_col_blocks(a), split.count};
   const auto launch = [&](auto several) {
-    if (split.by_keys)
-      compact_prefill_keys_kernel<Fp8, several><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
+    if (split.by_keys && a.weights != nullptr)
+      compact_prefill_keys_kernel<Fp8, several, true><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
+    else if (split.by_keys)
+      compact_prefill_keys_kernel<Fp8, several, false><<<keys_grid, kPThreads, 0, stream>>>(a, sc);
     else if (a.weights != nullptr)
       compact_prefill_kernel<Fp8, several, true><<<grid, kPThreads, 0, stream>>>(a, sc);
     else

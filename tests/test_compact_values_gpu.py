@@ -10,8 +10,9 @@ from test_compact_gpu import BF16, D, FP8, WIDE, Cache, dev, filled, host, rows
 
 pytestmark = pytest.mark.gpu
 
-# (KV heads, group, tokens, past, window, sinks): many columns, keys whole and in ranges
-SHAPES = [WIDE[i] for i in (0, 1, 4, 7)]
+# (KV heads, group, tokens, past, window, sinks): few columns and many, keys whole and in ranges
+SHAPES = [(2, 4, 2, 0, 0, 0), (2, 4, 40, 100, 0, 0), (1, 4, 5, 3001, 0, 0), (4, 4, 70, 333, 100, 40)] + \
+    [WIDE[i] for i in (0, 1, 4, 7, 8)]
 
 
 def prefill(c, x, t, heads, past, window=0, sinks=0, observed=0):
