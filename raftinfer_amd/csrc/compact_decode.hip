@@ -65,6 +65,10 @@ __device__ __forceinline__ u32x4 bf16x16_to_fp8(u32x4 lo, u32x4 hi, float inv) {
   }
   return r;
 }
+// Two values cut to bf16.
+__device__ __forceinline__ std::uint32_t cut_bf16x2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(x)), lane)));
 }
@@ -83,7 +87,8 @@ __device__ __forceinline__ u32x4 rescale_fp8x16(u32x4 w, float ratio) {
 // v_mfma_f32_16x16x32_bf16 with the query heads of the group as the 16 columns
 // (those past the group repeat the last): S = K q^T with K rows as loaded, O^T = V^T P^T
 // with V transposed by the LDS read.  Codes become bf16 behind the reads, without loss; the block's
-// K scale multiplies the scores, its V scale the probabilities.
+// K scale multiplies the scores, its V scale the probabilities.  These go into the product in two bf16
+// parts, 16 bits together (one part: an average of equal values was up to a step of bf16 off).
 //
 // The kernel is bound by its cache reads, so a wave (32 8-bit or 16 bf16 rows a
 // step) asks for rows a step ahead: K(t + 1) goes out when S(t) is formed, V(t + 1)
@@ -348,7 +353,9 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
       for (int i = 0; i < kVLoads; ++i)
         if (kVRows * i + lane / kRowLanes == static_cast<int>(r_new)) vr[i] = fresh;
     }
-    std::uint32_t pw[2 * kRB];
+    // In two parts: pw, cut to bf16 below p (1 - 2^-9), and pl, what it leaves.  Neither is 0 or
+    // negative where p is not, so that an infinite value gives that and no NaN.
+    std::uint32_t pw[2 * kRB], pl[2 * kRB];
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
       float e[4];
@@ -358,10 +365,15 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
         l_run += e[i];
         e[i] *= vs;
       }
-      pw[2 * rb] = pack_bf16x2(e[0], e[1]);
-      pw[2 * rb + 1] = pack_bf16x2(e[2], e[3]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = e[2 * i], y = e[2 * i + 1];
+        const std::uint32_t w = cut_bf16x2(fmaf(x, -0x1p-9f, x), fmaf(y, -0x1p-9f, y));
+        pw[2 * rb + i] = w;
+        pl[2 * rb + i] = pack_bf16x2(x - bf16_lo(w), y - bf16_hi(w));
+      }
     }
-    // V rows into LDS as bf16; a key that is not seen gives a row of zeros (its
+    // V rows into LDS as cached; a key that is not seen gives a row of zeros (its
     // probability is 0, and 0 times what an unused row holds may be NaN).
     if (!whole) {
 #pragma unroll
@@ -387,19 +399,27 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
     u32x2 op[kRing];
 #pragma unroll
     for (int db = 0; db < kRing; ++db) op[db] = read_v(db);
+    [[maybe_unused]] bf16x8 before; // 8 bit: the operand of product db - 1, whose second one follows product db
+    const auto second = [&](int db) {
+      if constexpr (Fp8)
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(before, __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]}), acc[db], 0, 0, 0);
+    };
 #pragma unroll
     for (int db = 0; db < 16; ++db) {
       const u32x2 w = op[db % kRing];
       if constexpr (Fp8) {
-        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1])),
-                                                          __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
-      } else {
-        acc[db] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
-            __builtin_bit_cast(prefill::short4v, w), __builtin_bit_cast(prefill::short4v, u32x2{pw[0], pw[1]}), acc[db], 0, 0, 0);
+        const bf16x8 v = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1]));
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
+        if (db > 0) second(db - 1);
+        before = v;
+      } else { // 16 keys: both parts in one product
+        acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[0], w[1]}),
+                                                          __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pl[0], pl[1]}), acc[db], 0, 0, 0);
       }
       if (db + kRing < 16) op[db % kRing] = read_v(db + kRing);
       __builtin_amdgcn_sched_barrier(0);
     }
+    second(15);
   };
   for (; it + WAVES < it_end; it += WAVES) step.template operator()<true>();
   if (it < it_end) step.template operator()<false>();

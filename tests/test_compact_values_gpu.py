@@ -24,6 +24,15 @@ def prefill(c, x, t, heads, past, window=0, sinks=0, observed=0):
     return out, w
 
 
+def decode(c, x, heads, past, window=0, sinks=0, weigh=False):
+    shape = c.shape(1, heads, past, window_tokens=window, sink_tokens=sinks, observed_tokens=int(weigh))
+    ws = torch.full((ops.qwen35_compact_decode_workspace_bytes(shape),), 0xFF, device="cuda", dtype=torch.uint8)
+    out = torch.empty(1, heads, D, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(c.hkv, c.cap, device="cuda") if weigh else None
+    ops.qwen35_compact_attention_decode(*x, out, c.buf, shape, ops.DTYPE_BF16, c.dtype, c.layout, ws, key_weights=w)
+    return out, w
+
+
 # ------------------------------------------------------------------ an average of equal values is that value
 
 ALIKE = 1.875  # a bf16 and an e4m3 number; its neighbours in bf16 are 2^-7 away
@@ -69,6 +78,23 @@ def test_prefill_of_equal_values(gpu, dtype, observed, hkv, group, t, past, wind
         assert np.abs(total / group - 1).max() < (past + t + 64) * 2.0 ** -23
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("n,window", [(1, 0), (17, 0), (300, 0), (301, 100), (700, 0), (4001, 0), (4001, 2100)])
+def test_decode_of_equal_values(gpu, dtype, weigh, n, window):
+    hkv, group = 2, 8
+    k, v = alike(hkv, n)
+    c = Cache(rng(2), dtype, 1, hkv, n)
+    if n > 1:
+        c.store(0, k[:-1], v[:-1])
+    q, g = queries(1, hkv * group)
+    out, w = decode(c, (q, dev(k[-1:]), dev(v[-1:]), g), hkv * group, n - 1, window, 0, weigh)
+    assert (host(out) == ALIKE).all()
+    if weigh:
+        total = host(w).astype(np.float64).sum(1)
+        assert np.abs(total / group - 1).max() < (n + 64) * 2.0 ** -23
+
+
 # ------------------------------------------------------------------ key weights change no output
 
 @pytest.mark.parametrize("dtype", [BF16, FP8])
@@ -83,3 +109,33 @@ def test_prefill_with_weights_gives_the_same_output(gpu, dtype, hkv, group, t, p
     c.buf.copy_(start)
     weighed, _ = prefill(c, x, t, heads, past, window, sinks, observed=min(t, 3))
     assert torch.equal(plain, weighed)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("n,window", [(1, 0), (300, 0), (4001, 0), (4001, 2100)])
+def test_decode_with_weights_gives_the_same_output(gpu, dtype, n, window):
+    r = rng(4)
+    hkv, heads = 2, 16
+    c = filled(r, dtype, 1, hkv, n, n - 1)
+    x = dev(normal(r, 1, heads, D)), dev(rows(r, 1, hkv)), dev(rows(r, 1, hkv)), dev(normal(r, 1, heads, D))
+    start = c.buf.clone()
+    plain, _ = decode(c, x, heads, n - 1, window)
+    c.buf.copy_(start)
+    weighed, _ = decode(c, x, heads, n - 1, window, weigh=True)
+    assert torch.equal(plain, weighed)
+
+
+@pytest.mark.parametrize("what", [np.inf, -np.inf])
+@pytest.mark.parametrize("n,at,k_size", [(1, 0, 1), (40, 3, 0), (40, 39, 1), (700, 500, 1), (4001, 17, 0)])
+def test_decode_of_infinite_values(gpu, what, n, at, k_size):
+    """A seen value of infinity gives infinity, also to keys whose probability is the largest (equal keys: all are)."""
+    r = rng(5)
+    hkv, heads = 2, 16
+    k, v = bf16(normal(r, n, hkv, D) * k_size), rows(r, n, hkv)
+    v[at, :, 5] = what
+    c = Cache(r, BF16, 1, hkv, n)
+    if n > 1:
+        c.store(0, k[:-1], v[:-1])
+    out, _ = decode(c, (dev(normal(r, 1, heads, D)), dev(k[-1:]), dev(v[-1:]), dev(normal(r, 1, heads, D))), heads, n - 1)
+    got = host(out)
+    assert (got[..., 5] == what).all() and np.isfinite(np.delete(got, 5, -1)).all()
