@@ -17,11 +17,12 @@
 // of e4m3 codes, then the scales, float [2][kv_heads][ceil(max_context_tokens /
 // 32)] in either layout.  A scale belongs to the 32 positions 32 b .. 32 b + 31 of
 // one plane and head.  It is the smallest power of two s with which every finite
-// value that was stored is at most 448 s, and a code stands for code * s.  A row
-// that needs a larger scale than its block has raises it, and the block's earlier
-// rows are rounded to the new one (exact but for codes that become subnormal).
-// Infinite and NaN values are stored as NaN.  A block's scale starts anew with
-// its first position, so a buffer needs no clearing between sequences.
+// value that was stored is at most 448 s, and a code stands for code * s; under the
+// largest scale, 2^120, codes end at 240, since 256 would stand for 2^128, which is
+// no f32.  A row that needs a larger scale than its block has raises it, and the
+// block's earlier rows are rounded to the new one (exact but for codes that become
+// subnormal).  Infinite and NaN values are stored as NaN.  A block's scale starts
+// anew with its first position, so a buffer needs no clearing between sequences.
 #pragma once
 
 #include "qwen35_attention.hpp"

@@ -88,6 +88,10 @@ __global__ __launch_bounds__(kStoreThreads) void compact_store_fp8_kernel(Compac
   if (threadIdx.x == 0) *scale = after;
   u32x4 out[2];
   if (fresh) {
+    if (after == kCompactTopScale) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = compact_below_top(x[e]);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       out[j >> 2][j & 3] = pack_fp8x4(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);

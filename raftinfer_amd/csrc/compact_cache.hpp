@@ -81,12 +81,20 @@ __device__ __forceinline__ float compact_scale(float amax) {
 __device__ __forceinline__ float compact_inverse(float s) {
   return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
 }
+// Under the largest scale, 2^120, codes end at 240: the next one, 256, would stand for 2^128,
+// which neither f32 nor bf16 holds.  (Finite values reach 255 / 128 2^127.)
+constexpr float kCompactTopScale = 0x1p120f;
+__device__ __forceinline__ float compact_below_top(float x) {
+  constexpr float kMost = 240 * kCompactTopScale;
+  return x > kMost ? kMost : x < -kMost ? -kMost : x; // (NaN stays)
+}
 // Four values, already divided by their scale, as e4m3 codes (nearest even).
 __device__ __forceinline__ std::uint32_t pack_fp8x4(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return static_cast<std::uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
 }
-// Eight codes as bf16 (exact: 4 significant bits, exponents -9 .. 8).
+// Eight codes as bf16 (exact: 4 significant bits, exponents -9 .. 8; times a scale, too, but for
+// what lies below 2^-126).
 __device__ __forceinline__ u32x4 fp8x8_to_bf16(std::uint32_t lo, std::uint32_t hi) {
   typedef __bf16 pair __attribute__((ext_vector_type(2)));
   const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);

@@ -54,14 +54,17 @@ __device__ __forceinline__ float max_finite_bf16x8(u32x4 w, float m) {
   return m;
 }
 __device__ __forceinline__ float finite_or_nan(float x) { return is_finite_f32(x) ? x : __builtin_nanf(""); }
-// Sixteen bf16 values as codes of scale 1 / inv.
-__device__ __forceinline__ u32x4 bf16x16_to_fp8(u32x4 lo, u32x4 hi, float inv) {
+// Sixteen bf16 values as codes of scale 1 / inv (Top: which may be the largest).
+template <bool Top> __device__ __forceinline__ u32x4 bf16x16_to_fp8(u32x4 lo, u32x4 hi, float inv) {
+  const auto part = [&](float x) {
+    const float f = finite_or_nan(x);
+    return (Top && inv == 1.0f / kCompactTopScale ? compact_below_top(f) : f) * inv;
+  };
   u32x4 r;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const std::uint32_t x = e < 2 ? lo[2 * e] : hi[2 * e - 4], y = e < 2 ? lo[2 * e + 1] : hi[2 * e - 3];
-    r[e] = pack_fp8x4(finite_or_nan(bf16_lo(x)) * inv, finite_or_nan(bf16_hi(x)) * inv,
-                      finite_or_nan(bf16_lo(y)) * inv, finite_or_nan(bf16_hi(y)) * inv);
+    r[e] = pack_fp8x4(part(bf16_lo(x)), part(bf16_hi(x)), part(bf16_lo(y)), part(bf16_hi(y)));
   }
   return r;
 }
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
       const float amax = row16_max(max_finite_bf16x8(hi, max_finite_bf16x8(lo, 0.f)));
       const float after = fmaxf(before, compact_scale(amax));
       const float inv = compact_inverse(after);
-      const u32x4 codes = bf16x16_to_fp8(lo, hi, inv);
+      u32x4 codes = bf16x16_to_fp8<false>(lo, hi, inv);
+      if (__builtin_amdgcn_ballot_w64(after == kCompactTopScale) != 0) codes = bf16x16_to_fp8<true>(lo, hi, inv);
       const float grow = before != 0.f && after != before ? before * inv : 0.f;
       if (lane < 32) {
         *reinterpret_cast<u32x4 *>(dst + 16 * piece) = codes;

@@ -397,6 +397,10 @@ __global__ __launch_bounds__(kMoveThreads) void compact_move_kernel(CompactEvict
     const float inv = compact_inverse(scale);
     if (threadIdx.x == 0) (plane ? dst.vs : dst.ks)[block] = scale;
     if (!real) return;
+    if (scale == kCompactTopScale) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = compact_below_top(x[e]);
+    }
     u32x4 out[2];
 #pragma unroll
     for (int j = 0; j < 8; ++j)

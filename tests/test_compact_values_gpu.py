@@ -4,9 +4,10 @@ import numpy as np
 import pytest
 import torch
 
+import compact_reference as ref
 from helpers import bf16, normal, rng
 from raftinfer_amd import ops
-from test_compact_gpu import BF16, D, FP8, WIDE, Cache, dev, filled, host, rows
+from test_compact_gpu import BF16, D, FP8, WIDE, Cache, dev, filled, host, near, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +140,85 @@ def test_decode_of_infinite_values(gpu, what, n, at, k_size):
     out, _ = decode(c, (dev(normal(r, 1, heads, D)), dev(k[-1:]), dev(v[-1:]), dev(normal(r, 1, heads, D))), heads, n - 1)
     got = host(out)
     assert (got[..., 5] == what).all() and np.isfinite(np.delete(got, 5, -1)).all()
+
+
+# ------------------------------------------------------------------ values up to the largest
+
+MOST = 255 * 2.0 ** 120  # of bf16
+TOP = 240 * 2.0 ** 120   # of an 8-bit cache: the next code would stand for 2^128
+
+
+def below_top(x, dtype):
+    return np.where(np.isfinite(x), np.clip(x, -TOP, TOP), x) if dtype == FP8 else x
+
+
+def append(c, past, k, v):
+    ops.qwen35_compact_cache_append(dev(k), dev(v), c.buf, c.shape(len(k), c.hkv, past), ops.DTYPE_BF16, c.dtype, c.layout)
+    c.want_store(past, below_top(k, c.dtype), below_top(v, c.dtype))
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+def test_store_of_the_largest_values(gpu, layout):
+    r = rng(6)
+    c = Cache(r, FP8, layout, 2, 100)
+    k, v = rows(r, 70, 2), rows(r, 70, 2)
+    k[3, 0, :4] = [MOST, -MOST, TOP, 248 * 2.0 ** 120]
+    k[4, 0, :2] = [np.inf, np.nan]
+    k[5, 1, 7] = 224 * 2.0 ** 120       # under the same scale, and no code above 224
+    v[40, 1, 9] = -249 * 2.0 ** 120
+    v[41, 0, 3] = 2.0 ** 126            # a scale below the largest
+    append(c, 0, k[:35], v[:35])
+    c.check("first")
+    append(c, 35, k[35:], v[35:])
+    c.check("second")
+    held = c.held(70)
+    assert np.nanmax(np.abs(held)) == TOP
+
+
+def largest(r, t, past, hkv, heads, v_at, k_at):
+    """A value of the largest size at the keys v_at, whose scores lie 2^7 above those of the keys before; a largest number
+    at the keys k_at, in a dim that no query looks at."""
+    n = past + t
+    k, v = bf16(normal(r, n, hkv, D) / 64), rows(r, n, hkv)
+    q = np.zeros((t, heads, D), np.float32)
+    q[..., 0] = 4
+    k[v_at, :, 0] = 19.5   # 19.5 * 4 / 16 / ln 2 = 7.03
+    v[v_at, :, 5], v[v_at, :, 6] = MOST, -MOST
+    k[k_at, :, 9] = MOST
+    return q, k, v, bf16(normal(r, t, heads, D))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("n,at", [(1, 0), (40, 39), (40, 7), (700, 500), (4001, 4000), (4001, 300)])
+def test_decode_of_the_largest_values(gpu, dtype, n, at):
+    r = rng(8)
+    hkv, heads = 2, 16
+    q, k, v, g = largest(r, 1, n - 1, hkv, heads, [at], [n // 7])
+    c = Cache(r, dtype, 1, hkv, n)
+    if n > 1:
+        append(c, 0, k[:-1], v[:-1])
+    out, _ = decode(c, (dev(q), dev(k[-1:]), dev(v[-1:]), dev(g)), heads, n - 1)
+    c.want_store(n - 1, below_top(k[-1:], dtype), below_top(v[-1:], dtype))
+    c.check()
+    want, bound, _, _ = ref.attention(q, g, c.held(n), n - 1)
+    near(host(out), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+def test_evict_of_the_largest_values(gpu, dtype):
+    r = rng(9)
+    hkv, n, keep = 2, 200, 90
+    k, v = rows(r, n, hkv), rows(r, n, hkv)
+    k[50, 0, 3], v[51, 1, 4] = MOST, -MOST
+    c, out = Cache(r, dtype, 1, hkv, n), Cache(r, FP8, 1, hkv, keep)
+    append(c, 0, k, v)
+    w = np.zeros((hkv, n), np.float32)
+    w[:, 30:120] = 1
+    out_w, kept = torch.empty(hkv, keep, device="cuda"), torch.empty(hkv, keep, device="cuda", dtype=torch.int32)
+    ops.qwen35_compact_cache_evict(c.buf, dev(w, torch.float32), out.buf, out_w, kept,
+                                   ops.Qwen35EvictShape(hkv, D, n, n, keep, keep), dtype, FP8, 1)
+    assert (kept.cpu().numpy() == np.arange(30, 120)).all()
+    held = below_top(c.held(n)[:, :, 30:120], FP8)
+    out.ref.store(0, held[0].transpose(1, 0, 2), held[1].transpose(1, 0, 2))
+    out.check()
+    assert np.nanmax(np.abs(out.held(keep))) == TOP
