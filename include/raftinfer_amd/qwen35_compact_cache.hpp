@@ -91,7 +91,10 @@ void qwen35_compact_cache_append(const void *key, const void *value, void *kv_ca
 // over the cache: softmax(q k / 16) over the keys that the token sees.  query,
 // gate, output: [tokens][query_heads][256] bf16.  key_weights: float
 // [kv_heads][max_context_tokens], to which each seen key's probabilities are
-// added, over the observed tokens and the head's group of query heads.
+// added, over the observed tokens and the head's group of query heads.  Before
+// the division by the softmax's sum the values are summed in f32 with
+// probabilities of at most 1: finite where |probability * value| over a token's
+// keys sums to less than 2^128.
 void qwen35_compact_attention_prefill(const void *query, const void *key, const void *value,
                                       const void *gate, void *output, void *kv_cache,
                                       std::size_t kv_cache_bytes, float *key_weights, void *workspace,

@@ -357,16 +357,16 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
     for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
     mx = max_xor32(mx) * kScale;
-    // The accumulators are scaled only where a max grows by more than 2^8, which
-    // the probabilities can exceed 1 by.
-    const bool grow = mx > m_run + kLazyRescale;
+    // m_run lies 2^8 above the max that it was last set to, and the accumulators are scaled
+    // only where a max grows past it: no probability exceeds 1.
+    const bool grow = mx > m_run;
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-      const float f = grow ? fexp2(m_run - mx) : 1.0f;
+      const float m_new = mx + kLazyRescale, f = grow ? fexp2(m_run - m_new) : 1.0f;
       l_run *= f;
       if constexpr (Weigh) lw_run *= f;
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) o[nb] *= f;
-      m_run = grow ? mx : m_run;
+      m_run = grow ? m_new : m_run;
     }
     // k-slot (kb, kh, e) of V^T P^T <-> key 16 kb + 8 (e / 4) + 4 kh + e % 4, the order of s.
     bf16x8 pb[2];
@@ -699,8 +699,9 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
           for (int i = 0; i < 4; ++i)
             s[cb][rb][i] = compact_sees(j0 + 16 * rb + 4 * kq + i, pos[cb], a.window, a.sinks) ? s[cb][rb][i] : -INFINITY;
     }
-    // The accumulators are scaled only where a max grows by more than 2^8, which the
-    // probabilities can exceed 1 by.
+    // m_run lies 2^8 above the max that it was last set to, and the accumulators are scaled
+    // only where a max grows past it.  (Not at the max itself, which the probabilities could exceed by
+    // 2^8: times the largest values that is no f32.)
     float mx[2];
     bool grow = false;
 #pragma unroll
@@ -709,12 +710,12 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
 #pragma unroll
       for (int i = 1; i < 4; ++i) x = fmaxf(fmaxf(x, s[cb][0][i]), s[cb][1][i]);
       mx[cb] = max_xor32(max_xor16(x)) * k_scale;
-      grow |= mx[cb] > m_run[cb] + kLazyRescale;
+      grow |= mx[cb] > m_run[cb];
     }
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) {
-        const float m_new = fmaxf(m_run[cb], mx[cb]), f = fexp2(m_run[cb] - m_new);
+        const float m_new = mx[cb] > m_run[cb] ? mx[cb] + kLazyRescale : m_run[cb], f = fexp2(m_run[cb] - m_new);
         l_run[cb] *= f;
         if constexpr (Weigh) lw_run[cb] *= f;
 #pragma unroll

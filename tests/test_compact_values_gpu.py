@@ -189,6 +189,25 @@ def largest(r, t, past, hkv, heads, v_at, k_at):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", SHAPES[1:])
+def test_prefill_of_the_largest_values(gpu, dtype, hkv, group, t, past, window, sinks):
+    r = rng(7)
+    heads, n = hkv * group, past + t
+    q, k, v, g = largest(r, t, past, hkv, heads, [past + t // 2], [n // 7])
+    c = Cache(r, dtype, 1, hkv, n)
+    if past:
+        append(c, 0, k[:past], v[:past])
+    out, _ = prefill(c, (dev(q), dev(k[past:]), dev(v[past:]), dev(g)), t, heads, past, window, sinks)
+    c.want_store(past, below_top(k[past:], dtype), below_top(v[past:], dtype))
+    c.check()
+    got = host(out)
+    assert np.isfinite(got).all()
+    for i in sorted({0, t // 2 - 1, t // 2, t // 2 + 1, t - 2, t - 1} & set(range(t))):
+        want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], c.held(past + i + 1), past + i, window, sinks)
+        near(got[i:i + 1], want, bound, f"token {i}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
 @pytest.mark.parametrize("n,at", [(1, 0), (40, 39), (40, 7), (700, 500), (4001, 4000), (4001, 300)])
 def test_decode_of_the_largest_values(gpu, dtype, n, at):
     r = rng(8)
