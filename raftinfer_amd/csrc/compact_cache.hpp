@@ -93,14 +93,13 @@ __device__ __forceinline__ std::uint32_t pack_fp8x4(float a, float b, float c, f
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return static_cast<std::uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
 }
-// Eight codes as bf16 (exact: 4 significant bits, exponents -9 .. 8; times a scale, too, but for
-// what lies below 2^-126).
-__device__ __forceinline__ u32x4 fp8x8_to_bf16(std::uint32_t lo, std::uint32_t hi) {
+// Eight codes times a scale as bf16 (exact: 4 significant bits; but for what lies below 2^-126).
+__device__ __forceinline__ u32x4 fp8x8_to_bf16(std::uint32_t lo, std::uint32_t hi, float scale = 1.0f) {
   typedef __bf16 pair __attribute__((ext_vector_type(2)));
-  const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
-  const pair b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-  const pair c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
-  const pair d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const pair b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const pair c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const pair d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
   return u32x4{__builtin_bit_cast(std::uint32_t, a), __builtin_bit_cast(std::uint32_t, b),
                __builtin_bit_cast(std::uint32_t, c), __builtin_bit_cast(std::uint32_t, d)};
 }

@@ -90,8 +90,9 @@ __device__ __forceinline__ u32x4 rescale_fp8x16(u32x4 w, float ratio) {
 // v_mfma_f32_16x16x32_bf16 with the query heads of the group as the 16 columns
 // (those past the group repeat the last): S = K q^T with K rows as loaded, O^T = V^T P^T
 // with V transposed by the LDS read.  Codes become bf16 behind the reads, without loss; the block's
-// K scale multiplies the scores, its V scale the probabilities.  These go into the product in two bf16
-// parts, 16 bits together (one part: an average of equal values was up to a step of bf16 off).
+// K scale multiplies the scores, its V scale V's operands (a probability times the least scales is no
+// normal number).  Probabilities go into the product in two bf16 parts, 16 bits together (one part:
+// an average of equal values was up to a step of bf16 off).
 //
 // The kernel is bound by its cache reads, so a wave (32 8-bit or 16 bf16 rows a
 // step) asks for rows a step ahead: K(t + 1) goes out when S(t) is formed, V(t + 1)
@@ -367,7 +368,6 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
       for (int i = 0; i < 4; ++i) {
         e[i] = fexp2(s[rb][i] - m_run);
         l_run += e[i];
-        e[i] *= vs;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -386,10 +386,12 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
         vr[i] &= u32x4{keep, keep, keep, keep};
       }
     }
+    if constexpr (Fp8) asm volatile("" : "+v"(vs)); // (one wait for all of V: 60001 tokens 25.6 -> 25.2 us)
     wave_lds_order();
 #pragma unroll
     for (int i = 0; i < kVLoads; ++i) // (v_key is linear in the bits of the row)
       *reinterpret_cast<u32x4 *>(&sh.v[wave][(v_put ^ (16 * v_key<Fp8>(kVRows * i))) + kVBytes * kVRows * i]) = vr[i];
+    [[maybe_unused]] const float v_scale = lane_value(vs, 0);
     if constexpr (kMore) load_v(first_key(it + WAVES));
     __builtin_amdgcn_sched_barrier(0);
     wave_lds_order();
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void compact_decode_kernel
     for (int db = 0; db < 16; ++db) {
       const u32x2 w = op[db % kRing];
       if constexpr (Fp8) {
-        const bf16x8 v = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1]));
+        const bf16x8 v = __builtin_bit_cast(bf16x8, fp8x8_to_bf16(w[0], w[1], v_scale));
         acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]}), acc[db], 0, 0, 0);
         if (db > 0) second(db - 1);
         before = v;

@@ -146,15 +146,6 @@ __device__ __forceinline__ void add_odd_values(const CompactHead<Fp8> &c, const 
     }
   }
 }
-__device__ __forceinline__ u32x4 fp8x8_to_bf16_scaled(std::uint32_t lo, std::uint32_t hi, float scale) {
-  typedef __bf16 pair __attribute__((ext_vector_type(2)));
-  const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-  const pair b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-  const pair c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-  const pair d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-  return u32x4{__builtin_bit_cast(std::uint32_t, a), __builtin_bit_cast(std::uint32_t, b),
-               __builtin_bit_cast(std::uint32_t, c), __builtin_bit_cast(std::uint32_t, d)};
-}
 
 // A workgroup takes 128 columns (column = token * group + head) of one KV head and a
 // contiguous range of the 32-key tiles that they see; a wave takes 32 columns.  The
@@ -271,7 +262,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       const int at = (l & 31) ^ row_key(8 * wave + (l >> 5));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u32x4 x = fp8x8_to_bf16_scaled(raw[i][0], raw[i][1], scale);
+        u32x4 x = fp8x8_to_bf16(raw[i][0], raw[i][1], scale);
         if (clean) odd |= __builtin_amdgcn_ballot_w64(without_odd(x));
         *reinterpret_cast<u32x4 *>(tile + (8 * wave + 2 * i + (l >> 5)) * kHeadDim + 8 * (at ^ (8 * (i & 1) + (i >> 1)))) = x;
       }

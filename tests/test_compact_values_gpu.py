@@ -241,3 +241,22 @@ def test_evict_of_the_largest_values(gpu, dtype):
     out.ref.store(0, held[0].transpose(1, 0, 2), held[1].transpose(1, 0, 2))
     out.check()
     assert np.nanmax(np.abs(out.held(keep))) == TOP
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("call,n", [("decode", 40), ("decode", 700), ("decode", 4001), ("few", 200), ("many", 700)])
+def test_small_values(gpu, dtype, call, n):
+    """Values of 1e-36, under the least scale of an 8-bit cache."""
+    r = rng(10)
+    hkv, heads, t = (16, 256, 130) if call == "many" else (2, 16, 1 if call == "decode" else 30)
+    k, v = rows(r, n, hkv), bf16(rows(r, n, hkv, heavy=False) * 1e-36)
+    q, g = bf16(normal(r, t, heads, D)), bf16(normal(r, t, heads, D))
+    c = Cache(r, dtype, 1, hkv, n)
+    c.store(0, k[:n - t], v[:n - t])
+    x = dev(q), dev(k[n - t:]), dev(v[n - t:]), dev(g)
+    out, _ = decode(c, x, heads, n - 1) if call == "decode" else prefill(c, x, t, heads, n - t)
+    c.want_store(n - t, k[n - t:], v[n - t:])
+    for i in sorted({0, t // 2, t - 1}):
+        want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], c.held(n - t + i + 1), n - t + i)
+        # (a code below 2^-6 and a product or result below 2^-126 may be rounded to a multiple of 2^-133)
+        near(host(out)[i:i + 1], want, bound + 2.0 ** -132, f"token {i}")
