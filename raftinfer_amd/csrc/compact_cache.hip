@@ -229,15 +229,22 @@ void validate_apart(std::initializer_list<Bytes> written, std::initializer_list<
     for (const Bytes &r : read) require<Err>(apart(*w, r), message);
   }
 }
+Bytes lengths_of(const Qwen35CompactShape &s, const std::uint32_t *lengths) {
+  return {lengths, lengths != nullptr ? s.sequences * sizeof(std::uint32_t) : 0};
+}
+void validate_lengths(const std::uint32_t *lengths) {
+  require<Err>((reinterpret_cast<std::uintptr_t>(lengths) & 3u) == 0, "compact attention context_lengths must be 4-byte aligned");
+}
 // Checked last: everything else about the call is valid.
 void validate_overlap(const Qwen35CompactShape &s, const void *q, const void *k, const void *v, const void *g,
-                      const void *output, const void *cache, std::size_t cache_bytes, const float *weights,
-                      const void *workspace, std::size_t workspace_bytes) {
+                      const void *output, const void *cache, std::size_t cache_bytes, const std::uint32_t *lengths,
+                      const float *weights, const void *workspace, std::size_t workspace_bytes) {
   const std::size_t tokens = s.sequences * s.tokens;
   const std::size_t heads = tokens * s.query_heads * kHeadDim * 2, rows = tokens * s.kv_heads * kHeadDim * 2;
   const std::size_t weight_bytes = weights != nullptr ? s.sequences * s.kv_heads * s.max_context_tokens * sizeof(float) : 0;
   validate_apart({{output, heads}, {cache, cache_bytes}, {weights, weight_bytes}, {workspace, workspace_bytes}},
-                 {{q, heads}, {k, rows}, {v, rows}, {g, heads}}, "compact attention outputs overlap other arguments");
+                 {{q, heads}, {k, rows}, {v, rows}, {g, heads}, lengths_of(s, lengths)},
+                 "compact attention outputs overlap other arguments");
 }
 
 std::size_t validate_cache(const Qwen35CompactShape &s, Qwen35CompactCacheDType dtype, const void *cache,
@@ -342,7 +349,9 @@ void qwen35_compact_cache_append(const void *key, const void *value, void *kv_ca
   const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
   require<Err>(aligned16(key) && aligned16(value), "compact attention inputs and output must be 16-byte aligned");
   const std::size_t rows = shape.sequences * shape.tokens * shape.kv_heads * kHeadDim * 2;
-  validate_apart({{kv_cache, used}}, {{key, rows}, {value, rows}}, "compact cache overlaps the rows to be stored");
+  validate_lengths(context_lengths);
+  validate_apart({{kv_cache, used}}, {{key, rows}, {value, rows}, lengths_of(shape, context_lengths)},
+                 "compact cache overlaps the rows to be stored or their lengths");
   CompactArgs a = to_args(shape);
   fill_pointers(a, nullptr, key, value, nullptr, nullptr, kv_cache, layout);
   a.lengths = context_lengths;
@@ -362,7 +371,7 @@ void qwen35_compact_attention_prefill(const void *query, const void *key, const 
   validate_call(query, key, value, gate, output, key_weights, workspace, workspace_bytes, need, shape, act, layout,
                 stream);
   const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
-  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, key_weights, workspace, need);
+  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, nullptr, key_weights, workspace, need);
   CompactArgs a = to_args(shape);
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;
@@ -383,7 +392,8 @@ void qwen35_compact_attention_decode(const void *query, const void *key, const v
   validate_call(query, key, value, gate, output, key_weights, workspace, workspace_bytes, need, shape, act, layout,
                 stream);
   const std::size_t used = validate_cache(shape, cache_dtype, kv_cache, kv_cache_bytes);
-  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, key_weights, workspace, need);
+  validate_lengths(context_lengths);
+  validate_overlap(shape, query, key, value, gate, output, kv_cache, used, context_lengths, key_weights, workspace, need);
   CompactArgs a = to_args(shape);
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;

@@ -206,3 +206,35 @@ def test_evict_refuses_too_many_segments():
     with pytest.raises(ops.Qwen35PrimitiveError, match="at most 65535"):
         ops.qwen35_compact_evict_workspace_bytes(shape)
     assert ops.qwen35_compact_evict_workspace_bytes(dataclasses.replace(shape, context_tokens=65535 * 4096)) > 0
+
+
+@pytest.mark.parametrize("written", [4, 5, 6, 7])   # output, cache, workspace, key weights
+def test_decode_refuses_lengths_that_it_would_write(written):
+    """The lengths are read again after the cache, the workspace and the outputs are written."""
+    shape = dataclasses.replace(MODEL, observed_tokens=1, sequences=3, cache_stride_bytes=ops.qwen35_compact_cache_bytes(MODEL, FP8))
+    need = ops.qwen35_compact_decode_workspace_bytes(shape)
+    head, row = 3 * 16 * 512, 3 * 4 * 512
+    sizes = [head, row, row, head, head, 3 * shape.cache_stride_bytes, need, 3 * 4 * 4096 * 4, 3 * 4]
+    for by in (12, 4):   # the whole of the lengths, and the first of them
+        t = places(sizes, (8, written, by))
+        with pytest.raises(ops.Qwen35PrimitiveError, match="outputs overlap other arguments"):
+            ops.qwen35_compact_attention_decode(*t[:6], shape, ops.DTYPE_BF16, FP8, 1, t[6], key_weights=t[7], context_lengths=t[8],
+                                                stream=0x1234)
+
+
+def test_append_refuses_lengths_that_it_would_write():
+    row, cache = 4 * 512, ops.qwen35_compact_cache_bytes(MODEL, FP8)
+    for by in (4, cache):   # the cache's last bytes, and its first
+        t = places([row, row, cache, 4], (3, 2, by))
+        with pytest.raises(ops.Qwen35PrimitiveError, match="overlaps the rows"):
+            ops.qwen35_compact_cache_append(*t[:3], MODEL, ops.DTYPE_BF16, FP8, 1, context_lengths=t[3], stream=0x1234)
+
+
+def test_refuses_lengths_that_are_not_aligned():
+    bad = FakeTensor(4, (1 << 60) + 2)
+    t = places([16 * 512, 4 * 512, 4 * 512, 16 * 512, 16 * 512, ops.qwen35_compact_cache_bytes(MODEL, FP8),
+                ops.qwen35_compact_decode_workspace_bytes(MODEL)])
+    with pytest.raises(ops.Qwen35PrimitiveError, match="context_lengths must be 4-byte aligned"):
+        ops.qwen35_compact_attention_decode(*t[:6], MODEL, ops.DTYPE_BF16, FP8, 1, t[6], context_lengths=bad, stream=0x1234)
+    with pytest.raises(ops.Qwen35PrimitiveError, match="context_lengths must be 4-byte aligned"):
+        ops.qwen35_compact_cache_append(*t[1:3], t[5], MODEL, ops.DTYPE_BF16, FP8, 1, context_lengths=bad, stream=0x1234)
