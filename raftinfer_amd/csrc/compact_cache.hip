@@ -136,7 +136,11 @@ using namespace raftinfer::amd;
 using Err = Qwen35PrimitiveError;
 
 // Positions, rows and columns are 32-bit in the kernels, and a grid holds fewer than
-// 2^32 threads in x and 2^16 workgroups in y and z.
+// 2^32 threads in x and 2^16 workgroups in y and z.  At these limits the threads in x are:
+// stores 2^26 rows * 32, or 2^26 / 32 blocks * 256; decode 2^17 units * 64 partitions * 256; its merge (2^31 /
+// 512 + 2^15 pieces of weights + 2^19 heads) * 512; prefill 2^26 / 128 + 2^15 column blocks * 256 (few
+// enough are cut that the merge of their columns, a wave or a workgroup each, is below 2^24); key weights 2^22 tiles * 512
+// (kWeighGrid; a launch more for others); eviction 2^15 heads * 1024 and 2^28 / 32 blocks * 256.
 constexpr std::size_t kMaxPositions = std::size_t{1} << 28;
 constexpr std::size_t kMaxHeadPositions = std::size_t{1} << 31; // over all KV heads
 constexpr std::size_t kMaxQueryRows = std::size_t{1} << 26;

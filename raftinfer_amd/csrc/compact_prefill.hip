@@ -970,8 +970,10 @@ __global__ __launch_bounds__(kPThreads) void compact_prefill_merge_kernel(Compac
 // nothing is added twice or in a changing order.  64 tokens over 2001 keys: 10.6 us, round
 // trips (q and the sums, K, the weights) and a wave's chain of products; 11.7 with 4 waves.
 constexpr int kWeighWaves = 8;
+constexpr std::uint32_t kWeighGrid = 1u << 22; // tiles of a launch: fewer than 2^32 threads in x
 template <bool Fp8>
-__global__ __launch_bounds__(kWeighWaves *kWave, 1) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc) {
+__global__ __launch_bounds__(kWeighWaves *kWave, 1) void compact_prefill_weigh_kernel(CompactArgs a, PrefillScratch sc,
+                                                                                           std::uint32_t before) {
   __shared__ float sum[kWeighWaves][kCompactBlock];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -979,7 +981,7 @@ __global__ __launch_bounds__(kWeighWaves *kWave, 1) void compact_prefill_weigh_k
   const std::uint32_t kvh = blockIdx.y;
   const std::uint32_t last = a.past + a.tokens - 1;
   const SeenTiles seen(a.past + a.tokens - a.observed, last, a.window, a.sinks);
-  const std::uint32_t tile = seen.tile(blockIdx.x), j0 = tile * kCompactBlock;
+  const std::uint32_t tile = seen.tile(before + blockIdx.x), j0 = tile * kCompactBlock;
   const CompactHead<Fp8> c(a.cache, kvh, a.kv_heads, a.max_ctx, a.head_major);
   float k_scale = kLog2e / 16.0f;
   if constexpr (Fp8) k_scale *= c.ks[tile];
@@ -1157,7 +1159,8 @@ template <bool Fp8> void launch_prefill(const CompactArgs &a, void *workspace, h
   const std::uint32_t last = a.past + a.tokens - 1;
   if (a.weights != nullptr) {
     const SeenTiles seen(last + 1 - a.observed, last, a.window, a.sinks);
-    compact_prefill_weigh_kernel<Fp8><<<dim3{seen.total, a.kv_heads}, kWeighWaves * kWave, 0, stream>>>(a, sc);
+    for (std::uint32_t before = 0; before < seen.total; before += kWeighGrid)
+      compact_prefill_weigh_kernel<Fp8><<<dim3{std::min(seen.total - before, kWeighGrid), a.kv_heads}, kWeighWaves * kWave, 0, stream>>>(a, sc, before);
   }
 }
 

@@ -260,3 +260,31 @@ def test_small_values(gpu, dtype, call, n):
         want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], c.held(n - t + i + 1), n - t + i)
         # (a code below 2^-6 and a product or result below 2^-126 may be rounded to a multiple of 2^-133)
         near(host(out)[i:i + 1], want, bound + 2.0 ** -132, f"token {i}")
+
+
+# ------------------------------------------------------------------ the largest cache
+
+def test_the_largest_cache(gpu):
+    """2^28 positions of equal keys and values, full: every weight is 2^-28 and the output the value.  (Sums of equal powers
+    of two are exact.)"""
+    cap = 1 << 28
+    torch.cuda.empty_cache()
+    shape = ops.Qwen35CompactShape(1, 1, 1, 1, D, cap, cap - 1, observed_tokens=1)
+    size = ops.qwen35_compact_cache_bytes(shape, FP8)
+    if torch.cuda.mem_get_info()[0] < size + (8 << 30):
+        pytest.skip(f"needs {size >> 30} GiB of GPU memory")
+    buf = torch.full((size,), 0x38, device="cuda", dtype=torch.uint8)   # the code of 1
+    buf[2 * cap * D:].view(torch.float32).fill_(1)
+    q, one = (torch.full((1, 1, D), x, device="cuda", dtype=torch.bfloat16) for x in (0, 1))
+    gate = torch.full((1, 1, D), 200, device="cuda", dtype=torch.bfloat16)
+    for call, need in ((ops.qwen35_compact_attention_prefill, ops.qwen35_compact_prefill_workspace_bytes),
+                       (ops.qwen35_compact_attention_decode, ops.qwen35_compact_decode_workspace_bytes)):
+        ws = torch.empty(need(shape), device="cuda", dtype=torch.uint8)
+        out, w = torch.zeros(1, 1, D, device="cuda", dtype=torch.bfloat16), torch.zeros(cap, device="cuda")
+        call(q, one, one, gate, out, buf, shape, ops.DTYPE_BF16, FP8, 1, ws, key_weights=w)
+        torch.cuda.synchronize()
+        assert (out == 1).all(), call
+        assert (w == 2.0 ** -28).all(), call
+        del ws, w
+    del buf
+    torch.cuda.empty_cache()
