@@ -146,7 +146,7 @@ constexpr std::size_t kMaxHeadPositions = std::size_t{1} << 31; // over all KV h
 constexpr std::size_t kMaxQueryRows = std::size_t{1} << 26;
 constexpr std::size_t kMaxUnits = std::size_t{1} << 17; // sequences times KV heads
 constexpr std::size_t kMaxGrid = 65535;
-constexpr std::size_t kMaxEvictContext = kMaxGrid * 4096; // segments of the selection
+constexpr std::size_t kMaxEvictContext = kMaxGrid * 4096; // (the documented limit)
 
 std::size_t cache_bytes_of(std::size_t positions, std::size_t kv_heads, Qwen35CompactCacheDType dtype) {
   const char *overflow = "compact cache byte size overflow";
