@@ -1,5 +1,5 @@
-"""The compact KV cache at values where roundings show: the weights that the values are averaged with sum to what the
-average is divided by, and key weights change no output."""
+"""The compact KV cache at values where roundings show and at the ends of their range: what the values are averaged with
+sums to what the average is divided by, key weights change no output, the largest and the smallest values, infinities and NaN."""
 import numpy as np
 import pytest
 import torch
@@ -288,3 +288,68 @@ def test_the_largest_cache(gpu):
         del ws, w
     del buf
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ NaN codes reach only the tokens that see them
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hkv,group,t,past,window,sinks", [
+    (2, 4, 40, 100, 0, 0), (2, 4, 40, 100, 30, 0), (2, 4, 40, 100, 30, 40), (2, 4, 40, 96, 0, 0), (2, 4, 1, 100, 30, 40),
+    (2, 8, 20, 3001, 2900, 0), (16, 16, 130, 600, 0, 0), (16, 16, 131, 700, 333, 40), (2, 16, 131, 4000, 3000, 70)])
+def test_bad_values_in_8_bit(gpu, layout, what, hkv, group, t, past, window, sinks):
+    """Rows of infinite or NaN values are stored as NaN: in K at 45, in V among the new tokens, at a window's edge and
+    where no window reaches."""
+    r = rng(11)
+    heads, n = hkv * group, past + t
+    k, v = rows(r, n, hkv), rows(r, n, hkv)
+    q, g = bf16(normal(r, t, heads, D)), bf16(normal(r, t, heads, D))
+    bad_k = [45] if window and sinks < 45 else []
+    bad_v = sorted({past + t // 2, n - 1} | ({past - window + t // 2, past - window - 3} if window else set()))
+    k[bad_k] = what
+    v[bad_v, 0] = what     # all of a row, and of another head one value
+    v[bad_v, 1, 77] = what
+    c = Cache(r, FP8, layout, hkv, n)
+    c.store(0, k[:past], v[:past])
+    x = dev(q), dev(k[past:]), dev(v[past:]), dev(g)
+    out, _ = prefill(c, x, t, heads, past, window, sinks) if t > 1 else decode(c, x, heads, past, window, sinks)
+    c.want_store(past, k[past:], v[past:])
+    c.check()
+    got = host(out)
+    for i in sorted({0, 1, t // 2 - 1, t // 2, t // 2 + 1, t - 2, t - 1} & set(range(t))):
+        ok = ref.sees(past + i, window, sinks, n)
+        seen_k, seen_v = ok[bad_k].any(), ok[bad_v].any()
+        held = np.where(ok[None, None, :, None], c.held(n), 0)
+        clean = np.nan_to_num(held, nan=0.0)
+        want, bound, _, _ = ref.attention(q[i:i + 1], g[i:i + 1], clean, past + i, window, sinks)
+        bad = np.zeros((heads, D), bool)
+        if seen_k:
+            bad[:] = True
+        if seen_v:
+            bad[:group] = True
+            bad[group:2 * group, 77] = True
+        assert np.isnan(got[i][bad]).all(), i
+        near(got[i][~bad], want[0][~bad], bound[0][~bad], f"token {i}")
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("n,at,window", [(1, 0, 0), (40, 39, 0), (40, 7, 0), (40, 7, 20), (700, 650, 0), (4001, 3990, 0), (4001, 300, 2000)])
+def test_decode_of_bad_values_in_8_bit(gpu, layout, n, at, window):
+    r = rng(12)
+    hkv, heads = 2, 16
+    k, v = rows(r, n, hkv), rows(r, n, hkv)
+    v[at, 1, 200] = np.nan
+    c = Cache(r, FP8, layout, hkv, n)
+    if n > 1:
+        c.store(0, k[:-1], v[:-1])
+    q, g = bf16(normal(r, 1, heads, D)), bf16(normal(r, 1, heads, D))
+    out, w = decode(c, (dev(q), dev(k[-1:]), dev(v[-1:]), dev(g)), heads, n - 1, window, weigh=True)
+    c.want_store(n - 1, k[-1:], v[-1:])
+    c.check()
+    seen = ref.sees(n - 1, window, 0, n)
+    want, bound, ww, rel = ref.attention(q, g, np.nan_to_num(c.held(n)), n - 1, window, 0, 1)
+    got, bad = host(out), np.zeros((1, heads, D), bool)
+    bad[0, heads // 2:, 200] = seen[at]
+    assert np.isnan(got[bad]).all()
+    near(got[~bad], want[~bad], bound[~bad])
+    near(host(w), ww, ww * rel + 2.0 ** -23 * ww + 1e-38, "weights")
