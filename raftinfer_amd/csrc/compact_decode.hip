@@ -96,9 +96,9 @@ __device__ __forceinline__ u32x4 rescale_fp8x16(u32x4 w, float ratio) {
 //
 // The kernel is bound by its cache reads, so a wave (32 8-bit or 16 bf16 rows a
 // step) asks for rows a step ahead: K(t + 1) goes out when S(t) is formed, V(t + 1)
-// when V(t) is in LDS.  32 ragged sequences of up to 32768, 8 bit, 4 KV heads: 197 us,
-// 5.5 TB/s; one of 60001 22.4 us, 5.5 TB/s; 16 behind a window of 4096, bf16, 43.5 us,
-// 5.8 TB/s.  201 tokens, 8.7 us, are round trips: lengths, then rows and scales, gate, output.
+// when V(t) is in LDS.  32 ragged sequences of up to 32768, 8 bit, 4 KV heads: 202 us,
+// 5.3 TB/s; one of 60001 23.0 us, 5.3 TB/s; 16 behind a window of 4096, bf16, 43.5 us,
+// 5.8 TB/s.  201 tokens, 8.9 us, are round trips: lengths, then rows and scales, gate, output.
 //
 // The step that holds the new token's position covers its scale block, so its wave also
 // stores the row: it raises the block's scale where the row needs that, rounds the
@@ -594,7 +594,9 @@ std::uint32_t most_tiles(const CompactArgs &a, std::uint32_t n) {
 // with key weights 27.7 / 32.7 / 28.4); no longer where there are more (32 ragged sequences,
 // 32 / 64 tiles: 203 / 210 us), and at most 64 partitions, which the merge takes in one
 // batch (60001 tokens, 64 / 128: 30.3 / 31.0 us, 16000 tokens 17.1 / 18.8).  Where that leaves
-// at most one workgroup per CU, it gets 8 waves (60001 tokens: 33.5 against 35.0 us).
+// at most one workgroup per CU, it gets 8 waves from 32 tiles on (60001 tokens: 33.5 against 35.0
+// us with 4); of fewer tiles 4 are faster (4 / 8 waves: 16000 tokens, 8 tiles, 12.9 / 13.1 us; 4 of
+// 8192 in bf16, 16 tiles, 28.9 / 30.3, with key weights 32.0 / 32.9; 45000 tokens, 24 tiles, 22.1 / 22.7).
 constexpr std::uint32_t kAlone = 16;
 constexpr std::uint32_t kMostParts = 64;
 struct DecodeSplit {

@@ -158,10 +158,13 @@ __device__ __forceinline__ void add_odd_values(const CompactHead<Fp8> &c, const 
 // that one's softmax runs beside the other's products.
 //
 // 500 tokens of 16 heads behind 30001, 8 bit: 285 us, 870 TFLOP/s; 6001 behind a window of
-// 1024, bf16, with the store: 155 us.  A wave's tile takes 4300 clocks, 1024 of them of matrix time (two
-// waves a SIMD, 50% busy): softmax 450, conversion 1000, barrier 200, products 2300; no
-// waits for loads, no bank conflicts.  One workgroup of 256 columns per CU took 174 us for
-// the window, 64 columns a wave do not fit its registers.
+// 1024, bf16, with the store: 152 us; 2001 with key weights 67 us.  An 8-bit tile takes a wave 4300 clocks,
+// 1024 of them of matrix time (two waves a SIMD, 50% busy): by time stamps softmax 450, conversion
+// 1000, barrier 200, products 2300, the rest between them; no waits for loads, no bank conflicts.  At
+// 128 B a clock, and 64 of transposed reads, LDS needs 4100 clocks for the eight waves of a CU: V's
+// operands 2048, K's 1024, codes in and out and bf16 tiles in 1024.  So it bounds the tile: every
+// operand serves 32 columns only.  (64 columns a wave spilled with the accumulators left to the
+// compiler.)  One workgroup of 256 columns per CU took 174 us for the window.
 template <bool Fp8, bool Split, bool Weigh>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void compact_prefill_kernel(
     CompactArgs a, PrefillScratch sc) {
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 // read; the block's scales go on the scores and on V's operands), asked for by
 // LDS-direct loads of the wave's own kStages tiles ahead.
 //
-// 500 tokens of 16 heads, 8 bit: 17.3 us for 2.1 GFLOP, of which 3.4 until q and the first
+// 500 tokens of 16 heads, 8 bit: 17.4 us for 2.1 GFLOP, of which 3.4 until q and the first
 // rows are there, 1.6 a tile (at one wave per SIMD, for 128 accumulators and q: products
 // with K 860 clocks, softmax and the next loads' issue 1290, products with V and loads 1180),
 // 3 for the join.  K and V through registers, as decode has them: 21.5.
