@@ -233,7 +233,8 @@ int raftinfer_amd_online_attention_prefill_kernel_only(
     int activation_dtype, uint8_t cache_dtype, uint8_t cache_layout, void *stream);
 /* Device capacity-guard counter (replaces the reference merge kernel's trap,
  * qwen35_online_attention.cu:714-717); also counts batched-decode and compact
- * decode sequences whose length is 0 or above the maximum context.  Synchronizes the device. */
+ * decode sequences whose length is 0 or above the maximum context, and the paged calls'
+ * bad sequences and pages.  Synchronizes the device. */
 int raftinfer_amd_consume_capacity_errors(uint32_t *out);
 
 /* ---- decode graphs (include/raftinfer_amd/hip_graph_decode.hpp) ---- */
@@ -338,6 +339,69 @@ int raftinfer_amd_compact_cache_evict(const void *kv_cache, size_t kv_cache_byte
                                       size_t workspace_bytes, raftinfer_amd_evict_shape shape,
                                       uint8_t cache_dtype, uint8_t out_cache_dtype,
                                       uint8_t cache_layout, void *stream);
+
+/* ---- rotary positions, paged KV cache (include/raftinfer_amd/qwen35_paged_cache.hpp) ---- */
+/* Additive.  Strides in elements, 0: dense. */
+enum {
+  RAFTINFER_AMD_ROTARY_SCALING_NONE = 0,
+  RAFTINFER_AMD_ROTARY_SCALING_LINEAR = 1,
+  RAFTINFER_AMD_ROTARY_SCALING_BY_PAIR = 2,
+  RAFTINFER_AMD_ROTARY_SCALING_BY_TURNS = 3
+};
+typedef struct raftinfer_amd_rotary_shape {
+  size_t rows, heads, head_dim, rotary_dim;
+  uint8_t interleaved;
+  float magnitude;
+  size_t input_row_stride, input_head_stride, output_row_stride, output_head_stride;
+} raftinfer_amd_rotary_shape;
+typedef struct raftinfer_amd_paged_shape {
+  size_t rows, sequences, query_heads, kv_heads, head_dim, pages, page_tokens, table_pages,
+      max_context_tokens, window_tokens;
+} raftinfer_amd_paged_shape;
+typedef struct raftinfer_amd_paged_rotary {
+  size_t rotary_dim;
+  uint8_t interleaved;
+  float magnitude, epsilon;
+  size_t query_row_stride, query_head_stride, key_row_stride, key_head_stride, value_row_stride,
+      value_head_stride, output_row_stride, output_head_stride;
+} raftinfer_amd_paged_rotary;
+typedef struct raftinfer_amd_paged_strides {
+  size_t query_row, query_head, gate_row, gate_head, output_row, output_head;
+} raftinfer_amd_paged_strides;
+/* Host: writes rotary_dim / 2 frequencies and their magnitude. */
+int raftinfer_amd_rotary_frequencies(double *frequencies, size_t rotary_dim, double base,
+                                     uint8_t scaling, double factor, double trained_tokens,
+                                     double fast_turns, double slow_turns, float *magnitude);
+/* weight may be null; positions uint32, frequencies double, on the device. */
+int raftinfer_amd_rotary(const void *input, const void *weight, void *output,
+                         const uint32_t *positions, const double *frequencies,
+                         raftinfer_amd_rotary_shape shape, float epsilon, int dtype,
+                         int weight_dtype, void *stream);
+int raftinfer_amd_paged_cache_bytes(raftinfer_amd_paged_shape shape, size_t *out);
+int raftinfer_amd_paged_decode_workspace_bytes(raftinfer_amd_paged_shape shape, size_t *out);
+int raftinfer_amd_paged_prefill_workspace_bytes(raftinfer_amd_paged_shape shape, size_t *out);
+int raftinfer_amd_paged_cache_append(const void *query, const void *key, const void *value,
+                                     void *query_output, void *pages, size_t pages_bytes,
+                                     const int32_t *page_table, const uint32_t *query_starts,
+                                     const uint32_t *context_lengths, const double *frequencies,
+                                     const void *query_weight, const void *key_weight,
+                                     raftinfer_amd_paged_shape shape,
+                                     raftinfer_amd_paged_rotary rotary, int activation_dtype,
+                                     int weight_dtype, uint8_t cache_layout, void *stream);
+int raftinfer_amd_paged_attention_prefill(const void *query, const void *gate, void *output,
+                                          const void *pages, size_t pages_bytes,
+                                          const int32_t *page_table, const uint32_t *query_starts,
+                                          const uint32_t *context_lengths, void *workspace,
+                                          size_t workspace_bytes, raftinfer_amd_paged_shape shape,
+                                          raftinfer_amd_paged_strides strides,
+                                          int activation_dtype, uint8_t cache_layout, void *stream);
+int raftinfer_amd_paged_attention_decode(const void *query, const void *gate, void *output,
+                                         const void *pages, size_t pages_bytes,
+                                         const int32_t *page_table,
+                                         const uint32_t *context_lengths, void *workspace,
+                                         size_t workspace_bytes, raftinfer_amd_paged_shape shape,
+                                         raftinfer_amd_paged_strides strides, int activation_dtype,
+                                         uint8_t cache_layout, void *stream);
 
 /* ---- attention producers ---- */
 /* qwen35_primitives.cuh:63-67 (qwen35_qk_norm_rope; device_position may be null). */

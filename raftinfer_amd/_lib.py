@@ -71,6 +71,30 @@ class EvictShape(ctypes.Structure):
                 ("sink_tokens", _sz), ("recent_tokens", _sz)]
 
 
+class RotaryShape(ctypes.Structure):
+    _fields_ = [("rows", _sz), ("heads", _sz), ("head_dim", _sz), ("rotary_dim", _sz),
+                ("interleaved", _u8), ("magnitude", ctypes.c_float), ("input_row_stride", _sz),
+                ("input_head_stride", _sz), ("output_row_stride", _sz), ("output_head_stride", _sz)]
+
+
+class PagedShape(ctypes.Structure):
+    _fields_ = [("rows", _sz), ("sequences", _sz), ("query_heads", _sz), ("kv_heads", _sz),
+                ("head_dim", _sz), ("pages", _sz), ("page_tokens", _sz), ("table_pages", _sz),
+                ("max_context_tokens", _sz), ("window_tokens", _sz)]
+
+
+class PagedRotary(ctypes.Structure):
+    _fields_ = [("rotary_dim", _sz), ("interleaved", _u8), ("magnitude", ctypes.c_float),
+                ("epsilon", ctypes.c_float), ("query_row_stride", _sz), ("query_head_stride", _sz),
+                ("key_row_stride", _sz), ("key_head_stride", _sz), ("value_row_stride", _sz),
+                ("value_head_stride", _sz), ("output_row_stride", _sz), ("output_head_stride", _sz)]
+
+
+class PagedStrides(ctypes.Structure):
+    _fields_ = [("query_row", _sz), ("query_head", _sz), ("gate_row", _sz), ("gate_head", _sz),
+                ("output_row", _sz), ("output_head", _sz)]
+
+
 class DeltaCoreShape(ctypes.Structure):
     _fields_ = [("tokens", _sz), ("key_heads", _sz), ("value_heads", _sz), ("key_dim", _sz),
                 ("value_dim", _sz)]
@@ -160,6 +184,18 @@ SIGNATURES = {
         ([_vp] * 6 + [_sz, _vp, _vp, _vp, _sz, CompactShape, _I, _u8, _u8, _vp], _I),
     "raftinfer_amd_compact_cache_evict":
         ([_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _sz, EvictShape, _u8, _u8, _u8, _vp], _I),
+    "raftinfer_amd_rotary_frequencies":
+        ([_vp, _sz, ctypes.c_double, _u8, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _PF], _I),
+    "raftinfer_amd_rotary": ([_vp] * 5 + [RotaryShape, _F, _I, _I, _vp], _I),
+    "raftinfer_amd_paged_cache_bytes": ([PagedShape, _PSZ], _I),
+    "raftinfer_amd_paged_decode_workspace_bytes": ([PagedShape, _PSZ], _I),
+    "raftinfer_amd_paged_prefill_workspace_bytes": ([PagedShape, _PSZ], _I),
+    "raftinfer_amd_paged_cache_append":
+        ([_vp] * 5 + [_sz] + [_vp] * 6 + [PagedShape, PagedRotary, _I, _I, _u8, _vp], _I),
+    "raftinfer_amd_paged_attention_prefill":
+        ([_vp] * 4 + [_sz] + [_vp] * 4 + [_sz, PagedShape, PagedStrides, _I, _u8, _vp], _I),
+    "raftinfer_amd_paged_attention_decode":
+        ([_vp] * 4 + [_sz] + [_vp] * 3 + [_sz, PagedShape, PagedStrides, _I, _u8, _vp], _I),
     "raftinfer_amd_qk_norm_rope":
         ([_vp, _vp, _vp, QkNormRopeShape, _F, _I, _I, _vp, _vp], _I),
     "raftinfer_amd_split_full_query_gate": ([_vp, _vp, _vp, _sz, _sz, _sz, _I, _vp], _I),

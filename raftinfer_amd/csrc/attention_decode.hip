@@ -10,6 +10,7 @@
 #include "decode_mfma.hpp"
 #include "decode_scan.hpp"
 #include "norm_rope.hpp"
+#include "paged_cache.hpp"
 #include "raftinfer_amd/qwen35_online_attention.hpp"
 
 #include <algorithm>
@@ -1233,7 +1234,7 @@ std::uint32_t qwen35_online_attention_consume_capacity_errors() {
                "reading the capacity error counter failed");
   require<Err>(hipMemcpyToSymbol(HIP_SYMBOL(g_capacity_errors), &zero, sizeof zero) == hipSuccess,
                "clearing the capacity error counter failed");
-  return value + compact_take_capacity_errors();
+  return value + compact_take_capacity_errors() + paged_take_capacity_errors() + paged_take_append_errors();
 }
 
 // ------------------------------------------------------ batched decode

@@ -8,6 +8,7 @@
 #include "raftinfer_amd/qwen35_compact_cache.hpp"
 #include "raftinfer_amd/qwen35_delta.hpp"
 #include "raftinfer_amd/qwen35_online_attention.hpp"
+#include "raftinfer_amd/qwen35_paged_cache.hpp"
 #include "raftinfer_amd/qwen35_primitives.hpp"
 
 #include <cstring>
@@ -80,6 +81,22 @@ Qwen35CompactShape to_compact(raftinfer_amd_compact_shape s) {
 Qwen35EvictShape to_evict(raftinfer_amd_evict_shape s) {
   return {s.kv_heads,    s.head_dim,               s.context_tokens, s.max_context_tokens,
           s.keep_tokens, s.out_max_context_tokens, s.sink_tokens,    s.recent_tokens};
+}
+Qwen35RotaryShape to_rotary(raftinfer_amd_rotary_shape s) {
+  return {s.rows,      s.heads,            s.head_dim,          s.rotary_dim,        s.interleaved != 0,
+          s.magnitude, s.input_row_stride, s.input_head_stride, s.output_row_stride, s.output_head_stride};
+}
+Qwen35PagedShape to_paged(raftinfer_amd_paged_shape s) {
+  return {s.rows,  s.sequences,   s.query_heads, s.kv_heads,           s.head_dim,
+          s.pages, s.page_tokens, s.table_pages, s.max_context_tokens, s.window_tokens};
+}
+Qwen35PagedRotary to_paged_rotary(raftinfer_amd_paged_rotary r) {
+  return {r.rotary_dim,        r.interleaved != 0,  r.magnitude,          r.epsilon,
+          r.query_row_stride,  r.query_head_stride, r.key_row_stride,     r.key_head_stride,
+          r.value_row_stride,  r.value_head_stride, r.output_row_stride,  r.output_head_stride};
+}
+Qwen35PagedStrides to_paged_strides(raftinfer_amd_paged_strides s) {
+  return {s.query_row, s.query_head, s.gate_row, s.gate_head, s.output_row, s.output_head};
 }
 Qwen35CompactCacheDType to_compact_dtype(uint8_t d) { return static_cast<Qwen35CompactCacheDType>(d); }
 
@@ -504,6 +521,73 @@ int raftinfer_amd_compact_cache_evict(const void *cache, size_t cache_bytes, con
                                ws, ws_bytes, to_evict(shape), to_compact_dtype(cache_dtype),
                                to_compact_dtype(out_cache_dtype), static_cast<Qwen35KvCacheLayout>(cache_layout),
                                to_stream(stream));
+  });
+}
+
+int raftinfer_amd_rotary_frequencies(double *frequencies, size_t rotary_dim, double base, uint8_t scaling, double factor,
+                                     double trained_tokens, double fast_turns, double slow_turns, float *magnitude) {
+  return guarded([&] {
+    out_ref(magnitude) = qwen35_rotary_frequencies(frequencies, rotary_dim, base, static_cast<Qwen35RotaryScaling>(scaling),
+                                                   factor, trained_tokens, fast_turns, slow_turns);
+  });
+}
+
+int raftinfer_amd_rotary(const void *input, const void *weight, void *output, const uint32_t *positions,
+                         const double *frequencies, raftinfer_amd_rotary_shape shape, float epsilon, int dtype,
+                         int weight_dtype, void *stream) {
+  return guarded([&] {
+    qwen35_rotary(input, weight, output, positions, frequencies, to_rotary(shape), epsilon, to_dtype(dtype),
+                  to_dtype(weight_dtype), to_stream(stream));
+  });
+}
+
+int raftinfer_amd_paged_cache_bytes(raftinfer_amd_paged_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_paged_cache_bytes(to_paged(shape)); });
+}
+
+int raftinfer_amd_paged_decode_workspace_bytes(raftinfer_amd_paged_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_paged_decode_workspace_bytes(to_paged(shape)); });
+}
+
+int raftinfer_amd_paged_prefill_workspace_bytes(raftinfer_amd_paged_shape shape, size_t *out) {
+  return guarded([&] { out_ref(out) = qwen35_paged_prefill_workspace_bytes(to_paged(shape)); });
+}
+
+int raftinfer_amd_paged_cache_append(const void *query, const void *key, const void *value, void *query_output,
+                                     void *pages, size_t pages_bytes, const int32_t *page_table,
+                                     const uint32_t *query_starts, const uint32_t *context_lengths,
+                                     const double *frequencies, const void *query_weight, const void *key_weight,
+                                     raftinfer_amd_paged_shape shape, raftinfer_amd_paged_rotary rotary, int act,
+                                     int weight_dtype, uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_paged_cache_append(query, key, value, query_output, pages, pages_bytes, page_table, query_starts,
+                              context_lengths, frequencies, query_weight, key_weight, to_paged(shape),
+                              to_paged_rotary(rotary), to_dtype(act), to_dtype(weight_dtype),
+                              static_cast<Qwen35KvCacheLayout>(cache_layout), to_stream(stream));
+  });
+}
+
+int raftinfer_amd_paged_attention_prefill(const void *q, const void *g, void *o, const void *pages, size_t pages_bytes,
+                                          const int32_t *page_table, const uint32_t *query_starts,
+                                          const uint32_t *context_lengths, void *ws, size_t ws_bytes,
+                                          raftinfer_amd_paged_shape shape, raftinfer_amd_paged_strides strides, int act,
+                                          uint8_t cache_layout, void *stream) {
+  return guarded([&] {
+    qwen35_paged_attention_prefill(q, g, o, pages, pages_bytes, page_table, query_starts, context_lengths, ws, ws_bytes,
+                                   to_paged(shape), to_paged_strides(strides), to_dtype(act),
+                                   static_cast<Qwen35KvCacheLayout>(cache_layout), to_stream(stream));
+  });
+}
+
+int raftinfer_amd_paged_attention_decode(const void *q, const void *g, void *o, const void *pages, size_t pages_bytes,
+                                         const int32_t *page_table, const uint32_t *context_lengths, void *ws,
+                                         size_t ws_bytes, raftinfer_amd_paged_shape shape,
+                                         raftinfer_amd_paged_strides strides, int act, uint8_t cache_layout,
+                                         void *stream) {
+  return guarded([&] {
+    qwen35_paged_attention_decode(q, g, o, pages, pages_bytes, page_table, context_lengths, ws, ws_bytes, to_paged(shape),
+                                  to_paged_strides(strides), to_dtype(act),
+                                  static_cast<Qwen35KvCacheLayout>(cache_layout), to_stream(stream));
   });
 }
 

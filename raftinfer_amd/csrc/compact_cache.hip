@@ -1,9 +1,8 @@
 // Entry points, sizing and the row store of the compact KV cache
 // (include/raftinfer_amd/qwen35_compact_cache.hpp).
+#include "call_checks.hpp"
 #include "compact_cache.hpp"
 #include "raftinfer_amd/qwen35_compact_cache.hpp"
-
-#include <initializer_list>
 
 namespace raftinfer::amd {
 namespace {
@@ -177,29 +176,6 @@ void validate_layout(Qwen35KvCacheLayout layout) {
                "unsupported compact cache layout");
 }
 
-// The stream's device for the launches of a call, where another one is current.
-class StreamDevice {
-public:
-  explicit StreamDevice(hipStream_t stream) {
-    int device = 0;
-    require<Err>(hipGetDevice(&current_) == hipSuccess && hipStreamGetDevice(stream, &device) == hipSuccess,
-                 "compact attention HIP stream has no device");
-    if (device == current_) return;
-    require<Err>(hipSetDevice(device) == hipSuccess, "compact attention cannot select the stream's device");
-    changed_ = true;
-  }
-  ~StreamDevice() {
-    if (changed_) (void)hipSetDevice(current_);
-  }
-  StreamDevice(const StreamDevice &) = delete;
-  StreamDevice &operator=(const StreamDevice &) = delete;
-
-private:
-  int current_ = 0;
-  bool changed_ = false;
-};
-
-bool aligned16(const void *p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
 
 // lengths_given: past_tokens is not read.
 void validate_shape(const Qwen35CompactShape &s, bool lengths_given) {
@@ -218,21 +194,6 @@ void validate_shape(const Qwen35CompactShape &s, bool lengths_given) {
   require<Err>(s.observed_tokens <= s.tokens, "compact attention observes more tokens than the call has");
 }
 
-struct Bytes {
-  const void *at;
-  std::size_t count;
-};
-// What a call writes overlaps neither what it reads nor what else it writes.
-void validate_apart(std::initializer_list<Bytes> written, std::initializer_list<Bytes> read, const char *message) {
-  const auto apart = [](const Bytes &a, const Bytes &b) {
-    const auto x = reinterpret_cast<std::uintptr_t>(a.at), y = reinterpret_cast<std::uintptr_t>(b.at);
-    return x <= y ? a.count <= y - x : b.count <= x - y;
-  };
-  for (auto w = written.begin(); w != written.end(); ++w) {
-    for (auto other = w + 1; other != written.end(); ++other) require<Err>(apart(*w, *other), message);
-    for (const Bytes &r : read) require<Err>(apart(*w, r), message);
-  }
-}
 Bytes lengths_of(const Qwen35CompactShape &s, const std::uint32_t *lengths) {
   return {lengths, lengths != nullptr ? s.sequences * sizeof(std::uint32_t) : 0};
 }
@@ -246,7 +207,7 @@ void validate_overlap(const Qwen35CompactShape &s, const void *q, const void *k,
   const std::size_t tokens = s.sequences * s.tokens;
   const std::size_t heads = tokens * s.query_heads * kHeadDim * 2, rows = tokens * s.kv_heads * kHeadDim * 2;
   const std::size_t weight_bytes = weights != nullptr ? s.sequences * s.kv_heads * s.max_context_tokens * sizeof(float) : 0;
-  validate_apart({{output, heads}, {cache, cache_bytes}, {weights, weight_bytes}, {workspace, workspace_bytes}},
+  validate_apart<Err>({{output, heads}, {cache, cache_bytes}, {weights, weight_bytes}, {workspace, workspace_bytes}},
                  {{q, heads}, {k, rows}, {v, rows}, {g, heads}, lengths_of(s, lengths)},
                  "compact attention outputs overlap other arguments");
 }
@@ -354,12 +315,12 @@ void qwen35_compact_cache_append(const void *key, const void *value, void *kv_ca
   require<Err>(aligned16(key) && aligned16(value), "compact attention inputs and output must be 16-byte aligned");
   const std::size_t rows = shape.sequences * shape.tokens * shape.kv_heads * kHeadDim * 2;
   validate_lengths(context_lengths);
-  validate_apart({{kv_cache, used}}, {{key, rows}, {value, rows}, lengths_of(shape, context_lengths)},
+  validate_apart<Err>({{kv_cache, used}}, {{key, rows}, {value, rows}, lengths_of(shape, context_lengths)},
                  "compact cache overlaps the rows to be stored or their lengths");
   CompactArgs a = to_args(shape);
   fill_pointers(a, nullptr, key, value, nullptr, nullptr, kv_cache, layout);
   a.lengths = context_lengths;
-  const StreamDevice device(stream);
+  const StreamDevice<Err> device(stream, "compact attention");
   compact_append(a, cache_dtype == Qwen35CompactCacheDType::fp8_e4m3, stream);
   check_launch<Err>("qwen35_compact_cache_append");
 }
@@ -379,7 +340,7 @@ void qwen35_compact_attention_prefill(const void *query, const void *key, const 
   CompactArgs a = to_args(shape);
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;
-  const StreamDevice device(stream);
+  const StreamDevice<Err> device(stream, "compact attention");
   compact_prefill(a, cache_dtype == Qwen35CompactCacheDType::fp8_e4m3, workspace, stream);
   check_launch<Err>("qwen35_compact_attention_prefill");
 }
@@ -402,7 +363,7 @@ void qwen35_compact_attention_decode(const void *query, const void *key, const v
   fill_pointers(a, query, key, value, gate, output, kv_cache, layout);
   a.weights = key_weights;
   a.lengths = context_lengths;
-  const StreamDevice device(stream);
+  const StreamDevice<Err> device(stream, "compact attention");
   compact_decode(a, cache_dtype == Qwen35CompactCacheDType::fp8_e4m3, workspace, stream);
   check_launch<Err>("qwen35_compact_attention_decode");
 }
@@ -465,7 +426,7 @@ void qwen35_compact_cache_evict(const void *kv_cache, std::size_t kv_cache_bytes
   require<Err>(aligned16(workspace), "compact attention workspace must be 16-byte aligned");
   const std::size_t in_bytes = cache_bytes_of(shape.max_context_tokens, shape.kv_heads, cache_dtype);
   const std::size_t out_bytes = cache_bytes_of(shape.out_max_context_tokens, shape.kv_heads, out_cache_dtype);
-  validate_apart({{out_cache, out_bytes},
+  validate_apart<Err>({{out_cache, out_bytes},
                   {out_weights, shape.kv_heads * shape.out_max_context_tokens * sizeof(float)},
                   {kept_indices, shape.kv_heads * shape.keep_tokens * sizeof(std::int32_t)},
                   {workspace, need}},
@@ -477,7 +438,7 @@ void qwen35_compact_cache_evict(const void *kv_cache, std::size_t kv_cache_bytes
   a.out_weights = out_weights;
   a.kept = kept_indices;
   a.head_major = layout == Qwen35KvCacheLayout::head_major;
-  const StreamDevice device(stream);
+  const StreamDevice<Err> device(stream, "compact attention");
   compact_evict(a, cache_dtype == Qwen35CompactCacheDType::fp8_e4m3,
                 out_cache_dtype == Qwen35CompactCacheDType::fp8_e4m3, workspace, stream);
   check_launch<Err>("qwen35_compact_cache_evict");

@@ -1,0 +1,236 @@
+// Device pieces of the paged KV cache: the pool's rows, a ragged batch's sequences,
+// and how a batch's work is dealt to workgroups.
+#pragma once
+
+#include "decode_scan.hpp"
+
+#include <cfloat>
+
+namespace raftinfer::amd {
+
+constexpr int kPageGranule = 16;      // positions that always lie in one page, next to each other
+constexpr int kPagedMaxGroup = 16;    // query heads per KV head
+constexpr int kRowBytes = kHeadDim * 2;
+
+// What the kernels read of one call.  Strides in elements; row_step, head_step and
+// plane_rows in rows of 512 bytes: between positions, KV heads, and K and V.
+struct PagedArgs {
+  const bf16_bits *query, *gate; // gate: or null
+  bf16_bits *output;
+  const unsigned char *pages;
+  const std::int32_t *table;
+  const std::uint32_t *starts; // or null: one row for each sequence
+  const std::uint32_t *lengths;
+  std::size_t q_row, q_head, g_row, g_head, o_row, o_head;
+  std::uint32_t rows, sequences, kv_heads, group, page_count, page_tokens, table_pages, max_ctx, window;
+  std::uint32_t row_step, head_step, plane_rows;
+  int page_shift; // log2 of page_tokens, or -1
+};
+
+// One sequence's share of a batch.  Not valid: its rows, as far as they are the call's,
+// become NaN.
+struct PagedSeq {
+  std::uint32_t row0, n, ctx;
+  bool valid;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, std::uint32_t s) {
+  const std::uint32_t c = a.lengths[s];
+  if (a.starts == nullptr) return {s, c != 0 ? 1u : 0u, c, c <= a.max_ctx};
+  const std::uint32_t b = a.starts[s], e = a.starts[s + 1];
+  PagedSeq q{b, 0, c, true};
+  if (b == e) return q;
+  if (b > e || b >= a.rows) {
+    q.valid = false;
+  } else {
+    q.valid = e <= a.rows && c >= e - b && c <= a.max_ctx;
+    q.n = (e < a.rows ? e : a.rows) - b;
+  }
+  return q;
+}
+
+// The page-table entry's place and the position in the page of position j.
+__device__ __forceinline__ void paged_place(const PagedArgs &a, std::uint32_t j, std::uint32_t &entry, std::uint32_t &in) {
+  entry = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_tokens;
+  in = j - entry * a.page_tokens;
+}
+// The K row (512 bytes each, from the pool's first) of position j of a KV head; a bad page: `bad` is
+// set and page 0 taken.  (The host sees to it that the pool has fewer than 2^32 rows.)
+__device__ __forceinline__ std::uint32_t paged_row(const PagedArgs &a, std::uint32_t seq, std::uint32_t kvh, std::uint32_t j,
+                                                   bool &bad) {
+  std::uint32_t entry, in;
+  paged_place(a, j, entry, in);
+  auto page = static_cast<std::uint32_t>(a.table[static_cast<std::size_t>(seq) * a.table_pages + entry]);
+  if (page >= a.page_count) {
+    bad = true;
+    page = 0;
+  }
+  return page * 2 * a.plane_rows + kvh * a.head_step + in * a.row_step;
+}
+
+// -------------------------------------------------------- dealing out the work
+// A column is a (token, head of the group) of one KV head; a workgroup takes block_cols
+// columns of a sequence and KV head, and of the tiles (of `unit` keys) that they see a
+// range.  All of a batch's workgroups deal the work out alike, each by itself, from the
+// sequences' lengths: no launch in front, nothing kept.  The whole batch has W (column
+// block, tile) pairs; ranges have at most T = max(least, W / slots) tiles of a sequence's
+// longest block, so that about `slots` = 2^slot_bits workgroups per KV head run.  Integers
+// throughout: every kernel of a call finds the same.
+struct PagedSplit {
+  std::uint32_t block_cols, unit, least, slot_bits;
+  std::uint32_t parts; // partial results that the workspace holds, each of a block and KV head
+};
+struct PagedScratch {
+  float *m, *l, *o; // [part][kv_head][column of the block]; o: 256 floats of each
+};
+
+struct PagedItem {
+  PagedSeq seq;
+  std::uint32_t id, blocks, ranges, range_tiles; // of its sequence
+  std::uint32_t local;      // index in the sequence's items, or split blocks
+  std::uint32_t first_part; // of its sequence
+};
+
+template <int Ctrl, int RowMask> __device__ __forceinline__ std::uint32_t dpp_zero(std::uint32_t x) {
+  return static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, RowMask, 0xF, false));
+}
+// Sum over this lane and those below it.
+__device__ __forceinline__ std::uint32_t wave_prefix(std::uint32_t x) {
+  x += dpp_zero<0x111, 0xF>(x); // row_shr 1, 2, 4, 8
+  x += dpp_zero<0x112, 0xF>(x);
+  x += dpp_zero<0x114, 0xF>(x);
+  x += dpp_zero<0x118, 0xF>(x);
+  x += dpp_zero<0x142, 0xA>(x); // lane 15 of the row below, into rows 1 and 3
+  x += dpp_zero<0x143, 0xC>(x); // lane 31, into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ std::uint32_t lane_u32(std::uint32_t x, int lane) {
+  return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+
+// Tiles that a sequence's longest column block sees (at least 1), and its blocks.
+__device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSplit &sp, const PagedSeq &q, std::uint32_t &blocks,
+                                             std::uint32_t &tiles) {
+  blocks = (q.n * a.group + sp.block_cols - 1) / sp.block_cols;
+  if (!q.valid) {
+    tiles = 1;
+    return;
+  }
+  tiles = (q.ctx + sp.unit - 1) / sp.unit;
+  if (a.window != 0) { // the window and the tokens of a block, both ends inside tiles
+    const std::uint32_t span = (sp.block_cols + a.group - 2) / a.group + 1;
+    const std::uint32_t some = (a.window + (span < q.n ? span : q.n) + sp.unit - 3) / sp.unit + 1;
+    tiles = some < tiles ? some : tiles;
+  }
+}
+
+// Finds item `index` of the batch (of_blocks: split column block `index`); false: there are
+// fewer.  By a whole wave, 64 sequences at a time; `count`: the caller is the one that counts bad
+// sequences.
+__device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, std::uint32_t index, bool of_blocks,
+                                           unsigned int *count, PagedItem &item) {
+  const std::uint32_t lane = threadIdx.x & 63;
+  std::uint64_t work = 0;
+  PagedSeq q{};
+  std::uint32_t blocks = 0, tiles = 1, bad = 0;
+  for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+    blocks = 0;
+    if (s0 + lane < a.sequences) {
+      q = paged_seq(a, s0 + lane);
+      paged_extent(a, sp, q, blocks, tiles);
+      bad += !q.valid;
+    }
+    const std::uint64_t w = static_cast<std::uint64_t>(blocks) * tiles;
+    work += lane_u32(wave_prefix(static_cast<std::uint32_t>(w) & 0xFFFFFFu), 63);
+    if (__builtin_amdgcn_ballot_w64(w >> 24 != 0) != 0)
+      work += static_cast<std::uint64_t>(lane_u32(wave_prefix(static_cast<std::uint32_t>(w >> 24)), 63)) << 24;
+  }
+  if (count != nullptr && bad != 0) atomicAdd(count, bad);
+  const std::uint64_t share = (work + (std::uint64_t{1} << sp.slot_bits) - 1) >> sp.slot_bits;
+  const std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
+  std::uint32_t before = 0, parts_before = 0;
+  for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+    if (a.sequences > 64) {
+      blocks = 0;
+      if (s0 + lane < a.sequences) {
+        q = paged_seq(a, s0 + lane);
+        paged_extent(a, sp, q, blocks, tiles);
+      }
+    }
+    const std::uint32_t ranges = (tiles + t - 1) / t;
+    const std::uint32_t parts = ranges > 1 ? blocks * ranges : 0;
+    const std::uint32_t mine = of_blocks ? (ranges > 1 ? blocks : 0) : blocks * ranges;
+    const std::uint32_t upto = before + wave_prefix(mine), parts_upto = parts_before + wave_prefix(parts);
+    const std::uint64_t hit = __builtin_amdgcn_ballot_w64(index < upto);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      item.seq.row0 = lane_u32(q.row0, at);
+      item.seq.n = lane_u32(q.n, at);
+      item.seq.ctx = lane_u32(q.ctx, at);
+      item.seq.valid = lane_u32(q.valid, at) != 0;
+      item.id = s0 + at;
+      item.blocks = lane_u32(blocks, at);
+      item.ranges = lane_u32(ranges, at);
+      item.range_tiles = t;
+      item.local = index - lane_u32(upto - mine, at);
+      item.first_part = lane_u32(parts_upto - parts, at);
+      return true;
+    }
+    before = lane_u32(upto, 63);
+    parts_before = lane_u32(parts_upto, 63);
+  }
+  return false;
+}
+
+// A column block's tokens and keys, and its ranges of about equal length.
+struct PagedBlock {
+  std::uint32_t col0, col_end;    // of its sequence's columns
+  std::uint32_t tok0;             // first token
+  std::uint32_t p_lo, p_hi;       // its tokens' positions
+  std::uint32_t first, total;     // tiles
+  std::uint32_t count, each, more; // ranges; the first `more` have a tile above `each`
+  __device__ __forceinline__ PagedBlock(const PagedArgs &a, const PagedSplit &sp, const PagedItem &it, std::uint32_t block) {
+    const std::uint32_t cols = it.seq.n * a.group, past = it.seq.ctx - it.seq.n;
+    col0 = block * sp.block_cols;
+    col_end = cols - col0 < sp.block_cols ? cols : col0 + sp.block_cols;
+    tok0 = col0 / a.group;
+    p_lo = past + tok0;
+    p_hi = past + (col_end - 1) / a.group;
+    first = (a.window != 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0) / sp.unit;
+    total = p_hi / sp.unit + 1 - first;
+    count = (total + it.range_tiles - 1) / it.range_tiles;
+    count = count < it.ranges ? count : it.ranges;
+    each = total / count;
+    more = total - each * count;
+  }
+  __device__ __forceinline__ std::uint32_t begin(std::uint32_t i) const { return first + i * each + (i < more ? i : more); }
+};
+
+// Whether a token at position p sees key j.  (no branches)
+__device__ __forceinline__ bool paged_sees(std::uint32_t j, std::uint32_t p, std::uint32_t window) {
+  return (j <= p) & ((window == 0) | (p - j < window));
+}
+
+// ------------------------------------------------------------- launches
+std::size_t paged_decode_workspace(const PagedArgs &a);
+void paged_decode(const PagedArgs &a, void *workspace, hipStream_t stream);
+std::size_t paged_prefill_workspace(const PagedArgs &a);
+void paged_prefill(const PagedArgs &a, void *workspace, hipStream_t stream);
+
+struct PagedAppendArgs {
+  PagedArgs paged; // query, output and their strides; no gate
+  const bf16_bits *key, *value;
+  unsigned char *pages;
+  const double *frequencies;
+  const void *q_weight, *k_weight;
+  bool weight_f32, interleaved;
+  std::size_t k_row, k_head, v_row, v_head;
+  std::uint32_t rotary_dim;
+  float magnitude, epsilon;
+};
+void paged_append(const PagedAppendArgs &a, hipStream_t stream);
+
+// Take (read and clear) the counts of bad sequences and pages, of attention calls and of appends.
+std::uint32_t paged_take_capacity_errors();
+std::uint32_t paged_take_append_errors();
+
+} // namespace raftinfer::amd

@@ -17,7 +17,8 @@ from dataclasses import dataclass
 
 from . import _lib
 from ._lib import (AttentionPolicy, AttentionShape, BatchedDecodeShape, CompactShape, DecodeLayout,
-                   DecodePlan, DeltaCoreShape, DeltaPolicy, DeltaShape, EvictShape, RaftInferError)
+                   DecodePlan, DeltaCoreShape, DeltaPolicy, DeltaShape, EvictShape, PagedRotary,
+                   PagedShape, PagedStrides, RaftInferError, RotaryShape)
 
 # cpp/execution/qwen35_execution_policy.hpp:7-27 and cpp/include/raftinfer/tensor.h:10-15
 MATERIALIZED, ONLINE_TILED = 0, 1
@@ -484,6 +485,149 @@ def qwen35_compact_cache_evict(kv_cache, key_weights, out_cache, out_weights, ke
         _raw(kept_indices), _raw(workspace),
         _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(), cache_dtype,
         out_cache_dtype, cache_layout, _stream_of(stream, kv_cache)))
+
+
+# ------------------------------------------- rotary positions, paged KV cache
+# include/raftinfer_amd/qwen35_paged_cache.hpp.  Tensors [rows, heads, dim] may have any strides
+# that the header allows; they are read off the tensors.
+SCALING_NONE, SCALING_LINEAR, SCALING_BY_PAIR, SCALING_BY_TURNS = 0, 1, 2, 3
+
+
+@dataclass(frozen=True)
+class Qwen35RotaryShape:
+    rows: int
+    heads: int
+    head_dim: int
+    rotary_dim: int
+    interleaved: bool = False
+    magnitude: float = 1.0
+
+
+@dataclass(frozen=True)
+class Qwen35PagedShape:
+    rows: int
+    sequences: int
+    query_heads: int
+    kv_heads: int
+    head_dim: int
+    pages: int
+    page_tokens: int
+    table_pages: int
+    max_context_tokens: int
+    window_tokens: int = 0
+
+    def c(self) -> PagedShape:
+        return PagedShape(self.rows, self.sequences, self.query_heads, self.kv_heads, self.head_dim,
+                          self.pages, self.page_tokens, self.table_pages, self.max_context_tokens,
+                          self.window_tokens)
+
+
+@dataclass(frozen=True)
+class Qwen35PagedRotary:
+    rotary_dim: int
+    interleaved: bool = False
+    magnitude: float = 1.0
+    epsilon: float = 1e-6
+
+
+def _strides(t) -> tuple:
+    """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else is dense."""
+    if t is None or getattr(t, "ndim", 0) != 3:
+        return 0, 0
+    row, head, dim = t.stride()
+    if dim != 1 and t.shape[2] != 1:
+        raise Qwen35PrimitiveError(1, "the last dimension of a tensor of heads must be contiguous")
+    # (the stride of a dimension of one element says nothing)
+    return (row if t.shape[0] > 1 else 0), (head if t.shape[1] > 1 else 0)
+
+
+def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
+                              factor: float = 1.0, trained_tokens: float = 0.0,
+                              fast_turns: float = 32.0, slow_turns: float = 1.0) -> tuple:
+    """(the rotary_dim / 2 angles per position, their magnitude), on the host."""
+    out = (ctypes.c_double * max(1, rotary_dim // 2))()
+    magnitude = ctypes.c_float()
+    _checked(_lib.load().raftinfer_amd_rotary_frequencies(
+        out, rotary_dim, base, scaling, factor, trained_tokens, fast_turns, slow_turns,
+        ctypes.byref(magnitude)))
+    return list(out), magnitude.value
+
+
+def qwen35_rotary(input, weight, output, positions, frequencies, shape: Qwen35RotaryShape,
+                  epsilon: float, stream=None) -> None:
+    """RoPE(input / rms(input) * weight) of every head by the rows' positions (int32/uint32); weight
+    None: no norm.  frequencies: float64 [rotary_dim / 2].  output may be input."""
+    dtype = _dtype_code(input)
+    _checked(_lib.load().raftinfer_amd_rotary(
+        input.data_ptr(), _raw(weight), output.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
+        RotaryShape(shape.rows, shape.heads, shape.head_dim, shape.rotary_dim, shape.interleaved,
+                    shape.magnitude, *_strides(input), *_strides(output)),
+        epsilon, dtype, dtype if weight is None else _dtype_code(weight), _stream_of(stream, input)))
+
+
+def qwen35_paged_cache_bytes(shape: Qwen35PagedShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_paged_cache_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_paged_decode_workspace_bytes(shape: Qwen35PagedShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_paged_decode_workspace_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_paged_prefill_workspace_bytes(shape: Qwen35PagedShape) -> int:
+    out = ctypes.c_size_t()
+    _checked(_lib.load().raftinfer_amd_paged_prefill_workspace_bytes(shape.c(), ctypes.byref(out)))
+    return out.value
+
+
+def qwen35_paged_cache_append(query, key, value, query_output, pages, page_table, query_starts,
+                              context_lengths, frequencies, query_weight, key_weight,
+                              shape: Qwen35PagedShape, rotary: Qwen35PagedRotary, cache_layout: int,
+                              activation_dtype: int = DTYPE_BF16, weight_dtype=None, stream=None,
+                              pages_bytes=None) -> None:
+    """The batch's queries normalised and turned to query_output, its keys (likewise) and values to
+    their positions in the pages."""
+    if weight_dtype is None:
+        weight = query_weight if query_weight is not None else key_weight
+        weight_dtype = DTYPE_BF16 if weight is None else _dtype_code(weight)
+    _checked(_lib.load().raftinfer_amd_paged_cache_append(
+        _raw(query), _raw(key), _raw(value), _raw(query_output), _raw(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table), _raw(query_starts),
+        _raw(context_lengths), _raw(frequencies), _raw(query_weight), _raw(key_weight), shape.c(),
+        PagedRotary(rotary.rotary_dim, rotary.interleaved, rotary.magnitude, rotary.epsilon,
+                    *_strides(query), *_strides(key), *_strides(value), *_strides(query_output)),
+        activation_dtype, weight_dtype, cache_layout, _stream_of(stream, key)))
+
+
+def qwen35_paged_attention_prefill(query, gate, output, pages, page_table, query_starts,
+                                   context_lengths, workspace, shape: Qwen35PagedShape,
+                                   cache_layout: int, activation_dtype: int = DTYPE_BF16, stream=None,
+                                   pages_bytes=None, workspace_bytes=None) -> None:
+    """Attention of every sequence's new tokens over its pages; gate None: no gate."""
+    _checked(_lib.load().raftinfer_amd_paged_attention_prefill(
+        _raw(query), _raw(gate), _raw(output), _raw(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table), _raw(query_starts),
+        _raw(context_lengths), _raw(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
+        cache_layout, _stream_of(stream, query)))
+
+
+def qwen35_paged_attention_decode(query, gate, output, pages, page_table, context_lengths, workspace,
+                                  shape: Qwen35PagedShape, cache_layout: int,
+                                  activation_dtype: int = DTYPE_BF16, stream=None, pages_bytes=None,
+                                  workspace_bytes=None) -> None:
+    """The same for one new token of every sequence; a context length of 0: an unused row."""
+    _checked(_lib.load().raftinfer_amd_paged_attention_decode(
+        _raw(query), _raw(gate), _raw(output), _raw(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table),
+        _raw(context_lengths), _raw(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
+        cache_layout, _stream_of(stream, query)))
 
 
 def qwen35_gated_delta(input, conv_weight, recurrent_a, dt_bias, output_norm_weight, output,

@@ -1,0 +1,220 @@
+"""CPU tests of rotary positions and the paged KV cache: frequencies, sizes, refusals before any launch."""
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+import paged_reference as ref
+from raftinfer_amd import ops
+from test_boundary import FakeTensor
+
+P, R, Q = ops.Qwen35PagedShape, ops.Qwen35PagedRotary, ops.Qwen35RotaryShape
+MODEL = P(rows=40, sequences=3, query_heads=16, kv_heads=4, head_dim=256, pages=100, page_tokens=16, table_pages=20,
+          max_context_tokens=320)
+STEP = dataclasses.replace(MODEL, rows=3)
+SCALINGS = {"none": ops.SCALING_NONE, "linear": ops.SCALING_LINEAR, "pair": ops.SCALING_BY_PAIR, "turns": ops.SCALING_BY_TURNS}
+
+
+def spaced(count):
+    """Arguments 1 TiB apart, so that none overlaps another."""
+    return [FakeTensor(addr=(i + 1) << 40, nbytes=1 << 39) for i in range(count)]
+
+
+@pytest.mark.parametrize("scaling", list(SCALINGS))
+@pytest.mark.parametrize("rotary,base,factor,trained", [(64, 1e7, 8.0, 32768.0), (2, 1e4, 2.0, 100.0), (256, 5e5, 32.0, 8192.0),
+                                                       (128, 1e4, 1.0, 4096.0)])
+def test_frequencies(scaling, rotary, base, factor, trained):
+    got, magnitude = ops.qwen35_rotary_frequencies(rotary, base, SCALINGS[scaling], factor, trained, 32.0, 1.0)
+    want, m = ref.frequencies(rotary, base, scaling, factor, trained)
+    assert np.allclose(got, want, rtol=1e-13, atol=0) and abs(magnitude - m) <= 2.0 ** -24 * m
+    assert len(got) == rotary // 2
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"rotary_dim": 0}, "rotary_dim must be even"), ({"rotary_dim": 3}, "rotary_dim must be even"), ({"rotary_dim": 16386}, "rotary_dim"),
+    ({"base": 1.0}, "base"), ({"base": float("nan")}, "base"), ({"scaling": 4}, "unsupported rotary scaling"),
+    ({"factor": 0.5}, "factor"), ({"factor": float("inf")}, "factor"), ({"trained_tokens": 0.0}, "trained_tokens"),
+    ({"slow_turns": 32.0}, "turns"), ({"slow_turns": 0.0}, "turns")])
+def test_frequencies_refusals(change, message):
+    args = {"rotary_dim": 64, "base": 1e7, "scaling": ops.SCALING_BY_PAIR, "factor": 2.0, "trained_tokens": 100.0, **change}
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_rotary_frequencies(**args)
+
+
+def test_sizes():
+    assert ops.qwen35_paged_cache_bytes(MODEL) == 100 * 2 * 4 * 16 * 256 * 2
+    # contexts that no call splits need nothing
+    assert ops.qwen35_paged_decode_workspace_bytes(dataclasses.replace(STEP, max_context_tokens=16)) == 0
+    long = dataclasses.replace(STEP, table_pages=5000, max_context_tokens=80000)
+    assert 0 < ops.qwen35_paged_decode_workspace_bytes(long) < 64 << 20
+    # a window bounds what is split
+    assert ops.qwen35_paged_decode_workspace_bytes(dataclasses.replace(long, window_tokens=10)) == 0
+    more = dataclasses.replace(MODEL, rows=4000, table_pages=5000, max_context_tokens=80000)
+    assert 0 < ops.qwen35_paged_prefill_workspace_bytes(more) < 512 << 20
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"rows": 0}, "rows must be positive"), ({"sequences": 0}, "sequences"), ({"sequences": 65536, "rows": 65536}, "sequences"),
+    ({"kv_heads": 0}, "kv_heads"), ({"kv_heads": 1025, "query_heads": 1025}, "kv_heads"), ({"query_heads": 0}, "query_heads"),
+    ({"query_heads": 6}, "query_heads"), ({"query_heads": 68}, "query_heads"), ({"head_dim": 128}, "head_dim must be 256"),
+    ({"rows": 2 ** 18 + 1}, "query rows"), ({"page_tokens": 0}, "page_tokens"), ({"page_tokens": 24}, "page_tokens"),
+    ({"pages": 0}, "pages must be"), ({"pages": 2 ** 24 + 1}, "pages must be"), ({"table_pages": 0}, "table_pages"),
+    ({"max_context_tokens": 0}, "max_context_tokens"), ({"max_context_tokens": 321}, "max_context_tokens"),
+    ({"max_context_tokens": 2 ** 28 + 1, "table_pages": 2 ** 27}, "max_context_tokens")])
+def test_shape_refusals(change, message):
+    shape = dataclasses.replace(MODEL, **change)
+    a = spaced(9)
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_paged_attention_prefill(*a[:7], a[7], shape, 1, stream=0x1234)
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_paged_cache_append(*a, None, None, shape, R(64), 1, stream=0x1234)
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_paged_cache_bytes(shape)
+
+
+@pytest.mark.parametrize("call", ["prefill", "decode"])
+def test_attention_refusals(call):
+    prefill = call == "prefill"
+    shape = MODEL if prefill else STEP
+    shape = dataclasses.replace(shape, pages=10000, table_pages=5000, max_context_tokens=80000)
+    names = ["query", "gate", "output", "pages", "page_table"] + ["query_starts"] * prefill + ["context_lengths", "workspace"]
+    fn = getattr(ops, f"qwen35_paged_attention_{call}")
+
+    def go(layout=1, act=ops.DTYPE_BF16, stream=0x1234, shape=shape, sizes={}, **put):
+        a = dict(zip(names, spaced(len(names))))
+        a.update(put)
+        fn(*a.values(), shape, layout, act, stream=stream, **sizes)
+
+    refused = lambda message: pytest.raises(ops.Qwen35PrimitiveError, match=message)  # noqa: E731
+    for name in names:
+        if name != "gate":
+            with refused(f"{name} .*is null|{name} is null"):
+                go(**{name: None})
+        align = 16 if name in ("query", "gate", "output", "pages", "workspace") else 4
+        with refused("aligned"):
+            go(**{name: FakeTensor(addr=(77 << 40) + align // 2, nbytes=1 << 39)})
+    with refused("stream is null"):
+        go(stream=0)
+    with refused("layout"):
+        go(layout=2)
+    with refused("must be bf16"):
+        go(act=ops.DTYPE_F16)
+    with refused("cache is too small"):
+        go(sizes={"pages_bytes": 10000 * 2 * 4 * 16 * 512 - 1})
+    need = getattr(ops, f"qwen35_paged_{call}_workspace_bytes")(shape)
+    with refused("workspace is too small"):
+        go(sizes={"workspace_bytes": need - 1})
+    for written in ("output", "workspace"):
+        for other in names:
+            if other != written:
+                with refused("overlap"):
+                    a = dict(zip(names, spaced(len(names))))
+                    go(**{written: a[other]})
+    if not prefill:
+        with refused("one row per sequence"):
+            go(shape=dataclasses.replace(shape, rows=4))
+        with refused("one row per sequence"):
+            ops.qwen35_paged_decode_workspace_bytes(dataclasses.replace(shape, rows=4))
+
+
+def test_strides_are_checked():
+    a = spaced(9)
+    rows, heads = STEP.rows, STEP.query_heads
+    for strides, message in [((heads * 256, 252, 1), "multiples of 8"), ((256, 256, 1), "output rows or heads overlap"),
+                             ((heads * 256, 128, 1), "output rows or heads overlap"), ((2 ** 62, 256, 1), "overflow")]:
+        out = FakeTensor(addr=50 << 40, nbytes=1 << 30)
+        out.ndim, out.shape, out.stride = 3, (rows, heads, 256), lambda s=strides: s
+        with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+            ops.qwen35_paged_attention_decode(a[0], a[1], out, *a[3:6], a[6], STEP, 1, stream=0x1234)
+    x = torch.empty(4, 16, 256, dtype=torch.bfloat16).transpose(1, 2)
+    with pytest.raises(ops.Qwen35PrimitiveError, match="contiguous"):
+        ops.qwen35_paged_attention_decode(x, *a[1:6], a[6], STEP, 1, stream=0x1234)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"rotary_dim": 258}, "rotary_dim"), ({"rotary_dim": 24}, "rotary_dim"), ({"rotary_dim": 12, "interleaved": True}, "rotary_dim"),
+    ({"rotary_dim": 0}, "frequencies go with"), ({"magnitude": float("nan")}, "magnitude"), ({"epsilon": -1.0}, "epsilon"),
+    ({"epsilon": float("inf")}, "epsilon")])
+def test_append_refuses_rotary(change, message):
+    a = spaced(9)
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_paged_cache_append(*a, None, None, MODEL, dataclasses.replace(R(64), **change), 1, stream=0x1234)
+
+
+def test_append_refusals():
+    names = ["query", "key", "value", "query_output", "pages", "page_table", "query_starts", "context_lengths", "frequencies",
+             "query_weight", "key_weight"]
+
+    def go(layout=1, act=ops.DTYPE_BF16, weight_dtype=ops.DTYPE_BF16, stream=0x1234, sizes={}, **put):
+        a = dict(zip(names, spaced(len(names))))
+        a.update(put)
+        ops.qwen35_paged_cache_append(*a.values(), MODEL, R(64), layout, act, weight_dtype, stream=stream, **sizes)
+
+    refused = lambda message: pytest.raises(ops.Qwen35PrimitiveError, match=message)  # noqa: E731
+    for name in ("key", "value", "pages", "page_table", "query_starts", "context_lengths"):
+        with refused(f"{name} pointer is null"):
+            go(**{name: None})
+    for name in ("query", "query_output"):
+        with refused("go together"):
+            go(**{name: None})
+    with refused("frequencies go with"):
+        go(frequencies=None)
+    for i, name in enumerate(names):
+        with refused("aligned"):
+            go(**{name: FakeTensor(addr=(77 << 40) + 1, nbytes=1 << 39)})
+    with refused("stream is null"):
+        go(stream=0)
+    with refused("layout"):
+        go(layout=9)
+    with refused("must be bf16"):
+        go(act=ops.DTYPE_F32)
+    with refused("weights must be"):
+        go(weight_dtype=ops.DTYPE_F16)
+    with refused("cache is too small"):
+        go(sizes={"pages_bytes": 100 * 2 * 4 * 16 * 512 - 1})
+    for written in ("query_output", "pages"):
+        for other in names:
+            if other != written:
+                with refused("overlap"):
+                    go(**{written: dict(zip(names, spaced(len(names))))[other]})
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"rows": 0}, "rows"), ({"rows": 2 ** 23}, "rows"), ({"heads": 0}, "heads"), ({"heads": 65536}, "heads"), ({"head_dim": 0}, "head_dim"),
+    ({"head_dim": 16385}, "head_dim"), ({"rotary_dim": 0}, "rotary_dim"), ({"rotary_dim": 63}, "rotary_dim"),
+    ({"rotary_dim": 258}, "rotary_dim"), ({"magnitude": float("inf")}, "magnitude")])
+def test_rotary_refuses_shapes(change, message):
+    x = torch.empty(8, dtype=torch.bfloat16)
+    a = spaced(5)
+    for t in a:
+        t.dtype = torch.bfloat16
+    with pytest.raises(ops.Qwen35PrimitiveError, match=message):
+        ops.qwen35_rotary(*a, dataclasses.replace(Q(10, 4, 256, 64), **change), 1e-6, stream=0x1234)
+
+
+def test_rotary_refusals():
+    def go(stream=0x1234, epsilon=1e-6, dtype=torch.bfloat16, wdt=torch.bfloat16, **put):
+        names = ["input", "weight", "output", "positions", "frequencies"]
+        a = dict(zip(names, spaced(5)))
+        a.update(put)
+        for k, t in a.items():
+            if t is not None:
+                t.dtype = wdt if k == "weight" else dtype
+        ops.qwen35_rotary(*a.values(), Q(10, 4, 256, 64), epsilon, stream=stream)
+
+    refused = lambda message: pytest.raises(ops.Qwen35PrimitiveError, match=message)  # noqa: E731
+    with refused("stream is null"):
+        go(stream=0)
+    with refused("epsilon"):
+        go(epsilon=float("nan"))
+    with refused("unsupported"):
+        go(dtype=torch.float64)
+    with refused("weight dtype"):
+        go(wdt=torch.float16)
+    for name in ("input", "weight", "output", "positions", "frequencies"):
+        with refused("aligned to their elements"):
+            go(**{name: FakeTensor(addr=(77 << 40) + 1, nbytes=1 << 39)})
+        if name != "output":  # one row of it lies in the output's
+            with refused("overlaps"):
+                go(**{name: FakeTensor(addr=(3 << 40) + 1024, nbytes=1 << 39)})

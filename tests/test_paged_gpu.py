@@ -1,0 +1,495 @@
+"""Rotary positions and the paged KV cache on the GPU, against the 64-bit reference."""
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+import paged_reference as ref
+from raftinfer_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+P = ops.Qwen35PagedShape
+
+
+def wide(t):
+    return t.detach().cpu().double().numpy()
+
+
+class Batch:
+    """A ragged batch over a shuffled pool.  each: (new tokens, context) of every sequence; places that no token may read
+    hold NaN, table entries that no call may use hold garbage."""
+
+    def __init__(self, each, kv_heads=4, group=4, page=16, head_major=True, window=0, gate=True, seed=0, lead=0, tail=0, spare=2,
+                 decode=False, scale=1.0):
+        g = self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.each, self.page, self.head_major, self.window = each, page, head_major, window
+        self.kv_heads, self.group, self.decode = kv_heads, group, decode
+        heads = kv_heads * group
+        self.rows = lead + sum(n for n, _ in each) + tail
+        need = [-(-c // page) for _, c in each]
+        pool = sum(need) + spare
+        starts = np.concatenate([[0], np.cumsum([n for n, _ in each])]) + lead
+        self.starts_host = starts
+        self.starts = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        self.lengths = torch.tensor([c for _, c in each], dtype=torch.int32, device="cuda")
+        where = torch.randperm(pool, generator=g, device="cuda", dtype=torch.int32).cpu().numpy()
+        width = max(max(need), 1) + 1
+        table = np.random.default_rng(seed).integers(-2 ** 31, 2 ** 31, (len(each), width)).astype(np.int32)
+        shape = (pool, 2, kv_heads, page, 256) if head_major else (pool, 2, page, kv_heads, 256)
+        pages = torch.full(shape, float("nan"), device="cuda", dtype=BF)
+        taken = 0
+        for i, ((n, c), k) in enumerate(zip(each, need)):
+            lo = max(0, c - n + 1 - window) if window else 0
+            for p in range(k):
+                if (p + 1) * page <= lo:
+                    taken += 1
+                    continue  # in front of the window: the entry names no page, the page holds NaN
+                table[i, p] = where[taken]
+                a, e = max(lo - p * page, 0), min(c - p * page, page)
+                x = torch.randn(2, kv_heads, e - a, 256, generator=g, device="cuda") * scale
+                x *= 1 + 7 * (torch.rand(2, kv_heads, e - a, 1, generator=g, device="cuda") < 0.02)
+                at = pages[int(where[taken])]
+                if head_major:
+                    at[:, :, a:e] = x.to(BF)
+                else:
+                    at[:, a:e] = x.transpose(1, 2).to(BF)
+                taken += 1
+        self.pages, self.table = pages, torch.tensor(table, device="cuda")
+        self.q = torch.randn(self.rows, heads, 256, generator=g, device="cuda").to(BF)
+        self.gate = torch.randn(self.rows, heads, 256, generator=g, device="cuda").to(BF) if gate else None
+        self.out = torch.full((self.rows, heads, 256), 7.0, device="cuda", dtype=BF)
+        self.shape = P(self.rows, len(each), heads, kv_heads, 256, pool, page, width, max(max(c for _, c in each), 1), window)
+
+    def workspace(self):
+        size = ops.qwen35_paged_decode_workspace_bytes if self.decode else ops.qwen35_paged_prefill_workspace_bytes
+        return torch.full((max(size(self.shape), 16),), 0xFF, device="cuda", dtype=torch.uint8)
+
+    def call(self, workspace=None, **kw):
+        ws = self.workspace() if workspace is None else workspace
+        layout = ops.HEAD_MAJOR if self.head_major else ops.TOKEN_MAJOR
+        shape = kw.pop("shape", self.shape)
+        if self.decode:
+            ops.qwen35_paged_attention_decode(self.q, self.gate, self.out, self.pages, self.table, self.lengths, ws, shape, layout, **kw)
+        else:
+            ops.qwen35_paged_attention_prefill(self.q, self.gate, self.out, self.pages, self.table, self.starts, self.lengths, ws, shape,
+                                               layout, **kw)
+        return self.out
+
+    def want(self, i):
+        """(rows, output, tolerance) of sequence i."""
+        n, c = self.each[i]
+        a = int(self.starts_host[i])
+        lo = max(0, c - n + 1 - self.window) if self.window else 0
+        table = self.table[i].cpu().numpy().copy()
+        table[:lo // self.page] = 0
+        kv = ref.rows_of(wide(self.pages), table, c, self.page, self.head_major)
+        gate = None if self.gate is None else wide(self.gate[a:a + n])
+        out, spread, reach = ref.attention(wide(self.q[a:a + n]), gate, kv, c, self.window)
+        return slice(a, a + n), out, ref.tolerance(out, spread, reach)
+
+    def check(self, only=None):
+        torch.cuda.synchronize()
+        got = wide(self.out)
+        touched = np.zeros(self.rows, bool)
+        for i, (n, _) in enumerate(self.each):
+            if n == 0 or (only is not None and i not in only):
+                continue
+            rows, want, tol = self.want(i)
+            touched[rows] = True
+            assert np.array_equal(np.isnan(got[rows]), np.isnan(want)), i
+            fine = np.isfinite(want)
+            assert np.array_equal(got[rows][~fine], want[~fine], equal_nan=True), i
+            off = np.abs(got[rows] - want)[fine] - tol[fine]
+            assert (off <= 0).all(), (i, self.each[i], off.max())
+        if only is None:
+            assert (got[~touched] == 7).all(), "rows of no sequence were written"
+
+
+def errors():
+    return ops.consume_capacity_errors()
+
+
+# ------------------------------------------------------------------- rotary
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, BF])
+@pytest.mark.parametrize("rows,heads,dim,rotary", [(1, 16, 256, 64), (37, 3, 256, 256), (5, 1, 128, 32), (9, 5, 80, 20), (3, 2, 96, 96),
+                                                   (2, 7, 64, 16), (1, 1, 2, 2), (4, 70, 256, 128), (2, 3, 1000, 400), (11, 2, 33, 30),
+                                                   (3, 4, 512, 512)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [None, "own", "f32"])
+def test_rotary(gpu, dtype, rows, heads, dim, rotary, interleaved, norm):
+    g = torch.Generator(device="cuda").manual_seed(rows * dim)
+    x = torch.randn(rows, heads, 2, dim, generator=g, device="cuda").to(dtype)[:, :, 1]  # strided
+    w = None if norm is None else (1 + 0.1 * torch.randn(dim, generator=g, device="cuda")).to(dtype if norm == "own" else torch.float32)
+    positions = torch.randint(0, 1 << 20, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    positions[0] = -1  # 2^32 - 1 as uint32
+    freq, magnitude = ops.qwen35_rotary_frequencies(rotary, 1e7, ops.SCALING_BY_PAIR, 4.0, 32768.0)
+    out = torch.full((heads, rows, dim), 9.0, device="cuda", dtype=dtype).transpose(0, 1)
+    shape = ops.Qwen35RotaryShape(rows, heads, dim, rotary, interleaved, magnitude)
+    f = torch.tensor(freq, dtype=torch.float64, device="cuda")
+    ops.qwen35_rotary(x, w, out, positions, f, shape, 1e-6)
+    torch.cuda.synchronize()
+    want = ref.rotate(wide(x), None if w is None else wide(w), positions.cpu().numpy().view(np.uint32), freq, magnitude, interleaved, 1e-6)
+    # sizes of a pair bound its two results; 32 bits: a norm's sum of dim squares, the reduced angle (up to pi, half a step of
+    # which is pi 2^-24) and its sine and cosine (2 steps), the products and the sum; the result is rounded once
+    pair = np.abs(ref.rotate(np.abs(wide(x)), None if w is None else np.abs(wide(w)), [0] * rows, freq, 1.0, interleaved, 1e-6))
+    n = rotary // 2
+    i, j = (np.arange(0, rotary, 2), np.arange(1, rotary, 2)) if interleaved else (np.arange(n), np.arange(n, rotary))
+    size = pair.copy()
+    size[..., i] = size[..., j] = (pair[..., i] + pair[..., j]) * magnitude
+    half = torch.finfo(dtype).eps / 2
+    tol = half * np.abs(want) + size * 2.0 ** -24 * (12 + (0 if w is None else dim / 2 + 4)) + torch.finfo(dtype).smallest_normal * half
+    assert (np.abs(wide(out) - want) <= tol).all()
+    # in place
+    same = x.clone() if dtype != BF else x
+    ops.qwen35_rotary(same, w, same, positions, f, shape, 1e-6)
+    torch.cuda.synchronize()
+    assert torch.equal(same, out)
+
+
+def test_rotary_at_zero_is_the_norm(gpu):
+    x = torch.randn(3, 4, 256, device="cuda").to(BF)
+    out = torch.empty_like(x)
+    f = torch.tensor(ops.qwen35_rotary_frequencies(64, 1e7)[0], dtype=torch.float64, device="cuda")
+    ops.qwen35_rotary(x, None, out, torch.zeros(3, dtype=torch.int32, device="cuda"), f, ops.Qwen35RotaryShape(3, 4, 256, 64), 1e-6)
+    torch.cuda.synchronize()
+    assert torch.equal(x, out)
+
+
+def test_rotary_matches_the_producer(gpu):
+    """The half layout without scaling is qwen35_qk_norm_rope at consecutive positions (both round once from 32 bits)."""
+    x, w = torch.randn(50, 4, 256, device="cuda").to(BF), (1 + 0.1 * torch.randn(256, device="cuda")).to(BF)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    ops.qwen35_qk_norm_rope(x, w, a, ops.QkNormRopeShape(50, 4, 256, 64, 1000, 1e7), 1e-6, 3, 3)
+    f = torch.tensor(ops.qwen35_rotary_frequencies(64, 1e7)[0], dtype=torch.float64, device="cuda")
+    ops.qwen35_rotary(x, w, b, torch.arange(1000, 1050, dtype=torch.int32, device="cuda"), f, ops.Qwen35RotaryShape(50, 4, 256, 64), 1e-6)
+    torch.cuda.synchronize()
+    # one step of bf16 where the 32-bit values straddle a border
+    assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * a.float().abs() + 1e-6).all() and (a == b).float().mean() > 0.999
+
+
+# ------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("head_major", [True, False])
+@pytest.mark.parametrize("each,page,kv_heads,group,rotary,interleaved,norm", [
+    ([(1, 1)], 16, 4, 4, 64, False, "bf16"), ([(5, 5), (1, 300), (0, 40), (33, 50)], 16, 4, 4, 64, False, "bf16"),
+    ([(17, 100), (1, 49)], 48, 3, 5, 256, True, "f32"), ([(64, 64)], 64, 1, 16, 32, False, None), ([(3, 10), (2, 2)], 32, 5, 1, 0, False, "q"),
+    ([(1, i + 1) for i in range(70)], 16, 2, 2, 128, True, "k")])
+def test_append(gpu, each, page, kv_heads, group, rotary, interleaved, norm, head_major):
+    b = Batch(each, kv_heads, group, page, head_major, seed=3, lead=2, tail=3)
+    before = b.pages.clone()
+    g, heads = b.g, kv_heads * group
+    proj = torch.randn(b.rows, heads, 2, 256, generator=g, device="cuda").to(BF)
+    k = torch.randn(kv_heads, b.rows, 256, generator=g, device="cuda").to(BF).transpose(0, 1)
+    v = torch.randn(b.rows, kv_heads + 1, 256, generator=g, device="cuda").to(BF)[:, 1:]
+    wq, wk = ((1 + 0.1 * torch.randn(256, generator=g, device="cuda")).to(torch.float32 if norm == "f32" else BF) for _ in (0, 1))
+    if norm in (None, "k"):
+        wq = None
+    if norm in (None, "q"):
+        wk = None
+    freq, magnitude = ops.qwen35_rotary_frequencies(rotary, 1e7, ops.SCALING_BY_TURNS, 8.0, 100.0) if rotary else ([], 1.0)
+    f = torch.tensor(freq, dtype=torch.float64, device="cuda") if rotary else None
+    out = torch.full((b.rows, heads, 256), 7.0, device="cuda", dtype=BF)
+    layout = ops.HEAD_MAJOR if head_major else ops.TOKEN_MAJOR
+    r = ops.Qwen35PagedRotary(rotary, interleaved, magnitude, 1e-6)
+    errors()
+    ops.qwen35_paged_cache_append(proj[:, :, 0], k, v, out, b.pages, b.table, b.starts, b.lengths, f, wq, wk, b.shape, r, layout)
+    torch.cuda.synchronize()
+    assert errors() == 0
+    expect, seen = wide(before), np.zeros(b.rows, bool)
+    got_q, got_pages = wide(out), wide(b.pages)
+    close = lambda x, y, ref_x: (np.abs(x - y) <= ref.HALF_BF16 * np.abs(y) + 2e-4 * np.abs(ref_x).max()).all()  # noqa: E731
+    table = b.table.cpu().numpy()
+    for i, (n, c) in enumerate(each):
+        a = int(b.starts_host[i])
+        seen[a:a + n] = True
+        at = np.arange(c - n, c)
+        turn = lambda x, w: ref.rotate(wide(x[a:a + n]), None if w is None else wide(w), at, freq, magnitude, interleaved, 1e-6)  # noqa: E731
+        if n:
+            y = turn(proj[:, :, 0], wq)
+            # (32 bits: 256 squares and a few roundings, 2e-5 of the largest value; 2e-4 leaves the angle's)
+            assert close(got_q[a:a + n], y, y)
+            y = turn(k, wk)
+            for t in range(n):
+                page_at, in_page = table[i, at[t] // page], at[t] % page
+                where = (page_at, slice(None), slice(None), in_page) if head_major else (page_at, slice(None), in_page)
+                assert close(got_pages[where][0], y[t], y) and np.array_equal(got_pages[where][1], wide(v[a + t]))
+                expect[where] = got_pages[where]
+    assert (got_q[~seen] == 7).all()
+    assert np.array_equal(got_pages, expect, equal_nan=True), "other places were written"
+    # without queries: the same pages
+    again = before.clone()
+    ops.qwen35_paged_cache_append(None, k, v, None, again, b.table, b.starts, b.lengths, f, None, wk, b.shape, r, layout)
+    torch.cuda.synchronize()
+    assert torch.equal(again.view(torch.int16), b.pages.view(torch.int16))
+
+
+def test_append_refuses_bad_sequences_on_the_device(gpu):
+    b = Batch([(3, 20), (3, 20), (3, 20), (3, 20), (3, 20)], seed=1)
+    b.lengths[0] = 2                              # below its new tokens
+    b.lengths[1] = b.shape.max_context_tokens + 1
+    b.table[2, 1] = b.shape.pages                 # the page of its positions 17 .. 19
+    b.table[3, 0] = -1                            # not needed: nothing is stored there
+    b.starts[5] = 99                              # behind the call's rows
+    k, v = (torch.randn(b.rows, 4, 256, device="cuda").to(BF) for _ in (0, 1))
+    before, out = b.pages.clone(), torch.full_like(b.q, 7.0)
+    errors()
+    ops.qwen35_paged_cache_append(b.q, k, v, out, b.pages, b.table, b.starts, b.lengths, None, None, None, b.shape,
+                                  ops.Qwen35PagedRotary(0), ops.HEAD_MAJOR)
+    torch.cuda.synchronize()
+    assert errors() >= 4
+    page = int(b.table[3, 1])
+    assert torch.equal(b.pages[page, 0, :, 1:4].transpose(0, 1), k[9:12]) and torch.equal(b.pages[page, 1, :, 1:4].transpose(0, 1), v[9:12])
+    b.pages[page] = before[page]
+    assert torch.equal(b.pages.view(torch.int16), before.view(torch.int16))
+    assert torch.equal(out[9:12], b.q[9:12]) and (out[:6] == 7).all() and (out[12:] == 7).all()
+
+
+# ---------------------------------------------------------------- attention
+
+RAGGED = [(1, 1), (2, 2), (0, 5), (16, 16), (17, 33), (1, 300), (40, 41), (5, 64)]
+
+
+@pytest.mark.parametrize("head_major", [True, False])
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("window", [0, 1, 20])
+def test_prefill_ragged(gpu, page, head_major, window):
+    b = Batch(RAGGED, page=page, head_major=head_major, window=window, lead=1, tail=2, seed=page)
+    b.call()
+    b.check()
+    assert errors() == 0
+
+
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (1, 16), (2, 3), (5, 7), (8, 2), (3, 12)])
+def test_prefill_heads(gpu, kv_heads, group):
+    b = Batch([(9, 40), (33, 70)], kv_heads, group, seed=group, gate=group != 3)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("n,c", [(1, 1), (15, 15), (31, 32), (32, 32), (33, 33), (64, 1000), (130, 700), (300, 300), (3, 1600), (200, 201)])
+@pytest.mark.parametrize("window", [0, 97])
+def test_prefill_lengths(gpu, n, c, window):
+    b = Batch([(n, c)], window=window, seed=n)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("each", [[(1, 1)], [(1, 15)], [(1, 16)], [(1, 17)], [(1, 3000)], [(1, c) for c in (1, 2, 700, 33, 64, 65, 1500)],
+                                  [(1, 7 * i + 1) for i in range(80)]])
+@pytest.mark.parametrize("page,head_major,window", [(16, True, 0), (80, False, 0), (32, True, 50)])
+def test_decode(gpu, each, page, head_major, window):
+    b = Batch(each, page=page, head_major=head_major, window=window, decode=True, seed=len(each), gate=window == 0)
+    b.call()
+    b.check()
+    assert errors() == 0
+
+
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (1, 16), (2, 3), (5, 7), (32, 1)])
+def test_decode_heads(gpu, kv_heads, group):
+    b = Batch([(1, 100), (1, 9)], kv_heads, group, decode=True, seed=group)
+    b.call()
+    b.check()
+
+
+def test_decode_leaves_unused_rows(gpu):
+    b = Batch([(1, 50), (1, 40), (1, 30)], decode=True, seed=5)
+    b.lengths[1] = 0
+    b.call()
+    b.check(only=(0, 2))
+    assert (b.out[1] == 7).all() and errors() == 0
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_bad_sequences_are_nan_and_counted(gpu, decode):
+    n = 1 if decode else 3
+    b = Batch([(n, 60), (n, 70), (n, 80), (n, 90), (n, 100)], decode=decode, seed=8)
+    top = b.shape.max_context_tokens
+    b.lengths[1] = top + 1
+    b.table[3, 2] = b.shape.pages
+    if not decode:
+        b.lengths[0] = 2          # below its new tokens
+        b.starts[5] = 1000        # behind the call's rows
+    errors()
+    b.call()
+    b.check(only=(2,) if not decode else (0, 2, 4))
+    assert errors() >= (2 if decode else 4)
+    bad = [1, 3] if decode else [0, 1, 3, 4]
+    for i in bad:
+        assert torch.isnan(b.out[n * i:n * i + n]).all(), i
+
+
+def test_falling_starts_write_nothing_else(gpu):
+    b = Batch([(4, 30), (4, 30), (4, 30)], seed=2, tail=4)
+    b.starts[1] = 9  # sequence 0 takes rows 0 .. 8, 1 falls from 9 to 8
+    b.lengths[0] = 30
+    errors()
+    b.call()
+    torch.cuda.synchronize()
+    rows, want, tol = b.want(2)
+    assert (np.abs(wide(b.out[9:12]) - want[1:]) <= tol[1:]).all()
+    assert errors() >= 1 and (b.out[12:] == 7).all()
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_odd_values_reach_only_who_sees_them(gpu, decode, value):
+    """An infinite or NaN V value of a seen key goes to the tokens that see it, and to no other; so do NaN keys."""
+    b = Batch([(1, 40), (1, 70)] if decode else [(20, 40), (45, 70), (3, 16)], decode=decode, seed=4, scale=0.2)
+    for i, j in ((0, 39), (1, 60), (1, 3)):
+        page, at = int(b.table[i, j // 16]), j % 16
+        b.pages[page, 1, i, at, 17 + i] = value
+    b.call()
+    b.check()
+    b.pages[int(b.table[0, 2]), 0, 1, 35 - 32] = float("nan")
+    b.out.fill_(7)
+    b.call()
+    b.check()
+
+
+def test_strided_tensors(gpu):
+    """Query and gate as the projection leaves them, [rows][heads][query, gate][256]; heads-first output."""
+    b = Batch([(20, 50), (3, 9)], seed=6)
+    proj = torch.stack((b.q, b.gate), 2).contiguous()
+    b.q, b.gate = proj[:, :, 0], proj[:, :, 1]
+    b.out = torch.full((16, b.rows, 256), 7.0, device="cuda", dtype=BF).transpose(0, 1)
+    b.call()
+    b.check()
+
+
+def test_another_stream_and_two_at_once(gpu):
+    a, b = Batch([(30, 400)], seed=1), Batch([(1, 500), (1, 2000)], seed=2, decode=True)
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    wa, wb = a.workspace(), b.workspace()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        a.call(wa, stream=s)
+        b.call(wb, stream=t)
+    torch.cuda.synchronize()
+    a.check()
+    b.check()
+
+
+def test_shared_pages(gpu):
+    """Two sequences whose first pages are the same."""
+    b = Batch([(2, 64), (3, 60)], seed=9)
+    b.table[1, :3] = b.table[0, :3]
+    b.call()
+    b.check()
+
+
+def test_largest_scores_and_values(gpu):
+    """Probabilities stay at most 1 while the maximum grows along the keys: 400 values of 2^119 sum to less than 2^128."""
+    b = Batch([(1, 400)], decode=True, seed=3)
+    top = 2.0 ** 119
+    table = b.table.cpu().numpy()
+    for j in range(400):
+        b.pages[int(table[0, j // 16]), 0, :, j % 16] = b.q[0, ::4].float().mul(j / 400).to(BF)
+        b.pages[int(table[0, j // 16]), 1, :, j % 16] = top
+    b.gate.fill_(100.0)
+    b.call()
+    torch.cuda.synchronize()
+    assert (b.out == top).all()
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_graph_replays(gpu, decode):
+    """One captured graph follows the device's lengths, tables and starts, also between eager calls on another workspace."""
+    each = [(1, 900), (1, 33)] if decode else [(40, 900), (7, 33)]
+    b = Batch(each, decode=decode, seed=11)
+    b.shape = dataclasses.replace(b.shape, max_context_tokens=b.shape.table_pages * b.page)
+    ws, eager_ws = b.workspace(), b.workspace()
+    b.call(ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=gpu):
+        b.call(ws, stream=torch.cuda.current_stream())
+    for step in range(4):
+        b.out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check()
+        got = b.out.clone()
+        b.out.fill_(7)
+        b.call(eager_ws)
+        torch.cuda.synchronize()
+        assert torch.equal(got, b.out)
+        # the longer sequence ends earlier
+        n, c = b.each[0]
+        c = c // 3 + n
+        b.each = [(n, c)] + b.each[1:]
+        b.lengths[0] = c
+
+
+def test_step_of_a_server(gpu):
+    """Append and attention over three steps (prompts, chunks with single tokens, single tokens) equal attention over the
+    whole sequences at once."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    total, page, hkv, hq = [75, 40, 130], 16, 4, 16
+    x = [[torch.randn(t, h, 256, generator=g, device="cuda").to(BF) for h in (hq, hkv, hkv, hq)] for t in total]
+    freq, m = ops.qwen35_rotary_frequencies(64, 1e7, ops.SCALING_BY_PAIR, 2.0, 64.0)
+    f = torch.tensor(freq, dtype=torch.float64, device="cuda")
+    wq, wk = ((1 + 0.1 * torch.randn(256, generator=g, device="cuda")).to(BF) for _ in (0, 1))
+    table = torch.randperm(30, generator=g, device="cuda", dtype=torch.int32).view(3, 10)
+    pages = torch.full((30, 2, hkv, page, 256), float("nan"), device="cuda", dtype=BF)
+    done, outs = [0, 0, 0], [[], [], []]
+    for new in ([30, 40, 1], [44, 0, 128], [1, 0, 1]):
+        rows, live = sum(new), [i for i in range(3) if new[i]]
+        parts = [torch.cat([x[i][k][done[i]:done[i] + new[i]] for i in range(3)]) for k in range(4)]
+        done = [d + n for d, n in zip(done, new)]
+        starts = torch.tensor([0, new[0], new[0] + new[1], rows], dtype=torch.int32, device="cuda")
+        lengths = torch.tensor(done, dtype=torch.int32, device="cuda")
+        q, out = torch.empty_like(parts[0]), torch.empty_like(parts[0])
+        shape = P(rows, 3, hq, hkv, 256, 30, page, 10, 160)
+        ops.qwen35_paged_cache_append(parts[0], parts[1], parts[2], q, pages, table, starts, lengths, f, wq, wk, shape,
+                                      ops.Qwen35PagedRotary(64, False, m), ops.HEAD_MAJOR)
+        if max(new) == 1:
+            only = torch.tensor(live, device="cuda")
+            shape = P(rows, rows, hq, hkv, 256, 30, page, 10, 160)
+            ws = torch.empty(max(16, ops.qwen35_paged_decode_workspace_bytes(shape)), device="cuda", dtype=torch.uint8)
+            ops.qwen35_paged_attention_decode(q, parts[3], out, pages, table[only].contiguous(), lengths[only].contiguous(), ws, shape, ops.HEAD_MAJOR)
+        else:
+            ws = torch.empty(max(16, ops.qwen35_paged_prefill_workspace_bytes(shape)), device="cuda", dtype=torch.uint8)
+            ops.qwen35_paged_attention_prefill(q, parts[3], out, pages, table, starts, lengths, ws, shape, ops.HEAD_MAJOR)
+        torch.cuda.synchronize()
+        for i in range(3):
+            a = sum(new[:i])
+            outs[i].append(out[a:a + new[i]])
+    for i in range(3):
+        at = np.arange(total[i])
+        turn = lambda y, w: torch.tensor(ref.rotate(wide(y), wide(w), at, freq, m, False, 1e-6)).to(BF).double().numpy()  # noqa: E731
+        k = turn(x[i][1], wk)
+        kv = np.stack([k, wide(x[i][2])]).transpose(0, 2, 1, 3)
+        want, spread, reach = ref.attention(turn(x[i][0], wq), wide(x[i][3]), kv, total[i])
+        # queries and keys can be rounded to a neighbour of the reference's: 2^-8 of each product, of which some are off
+        loose = 2.0 ** -7 * 16 * np.abs(want).max()
+        assert (np.abs(wide(torch.cat(outs[i])) - want) <= ref.tolerance(want, spread, reach) + loose * 0.05).all()
+
+
+def test_offsets_beyond_4_gib(gpu):
+    """Rows behind 2^32 bytes of the pool, and a query tensor's rows far apart."""
+    page, hkv = 256, 4
+    pages = torch.zeros(5000, 2, hkv, page, 256, device="cuda", dtype=BF)  # 5.2 GB
+    b = Batch([(2, 300)], page=page, seed=12, spare=0)
+    pages[4998:5000] = b.pages
+    b.table[0, :2] += 4998
+    b.pages = pages
+    b.shape = dataclasses.replace(b.shape, pages=5000)
+    b.call()
+    torch.cuda.synchronize()
+    got = b.out.clone()
+    b.pages, b.table = pages[4998:].clone(), b.table - 4998
+    b.check()
+    b.shape = dataclasses.replace(b.shape, pages=2)
+    b.call()
+    torch.cuda.synchronize()
+    assert torch.equal(got, b.out)
+    k = torch.randn(2, hkv, 256, device="cuda").to(BF)
+    table = torch.tensor([[4999, 4998]], dtype=torch.int32, device="cuda")
+    ops.qwen35_paged_cache_append(None, k, k, None, pages, table, b.starts, b.lengths, None, None, None,
+                                  dataclasses.replace(b.shape, pages=5000, table_pages=2), ops.Qwen35PagedRotary(0), ops.HEAD_MAJOR)
+    torch.cuda.synchronize()
+    assert torch.equal(pages[4998, 0, :, 42:44].transpose(0, 1), k) and torch.equal(pages[4998, 1, :, 42:44].transpose(0, 1), k)
