@@ -27,6 +27,7 @@ OPERAND_WAIT_STATES = 2
 
 _INDEX = r"(0x[0-9a-f]+|\d+)"
 _REGISTER = re.compile(rf"\b([av])\[{_INDEX}:{_INDEX}\]|\b([av])\[?{_INDEX}\b")
+_LABEL = re.compile(r"^([\w.$]+):")
 _NOP = re.compile(r"^s_nop\s+(\d+)")
 
 
@@ -54,13 +55,27 @@ def _overlap(x, y) -> bool:
 
 def asm_mfma_hazards(assembly: str, owned_agprs: bool = False) -> list[str]:
     """The violations of the rules above (s_nop n counts n + 1 wait states, any
-    other instruction 1).  Code is followed in listing order, labels included,
-    so a fall-through is checked like straight-line code; a taken branch is not
-    followed (prefill_mfma_kernel drains its asm MFMAs before each loop
-    back-edge, prefill_wide_kernel has the next tile's first operand reads and
-    the max of its scores there).  Reads by other MFMAs are not checked: an
-    accumulator feeds only the next MFMA of its own chain, which the hardware's
-    dependency check covers."""
+    other instruction 1), along every path: what is under way at a branch reaches
+    its label too, and nothing falls through an unconditional one.  Reads by other
+    MFMAs are not checked: an accumulator feeds only the next MFMA of its own chain,
+    which the hardware's dependency check covers."""
+    arrivals: dict[str, tuple[dict, dict]] = {}
+    while True:
+        hazards, found = _one_pass(assembly, owned_agprs, arrivals)
+        if found == arrivals:
+            return hazards
+        arrivals = found
+
+
+def _merge(into: dict, entries) -> None:
+    for register, left, line in entries:
+        into[register, line] = max(into.get((register, line), 0), left)
+
+
+def _one_pass(assembly: str, owned_agprs: bool, arrivals):
+    """The hazards in listing order, entering each label with what falls into it and
+    with its arrivals; and the arrivals that this pass saw (a label's only grow)."""
+    found = {label: (dict(p), dict(w)) for label, (p, w) in arrivals.items()}
     hazards: list[str] = []
     pending: list[list] = []  # [destination, wait states left, line] of asm MFMAs
     written: list[list] = []  # [register, wait states left, line] of VALU writes
@@ -73,6 +88,14 @@ def asm_mfma_hazards(assembly: str, owned_agprs: bool = False) -> list[str]:
         if text.startswith(";;#ASMEND"):
             in_asm = False
             continue
+        label = _LABEL.match(text)
+        if label and label.group(1) in arrivals:
+            both = ({}, {})
+            _merge(both[0], [(tuple(r), left, line) for r, left, line in pending])
+            _merge(both[1], [(tuple(r), left, line) for r, left, line in written])
+            for mine, more in zip(both, arrivals[label.group(1)]):
+                _merge(mine, [(r, left, line) for (r, line), left in more.items()])
+            pending, written = ([[r, left, line] for (r, line), left in mine.items()] for mine in both)
         text = text.split(";")[0].strip()
         if not text or text.startswith(".") or text.endswith(":"):
             continue
@@ -104,10 +127,16 @@ def asm_mfma_hazards(assembly: str, owned_agprs: bool = False) -> list[str]:
         step = int(nop.group(1)) + 1 if nop else 1
         for entry in pending + written:
             entry[1] -= step
+        if opcode.startswith(("s_branch", "s_cbranch")):
+            to = found.setdefault(text.split()[1], ({}, {}))
+            _merge(to[0], [(tuple(r), left, line) for r, left, line in pending if left > 0])
+            _merge(to[1], [(tuple(r), left, line) for r, left, line in written if left > 0])
+        if opcode.startswith(("s_branch", "s_endpgm")):
+            pending, written = [], []
         pending = [e for e in pending if e[1] > 0]
         if issued is not None:
             pending.append([issued, RESULT_WAIT_STATES, number])
         written = [e for e in written if e[1] > 0]
         if not opcode.startswith("v_mfma"):
             written += [[r, OPERAND_WAIT_STATES, number] for r in _vector_writes(opcode, operands)]
-    return hazards
+    return hazards, found

@@ -46,7 +46,8 @@ def _compile(src: pathlib.Path) -> pathlib.Path:
 # Sources whose kernels issue MFMAs from inline asm; their gfx950 assembly is
 # checked for the hazards that the compiler cannot see (asm_check.py).  The
 # second entry: whether the kernel owns the accumulation registers by number.
-ASM_CHECKED = {"attention_prefill_mfma.hip": False, "attention_prefill_wide.hip": True}
+ASM_CHECKED = {"attention_prefill_mfma.hip": False, "attention_prefill_wide.hip": True,
+               "paged_prefill.hip": True}
 
 
 def _check_asm(name: str) -> None:

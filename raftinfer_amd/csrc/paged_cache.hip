@@ -178,6 +178,8 @@ PagedArgs to_args(const Qwen35PagedShape &s, Qwen35KvCacheLayout layout) {
   a.sequences = u32(s.sequences);
   a.kv_heads = u32(s.kv_heads);
   a.group = u32(s.query_heads / s.kv_heads);
+  a.group_inverse = 65536 / a.group + 1;
+  a.group_inverse30 = (1u << 30) / a.group + 1;
   a.page_count = u32(s.pages);
   a.page_tokens = u32(s.page_tokens);
   a.table_pages = u32(s.table_pages);

@@ -24,6 +24,7 @@ struct PagedArgs {
   std::size_t q_row, q_head, g_row, g_head, o_row, o_head;
   std::uint32_t rows, sequences, kv_heads, group, page_count, page_tokens, table_pages, max_ctx, window;
   std::uint32_t row_step, head_step, plane_rows;
+  std::uint32_t group_inverse, group_inverse30; // 2^16 / group + 1, 2^30 / group + 1
   int page_shift; // log2 of page_tokens, or -1
 };
 
@@ -50,8 +51,10 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, std::uint32_t 
 
 // The page-table entry's place and the position in the page of position j.
 __device__ __forceinline__ void paged_place(const PagedArgs &a, std::uint32_t j, std::uint32_t &entry, std::uint32_t &in) {
-  entry = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_tokens;
-  in = j - entry * a.page_tokens;
+  std::uint32_t page = a.page_tokens;
+  asm volatile("" : "+s"(page)); // (no reciprocal of it is kept in registers)
+  if (a.page_shift >= 0) entry = j >> a.page_shift; else entry = j / page;
+  in = j - entry * page;
 }
 // The K row (512 bytes each, from the pool's first) of position j of a KV head; a bad page: `bad` is
 // set and page 0 taken.  (The host sees to it that the pool has fewer than 2^32 rows.)
@@ -68,15 +71,14 @@ __device__ __forceinline__ std::uint32_t paged_row(const PagedArgs &a, std::uint
 }
 
 // -------------------------------------------------------- dealing out the work
-// A column is a (token, head of the group) of one KV head; a workgroup takes block_cols
-// columns of a sequence and KV head, and of the tiles (of `unit` keys) that they see a
-// range.  All of a batch's workgroups deal the work out alike, each by itself, from the
+// A column is a (token, head of the group) of one KV head; a workgroup takes kCols columns
+// of a sequence and KV head, and of the tiles (of kUnit keys) that they see a range.  All of a batch's workgroups deal the work out alike, each by itself, from the
 // sequences' lengths: no launch in front, nothing kept.  The whole batch has W (column
 // block, tile) pairs; ranges have at most T = max(least, W / slots) tiles of a sequence's
 // longest block, so that about `slots` = 2^slot_bits workgroups per KV head run.  Integers
 // throughout: every kernel of a call finds the same.
 struct PagedSplit {
-  std::uint32_t block_cols, unit, least, slot_bits;
+  std::uint32_t least, slot_bits;
   std::uint32_t parts; // partial results that the workspace holds, each of a block and KV head
 };
 struct PagedScratch {
@@ -108,17 +110,17 @@ __device__ __forceinline__ std::uint32_t lane_u32(std::uint32_t x, int lane) {
 }
 
 // Tiles that a sequence's longest column block sees (at least 1), and its blocks.
-__device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSplit &sp, const PagedSeq &q, std::uint32_t &blocks,
-                                             std::uint32_t &tiles) {
-  blocks = (q.n * a.group + sp.block_cols - 1) / sp.block_cols;
+template <int kCols, int kUnit>
+__device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSeq &q, std::uint32_t &blocks, std::uint32_t &tiles) {
+  blocks = (q.n * a.group + kCols - 1) / kCols;
   if (!q.valid) {
     tiles = 1;
     return;
   }
-  tiles = (q.ctx + sp.unit - 1) / sp.unit;
+  tiles = (q.ctx + kUnit - 1) / kUnit;
   if (a.window != 0) { // the window and the tokens of a block, both ends inside tiles
-    const std::uint32_t span = (sp.block_cols + a.group - 2) / a.group + 1;
-    const std::uint32_t some = (a.window + (span < q.n ? span : q.n) + sp.unit - 3) / sp.unit + 1;
+    const std::uint32_t span = (kCols + a.group - 2) * a.group_inverse / 65536 + 1;
+    const std::uint32_t some = (a.window + (span < q.n ? span : q.n) + kUnit - 3) / kUnit + 1;
     tiles = some < tiles ? some : tiles;
   }
 }
@@ -126,6 +128,7 @@ __device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSpli
 // Finds item `index` of the batch (of_blocks: split column block `index`); false: there are
 // fewer.  By a whole wave, 64 sequences at a time; `count`: the caller is the one that counts bad
 // sequences.
+template <int kCols, int kUnit>
 __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, std::uint32_t index, bool of_blocks,
                                            unsigned int *count, PagedItem &item) {
   const std::uint32_t lane = threadIdx.x & 63;
@@ -136,7 +139,7 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
     blocks = 0;
     if (s0 + lane < a.sequences) {
       q = paged_seq(a, s0 + lane);
-      paged_extent(a, sp, q, blocks, tiles);
+      paged_extent<kCols, kUnit>(a, q, blocks, tiles);
       bad += !q.valid;
     }
     const std::uint64_t w = static_cast<std::uint64_t>(blocks) * tiles;
@@ -153,7 +156,7 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
       blocks = 0;
       if (s0 + lane < a.sequences) {
         q = paged_seq(a, s0 + lane);
-        paged_extent(a, sp, q, blocks, tiles);
+        paged_extent<kCols, kUnit>(a, q, blocks, tiles);
       }
     }
     const std::uint32_t ranges = (tiles + t - 1) / t;
@@ -181,36 +184,73 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
   return false;
 }
 
+// A value that is the same in every lane, in a scalar register (a quotient comes out of the
+// vector unit and would stay in a vector register).
+__device__ __forceinline__ std::uint32_t scalar(std::uint32_t x) {
+  return static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
 // A column block's tokens and keys, and its ranges of about equal length.
 struct PagedBlock {
   std::uint32_t col0, col_end;    // of its sequence's columns
   std::uint32_t tok0;             // first token
   std::uint32_t p_lo, p_hi;       // its tokens' positions
+  std::uint32_t first_key;        // that any of them sees
   std::uint32_t first, total;     // tiles
   std::uint32_t count, each, more; // ranges; the first `more` have a tile above `each`
-  __device__ __forceinline__ PagedBlock(const PagedArgs &a, const PagedSplit &sp, const PagedItem &it, std::uint32_t block) {
-    const std::uint32_t cols = it.seq.n * a.group, past = it.seq.ctx - it.seq.n;
-    col0 = block * sp.block_cols;
-    col_end = cols - col0 < sp.block_cols ? cols : col0 + sp.block_cols;
-    tok0 = col0 / a.group;
-    p_lo = past + tok0;
-    p_hi = past + (col_end - 1) / a.group;
-    first = (a.window != 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0) / sp.unit;
-    total = p_hi / sp.unit + 1 - first;
-    count = (total + it.range_tiles - 1) / it.range_tiles;
-    count = count < it.ranges ? count : it.ranges;
-    each = total / count;
-    more = total - each * count;
-  }
   __device__ __forceinline__ std::uint32_t begin(std::uint32_t i) const { return first + i * each + (i < more ? i : more); }
 };
+
+template <int kCols, int kUnit>
+__device__ __forceinline__ PagedBlock paged_block(const PagedArgs &a, const PagedItem &it, std::uint32_t block) {
+  // (columns are fewer than 2^22: the quotient is column * (2^30 / group + 1) >> 30)
+  const auto token = [&](std::uint32_t col) {
+    return static_cast<std::uint32_t>(static_cast<std::uint64_t>(col) * a.group_inverse30 >> 30);
+  };
+  const std::uint32_t cols = it.seq.n * a.group, past = it.seq.ctx - it.seq.n;
+  PagedBlock b;
+  b.col0 = block * kCols;
+  b.col_end = cols - b.col0 < kCols ? cols : b.col0 + kCols;
+  b.tok0 = token(b.col0);
+  b.p_lo = past + b.tok0;
+  b.p_hi = past + token(b.col_end - 1);
+  b.first_key = a.window != 0 && b.p_lo >= a.window ? b.p_lo - a.window + 1 : 0;
+  b.first = b.first_key / kUnit;
+  b.total = b.p_hi / kUnit + 1 - b.first;
+  b.count = 1;
+  b.each = b.total;
+  b.more = 0;
+  if (it.ranges > 1) {
+    b.count = scalar((b.total + it.range_tiles - 1) / it.range_tiles);
+    b.count = b.count < it.ranges ? b.count : it.ranges;
+    b.each = scalar(b.total / b.count);
+    b.more = b.total - b.each * b.count;
+  }
+  return b;
+}
 
 // Whether a token at position p sees key j.  (no branches)
 __device__ __forceinline__ bool paged_sees(std::uint32_t j, std::uint32_t p, std::uint32_t window) {
   return (j <= p) & ((window == 0) | (p - j < window));
 }
 
+// NaN to the rows of a block's columns.
+template <int kThreads>
+__device__ __forceinline__ void paged_fill_nan(const PagedArgs &a, const PagedItem &it, std::uint32_t col0, std::uint32_t cols,
+                                               std::uint32_t kvh) {
+  const std::uint32_t all = it.seq.n * a.group;
+  for (std::uint32_t i = threadIdx.x; i < cols * (kHeadDim / 2); i += kThreads) {
+    const std::uint32_t col = col0 + i / (kHeadDim / 2), d = i % (kHeadDim / 2);
+    if (col >= all) break;
+    const std::uint32_t tok = col / a.group, h = col - tok * a.group;
+    *reinterpret_cast<std::uint32_t *>(a.output + (it.seq.row0 + tok) * a.o_row + (kvh * a.group + h) * a.o_head + 2 * d) = 0x7FC07FC0u;
+  }
+}
+
 // ------------------------------------------------------------- launches
+// Chunks with much work (paged_prefill.hip).
+constexpr std::uint32_t kStreamBlockCols = 128, kStreamUnit = 32;
+void launch_paged_stream(const PagedArgs &a, const PagedScratch &sc, const PagedSplit &sp, std::uint32_t items,
+                         std::uint32_t split_blocks, unsigned int *bad_count, hipStream_t stream);
 std::size_t paged_decode_workspace(const PagedArgs &a);
 void paged_decode(const PagedArgs &a, void *workspace, hipStream_t stream);
 std::size_t paged_prefill_workspace(const PagedArgs &a);

@@ -37,18 +37,6 @@ __device__ __forceinline__ std::uint32_t cut_bf16x2(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
-// NaN to the rows of a block's columns.
-template <int kThreads> __device__ __forceinline__ void fill_nan(const PagedArgs &a, const PagedItem &it, std::uint32_t col0,
-                                                                 std::uint32_t cols, std::uint32_t kvh) {
-  const std::uint32_t all = it.seq.n * a.group;
-  for (std::uint32_t i = threadIdx.x; i < cols * (kHeadDim / 2); i += kThreads) {
-    const std::uint32_t col = col0 + i / (kHeadDim / 2), d = i % (kHeadDim / 2);
-    if (col >= all) break;
-    const std::uint32_t tok = col / a.group, h = col - tok * a.group;
-    *reinterpret_cast<std::uint32_t *>(a.output + (it.seq.row0 + tok) * a.o_row + (kvh * a.group + h) * a.o_head + 2 * d) = 0x7FC07FC0u;
-  }
-}
-
 // A workgroup takes 16 CB columns of one sequence and KV head and a range of their keys; wave
 // w takes the range's steps (16 keys) w, w + WAVES, ..  S = K q^T and O^T = V^T P^T on
 // v_mfma_f32_16x16x32_bf16, operands out of LDS, where LDS-direct loads put the rows as
@@ -61,26 +49,28 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void paged_rows_kernel(Pag
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col16 = lane & 15, kq = lane >> 4;
-  const std::uint32_t kvh = blockIdx.x % a.kv_heads;
+  const std::uint32_t index = scalar(blockIdx.x / a.kv_heads), kvh = blockIdx.x - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find(a, sp, blockIdx.x / a.kv_heads, false, blockIdx.x == 0 && wave == 0 ? &g_paged_capacity_errors : nullptr, it)) return;
-  const std::uint32_t block = it.blocks - 1 - it.local % it.blocks, range = it.local / it.blocks; // longest first
+  if (!paged_find<16 * CB, kPageGranule>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_paged_capacity_errors : nullptr, it)) return;
+  const std::uint32_t range = scalar(it.local / it.blocks), block = it.blocks - 1 - (it.local - range * it.blocks); // longest first
   if (!it.seq.valid) {
-    fill_nan<WAVES * kWave>(a, it, block * sp.block_cols, 16 * CB, kvh);
+    paged_fill_nan<WAVES * kWave>(a, it, block * 16 * CB, 16 * CB, kvh);
     return;
   }
-  const PagedBlock b(a, sp, it, block);
+  const PagedBlock b = paged_block<16 * CB, kPageGranule>(a, it, block);
   if (range >= b.count) return;
   const std::uint32_t begin = b.begin(range), end = b.begin(range + 1);
   const bool part = b.count > 1;
   const std::uint32_t slot = it.first_part + block * it.ranges + range;
   if (part && slot >= sp.parts) return; // (only where sequences share rows)
 
-  // Column x of the block (those past the last repeat it): its row of query, gate, output.
+  // Column x of the block (those past the last repeat it): its row of query, gate, output.  (The
+  // quotient of fewer than 2^8 columns from a token's first.)
+  const std::uint32_t in_first = b.col0 - b.tok0 * a.group, last_x = b.col_end - 1 - b.col0;
   const auto place = [&](std::uint32_t x, std::uint32_t &tok, std::uint32_t &head) {
-    const std::uint32_t col = b.col0 + x < b.col_end ? b.col0 + x : b.col_end - 1;
-    tok = col / a.group;
-    head = kvh * a.group + (col - tok * a.group);
+    const std::uint32_t c = in_first + (x < last_x ? x : last_x), t = c * a.group_inverse >> 16;
+    tok = b.tok0 + t;
+    head = kvh * a.group + (c - t * a.group);
   };
   bf16x8 qb[CB][8];
   std::uint32_t pos[CB];
@@ -340,15 +330,16 @@ __global__ __launch_bounds__(WAVES *kWave, 8 / WAVES) void paged_rows_kernel(Pag
 // Joins the ranges of the split column blocks: grid (columns of a block / (4 / W), split blocks times
 // KV heads); W waves per column take its ranges in turn, a lane four dims.
 constexpr int kMergeWaves = 4;
-template <int W>
+template <int CB, int W>
 __global__ __launch_bounds__(kMergeWaves *kWave) void paged_merge_kernel(PagedArgs a, PagedScratch sc, PagedSplit sp) {
   __shared__ float o_of[kMergeWaves][kHeadDim];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::uint32_t kvh = blockIdx.y % a.kv_heads;
+  constexpr std::uint32_t kCols = 16 * CB;
+  const std::uint32_t index = scalar(blockIdx.y / a.kv_heads), kvh = blockIdx.y - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find(a, sp, blockIdx.y / a.kv_heads, true, nullptr, it)) return;
-  const PagedBlock b(a, sp, it, it.local);
+  if (!paged_find<kCols, kPageGranule>(a, sp, index, true, nullptr, it)) return;
+  const PagedBlock b = paged_block<kCols, kPageGranule>(a, it, it.local);
   if (b.count == 1) return;
   const std::uint32_t x = blockIdx.x * (kMergeWaves / W) + wave / W, col = b.col0 + x;
   const bool mine = col < b.col_end;
@@ -356,8 +347,8 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void paged_merge_kernel(PagedAr
   const std::uint32_t part0 = it.first_part + it.local * it.ranges;
   if (part0 + b.count > sp.parts) return; // (only where sequences share rows)
   if (W > 1 && b.col0 + blockIdx.x * (kMergeWaves / W) >= b.col_end) return; // (uniform)
-  const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * sp.block_cols; // between parts
-  const std::size_t at0 = part0 * stride + static_cast<std::size_t>(kvh) * sp.block_cols + (mine ? x : b.col_end - 1 - b.col0);
+  const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * kCols; // between parts
+  const std::size_t at0 = part0 * stride + static_cast<std::size_t>(kvh) * kCols + (mine ? x : b.col_end - 1 - b.col0);
   const std::uint32_t tok = (mine ? col : b.col_end - 1) / a.group, head = kvh * a.group + ((mine ? col : b.col_end - 1) - tok * a.group);
   u32x2 g{};
   if (a.gate != nullptr) g = *reinterpret_cast<const u32x2 *>(a.gate + (it.seq.row0 + tok) * a.g_row + head * a.g_head + 4 * lane);
@@ -422,7 +413,7 @@ std::uint32_t floor_log2(std::uint32_t x) {
 Bounds bounds_of(const PagedArgs &a, std::uint32_t block_cols, std::uint32_t unit, std::uint32_t least, std::uint32_t workgroups) {
   Bounds r{};
   const std::uint32_t slot_bits = workgroups > a.kv_heads ? floor_log2(workgroups / a.kv_heads) : 0;
-  r.split = {block_cols, unit, least, slot_bits, 0};
+  r.split = {least, slot_bits, 0};
   const std::uint64_t seqs = std::min(a.sequences, a.rows);
   const std::uint64_t blocks = (static_cast<std::uint64_t>(a.rows) * a.group + seqs * (block_cols - 1)) / block_cols;
   std::uint64_t tiles = (static_cast<std::uint64_t>(a.max_ctx) + unit - 1) / unit;
@@ -433,46 +424,57 @@ Bounds bounds_of(const PagedArgs &a, std::uint32_t block_cols, std::uint32_t uni
   r.split.parts = ranges == 1 ? 0 : static_cast<std::uint32_t>(std::min(blocks * ranges, 2 * slots));
   return r;
 }
-PagedScratch scratch_of(const PagedArgs &a, const PagedSplit &sp, void *workspace, std::size_t *bytes) {
-  const std::size_t cols = static_cast<std::size_t>(sp.parts) * a.kv_heads * sp.block_cols;
+PagedScratch scratch_of(const PagedArgs &a, const PagedSplit &sp, std::uint32_t block_cols, void *workspace, std::size_t *bytes) {
+  const std::size_t cols = static_cast<std::size_t>(sp.parts) * a.kv_heads * block_cols;
   auto *p = static_cast<float *>(workspace);
   if (bytes != nullptr) *bytes = cols * (kHeadDim + 2) * sizeof(float);
   return {p, p + cols, p + 2 * cols};
 }
 
 Bounds decode_bounds(const PagedArgs &a) { return bounds_of(a, 16, kPageGranule, 32, 512); }
-Bounds prefill_bounds(const PagedArgs &a) { return bounds_of(a, 32, kPageGranule, 32, 512); }
+Bounds few_bounds(const PagedArgs &a) { return bounds_of(a, 32, kPageGranule, 32, 512); }
+Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols, kStreamUnit, 8, 256); }
+bool streams(const PagedArgs &a) { return a.rows * a.group >= 1024; }
 
-template <int W> void launch_merge(const PagedArgs &a, const PagedScratch &sc, const Bounds &bd, hipStream_t stream) {
+template <int CB, int W> void launch_merge(const PagedArgs &a, const PagedScratch &sc, const Bounds &bd, hipStream_t stream) {
   if (bd.split_blocks == 0) return;
-  const dim3 grid{bd.split.block_cols / (kMergeWaves / W), bd.split_blocks * a.kv_heads};
-  paged_merge_kernel<W><<<grid, kMergeWaves * kWave, 0, stream>>>(a, sc, bd.split);
+  const dim3 grid{16 * CB / (kMergeWaves / W), bd.split_blocks * a.kv_heads};
+  paged_merge_kernel<CB, W><<<grid, kMergeWaves * kWave, 0, stream>>>(a, sc, bd.split);
 }
 
 } // namespace
 
 std::size_t paged_decode_workspace(const PagedArgs &a) {
   std::size_t bytes = 0;
-  (void)scratch_of(a, decode_bounds(a).split, nullptr, &bytes);
+  (void)scratch_of(a, decode_bounds(a).split, 16, nullptr, &bytes);
   return bytes;
 }
 void paged_decode(const PagedArgs &a, void *workspace, hipStream_t stream) {
   const Bounds bd = decode_bounds(a);
-  const PagedScratch sc = scratch_of(a, bd.split, workspace, nullptr);
+  const PagedScratch sc = scratch_of(a, bd.split, 16, workspace, nullptr);
   paged_rows_kernel<1, 4, true><<<bd.items * a.kv_heads, 4 * kWave, 0, stream>>>(a, sc, bd.split);
-  launch_merge<4>(a, sc, bd, stream);
+  launch_merge<1, 4>(a, sc, bd, stream);
 }
 
 std::size_t paged_prefill_workspace(const PagedArgs &a) {
-  std::size_t bytes = 0;
-  (void)scratch_of(a, prefill_bounds(a).split, nullptr, &bytes);
-  return bytes;
+  std::size_t few = 0, much = 0;
+  (void)scratch_of(a, few_bounds(a).split, 32, nullptr, &few);
+  (void)scratch_of(a, stream_bounds(a).split, kStreamBlockCols, nullptr, &much);
+  return std::max(few, much);
 }
 void paged_prefill(const PagedArgs &a, void *workspace, hipStream_t stream) {
-  const Bounds bd = prefill_bounds(a);
-  const PagedScratch sc = scratch_of(a, bd.split, workspace, nullptr);
+  if (streams(a)) {
+    const Bounds bd = stream_bounds(a);
+    const PagedScratch sc = scratch_of(a, bd.split, kStreamBlockCols, workspace, nullptr);
+    void *count = nullptr;
+    if (hipGetSymbolAddress(&count, HIP_SYMBOL(g_paged_capacity_errors)) != hipSuccess) return;
+    launch_paged_stream(a, sc, bd.split, bd.items, bd.split_blocks, static_cast<unsigned int *>(count), stream);
+    return;
+  }
+  const Bounds bd = few_bounds(a);
+  const PagedScratch sc = scratch_of(a, bd.split, 32, workspace, nullptr);
   paged_rows_kernel<2, 4, false><<<bd.items * a.kv_heads, 4 * kWave, 0, stream>>>(a, sc, bd.split);
-  launch_merge<1>(a, sc, bd, stream);
+  launch_merge<2, 1>(a, sc, bd, stream);
 }
 
 std::uint32_t paged_take_capacity_errors() {
