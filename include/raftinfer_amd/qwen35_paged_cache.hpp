@@ -127,7 +127,8 @@ void qwen35_paged_cache_append(const void *query, const void *key, const void *v
 // sees, which the pages hold; gate null: without the sigmoid.  query, gate, output: bf16
 // [rows][query_heads][256].  Before the division by the softmax's sum the values are
 // summed in f32 with probabilities of at most 1: finite where |probability * value|
-// over a token's keys sums to less than 2^128.
+// over a token's keys sums to less than 2^128.  (The sums are held scaled down by up to
+// 2^16, so products below 2^-110 lose bits.)
 void qwen35_paged_attention_prefill(const void *query, const void *gate, void *output, const void *pages,
                                     std::size_t pages_bytes, const std::int32_t *page_table,
                                     const std::uint32_t *query_starts, const std::uint32_t *context_lengths,

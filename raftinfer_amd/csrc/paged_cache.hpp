@@ -75,10 +75,11 @@ __device__ __forceinline__ std::uint32_t paged_row(const PagedArgs &a, std::uint
 // of a sequence and KV head, and of the tiles (of kUnit keys) that they see a range.  All of a batch's workgroups deal the work out alike, each by itself, from the
 // sequences' lengths: no launch in front, nothing kept.  The whole batch has W (column
 // block, tile) pairs; ranges have at most T = max(least, W / slots) tiles of a sequence's
-// longest block, so that about `slots` = 2^slot_bits workgroups per KV head run.  Integers
-// throughout: every kernel of a call finds the same.
+// longest block, so that about `slots` = 2^slot_bits workgroups per KV head run; 2^many_bits
+// times as many for `many` sequences and more, whose blocks are of different lengths.
+// Integers throughout: every kernel of a call finds the same.
 struct PagedSplit {
-  std::uint32_t least, slot_bits;
+  std::uint32_t least, slot_bits, many, many_bits;
   std::uint32_t parts; // partial results that the workspace holds, each of a block and KV head
 };
 struct PagedScratch {
@@ -133,6 +134,7 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
                                            unsigned int *count, PagedItem &item) {
   const std::uint32_t lane = threadIdx.x & 63;
   std::uint64_t work = 0;
+  std::uint32_t live = 0;
   PagedSeq q{};
   std::uint32_t blocks = 0, tiles = 1, bad = 0;
   for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
@@ -143,12 +145,14 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
       bad += !q.valid;
     }
     const std::uint64_t w = static_cast<std::uint64_t>(blocks) * tiles;
+    live += __builtin_popcountll(__builtin_amdgcn_ballot_w64(blocks != 0));
     work += lane_u32(wave_prefix(static_cast<std::uint32_t>(w) & 0xFFFFFFu), 63);
     if (__builtin_amdgcn_ballot_w64(w >> 24 != 0) != 0)
       work += static_cast<std::uint64_t>(lane_u32(wave_prefix(static_cast<std::uint32_t>(w >> 24)), 63)) << 24;
   }
   if (count != nullptr && bad != 0) atomicAdd(count, bad);
-  const std::uint64_t share = (work + (std::uint64_t{1} << sp.slot_bits) - 1) >> sp.slot_bits;
+  const std::uint32_t bits = sp.slot_bits + (live >= sp.many ? sp.many_bits : 0);
+  const std::uint64_t share = (work + (std::uint64_t{1} << bits) - 1) >> bits;
   const std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
   std::uint32_t before = 0, parts_before = 0;
   for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
@@ -250,7 +254,8 @@ __device__ __forceinline__ void paged_fill_nan(const PagedArgs &a, const PagedIt
 // Chunks with much work (paged_prefill.hip).
 constexpr std::uint32_t kStreamBlockCols = 128, kStreamUnit = 32;
 void launch_paged_stream(const PagedArgs &a, const PagedScratch &sc, const PagedSplit &sp, std::uint32_t items,
-                         std::uint32_t split_blocks, unsigned int *bad_count, hipStream_t stream);
+                         std::uint32_t split_blocks, hipStream_t stream);
+std::uint32_t paged_take_stream_errors();
 std::size_t paged_decode_workspace(const PagedArgs &a);
 void paged_decode(const PagedArgs &a, void *workspace, hipStream_t stream);
 std::size_t paged_prefill_workspace(const PagedArgs &a);

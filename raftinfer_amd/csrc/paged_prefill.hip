@@ -8,6 +8,8 @@ namespace {
 
 using namespace prefill;
 
+__device__ unsigned int g_stream_capacity_errors = 0;
+
 // Two key groups of two waves; the waves of a group share its tiles, each has 64 columns of its
 // own.  A ring slot holds a tile's K or V: 32 rows of 512 bytes.  (One group of four waves, which
 // halves the bytes that go into LDS for a column, was no faster over long contexts, 1159 against 1151
@@ -28,7 +30,7 @@ __device__ __forceinline__ bool stream_masked(const PagedArgs &a, std::uint32_t 
 
 template <bool HeadMajor>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_stream_kernel(
-    PagedArgs a, PagedScratch sc, PagedSplit sp, unsigned int *bad_count) {
+    PagedArgs a, PagedScratch sc, PagedSplit sp) {
   constexpr int L = kLoads;
   __shared__ __attribute__((aligned(16384))) unsigned char sh[kGroups * kArea];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -36,7 +38,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int kg = wave % kGroups, cg = wave / kGroups; // key group, column group
   const std::uint32_t index = scalar(blockIdx.x / a.kv_heads), kvh = blockIdx.x - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<kStreamCols, kKTile>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? bad_count : nullptr, it)) return;
+  if (!paged_find<kStreamCols, kKTile>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_stream_capacity_errors : nullptr, it)) return;
   const std::uint32_t range = scalar(it.local / it.blocks), block = it.blocks - 1 - (it.local - range * it.blocks); // longest first
   if (!it.seq.valid) {
     paged_fill_nan<kThreads>(a, it, block * kStreamCols, kStreamCols, kvh);
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   max_of[128 * wave + kWave + le] = kg == 0 ? l_run[1] : l_run[0];
   auto *flag_of = lds_ptr<std::uint32_t>(lds0 + kFlagsAt);
   if (le == 0) flag_of[wave] = (odd != 0 ? 1u : 0u) | (bad != 0 ? 2u : 0u);
-  if ((bad != 0) & (le == 0)) atomicAdd(bad_count, 1u);
+  if ((bad != 0) & (le == 0)) atomicAdd(&g_stream_capacity_errors, 1u);
   float mm = kg == 0 ? m_run[0] : m_run[1], ll = kg == 0 ? l_run[0] : l_run[1]; // of column col_e
   floatx4 f[32]; // quad i: dims 8 i + 4 half_e .. + 3
   auto *to = lds_ptr<floatx4>(lds0 + 16384u * wave) + le;
@@ -608,11 +610,20 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void paged_stream_merge_kernel(P
 } // namespace
 
 void launch_paged_stream(const PagedArgs &a, const PagedScratch &sc, const PagedSplit &sp, std::uint32_t items,
-                         std::uint32_t split_blocks, unsigned int *bad_count, hipStream_t stream) {
-  const auto go = [&](auto kernel) { kernel<<<items * a.kv_heads, kThreads, 0, stream>>>(a, sc, sp, bad_count); };
+                         std::uint32_t split_blocks, hipStream_t stream) {
+  const auto go = [&](auto kernel) { kernel<<<items * a.kv_heads, kThreads, 0, stream>>>(a, sc, sp); };
   go(a.row_step == 1 ? paged_stream_kernel<true> : paged_stream_kernel<false>);
   if (split_blocks != 0)
     paged_stream_merge_kernel<<<dim3{kStreamCols / 32, split_blocks * a.kv_heads}, kJoinWaves * kWave, 0, stream>>>(a, sc, sp);
+}
+
+std::uint32_t paged_take_stream_errors() {
+  unsigned int value = 0;
+  const unsigned int zero = 0;
+  if (hipMemcpyFromSymbol(&value, HIP_SYMBOL(g_stream_capacity_errors), sizeof value) != hipSuccess ||
+      hipMemcpyToSymbol(HIP_SYMBOL(g_stream_capacity_errors), &zero, sizeof zero) != hipSuccess)
+    throw std::runtime_error("reading the capacity error counter failed");
+  return value;
 }
 
 } // namespace raftinfer::amd

@@ -493,3 +493,155 @@ def test_offsets_beyond_4_gib(gpu):
                                   dataclasses.replace(b.shape, pages=5000, table_pages=2), ops.Qwen35PagedRotary(0), ops.HEAD_MAJOR)
     torch.cuda.synchronize()
     assert torch.equal(pages[4998, 0, :, 42:44].transpose(0, 1), k) and torch.equal(pages[4998, 1, :, 42:44].transpose(0, 1), k)
+
+
+# ------------------------------------- chunks of much work, as far as the host can tell
+
+def roomy(b):
+    """The batch with a page table of a million positions, which makes a call take the kernel for chunks of much work."""
+    extra = (1 << 20) // b.page - b.table.shape[1]
+    garbage = torch.randint(-2 ** 31, 2 ** 31 - 1, (b.table.shape[0], extra), generator=b.g, device="cuda", dtype=torch.int64).to(torch.int32)
+    b.table = torch.cat([b.table, garbage], 1).contiguous()
+    b.shape = dataclasses.replace(b.shape, table_pages=b.table.shape[1], max_context_tokens=b.table.shape[1] * b.page)
+    return b
+
+
+@pytest.mark.parametrize("head_major", [True, False])
+@pytest.mark.parametrize("page", [16, 48, 64])
+def test_roomy_ragged(gpu, page, head_major):
+    errors()
+    b = Batch(RAGGED, page=page, head_major=head_major, lead=1, tail=2, seed=page)
+    roomy(b).call()
+    b.check()
+    assert errors() == 0
+
+
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (1, 16), (2, 3), (5, 7), (8, 2), (3, 12)])
+@pytest.mark.parametrize("head_major", [True, False])
+def test_roomy_heads(gpu, kv_heads, group, head_major):
+    b = Batch([(9, 40), (33, 70), (150, 400)], kv_heads, group, seed=group, gate=group != 3, head_major=head_major)
+    roomy(b).call()
+    b.check()
+
+
+@pytest.mark.parametrize("n,c", [(31, 32), (32, 32), (33, 33), (64, 1000), (130, 700), (300, 300), (40, 3000), (65, 2049), (257, 1025)])
+def test_roomy_lengths(gpu, n, c):
+    b = roomy(Batch([(n, c)], seed=n))
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("kv_heads,each,window,page,head_major", [
+    (8, [(600, 620), (33, 400), (80, 80), (1, 300)], 97, 16, True), (8, [(400, 900), (500, 501)], 66, 48, False),
+    (4, [(300, 1000), (1, 800), (260, 260), (40, 340)], 300, 32, True)])
+def test_roomy_window(gpu, kv_heads, each, window, page, head_major):
+    b = Batch(each, kv_heads, 16, page, head_major, window, seed=window, lead=2, tail=1)
+    rows = sum(n for n, _ in each)
+    assert rows * 16 * kv_heads * window > 40 * 2 ** 18 * 0.7
+    roomy(b).call()
+    b.check()
+
+
+def test_roomy_bad_sequences(gpu):
+    b = Batch([(9, 60), (9, 70), (9, 80), (9, 90), (9, 100)], seed=8)
+    b.table[3, 2] = b.shape.pages
+    roomy(b)
+    b.lengths[0] = 2              # below its new tokens
+    b.lengths[1] = b.shape.max_context_tokens + 1
+    b.starts[5] = 1000            # behind the call's rows
+    errors()
+    b.call()
+    b.check(only=(2,))
+    assert errors() >= 4
+    for i in [0, 1, 3, 4]:
+        assert torch.isnan(b.out[9 * i:9 * i + 9]).all(), i
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_roomy_odd_values(gpu, value):
+    b = Batch([(20, 40), (45, 70), (30, 36), (200, 400)], seed=4, scale=0.2)
+    for i, j in ((0, 39), (1, 60), (1, 3), (3, 130), (3, 350), (3, 399)):
+        b.pages[int(b.table[i, j // 16]), 1, i, j % 16, 17 + i] = value
+    roomy(b).call()
+    b.check()
+    b.pages[int(b.table[0, 2]), 0, 1, 35 - 32] = float("nan")
+    b.out.fill_(7)
+    b.call()
+    b.check()
+
+
+def test_roomy_strided_and_shared(gpu):
+    b = Batch([(64, 64), (33, 90), (60, 64)], seed=9)
+    b.table[2, :4] = b.table[0, :4]
+    proj = torch.stack((b.q, b.gate), 2).contiguous()
+    b.q, b.gate = proj[:, :, 0], proj[:, :, 1]
+    b.out = torch.full((16, b.rows, 256), 7.0, device="cuda", dtype=BF).transpose(0, 1)
+    roomy(b).call()
+    b.check()
+
+
+@pytest.mark.parametrize("chunk", [True, False])
+def test_values_of_every_size(gpu, chunk):
+    """Scores grow along the keys, so that the kept maximum moves; values near the smallest that keep their bits and near the largest."""
+    for size in (2.0 ** -96, 2.0 ** 118):
+        b = Batch([(40, 500)], seed=3)
+        if chunk:
+            roomy(b)
+        table = b.table.cpu().numpy()
+        mean = b.q[:, ::4].float().mean(0)
+        for j in range(500):
+            b.pages[int(table[0, j // 16]), 0, :, j % 16] = (mean * (j / 25)).to(BF)
+            b.pages[int(table[0, j // 16]), 1, :, j % 16] = b.pages[int(table[0, j // 16]), 1, :, j % 16].float().clamp(-1, 1).mul(size).to(BF)
+        b.call()
+        b.check()
+
+
+def test_roomy_two_at_once_on_streams(gpu):
+    a, b = roomy(Batch([(30, 400), (1, 90)], seed=1)), roomy(Batch([(77, 500), (90, 2000)], seed=2))
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    wa, wb = a.workspace(), b.workspace()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        a.call(wa, stream=s)
+        b.call(wb, stream=t)
+    torch.cuda.synchronize()
+    a.check()
+    b.check()
+
+
+def test_roomy_graph_replays(gpu):
+    b = roomy(Batch([(40, 900), (200, 333)], seed=11))
+    ws, eager_ws = b.workspace(), b.workspace()
+    b.call(ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=gpu):
+        b.call(ws, stream=torch.cuda.current_stream())
+    for step in range(4):
+        b.out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check()
+        got = b.out.clone()
+        b.out.fill_(7)
+        b.call(eager_ws)
+        torch.cuda.synchronize()
+        assert torch.equal(got, b.out)
+        n, c = b.each[0]
+        c = c // 3 + n
+        b.each = [(n, c)] + b.each[1:]
+        b.lengths[0] = c
+
+
+def test_same_sequence_in_every_kernel(gpu):
+    """A sequence's rows do not depend on what else is in the batch by more than the tolerance; the same call twice gives the same bits."""
+    b = Batch([(40, 900)], seed=13)
+    first = b.call().clone()
+    b.out.fill_(7)
+    assert torch.equal(b.call(), first)
+    roomy(b)
+    b.out.fill_(7)
+    second = b.call().clone()
+    b.check()
+    b.out.fill_(7)
+    assert torch.equal(b.call(), second)
