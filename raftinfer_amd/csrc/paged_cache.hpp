@@ -110,6 +110,12 @@ __device__ __forceinline__ std::uint32_t lane_u32(std::uint32_t x, int lane) {
   return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
 }
 
+// A value that is the same in every lane, in a scalar register (a quotient comes out of the
+// vector unit and would stay in a vector register).
+__device__ __forceinline__ std::uint32_t scalar(std::uint32_t x) {
+  return static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
+
 // Tiles that a sequence's longest column block sees (at least 1), and its blocks.
 template <int kCols, int kUnit>
 __device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSeq &q, std::uint32_t &blocks, std::uint32_t &tiles) {
@@ -126,10 +132,51 @@ __device__ __forceinline__ void paged_extent(const PagedArgs &a, const PagedSeq 
   }
 }
 
+template <int Ctrl, int RowMask> __device__ __forceinline__ std::uint32_t dpp_most(std::uint32_t x) {
+  const std::uint32_t y = dpp_zero<Ctrl, RowMask>(x);
+  return x > y ? x : y;
+}
+__device__ __forceinline__ std::uint32_t wave_most(std::uint32_t x) {
+  x = dpp_most<0x118, 0xF>(dpp_most<0x114, 0xF>(dpp_most<0x112, 0xF>(dpp_most<0x111, 0xF>(x))));
+  return lane_u32(dpp_most<0x143, 0xC>(dpp_most<0x142, 0xA>(x)), 63);
+}
+// Workgroups that fill a compute unit run in rounds of `slots`; ranges of an even share can end a few
+// above a round, which then costs as much as a whole one.  Among ranges of `share` tiles and more, and of half of
+// it and more (two rounds), those whose rounds times (length + start and end) are fewest.  Only where
+// a sequence's blocks are of about equal length: blocks that grow from little to much, longest first,
+// fill the rounds by themselves.  (16 query and 4 KV heads, without and with it: 300 tokens of 30000 284 and 190 us,
+// 900 of 4000 125 and 99, 1100 of 8000 254 and 210, 200 of 60000 359 and 241.)
+template <int kUnit>
+__device__ __forceinline__ std::uint32_t paged_rounds(const PagedSeq &q, std::uint32_t blocks, std::uint32_t tiles, std::uint32_t share,
+                                                      std::uint32_t bits, const PagedSplit &sp) {
+  constexpr std::uint32_t kEnds = 20; // tiles that a workgroup's start and end take as long as
+  const std::uint32_t front = (q.ctx - q.n) / kUnit + 1, lo = q.valid && front < tiles ? front : tiles, mid = (lo + tiles) / 2;
+  if (__builtin_amdgcn_ballot_w64(blocks > 1 && 2 * lo < tiles) != 0) return share;
+  const std::uint32_t most = wave_most(blocks != 0 ? tiles : 0);
+  std::uint32_t best = share, least_cost = ~0u;
+  for (std::uint32_t r = 0; r <= sp.many_bits; ++r) {
+    std::uint32_t t = (share + (1u << r) - 1) >> r; // (rounded up: items stay within blocks + `want`)
+    t = t > sp.least ? t : sp.least;
+    const std::uint32_t want = 1u << bits << r;
+    for (int i = 0; i < 4; ++i) {
+      const std::uint32_t ranges = (lo + t - 1) / t + 2 * ((mid + t - 1) / t) + (tiles + t - 1) / t;
+      const std::uint32_t items = lane_u32(wave_prefix(blocks * ranges), 63) / 4;
+      const std::uint32_t rounds = (items + (1u << bits) - 1) >> bits, cost = rounds * ((t < most ? t : most) + kEnds);
+      if (cost < least_cost) {
+        least_cost = cost;
+        best = t;
+      }
+      if ((items <= want) | (items >= 2 * want) | (t >= most)) break;
+      t = scalar(t + 1 + static_cast<std::uint32_t>(static_cast<std::uint64_t>(t) * (items - want) >> (bits + r)));
+    }
+  }
+  return best;
+}
+
 // Finds item `index` of the batch (of_blocks: split column block `index`); false: there are
 // fewer.  By a whole wave, 64 sequences at a time; `count`: the caller is the one that counts bad
 // sequences.
-template <int kCols, int kUnit>
+template <int kCols, int kUnit, bool kRounds = false>
 __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, std::uint32_t index, bool of_blocks,
                                            unsigned int *count, PagedItem &item) {
   const std::uint32_t lane = threadIdx.x & 63;
@@ -153,7 +200,8 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
   if (count != nullptr && bad != 0) atomicAdd(count, bad);
   const std::uint32_t bits = sp.slot_bits + (live >= sp.many ? sp.many_bits : 0);
   const std::uint64_t share = (work + (std::uint64_t{1} << bits) - 1) >> bits;
-  const std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
+  std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
+  if (kRounds && (a.sequences <= 64) & (live < sp.many)) t = paged_rounds<kUnit>(q, blocks, tiles, t, bits, sp);
   std::uint32_t before = 0, parts_before = 0;
   for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
     if (a.sequences > 64) {
@@ -188,11 +236,6 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
   return false;
 }
 
-// A value that is the same in every lane, in a scalar register (a quotient comes out of the
-// vector unit and would stay in a vector register).
-__device__ __forceinline__ std::uint32_t scalar(std::uint32_t x) {
-  return static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
-}
 // A column block's tokens and keys, and its ranges of about equal length.
 struct PagedBlock {
   std::uint32_t col0, col_end;    // of its sequence's columns

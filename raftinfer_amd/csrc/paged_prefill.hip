@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int kg = wave % kGroups, cg = wave / kGroups; // key group, column group
   const std::uint32_t index = scalar(blockIdx.x / a.kv_heads), kvh = blockIdx.x - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<kStreamCols, kKTile>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_stream_capacity_errors : nullptr, it)) return;
+  if (!paged_find<kStreamCols, kKTile, true>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_stream_capacity_errors : nullptr, it)) return;
   const std::uint32_t range = scalar(it.local / it.blocks), block = it.blocks - 1 - (it.local - range * it.blocks); // longest first
   if (!it.seq.valid) {
     paged_fill_nan<kThreads>(a, it, block * kStreamCols, kStreamCols, kvh);
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void paged_stream_merge_kernel(P
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const std::uint32_t index = scalar(blockIdx.y / a.kv_heads), kvh = blockIdx.y - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<kStreamCols, kKTile>(a, sp, index, true, nullptr, it)) return;
+  if (!paged_find<kStreamCols, kKTile, true>(a, sp, index, true, nullptr, it)) return;
   const PagedBlock b = paged_block<kStreamCols, kKTile>(a, it, it.local);
   const std::uint32_t x0 = 32 * blockIdx.x, part0 = it.first_part + it.local * it.ranges;
   if (b.count == 1 || b.col0 + x0 >= b.col_end) return;

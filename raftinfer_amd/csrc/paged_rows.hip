@@ -567,7 +567,7 @@ std::uint32_t floor_log2(std::uint32_t x) {
   return n;
 }
 Bounds bounds_of(const PagedArgs &a, std::uint32_t block_cols, std::uint32_t unit, std::uint32_t least, std::uint32_t workgroups,
-                 std::uint32_t many, std::uint32_t many_bits) {
+                 std::uint32_t many, std::uint32_t many_bits, bool rounds = false) {
   Bounds r{};
   const std::uint32_t slot_bits = workgroups > a.kv_heads ? floor_log2(workgroups / a.kv_heads) : 0;
   r.split = {least, slot_bits, many, many_bits, 0};
@@ -575,10 +575,10 @@ Bounds bounds_of(const PagedArgs &a, std::uint32_t block_cols, std::uint32_t uni
   const std::uint64_t blocks = (static_cast<std::uint64_t>(a.rows) * a.group + seqs * (block_cols - 1)) / block_cols;
   std::uint64_t tiles = (static_cast<std::uint64_t>(a.max_ctx) + unit - 1) / unit;
   if (a.window != 0) tiles = std::min<std::uint64_t>(tiles, (static_cast<std::uint64_t>(a.window) + block_cols + unit) / unit + 2);
-  const std::uint64_t ranges = (tiles + least - 1) / least, slots = std::uint64_t{1} << (slot_bits + (seqs >= many ? many_bits : 0));
+  const std::uint64_t ranges = (tiles + least - 1) / least, slots = std::uint64_t{1} << (slot_bits + (seqs >= many || rounds ? many_bits : 0));
   r.items = static_cast<std::uint32_t>(std::min(blocks * ranges, blocks + slots));
   r.split_blocks = ranges == 1 ? 0 : static_cast<std::uint32_t>(std::min(blocks, slots));
-  r.split.parts = ranges == 1 ? 0 : static_cast<std::uint32_t>(std::min(blocks * ranges, 2 * slots));
+  r.split.parts = ranges == 1 ? 0 : static_cast<std::uint32_t>(std::min({blocks * ranges, blocks + slots, 2 * slots}));
   return r;
 }
 PagedScratch scratch_of(const PagedArgs &a, const PagedSplit &sp, std::uint32_t block_cols, void *workspace, std::size_t *bytes) {
@@ -594,7 +594,7 @@ bool reads_once(const PagedArgs &a) {
   return static_cast<std::uint64_t>(a.sequences) * a.max_ctx * a.kv_heads * 2 * kRowBytes > (16u << 20);
 }
 Bounds few_bounds(const PagedArgs &a) { return bounds_of(a, FewForm::kCols, FewForm::kKeys, 16, 256, 8, 1); }
-Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols, kStreamUnit, 8, 256, 8, 1); }
+Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols, kStreamUnit, 8, 256, 8, 1, true); }
 // Which kernel a chunk takes, by the (column, key) pairs of all heads that the sequences can have: the
 // stream kernel fetches a key once for 128 columns and keeps the matrix units busy, but its start and end cost
 // about 15 us of every workgroup (ring, 256 accumulator registers, the joining of its key groups).  Up to 40
