@@ -84,6 +84,7 @@ struct PagedSplit {
 };
 struct PagedScratch {
   float *m, *l, *o; // [part][kv_head][column of the block]; o: 256 floats of each
+  std::uint32_t *plan; // where there are parts: tiles of a range, and split column blocks of a KV head
 };
 
 struct PagedItem {
@@ -140,74 +141,19 @@ __device__ __forceinline__ std::uint32_t wave_most(std::uint32_t x) {
   x = dpp_most<0x118, 0xF>(dpp_most<0x114, 0xF>(dpp_most<0x112, 0xF>(dpp_most<0x111, 0xF>(x))));
   return lane_u32(dpp_most<0x143, 0xC>(dpp_most<0x142, 0xA>(x)), 63);
 }
-// Workgroups that fill a compute unit run in rounds of `slots`; ranges of an even share can end a few
-// above a round, which then costs as much as a whole one.  Among ranges of `share` tiles and more, and of half of
-// it and more (two rounds), those whose rounds times (length + start and end) are fewest.  Only where
-// a sequence's blocks are of about equal length: blocks that grow from little to much, longest first,
-// fill the rounds by themselves.  (16 query and 4 KV heads, without and with it: 300 tokens of 30000 284 and 190 us,
-// 900 of 4000 125 and 99, 1100 of 8000 254 and 210, 200 of 60000 359 and 241.)
-template <int kUnit>
-__device__ __forceinline__ std::uint32_t paged_rounds(const PagedSeq &q, std::uint32_t blocks, std::uint32_t tiles, std::uint32_t share,
-                                                      std::uint32_t bits, const PagedSplit &sp) {
-  constexpr std::uint32_t kEnds = 20; // tiles that a workgroup's start and end take as long as
-  const std::uint32_t front = (q.ctx - q.n) / kUnit + 1, lo = q.valid && front < tiles ? front : tiles, mid = (lo + tiles) / 2;
-  if (__builtin_amdgcn_ballot_w64(blocks > 1 && 2 * lo < tiles) != 0) return share;
-  const std::uint32_t most = wave_most(blocks != 0 ? tiles : 0);
-  std::uint32_t best = share, least_cost = ~0u;
-  for (std::uint32_t r = 0; r <= sp.many_bits; ++r) {
-    std::uint32_t t = (share + (1u << r) - 1) >> r; // (rounded up: items stay within blocks + `want`)
-    t = t > sp.least ? t : sp.least;
-    const std::uint32_t want = 1u << bits << r;
-    for (int i = 0; i < 4; ++i) {
-      const std::uint32_t ranges = (lo + t - 1) / t + 2 * ((mid + t - 1) / t) + (tiles + t - 1) / t;
-      const std::uint32_t items = lane_u32(wave_prefix(blocks * ranges), 63) / 4;
-      const std::uint32_t rounds = (items + (1u << bits) - 1) >> bits, cost = rounds * ((t < most ? t : most) + kEnds);
-      if (cost < least_cost) {
-        least_cost = cost;
-        best = t;
-      }
-      if ((items <= want) | (items >= 2 * want) | (t >= most)) break;
-      t = scalar(t + 1 + static_cast<std::uint32_t>(static_cast<std::uint64_t>(t) * (items - want) >> (bits + r)));
-    }
-  }
-  return best;
-}
-
-// Finds item `index` of the batch (of_blocks: split column block `index`); false: there are
-// fewer.  By a whole wave, 64 sequences at a time; `count`: the caller is the one that counts bad
-// sequences.
-template <int kCols, int kUnit, bool kRounds = false>
-__device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, std::uint32_t index, bool of_blocks,
-                                           unsigned int *count, PagedItem &item) {
+// Item `index` (of_blocks: split column block `index`) of sequences with ranges of t tiles: q, id, blocks and
+// tiles are those of up to 64 sequences, or of the batch's first, which are then read again.
+template <int kCols, int kUnit>
+__device__ __forceinline__ bool paged_pick(const PagedArgs &a, std::uint32_t index, bool of_blocks, std::uint32_t t, PagedSeq q, std::uint32_t id,
+                                           std::uint32_t blocks, std::uint32_t tiles, PagedItem &item) {
   const std::uint32_t lane = threadIdx.x & 63;
-  std::uint64_t work = 0;
-  std::uint32_t live = 0;
-  PagedSeq q{};
-  std::uint32_t blocks = 0, tiles = 1, bad = 0;
-  for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
-    blocks = 0;
-    if (s0 + lane < a.sequences) {
-      q = paged_seq(a, s0 + lane);
-      paged_extent<kCols, kUnit>(a, q, blocks, tiles);
-      bad += !q.valid;
-    }
-    const std::uint64_t w = static_cast<std::uint64_t>(blocks) * tiles;
-    live += __builtin_popcountll(__builtin_amdgcn_ballot_w64(blocks != 0));
-    work += lane_u32(wave_prefix(static_cast<std::uint32_t>(w) & 0xFFFFFFu), 63);
-    if (__builtin_amdgcn_ballot_w64(w >> 24 != 0) != 0)
-      work += static_cast<std::uint64_t>(lane_u32(wave_prefix(static_cast<std::uint32_t>(w >> 24)), 63)) << 24;
-  }
-  if (count != nullptr && bad != 0) atomicAdd(count, bad);
-  const std::uint32_t bits = sp.slot_bits + (live >= sp.many ? sp.many_bits : 0);
-  const std::uint64_t share = (work + (std::uint64_t{1} << bits) - 1) >> bits;
-  std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
-  if (kRounds && (a.sequences <= 64) & (live < sp.many)) t = paged_rounds<kUnit>(q, blocks, tiles, t, bits, sp);
   std::uint32_t before = 0, parts_before = 0;
   for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
     if (a.sequences > 64) {
       blocks = 0;
-      if (s0 + lane < a.sequences) {
-        q = paged_seq(a, s0 + lane);
+      id = s0 + lane;
+      if (id < a.sequences) {
+        q = paged_seq(a, id);
         paged_extent<kCols, kUnit>(a, q, blocks, tiles);
       }
     }
@@ -222,7 +168,7 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
       item.seq.n = lane_u32(q.n, at);
       item.seq.ctx = lane_u32(q.ctx, at);
       item.seq.valid = lane_u32(q.valid, at) != 0;
-      item.id = s0 + at;
+      item.id = lane_u32(id, at);
       item.blocks = lane_u32(blocks, at);
       item.ranges = lane_u32(ranges, at);
       item.range_tiles = t;
@@ -234,6 +180,146 @@ __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit 
     parts_before = lane_u32(parts_upto, 63);
   }
   return false;
+}
+
+// Workgroups that fill a compute unit, `slots` of a KV head at once: the range length whose last workgroup
+// should end first, one candidate a lane, from half of the share to twice of it.  A candidate's cost is the
+// larger of the mean load, and over the sequences, which lie longest first, of ceil(N / slots) x: N items so far,
+// of x tiles and more (a workgroup's start and end among them), of which some place takes as many.  Not for a
+// sequence whose unsplit blocks grow from little to much, which fill places up by themselves.  (Measured beside
+// paged_find.)
+constexpr float kEnds = 20; // tiles that a workgroup's start and end take as long as
+constexpr float kJoin = 12; // the same for the joining of ranges
+__device__ __forceinline__ std::uint32_t paged_rounds(std::uint32_t blocks, std::uint32_t lo, std::uint32_t tiles, std::uint32_t share,
+                                                      std::uint32_t bits, std::uint32_t sequences, std::uint32_t least) {
+  if (share >> 16 != 0) return share;
+  const std::uint32_t lane = threadIdx.x & 63;
+  std::uint32_t t = (share * (64 + 3 * lane) + 127) / 128; // (at least half of the share: items stay within blocks + 2 slots)
+  t = t > least ? t : least;
+  const float length = static_cast<float>(t), inverse = __builtin_amdgcn_rcpf(length);
+  // the sum of ceil(x) from 0 to u, by parts: (n + 1) (u - n / 2), n whole
+  const auto area = [](float u, float &n) {
+    n = floorf(u);
+    return fmaf(-0.5f, n, u);
+  };
+  float load = 0, longest = 0, shortest = FLT_MAX;
+  std::uint32_t ahead = 0;
+  for (std::uint32_t j = 0; j < sequences; ++j) {
+    const std::uint32_t b = lane_u32(blocks, j), last = lane_u32(tiles, j), first = lane_u32(lo, j);
+    if (b == 0) break;
+    const float l = static_cast<float>(last), f = static_cast<float>(first), mid = 0.5f * (f + l);
+    // the mean of a block's items: ceil(tiles / t), over tiles that grow from first to last
+    float n0, n1;
+    const float u0 = f * inverse, u1 = l * inverse, a0 = area(u0, n0), a1 = area(u1, n1);
+    const float grown = fmaf(n1, a1, a1 - fmaf(n0, a0, a0)) * __builtin_amdgcn_rcpf(fmaxf(u1 - u0, 1e-6f));
+    const float each = t >= last ? 1.0f : last - first < 2 ? ceilf(u1) : grown;
+    const float x = fmaf(mid, __builtin_amdgcn_rcpf(each), kEnds);
+    const std::uint32_t items = static_cast<std::uint32_t>(fmaf(static_cast<float>(b), each, 0.999f));
+    ahead += items;
+    shortest = fminf(shortest, x);
+    const float some = static_cast<float>((ahead + (1u << bits) - 1) >> bits) * shortest;
+    longest = fmaxf(longest, b > 1 && 2 * first < last && t >= last ? l + kEnds : some);
+    load = fmaf(static_cast<float>(items), x, load);
+  }
+  float cost = fmaxf(longest, load * (1.0f / static_cast<float>(1u << bits)));
+  if (t < lane_u32(tiles, 0)) cost += kJoin;
+  const std::uint32_t best = ~wave_most(~((__float_as_uint(cost) & ~63u) | lane)); // (costs are not negative)
+  return lane_u32(t, best & 63);
+}
+// Lays the sequences of a wave so that the longest come first.
+template <int kUnit>
+__device__ __forceinline__ void paged_sort(PagedSeq &q, std::uint32_t &id, std::uint32_t &blocks, std::uint32_t &lo, std::uint32_t &tiles,
+                                           std::uint32_t sequences) {
+  const std::uint32_t lane = threadIdx.x & 63, front = (q.ctx - q.n) / kUnit + 1;
+  lo = q.valid && front < tiles ? front : tiles; // of the first block; the last has `tiles`
+  if (sequences == 1) return;
+  const std::uint32_t key = blocks != 0 ? lo + tiles : 0;
+  std::uint32_t rank = lane;
+  if (lane < sequences) {
+    rank = 0;
+    for (std::uint32_t j = 0; j < sequences; ++j) {
+      const std::uint32_t other = lane_u32(key, j);
+      rank += static_cast<std::uint32_t>((other > key) | ((other == key) & (j < lane)));
+    }
+  }
+  const auto sorted = [&](std::uint32_t x) {
+    return static_cast<std::uint32_t>(__builtin_amdgcn_ds_permute(static_cast<int>(4 * rank), static_cast<int>(x)));
+  };
+  q.row0 = sorted(q.row0);
+  q.n = sorted(q.n);
+  q.ctx = sorted(q.ctx);
+  q.valid = sorted(q.valid) != 0;
+  id = sorted(id);
+  blocks = sorted(blocks);
+  lo = sorted(lo);
+  tiles = sorted(tiles);
+}
+
+// Finds item `index` of the batch; false: there are fewer.  By a whole wave, 64 sequences at a
+// time.  `first`: the caller is the one wave that counts bad sequences, in `count`, and writes the
+// plan for the kernel that joins the ranges.  With kRounds the items of up to 64 sequences are
+// the longest first and their ranges' length is chosen (16 query and 4 KV heads, against an even
+// share in the batch's order, us: 300 tokens of 30000 284 -> 190, 200 of 60000 359 -> 243, 16 sequences of
+// up to 8192 behind a window of 4096, ten of them single tokens, 222 -> 176; it takes a workgroup 2 to 7 us, of 1 to 32
+// sequences).
+template <int kCols, int kUnit, bool kRounds = false>
+__device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, const PagedScratch &sc, std::uint32_t index, bool first,
+                                           unsigned int *count, PagedItem &item) {
+  const std::uint32_t lane = threadIdx.x & 63;
+  std::uint64_t work = 0;
+  std::uint32_t live = 0;
+  PagedSeq q{};
+  std::uint32_t blocks = 0, lo = 1, tiles = 1, bad = 0, id = lane;
+  for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+    blocks = 0;
+    if (s0 + lane < a.sequences) {
+      q = paged_seq(a, s0 + lane);
+      paged_extent<kCols, kUnit>(a, q, blocks, tiles);
+      bad += !q.valid;
+    }
+    const std::uint64_t w = static_cast<std::uint64_t>(blocks) * tiles;
+    live += __builtin_popcountll(__builtin_amdgcn_ballot_w64(blocks != 0));
+    work += lane_u32(wave_prefix(static_cast<std::uint32_t>(w) & 0xFFFFFFu), 63);
+    if (__builtin_amdgcn_ballot_w64(w >> 24 != 0) != 0)
+      work += static_cast<std::uint64_t>(lane_u32(wave_prefix(static_cast<std::uint32_t>(w >> 24)), 63)) << 24;
+  }
+  if (first && bad != 0) atomicAdd(count, bad);
+  const std::uint32_t bits = sp.slot_bits + (live >= sp.many ? sp.many_bits : 0);
+  const std::uint64_t share = (work + (std::uint64_t{1} << bits) - 1) >> bits;
+  std::uint32_t t = share >> 28 != 0 ? 1u << 28 : share > sp.least ? static_cast<std::uint32_t>(share) : sp.least;
+  if (kRounds && a.sequences <= 64) {
+    paged_sort<kUnit>(q, id, blocks, lo, tiles, a.sequences);
+    t = paged_rounds(blocks, lo, tiles, t, bits, a.sequences, sp.least);
+  }
+  if (first && sp.parts != 0) {
+    std::uint32_t split = 0;
+    for (std::uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+      if (a.sequences > 64) {
+        blocks = 0;
+        if (s0 + lane < a.sequences) paged_extent<kCols, kUnit>(a, paged_seq(a, s0 + lane), blocks, tiles);
+      }
+      split += lane_u32(wave_prefix(tiles > t ? blocks : 0), 63);
+    }
+    if (lane == 0) {
+      sc.plan[0] = t;
+      sc.plan[1] = split;
+    }
+  }
+  return paged_pick<kCols, kUnit>(a, index, false, t, q, id, blocks, tiles, item);
+}
+// Finds split column block `index` for the kernel that joins its ranges.
+template <int kCols, int kUnit, bool kRounds = false>
+__device__ __forceinline__ bool paged_find_split(const PagedArgs &a, const PagedScratch &sc, std::uint32_t index, PagedItem &item) {
+  const std::uint32_t lane = threadIdx.x & 63;
+  const std::uint32_t t = sc.plan[0];
+  PagedSeq q{};
+  std::uint32_t blocks = 0, lo = 1, tiles = 1, id = lane;
+  if (lane < a.sequences) {
+    q = paged_seq(a, lane);
+    paged_extent<kCols, kUnit>(a, q, blocks, tiles);
+  }
+  if (kRounds && a.sequences <= 64) paged_sort<kUnit>(q, id, blocks, lo, tiles, a.sequences);
+  return paged_pick<kCols, kUnit>(a, index, true, t, q, id, blocks, tiles, item);
 }
 
 // A column block's tokens and keys, and its ranges of about equal length.

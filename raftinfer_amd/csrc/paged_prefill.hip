@@ -3,6 +3,8 @@
 #include "paged_cache.hpp"
 #include "prefill_stream.hpp"
 
+#include <algorithm>
+
 namespace raftinfer::amd {
 namespace {
 
@@ -36,9 +38,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave % kGroups, cg = wave / kGroups; // key group, column group
-  const std::uint32_t index = scalar(blockIdx.x / a.kv_heads), kvh = blockIdx.x - index * a.kv_heads;
+  // The hardware deals workgroups to the 8 dies in turn and of a die's to its 4 engines in turn, whatever has
+  // become free: every other row of 32 takes the engines the other way round, so that of items that lie
+  // longest first each engine gets about as much.  (16 sequences, 268 workgroups for 256 places: 219 -> 182 us.)
+  const std::uint32_t turned = (blockIdx.x & 32) != 0 ? blockIdx.x ^ 24 : blockIdx.x;
+  const std::uint32_t index = scalar(turned / a.kv_heads), kvh = turned - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<kStreamCols, kKTile, true>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_stream_capacity_errors : nullptr, it)) return;
+  if (!paged_find<kStreamCols, kKTile, true>(a, sp, sc, index, blockIdx.x == 0 && wave == 0, &g_stream_capacity_errors, it)) return;
   const std::uint32_t range = scalar(it.local / it.blocks), block = it.blocks - 1 - (it.local - range * it.blocks); // longest first
   if (!it.seq.valid) {
     paged_fill_nan<kThreads>(a, it, block * kStreamCols, kStreamCols, kvh);
@@ -537,73 +543,78 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   }
 }
 
-// Joins the ranges of split column blocks: grid (blocks of 32 columns, split blocks times KV heads).  A
-// wave takes four quads of every lane's column, eight ranges' at a time on the way.
-constexpr int kJoinWaves = 8;
+// Joins the ranges of split column blocks, 32 columns of a KV head at a time: by as many workgroups as work
+// side by side, since only the device knows how many blocks there are (one for each that could be: 9.6 us where none
+// is split, 16 sequences).  A wave takes four quads of every lane's column, eight ranges' at a time on the way.
+constexpr int kJoinWaves = 8, kJoinGrid = 1024;
 __global__ __launch_bounds__(kJoinWaves *kWave) void paged_stream_merge_kernel(PagedArgs a, PagedScratch sc, PagedSplit sp) {
+  constexpr std::uint32_t kSlices = kStreamCols / 32;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::uint32_t index = scalar(blockIdx.y / a.kv_heads), kvh = blockIdx.y - index * a.kv_heads;
-  PagedItem it;
-  if (!paged_find<kStreamCols, kKTile, true>(a, sp, index, true, nullptr, it)) return;
-  const PagedBlock b = paged_block<kStreamCols, kKTile>(a, it, it.local);
-  const std::uint32_t x0 = 32 * blockIdx.x, part0 = it.first_part + it.local * it.ranges;
-  if (b.count == 1 || b.col0 + x0 >= b.col_end) return;
-  if (part0 + b.count > sp.parts) return; // (only where sequences share rows)
-  const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * kStreamCols; // between parts
-  const std::size_t at0 = part0 * stride + static_cast<std::size_t>(kvh) * kStreamCols + x0;
-  const std::uint32_t last_x = b.col_end - 1 - b.col0, x = x0 + col < last_x ? x0 + col : last_x;
-  const std::uint32_t c = b.col0 - b.tok0 * a.group + x, tok = c * a.group_inverse >> 16, head = c - tok * a.group;
-  const std::size_t row = it.seq.row0 + b.tok0 + tok, h = kvh * a.group + head;
-  const int dim = 32 * wave + 4 * half; // quad 4 wave + i: dims 32 wave + 8 i + 4 half
-  u32x2 g[4];
-  if (a.gate != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = *reinterpret_cast<const u32x2 *>(a.gate + row * a.g_row + h * a.g_head + dim + 8 * i);
-  }
-  const auto *o = reinterpret_cast<const floatx4 *>(sc.o + at0 * kHeadDim) + 4 * kWave * wave + lane;
-  float m_run = -FLT_MAX, l = 0.f;
-  floatx4 sum[4]{};
-  constexpr int kBatch = 8;
-  for (std::uint32_t s0 = 0; s0 < b.count; s0 += kBatch) {
-    floatx4 in[kBatch][4];
-    float m[kBatch], ls[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const std::uint32_t s = s0 + k < b.count ? s0 + k : b.count - 1;
-      m[k] = sc.m[at0 + s * stride + col];
-      ls[k] = s0 + k < b.count ? sc.l[at0 + s * stride + col] : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) in[k][i] = o[s * stride * (kHeadDim / 4) + kWave * i];
-    }
-    float m_new = m_run;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, m[k]);
-    const float f = fexp2(m_run - m_new);
-    l *= f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] *= f;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (s0 + k >= b.count) break;
-      const float fk = fexp2(m[k] - m_new);
-      l += ls[k] * fk;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += in[k][i] * fk;
-    }
-    m_run = m_new;
-  }
-  if (x0 + col > last_x) return;
-  const float inv = 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    floatx4 y = sum[i] * inv;
+  const std::uint32_t all = sc.plan[1] * a.kv_heads * kSlices;
+  for (std::uint32_t at = blockIdx.x; at < all; at += gridDim.x) {
+    const std::uint32_t of_heads = at / kSlices, index = scalar(of_heads / a.kv_heads), kvh = of_heads - index * a.kv_heads;
+    PagedItem it;
+    if (!paged_find_split<kStreamCols, kKTile, true>(a, sc, index, it)) return;
+    const PagedBlock b = paged_block<kStreamCols, kKTile>(a, it, it.local);
+    const std::uint32_t x0 = 32 * (at % kSlices), part0 = it.first_part + it.local * it.ranges;
+    if (b.count == 1 || b.col0 + x0 >= b.col_end) continue;
+    if (part0 + b.count > sp.parts) return; // (only where sequences share rows)
+    const std::size_t stride = static_cast<std::size_t>(a.kv_heads) * kStreamCols; // between parts
+    const std::size_t at0 = part0 * stride + static_cast<std::size_t>(kvh) * kStreamCols + x0;
+    const std::uint32_t last_x = b.col_end - 1 - b.col0, x = x0 + col < last_x ? x0 + col : last_x;
+    const std::uint32_t c = b.col0 - b.tok0 * a.group + x, tok = c * a.group_inverse >> 16, head = c - tok * a.group;
+    const std::size_t row = it.seq.row0 + b.tok0 + tok, h = kvh * a.group + head;
+    const int dim = 32 * wave + 4 * half; // quad 4 wave + i: dims 32 wave + 8 i + 4 half
+    u32x2 g[4];
     if (a.gate != nullptr) {
-      y[0] *= sigmoid_gate(bf16_lo(g[i][0])); y[1] *= sigmoid_gate(bf16_hi(g[i][0]));
-      y[2] *= sigmoid_gate(bf16_lo(g[i][1])); y[3] *= sigmoid_gate(bf16_hi(g[i][1]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = *reinterpret_cast<const u32x2 *>(a.gate + row * a.g_row + h * a.g_head + dim + 8 * i);
     }
-    *reinterpret_cast<u32x2 *>(a.output + row * a.o_row + h * a.o_head + dim + 8 * i) =
-        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    const auto *o = reinterpret_cast<const floatx4 *>(sc.o + at0 * kHeadDim) + 4 * kWave * wave + lane;
+    float m_run = -FLT_MAX, l = 0.f;
+    floatx4 sum[4]{};
+    constexpr int kBatch = 8;
+    for (std::uint32_t s0 = 0; s0 < b.count; s0 += kBatch) {
+      floatx4 in[kBatch][4];
+      float m[kBatch], ls[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const std::uint32_t s = s0 + k < b.count ? s0 + k : b.count - 1;
+        m[k] = sc.m[at0 + s * stride + col];
+        ls[k] = s0 + k < b.count ? sc.l[at0 + s * stride + col] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) in[k][i] = o[s * stride * (kHeadDim / 4) + kWave * i];
+      }
+      float m_new = m_run;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, m[k]);
+      const float f = fexp2(m_run - m_new);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] *= f;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (s0 + k >= b.count) break;
+        const float fk = fexp2(m[k] - m_new);
+        l += ls[k] * fk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += in[k][i] * fk;
+      }
+      m_run = m_new;
+    }
+    if (x0 + col > last_x) continue;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      floatx4 y = sum[i] * inv;
+      if (a.gate != nullptr) {
+        y[0] *= sigmoid_gate(bf16_lo(g[i][0])); y[1] *= sigmoid_gate(bf16_hi(g[i][0]));
+        y[2] *= sigmoid_gate(bf16_lo(g[i][1])); y[3] *= sigmoid_gate(bf16_hi(g[i][1]));
+      }
+      *reinterpret_cast<u32x2 *>(a.output + row * a.o_row + h * a.o_head + dim + 8 * i) =
+          u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    }
   }
 }
 
@@ -611,10 +622,10 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void paged_stream_merge_kernel(P
 
 void launch_paged_stream(const PagedArgs &a, const PagedScratch &sc, const PagedSplit &sp, std::uint32_t items,
                          std::uint32_t split_blocks, hipStream_t stream) {
-  const auto go = [&](auto kernel) { kernel<<<items * a.kv_heads, kThreads, 0, stream>>>(a, sc, sp); };
+  const auto go = [&](auto kernel) { kernel<<<(items * a.kv_heads + 31) / 32 * 32, kThreads, 0, stream>>>(a, sc, sp); };
   go(a.row_step == 1 ? paged_stream_kernel<true> : paged_stream_kernel<false>);
   if (split_blocks != 0)
-    paged_stream_merge_kernel<<<dim3{kStreamCols / 32, split_blocks * a.kv_heads}, kJoinWaves * kWave, 0, stream>>>(a, sc, sp);
+    paged_stream_merge_kernel<<<std::min<std::uint32_t>(split_blocks * a.kv_heads * (kStreamCols / 32), kJoinGrid), kJoinWaves * kWave, 0, stream>>>(a, sc, sp);
 }
 
 std::uint32_t paged_take_stream_errors() {

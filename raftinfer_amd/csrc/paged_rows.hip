@@ -69,7 +69,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
   const int col16 = lane & 15, kq = lane >> 4;
   const std::uint32_t index = scalar(blockIdx.x / a.kv_heads), kvh = blockIdx.x - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<F::kCols, F::kKeys>(a, sp, index, false, blockIdx.x == 0 && wave == 0 ? &g_paged_capacity_errors : nullptr, it)) return;
+  if (!paged_find<F::kCols, F::kKeys>(a, sp, sc, index, blockIdx.x == 0 && wave == 0, &g_paged_capacity_errors, it)) return;
   const std::uint32_t range = scalar(it.local / it.blocks), block = it.blocks - 1 - (it.local - range * it.blocks); // longest first
   if (!it.seq.valid) {
     paged_fill_nan<F::kThreads>(a, it, block * F::kCols, F::kCols, kvh);
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(WAVES *kWave) void paged_merge_kernel(PagedArgs a, 
   constexpr std::uint32_t kCols = F::kCols;
   const std::uint32_t index = scalar(blockIdx.y / a.kv_heads), kvh = blockIdx.y - index * a.kv_heads;
   PagedItem it;
-  if (!paged_find<kCols, F::kKeys>(a, sp, index, true, nullptr, it)) return;
+  if (!paged_find_split<kCols, F::kKeys>(a, sc, index, it)) return;
   const PagedBlock b = paged_block<kCols, F::kKeys>(a, it, it.local);
   if (b.count == 1) return;
   const std::uint32_t x = blockIdx.x * WAVES + wave, col = b.col0 + x;
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(kDecodeJoin *kWave) void paged_decode_merge_kernel(
   const std::uint32_t x = blockIdx.x >> 2; // head of the group
   const int dim = 64 * (blockIdx.x & 3) + 4 * quad;
   PagedItem it;
-  if (!paged_find<F::kCols, F::kKeys>(a, sp, index, true, nullptr, it)) return;
+  if (!paged_find_split<F::kCols, F::kKeys>(a, sc, index, it)) return;
   const PagedBlock b = paged_block<F::kCols, F::kKeys>(a, it, it.local);
   if (b.count == 1) return;
   const std::uint32_t part0 = it.first_part + it.local * it.ranges;
@@ -584,8 +584,8 @@ Bounds bounds_of(const PagedArgs &a, std::uint32_t block_cols, std::uint32_t uni
 PagedScratch scratch_of(const PagedArgs &a, const PagedSplit &sp, std::uint32_t block_cols, void *workspace, std::size_t *bytes) {
   const std::size_t cols = static_cast<std::size_t>(sp.parts) * a.kv_heads * block_cols;
   auto *p = static_cast<float *>(workspace);
-  if (bytes != nullptr) *bytes = cols * (kHeadDim + 2) * sizeof(float);
-  return {p, p + cols, p + 2 * cols};
+  if (bytes != nullptr) *bytes = sp.parts == 0 ? 0 : cols * (kHeadDim + 2) * sizeof(float) + 16;
+  return {p, p + cols, p + 2 * cols, reinterpret_cast<std::uint32_t *>(p + cols * (kHeadDim + 2))};
 }
 
 Bounds decode_bounds(const PagedArgs &a) { return bounds_of(a, DecodeForm::kCols, DecodeForm::kKeys, 32, 256, 2, 2); }
@@ -594,7 +594,7 @@ bool reads_once(const PagedArgs &a) {
   return static_cast<std::uint64_t>(a.sequences) * a.max_ctx * a.kv_heads * 2 * kRowBytes > (16u << 20);
 }
 Bounds few_bounds(const PagedArgs &a) { return bounds_of(a, FewForm::kCols, FewForm::kKeys, 16, 256, 8, 1); }
-Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols, kStreamUnit, 8, 256, 8, 1, true); }
+Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols, kStreamUnit, 8, 256, 1u << 31, 1, true); }
 // Which kernel a chunk takes, by the (column, key) pairs of all heads that the sequences can have: the
 // stream kernel fetches a key once for 128 columns and keeps the matrix units busy, but its start and end cost
 // about 15 us of every workgroup (ring, 256 accumulator registers, the joining of its key groups).  Up to 40

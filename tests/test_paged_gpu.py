@@ -645,3 +645,16 @@ def test_same_sequence_in_every_kernel(gpu):
     b.check()
     b.out.fill_(7)
     assert torch.equal(b.call(), second)
+
+
+@pytest.mark.parametrize("sequences", [2, 13, 64, 65, 130])
+@pytest.mark.parametrize("chunk", [False, True])
+def test_many_sequences(gpu, sequences, chunk):
+    """Up to and beyond what one wave holds, some without rows, in no order of length."""
+    rng = np.random.default_rng(sequences)
+    each = [(0, int(rng.integers(0, 50))) if i % 7 == 3 else (int(rng.integers(1, 9 if i % 5 else 60)), int(rng.integers(60, 500 if i % 11 else 2500)))
+            for i in range(sequences)]
+    b = Batch(each, 2, 3, seed=sequences, lead=1)
+    (roomy(b) if chunk else b).call()
+    b.check()
+    assert errors() == 0
