@@ -30,30 +30,37 @@ __device__ __forceinline__ std::uint32_t sequence_of(const PagedArgs &a, std::ui
   return lo;
 }
 
-// A workgroup per row.  Its heads (query, key, value) lie in 32 lanes each, asked for before
-// the row's sequence, position and page are known.
-__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppendArgs x) {
-  __shared__ float rot[kHeadDim]; // cos of the pairs, then sin
+// A workgroup takes kRows rows: its waves look up the rows' sequences, positions and pages, one wave a row, while the
+// first heads (query, key, value; 32 lanes each, 16 bytes a lane) are on their way, and four heads of a lane's
+// group are asked for at a time, the next four before these are used.  What bounds a workgroup is the chain of loads in front of a store
+// (starts, lengths, table: 10 us of a workgroup with five of them on a compute unit); one row each keeps short calls
+// short (32 rows 7.0 us), four share the chain in long ones.
+template <int kRows> __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppendArgs x) {
+  __shared__ float rot[kRows][kHeadDim]; // cos of the pairs, then sin
+  __shared__ std::uint32_t place[kRows][2]; // the K row of head 0, and whether: 0 the row is not stored, 1 its query only, 2 all
   const PagedArgs &a = x.paged;
-  const std::uint32_t row = blockIdx.x, lane = threadIdx.x & 63;
+  const std::uint32_t row0 = blockIdx.x * kRows, rows = a.rows - row0 < kRows ? a.rows - row0 : kRows, lane = threadIdx.x & 63;
   const std::uint32_t q_heads = a.query != nullptr ? a.kv_heads * a.group : 0;
-  const std::uint32_t units = q_heads + 2 * a.kv_heads;
+  const std::uint32_t units = q_heads + 2 * a.kv_heads, all = units * rows;
   const int c = threadIdx.x % kAppendLanes;
   constexpr std::uint32_t kGroups = kAppendThreads / kAppendLanes;
   constexpr int kBatch = 4;
   const std::uint32_t u0 = threadIdx.x / kAppendLanes;
-  u32x4 raw[kBatch];
-  const auto load = [&](std::uint32_t first) {
+  const auto row_of = [&](std::uint32_t u) { return kRows == 1 ? 0u : __umulhi(u, x.units_inverse); };
+  const auto load = [&](std::uint32_t first, u32x4 (&raw)[kBatch]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const std::uint32_t u = first + kGroups * i < units ? first + kGroups * i : units - 1;
+      const std::uint32_t n = first + kGroups * i < all ? first + kGroups * i : all - 1;
+      const std::uint32_t r = row_of(n), u = n - r * units;
+      const std::size_t row = row0 + r;
       const bf16_bits *src = u < q_heads ? a.query + row * a.q_row + u * a.q_head
                              : u < q_heads + a.kv_heads ? x.key + row * x.k_row + (u - q_heads) * x.k_head
                                                         : x.value + row * x.v_row + (u - q_heads - a.kv_heads) * x.v_head;
       raw[i] = *reinterpret_cast<const u32x4 *>(src + 8 * c);
     }
   };
-  load(u0);
+  u32x4 raw[kBatch];
+  load(u0, raw);
   float qw[8], kw[8];
   const auto weights = [&](const void *weight, float (&w)[8]) {
 #pragma unroll
@@ -63,32 +70,47 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
   };
   weights(x.q_weight, qw);
   weights(x.k_weight, kw);
-  if (row == 0 && threadIdx.x < 64) { // bad sequences are counted here
+  if (row0 == 0 && threadIdx.x < 64) { // bad sequences are counted here
     std::uint32_t bad = 0;
     for (std::uint32_t s = lane; s < a.sequences; s += 64) bad += !paged_seq(a, s).valid;
     if (bad != 0) atomicAdd(&g_append_capacity_errors, bad);
   }
-  const std::uint32_t seq = __builtin_amdgcn_readfirstlane(sequence_of(a, row));
-  if (seq >= a.sequences) return; // behind the last sequence's rows (uniform)
-  const PagedSeq q = paged_seq(a, seq);
-  if (!q.valid || row < q.row0 || row - q.row0 >= q.n) return; // (uniform)
-  const std::uint32_t position = q.ctx - q.n + (row - q.row0);
-  bool bad = false;
-  const std::uint32_t to = paged_row(a, seq, 0, position, bad);
-  const std::uint32_t pairs = x.rotary_dim / 2;
-  if (threadIdx.x < pairs) {
-    float cs, sn;
-    rotary_cos_sin(position, x.frequencies[threadIdx.x], x.magnitude, cs, sn);
-    rot[threadIdx.x] = cs;
-    rot[pairs + threadIdx.x] = sn;
+  const std::uint32_t pairs = x.rotary_dim / 2, wave = scalar(threadIdx.x >> 6);
+  // (of one row every wave, and its angles by the first pairs / 64 of them; else wave w the rows w, w + 4, ..)
+  for (std::uint32_t r = kRows == 1 ? 0 : wave; r < rows; r += kRows == 1 ? 1 : kAppendThreads / 64) {
+    const std::uint32_t row = row0 + r, seq = scalar(sequence_of(a, row));
+    std::uint32_t to = 0, what = 0;
+    if (seq < a.sequences) { // (else behind the last sequence's rows)
+      const PagedSeq q = paged_seq(a, seq);
+      if (q.valid && row >= q.row0 && row - q.row0 < q.n) {
+        const std::uint32_t position = q.ctx - q.n + (row - q.row0);
+        bool bad = false;
+        to = paged_row(a, seq, 0, position, bad);
+        what = bad ? 1 : 2;
+        for (std::uint32_t p = kRows == 1 ? threadIdx.x : lane; p < pairs; p += kRows == 1 ? kAppendThreads : 64) {
+          float cs, sn;
+          rotary_cos_sin(position, x.frequencies[p], x.magnitude, cs, sn);
+          rot[r][p] = cs;
+          rot[r][pairs + p] = sn;
+        }
+        if (bad && (kRows == 1 ? threadIdx.x : lane) == 0) atomicAdd(&g_append_capacity_errors, 1u);
+      }
+    }
+    if (kRows == 1 && what == 0) return; // (uniform)
+    if (lane == 0) {
+      place[r][0] = to;
+      place[r][1] = what;
+    }
   }
-  if (bad && threadIdx.x == 0) atomicAdd(&g_append_capacity_errors, 1u);
   __syncthreads();
-  for (std::uint32_t first = u0; first - u0 < units; first += kGroups * kBatch) {
-    if (first != u0) load(first);
+  for (std::uint32_t first = u0; first - u0 < all; first += kGroups * kBatch) {
+    u32x4 next[kBatch];
+    const bool more = first - u0 + kGroups * kBatch < all; // (uniform)
+    if (more) load(first + kGroups * kBatch, next);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const std::uint32_t u = first + kGroups * i;
+      const std::uint32_t n = first + kGroups * i < all ? first + kGroups * i : all - 1;
+      const std::uint32_t r = row_of(n), u = n - r * units;
       const bool is_q = u < q_heads, is_v = u >= q_heads + a.kv_heads;
       float v[8], w[8];
       Piece16<bf16_bits>::unpack(raw[i], v);
@@ -98,30 +120,42 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = v[e];
-      if (x.q_weight != nullptr || x.k_weight != nullptr) {
-        norm_rotate<8, kAppendLanes>(y, w, true, false, c, 0, kHeadDim, rot, x.epsilon);
-        const bool norm = (is_q ? x.q_weight : x.k_weight) != nullptr;
+      if (__builtin_amdgcn_ballot_w64(!is_v) != 0) { // (a wave of values only: as they are)
+        if (x.q_weight != nullptr || x.k_weight != nullptr) {
+          norm_rotate<8, kAppendLanes>(y, w, true, false, c, 0, kHeadDim, rot[r], x.epsilon);
+          const bool norm = (is_q ? x.q_weight : x.k_weight) != nullptr;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = norm ? y[e] : v[e];
+          for (int e = 0; e < 8; ++e) y[e] = norm ? y[e] : v[e];
+        }
+        norm_rotate<8, kAppendLanes>(y, w, false, x.interleaved, c, pairs, kHeadDim, rot[r], x.epsilon);
       }
-      norm_rotate<8, kAppendLanes>(y, w, false, x.interleaved, c, pairs, kHeadDim, rot, x.epsilon);
       const u32x4 out = is_v ? raw[i] : Piece16<bf16_bits>::pack(y);
-      if (u >= units) continue;
+      const std::uint32_t what = place[r][1];
+      if (first + kGroups * i >= all || what == 0) continue;
+      const std::size_t row = row0 + r;
       if (is_q) {
         *reinterpret_cast<u32x4 *>(a.output + row * a.o_row + u * a.o_head + 8 * c) = out;
-      } else if (!bad) {
+      } else if (what == 2) {
         const std::uint32_t kvh = is_v ? u - q_heads - a.kv_heads : u - q_heads;
-        const std::size_t at = to + kvh * a.head_step + (is_v ? a.plane_rows : 0);
+        const std::size_t at = place[r][0] + kvh * a.head_step + (is_v ? a.plane_rows : 0);
         *reinterpret_cast<u32x4 *>(x.pages + at * kRowBytes + 16 * c) = out;
       }
+    }
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) raw[i] = next[i];
     }
   }
 }
 
 } // namespace
 
-void paged_append(const PagedAppendArgs &a, hipStream_t stream) {
-  paged_append_kernel<<<a.paged.rows, kAppendThreads, 0, stream>>>(a);
+void paged_append(const PagedAppendArgs &args, hipStream_t stream) {
+  PagedAppendArgs a = args;
+  const std::uint32_t units = (a.paged.query != nullptr ? a.paged.kv_heads * a.paged.group : 0) + 2 * a.paged.kv_heads;
+  a.units_inverse = 0xFFFFFFFFu / units + 1; // (of products below 2^32: units and four rows of them)
+  if (a.paged.rows >= 1024) paged_append_kernel<4><<<(a.paged.rows + 3) / 4, kAppendThreads, 0, stream>>>(a);
+  else paged_append_kernel<1><<<a.paged.rows, kAppendThreads, 0, stream>>>(a);
 }
 
 std::uint32_t paged_take_append_errors() {

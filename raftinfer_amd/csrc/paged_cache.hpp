@@ -398,7 +398,7 @@ struct PagedAppendArgs {
   const void *q_weight, *k_weight;
   bool weight_f32, interleaved;
   std::size_t k_row, k_head, v_row, v_head;
-  std::uint32_t rotary_dim;
+  std::uint32_t rotary_dim, units_inverse; // 2^32 / heads of a row + 1 (set by paged_append)
   float magnitude, epsilon;
 };
 void paged_append(const PagedAppendArgs &a, hipStream_t stream);

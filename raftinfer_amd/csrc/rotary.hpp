@@ -80,7 +80,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[N], const float (&w)[N], 
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], ss);
-    const float scale = 1.0f / sqrtf(lanes_sum<LANES>(ss) / head_dim + epsilon);
+    const float scale = __builtin_amdgcn_rsqf(fmaf(lanes_sum<LANES>(ss), 1.0f / head_dim, epsilon)); // (off by one step of 32 bits)
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = x[e] * scale * w[e];
   }
