@@ -402,6 +402,9 @@ def _stream_of(stream, tensor) -> int:
     """The stream's handle; None: the current stream of the tensor's device."""
     if stream is None:
         import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (0.1 us; a Stream object takes 1.8 us to make)
+        if raw is not None and tensor.is_cuda:
+            return raw(tensor.get_device())
         return torch.cuda.current_stream(tensor.device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
 
@@ -535,10 +538,11 @@ def _strides(t) -> tuple:
     if t is None or getattr(t, "ndim", 0) != 3:
         return 0, 0
     row, head, dim = t.stride()
-    if dim != 1 and t.shape[2] != 1:
+    rows, heads, dims = t.shape
+    if dim != 1 and dims != 1:
         raise Qwen35PrimitiveError(1, "the last dimension of a tensor of heads must be contiguous")
     # (the stride of a dimension of one element says nothing)
-    return (row if t.shape[0] > 1 else 0), (head if t.shape[1] > 1 else 0)
+    return (row if rows > 1 else 0), (head if heads > 1 else 0)
 
 
 def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
