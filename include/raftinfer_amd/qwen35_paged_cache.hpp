@@ -29,7 +29,9 @@
 // attention calls make such a sequence's rows NaN (a bad page: at least the rows that
 // see it; rows behind the call's are not written), the append stores none of it (a bad
 // page: none of the rows that belong there).  Each is counted at least once
-// (qwen35_online_attention_consume_capacity_errors).
+// (qwen35_online_attention_consume_capacity_errors).  Where query_starts fall, sequences
+// can share rows: such rows, and any row of that batch, may hold NaN, what another of the
+// sequences gives them, or what they held; nothing else is written.
 #pragma once
 
 #include "qwen35_attention.hpp"

@@ -534,15 +534,33 @@ class Qwen35PagedRotary:
 
 
 def _strides(t) -> tuple:
-    """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else is dense."""
-    if t is None or getattr(t, "ndim", 0) != 3:
+    """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else must be dense."""
+    if t is None:
+        return 0, 0
+    if getattr(t, "ndim", 0) != 3:
+        _dense(t)
         return 0, 0
     row, head, dim = t.stride()
     rows, heads, dims = t.shape
     if dim != 1 and dims != 1:
         raise Qwen35PrimitiveError(1, "the last dimension of a tensor of heads must be contiguous")
+    if (row == 0 and rows > 1) or (head == 0 and heads > 1):
+        raise Qwen35PrimitiveError(1, "rows and heads must not be broadcast")
     # (the stride of a dimension of one element says nothing)
     return (row if rows > 1 else 0), (head if heads > 1 else 0)
+
+
+def _dense(t):
+    """The address of an argument without strides of its own."""
+    if t is None:
+        return None
+    if not getattr(t, "is_contiguous", _yes)():
+        raise Qwen35PrimitiveError(1, "indices, pages, weights and workspaces must be contiguous")
+    return t.data_ptr()
+
+
+def _yes() -> bool:
+    return True
 
 
 def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
@@ -563,7 +581,7 @@ def qwen35_rotary(input, weight, output, positions, frequencies, shape: Qwen35Ro
     None: no norm.  frequencies: float64 [rotary_dim / 2].  output may be input."""
     dtype = _dtype_code(input)
     _checked(_lib.load().raftinfer_amd_rotary(
-        input.data_ptr(), _raw(weight), output.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
+        input.data_ptr(), _dense(weight), output.data_ptr(), _dense(positions), _dense(frequencies),
         RotaryShape(shape.rows, shape.heads, shape.head_dim, shape.rotary_dim, shape.interleaved,
                     shape.magnitude, *_strides(input), *_strides(output)),
         epsilon, dtype, dtype if weight is None else _dtype_code(weight), _stream_of(stream, input)))
@@ -597,10 +615,12 @@ def qwen35_paged_cache_append(query, key, value, query_output, pages, page_table
     if weight_dtype is None:
         weight = query_weight if query_weight is not None else key_weight
         weight_dtype = DTYPE_BF16 if weight is None else _dtype_code(weight)
+        if key_weight is not None and _dtype_code(key_weight) != weight_dtype:
+            raise Qwen35PrimitiveError(1, "query_weight and key_weight must be of one type")
     _checked(_lib.load().raftinfer_amd_paged_cache_append(
-        _raw(query), _raw(key), _raw(value), _raw(query_output), _raw(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table), _raw(query_starts),
-        _raw(context_lengths), _raw(frequencies), _raw(query_weight), _raw(key_weight), shape.c(),
+        _raw(query), _raw(key), _raw(value), _raw(query_output), _dense(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
+        _dense(context_lengths), _dense(frequencies), _dense(query_weight), _dense(key_weight), shape.c(),
         PagedRotary(rotary.rotary_dim, rotary.interleaved, rotary.magnitude, rotary.epsilon,
                     *_strides(query), *_strides(key), *_strides(value), *_strides(query_output)),
         activation_dtype, weight_dtype, cache_layout, _stream_of(stream, key)))
@@ -612,9 +632,9 @@ def qwen35_paged_attention_prefill(query, gate, output, pages, page_table, query
                                    pages_bytes=None, workspace_bytes=None) -> None:
     """Attention of every sequence's new tokens over its pages; gate None: no gate."""
     _checked(_lib.load().raftinfer_amd_paged_attention_prefill(
-        _raw(query), _raw(gate), _raw(output), _raw(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table), _raw(query_starts),
-        _raw(context_lengths), _raw(workspace),
+        _raw(query), _raw(gate), _raw(output), _dense(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
+        _dense(context_lengths), _dense(workspace),
         _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
         PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
         cache_layout, _stream_of(stream, query)))
@@ -626,9 +646,9 @@ def qwen35_paged_attention_decode(query, gate, output, pages, page_table, contex
                                   workspace_bytes=None) -> None:
     """The same for one new token of every sequence; a context length of 0: an unused row."""
     _checked(_lib.load().raftinfer_amd_paged_attention_decode(
-        _raw(query), _raw(gate), _raw(output), _raw(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _raw(page_table),
-        _raw(context_lengths), _raw(workspace),
+        _raw(query), _raw(gate), _raw(output), _dense(pages),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table),
+        _dense(context_lengths), _dense(workspace),
         _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
         PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
         cache_layout, _stream_of(stream, query)))

@@ -218,3 +218,30 @@ def test_rotary_refusals():
         if name != "output":  # one row of it lies in the output's
             with refused("overlaps"):
                 go(**{name: FakeTensor(addr=(3 << 40) + 1024, nbytes=1 << 39)})
+
+
+def test_views_that_have_no_strides_to_pass():
+    """Broadcast rows or heads, and index tensors with gaps, are refused before any address is taken."""
+    q = torch.zeros(3, 16, 256, dtype=torch.bfloat16)
+    rest = [FakeTensor(addr=(i + 1) << 40, nbytes=1 << 39) for i in range(5)]
+    out = torch.zeros(3, 16, 256, dtype=torch.bfloat16)
+    table = torch.zeros(3, 40, dtype=torch.int32)
+    refused = lambda message: pytest.raises(ops.Qwen35PrimitiveError, match=message)  # noqa: E731
+    decode = lambda q, table: ops.qwen35_paged_attention_decode(q, None, out, rest[0], table, rest[1], rest[2], STEP, 1, stream=0x1234,  # noqa: E731
+                                                                workspace_bytes=1 << 39)
+    for bad in (q[:1].expand(3, 16, 256), q[:, :1].expand(3, 16, 256)):
+        with refused("broadcast"):
+            decode(bad, rest[3])
+    with refused("last dimension"):
+        decode(q.transpose(1, 2), rest[3])
+    with refused("contiguous"):
+        decode(q, table[:, ::2])
+    with refused("contiguous"):
+        decode(q, table[:, :20])
+    with refused("contiguous"):
+        decode(q.reshape(3, 4096)[:, ::2], rest[3])
+    with refused("contiguous"):
+        ops.qwen35_rotary(q, None, out, torch.zeros(6, dtype=torch.int32)[::2], rest[0], Q(3, 16, 256, 64), 1e-6, stream=0x1234)
+    with refused("one type"):
+        ops.qwen35_paged_cache_append(rest[0], rest[1], rest[2], rest[3], rest[4], rest[0], rest[1], rest[2], rest[3],
+                                      torch.ones(256), torch.ones(256, dtype=torch.bfloat16), STEP, R(64), 1, stream=0x1234)
