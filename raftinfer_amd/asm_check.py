@@ -1,8 +1,8 @@
 """Build-time checks of the prefill kernels' inline-asm MFMAs.
 
 `prefill_mfma_kernel` issues its PV MFMAs as inline asm (so that the O^T
-accumulators stay in AGPRs), `prefill_wide_kernel` all of its MFMAs.  The
-compiler cannot see an MFMA inside asm, so it neither inserts the wait states
+accumulators stay in AGPRs), `prefill_wide_kernel` and `paged_stream_kernel` all of
+theirs.  The compiler cannot see an MFMA inside asm, so it neither inserts the wait states
 the MFMA needs around it nor avoids placing a register copy right behind it.
 The build therefore scans the kernels' gfx950 assembly and fails on
 

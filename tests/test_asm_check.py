@@ -75,3 +75,38 @@ def test_built_prefill_kernel_has_no_hazard():
     assert asm_mfma_hazards(s.read_text()) == []
     wide = s.with_name("attention_prefill_wide.hip.s")
     assert asm_mfma_hazards(wide.read_text(), owned_agprs=True) == []
+
+
+def test_what_is_under_way_follows_branches():
+    read = "\tv_add_f32 v1, a20, v2\n"
+    gap = "\ts_nop 7\n" * 3
+    # to a label further down, past code that falls out of the listing's order
+    ahead = MFMA + "\ts_cbranch_scc1 .LBB0_2\n" + gap + "\ts_endpgm\n.LBB0_2:\n" + read
+    assert len(asm_mfma_hazards(ahead)) == 1
+    assert asm_mfma_hazards(ahead.replace(".LBB0_2:\n", ".LBB0_2:\n" + gap)) == []
+    # back to a loop's head: the read stands in front of the MFMA
+    loop = "\ts_nop 0\n.LBB0_1:\n" + read + MFMA + "\ts_cbranch_scc0 .LBB0_1\n\ts_endpgm\n"
+    assert len(asm_mfma_hazards(loop)) == 1
+    assert asm_mfma_hazards(loop.replace(MFMA, MFMA + gap)) == []
+    # over two branches, whose own wait states count
+    chain = MFMA + "\ts_branch .LBB0_4\n.LBB0_3:\n" + read + "\ts_endpgm\n.LBB0_4:\n\ts_branch .LBB0_3\n"
+    hazards = asm_mfma_hazards(chain)
+    assert len(hazards) == 1 and "after 2 wait states" in hazards[0]
+
+
+def test_nothing_falls_through_an_unconditional_branch():
+    read = "\tv_add_f32 v1, a20, v2\n"
+    for end in ("\ts_branch .LBB0_9\n", "\ts_endpgm\n"):
+        assert asm_mfma_hazards(MFMA + end + ".LBB0_1:\n" + read) == [], end
+    # the longest wait of all ways into a label is the one that counts
+    both = MFMA + "\ts_cbranch_scc1 .LBB0_1\n" + "\ts_nop 7\n" * 2 + ".LBB0_1:\n" + read
+    hazards = asm_mfma_hazards(both)
+    assert len(hazards) == 1 and "after 1 wait states" in hazards[0]
+
+
+def test_built_paged_kernel_has_no_hazard():
+    s = pathlib.Path(asm_check.__file__).resolve().parent / "_build" / "paged_prefill.hip.s"
+    if not s.exists():
+        import pytest
+        pytest.skip("the library has not been built here")
+    assert asm_mfma_hazards(s.read_text(), owned_agprs=True) == []
