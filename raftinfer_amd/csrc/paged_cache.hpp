@@ -209,10 +209,14 @@ __device__ __forceinline__ std::uint32_t paged_rounds(std::uint32_t blocks, std:
     if (b == 0) break;
     const float l = static_cast<float>(last), f = static_cast<float>(first), mid = 0.5f * (f + l);
     // the mean of a block's items: ceil(tiles / t), over tiles that grow from first to last
-    float n0, n1;
-    const float u0 = f * inverse, u1 = l * inverse, a0 = area(u0, n0), a1 = area(u1, n1);
-    const float grown = fmaf(n1, a1, a1 - fmaf(n0, a0, a0)) * __builtin_amdgcn_rcpf(fmaxf(u1 - u0, 1e-6f));
-    const float each = t >= last ? 1.0f : last - first < 2 ? ceilf(u1) : grown;
+    const float u1 = l * inverse;
+    float each = ceilf(u1);
+    if (last - first >= 2) { // (uniform)
+      float n0, n1;
+      const float u0 = f * inverse, a0 = area(u0, n0), a1 = area(u1, n1);
+      each = fmaf(n1, a1, a1 - fmaf(n0, a0, a0)) * __builtin_amdgcn_rcpf(fmaxf(u1 - u0, 1e-6f));
+    }
+    each = t >= last ? 1.0f : each;
     const float x = fmaf(mid, __builtin_amdgcn_rcpf(each), kEnds);
     const std::uint32_t items = static_cast<std::uint32_t>(fmaf(static_cast<float>(b), each, 0.999f));
     ahead += items;
@@ -233,14 +237,11 @@ __device__ __forceinline__ void paged_sort(PagedSeq &q, std::uint32_t &id, std::
   const std::uint32_t lane = threadIdx.x & 63, front = (q.ctx - q.n) / kUnit + 1;
   lo = q.valid && front < tiles ? front : tiles; // of the first block; the last has `tiles`
   if (sequences == 1) return;
-  const std::uint32_t key = blocks != 0 ? lo + tiles : 0;
+  const std::uint32_t key = (blocks != 0 ? lo + tiles : 0) << 6 | (63 - lane); // (tiles are fewer than 2^24)
   std::uint32_t rank = lane;
   if (lane < sequences) {
     rank = 0;
-    for (std::uint32_t j = 0; j < sequences; ++j) {
-      const std::uint32_t other = lane_u32(key, j);
-      rank += static_cast<std::uint32_t>((other > key) | ((other == key) & (j < lane)));
-    }
+    for (std::uint32_t j = 0; j < sequences; ++j) rank += static_cast<std::uint32_t>(lane_u32(key, j) > key);
   }
   const auto sorted = [&](std::uint32_t x) {
     return static_cast<std::uint32_t>(__builtin_amdgcn_ds_permute(static_cast<int>(4 * rank), static_cast<int>(x)));

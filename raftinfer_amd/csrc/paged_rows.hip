@@ -605,13 +605,16 @@ Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols,
 // kernel first: 512 tokens 20.4 / 34.9, 1000 43.4 / 49.3, 500 of 1500 37.5 / 44.2, 64 of 4000 25.7 / 37.6, 16 of
 // 30000 56.7 / 69.6), above it the stream kernel (100 of 8000 68.3 / 52.1, 300 of 4000 76.5 / 71.8, 500 of 30501 and
 // 8001: twice as fast and more).  Several sequences: 4 of 125 41.5 / 41.1, 8 with 7 single tokens up to 8000
-// 105 / 92, 16 with up to 8192 behind a window of 4096 275 / 232.
+// 105 / 92, 16 with up to 8192 behind a window of 4096 275 / 232.  Where the rows kernel would take a third round of
+// workgroups, few keys or not, the stream kernel is the faster too (windows of 32 and 200: 900 tokens 26.7 / 26.6 and 31.4 / 35.3,
+// 1200 38.1 / 22.3 and 46.1 / 36.3), unless its blocks would be half empty (600 sequences of 2 tokens 136 / 195).
 bool streams(const PagedArgs &a) {
   const std::uint64_t seqs = std::min(a.sequences, a.rows);
   const std::uint64_t each = std::min<std::uint64_t>((a.rows + seqs - 1) / seqs, a.max_ctx);
   std::uint64_t keys = a.max_ctx - each / 2; // in the mean
   if (a.window != 0) keys = std::min<std::uint64_t>(keys, std::uint64_t{a.window} + 32);
-  return static_cast<std::uint64_t>(a.rows) * a.group * a.kv_heads * keys > 40u * 256 * 32 * 32;
+  const std::uint64_t columns = static_cast<std::uint64_t>(a.rows) * a.group * a.kv_heads;
+  return columns * keys > 40u * 256 * 32 * 32 || (columns > 2u * 256 * 32 && each * a.group >= 2 * 32);
 }
 
 template <class F, bool Once> void launch_rows(const PagedArgs &a, const PagedScratch &sc, const Bounds &bd, hipStream_t stream) {

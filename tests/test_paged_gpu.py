@@ -658,3 +658,33 @@ def test_many_sequences(gpu, sequences, chunk):
     (roomy(b) if chunk else b).call()
     b.check()
     assert errors() == 0
+
+
+@pytest.mark.parametrize("window", [1, 7, 40])
+def test_small_windows_of_long_chunks(gpu, window):
+    """Rows enough for the kernel for chunks of much work, with next to no keys each."""
+    b = Batch([(1100, 1100), (40, 300)], window=window, seed=window, head_major=window != 7)
+    b.call()
+    b.check()
+
+
+def test_graphs_that_share_a_workspace(gpu):
+    """Two captured graphs, of a chunk and of single tokens, use one workspace in turn."""
+    a, b = roomy(Batch([(60, 900), (30, 500)], seed=21)), Batch([(1, 3000), (1, 700)], seed=22, decode=True)
+    shared = torch.full((max(a.workspace().numel(), b.workspace().numel()),), 0xFF, device="cuda", dtype=torch.uint8)
+    graphs = []
+    for x in (a, b):
+        x.call(shared)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=gpu):
+            x.call(shared, stream=torch.cuda.current_stream())
+        graphs.append(graph)
+    for _ in range(3):
+        for x in (a, b):
+            x.out.fill_(7)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        a.check()
+        b.check()
