@@ -194,6 +194,27 @@ __device__ __forceinline__ std::uint32_t paged_rounds(std::uint32_t blocks, std:
                                                       std::uint32_t bits, std::uint32_t sequences, std::uint32_t least) {
   if (share >> 16 != 0) return share;
   const std::uint32_t lane = threadIdx.x & 63;
+  if (sequences > 16) { // neighbours as one, so that 16 remain at most (400 clocks each: 64 took 28,800)
+    const std::uint32_t width = scalar((sequences + 15) / 16);
+    std::uint32_t all = 0;
+    float l = 0, f = 0;
+    for (std::uint32_t i = 0; i < width; ++i) {
+      const std::uint32_t at = lane * width + i;
+      const auto of = [&](std::uint32_t x) {
+        return static_cast<std::uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4 * (at & 63)), static_cast<int>(x)));
+      };
+      const std::uint32_t b = of(blocks), last = of(tiles), first = of(lo);
+      if (at >= sequences) continue;
+      all += b;
+      l = fmaf(static_cast<float>(b), static_cast<float>(last), l);
+      f = fmaf(static_cast<float>(b), static_cast<float>(first), f);
+    }
+    const float each = __builtin_amdgcn_rcpf(static_cast<float>(all != 0 ? all : 1));
+    blocks = all;
+    tiles = static_cast<std::uint32_t>(fmaf(l, each, 0.5f));
+    lo = static_cast<std::uint32_t>(fmaf(f, each, 0.5f));
+    sequences = (sequences + width - 1) / width;
+  }
   std::uint32_t t = (share * (64 + 3 * lane) + 127) / 128; // (at least half of the share: items stay within blocks + 2 slots)
   t = t > least ? t : least;
   const float length = static_cast<float>(t), inverse = __builtin_amdgcn_rcpf(length);
@@ -261,7 +282,7 @@ __device__ __forceinline__ void paged_sort(PagedSeq &q, std::uint32_t &id, std::
 // plan for the kernel that joins the ranges.  With kRounds the items of up to 64 sequences are
 // the longest first and their ranges' length is chosen (16 query and 4 KV heads, against an even
 // share in the batch's order, us: 300 tokens of 30000 284 -> 190, 200 of 60000 359 -> 243, 16 sequences of
-// up to 8192 behind a window of 4096, ten of them single tokens, 222 -> 176; it takes a workgroup 2 to 7 us, of 1 to 32
+// up to 8192 behind a window of 4096, ten of them single tokens, 222 -> 176; it takes a workgroup 1.6 to 6 us, of 1 to 64
 // sequences).
 template <int kCols, int kUnit, bool kRounds = false>
 __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, const PagedScratch &sc, std::uint32_t index, bool first,
