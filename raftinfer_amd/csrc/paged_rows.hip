@@ -602,10 +602,10 @@ Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols,
 // stream kernel fetches a key once for 128 columns and keeps the matrix units busy, but its start and end cost
 // about 15 us of every workgroup (ring, 256 accumulator registers, the joining of its key groups).  Up to 40
 // squares of 32 x 32 pairs for each of 256 workgroups the rows kernel is the faster (16 query and 4 KV heads, us, rows
-// kernel first: 512 tokens 20.4 / 34.9, 1000 43.4 / 49.3, 500 of 1500 37.5 / 44.2, 64 of 4000 25.7 / 37.6, 16 of
-// 30000 56.7 / 69.6), above it the stream kernel (100 of 8000 68.3 / 52.1, 300 of 4000 76.5 / 71.8, 500 of 30501 and
-// 8001: twice as fast and more).  Several sequences: 4 of 125 41.5 / 41.1, 8 with 7 single tokens up to 8000
-// 105 / 92, 16 with up to 8192 behind a window of 4096 275 / 232.  Where the rows kernel would take a third round of
+// kernel first: 512 tokens 20.5 / 38.6, 1000 43.7 / 57.4, 500 of 1500 37.5 / 44.2, 64 of 4000 25.3 / 37.6, 16 of
+// 30000 56.7 / 69.6), above it the stream kernel (100 of 8000 68.3 / 51.5, 300 of 4000 78.4 / 56.4, 500 of 30501 and
+// 8001: twice as fast and more).  Several sequences: 4 of up to 500 tokens 41.5 / 42.6, 8 with 7 single tokens up to 8000
+// 105 / 80, 16 with up to 8192 behind a window of 4096 275 / 172.  Where the rows kernel would take a third round of
 // workgroups, few keys or not, the stream kernel is the faster too (windows of 32 and 200: 900 tokens 26.7 / 26.6 and 31.4 / 35.3,
 // 1200 38.1 / 22.3 and 46.1 / 36.3), unless its blocks would be half empty (600 sequences of 2 tokens 136 / 195).
 bool streams(const PagedArgs &a) {
