@@ -114,10 +114,14 @@ def _stream(stream) -> ctypes.c_void_p:
     return ctypes.c_void_p(handle)
 
 
+_DTYPE_CODES: dict = {}
+
+
 def _dtype_code(t) -> int:
-    import torch
-    return {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(
-        t.dtype, 0)
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
+    return _DTYPE_CODES.get(t.dtype, 0)
 
 
 # ------------------------------------------------------------- sizing API
@@ -537,10 +541,11 @@ def _strides(t) -> tuple:
     """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else must be dense."""
     if t is None:
         return 0, 0
-    if getattr(t, "ndim", 0) != 3:
+    try:
+        row, head, dim = t.stride()
+    except (AttributeError, ValueError):  # not three dimensions
         _dense(t)
         return 0, 0
-    row, head, dim = t.stride()
     rows, heads, dims = t.shape
     if dim != 1 and dims != 1:
         raise Qwen35PrimitiveError(1, "the last dimension of a tensor of heads must be contiguous")
@@ -554,13 +559,12 @@ def _dense(t):
     """The address of an argument without strides of its own."""
     if t is None:
         return None
-    if not getattr(t, "is_contiguous", _yes)():
-        raise Qwen35PrimitiveError(1, "indices, pages, weights and workspaces must be contiguous")
+    try:
+        if not t.is_contiguous():
+            raise Qwen35PrimitiveError(1, "indices, pages, weights and workspaces must be contiguous")
+    except AttributeError:  # not a tensor: it has an address only
+        pass
     return t.data_ptr()
-
-
-def _yes() -> bool:
-    return True
 
 
 def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
