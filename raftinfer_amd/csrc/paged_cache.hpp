@@ -72,12 +72,12 @@ __device__ __forceinline__ std::uint32_t paged_row(const PagedArgs &a, std::uint
 
 // -------------------------------------------------------- dealing out the work
 // A column is a (token, head of the group) of one KV head; a workgroup takes kCols columns
-// of a sequence and KV head, and of the tiles (of kUnit keys) that they see a range.  All of a batch's workgroups deal the work out alike, each by itself, from the
-// sequences' lengths: no launch in front, nothing kept.  The whole batch has W (column
-// block, tile) pairs; ranges have at most T = max(least, W / slots) tiles of a sequence's
-// longest block, so that about `slots` = 2^slot_bits workgroups per KV head run; 2^many_bits
-// times as many for `many` sequences and more, whose blocks are of different lengths.
-// Integers throughout: every kernel of a call finds the same.
+// of a sequence and KV head, and of the tiles (of kUnit keys) that they see a range.  All of a batch's
+// workgroups deal the work out alike, each by itself, from the sequences' lengths: no launch in front.  The
+// whole batch has W (column block, tile) pairs; ranges have at most T = max(least, W / slots) tiles of
+// a sequence's longest block, so that about `slots` = 2^slot_bits workgroups per KV head run; 2^many_bits
+// times as many for `many` sequences and more, whose blocks are of different lengths.  (Chunks of much
+// work weigh T against others, see paged_rounds.)  The kernel that joins the ranges reads T from the workspace.
 struct PagedSplit {
   std::uint32_t least, slot_bits, many, many_bits;
   std::uint32_t parts; // partial results that the workspace holds, each of a block and KV head

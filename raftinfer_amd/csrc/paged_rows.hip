@@ -14,16 +14,15 @@ using prefill::kLazyRescale;
 
 __device__ unsigned int g_paged_capacity_errors = 0;
 
-// A form of the kernel: 16 CB columns a workgroup, WAVES waves, steps of 16 G keys, of which a wave has
-// ST on the way.
-template <int CB_, int WAVES_, int G_, int ST_> struct Form {
-  static constexpr int CB = CB_, WAVES = WAVES_, G = G_, ST = ST_;
+// A form of the kernel: 16 CB columns a workgroup, WAVES waves, steps of 16 G keys.
+template <int CB_, int WAVES_, int G_> struct Form {
+  static constexpr int CB = CB_, WAVES = WAVES_, G = G_;
   static constexpr int kCols = 16 * CB, kKeys = kPageGranule * G, kThreads = WAVES * kWave;
   static constexpr int kLoads = 8 * G;                 // of a plane of a step, 1 KiB each
   static constexpr unsigned kPlane = kLoads * 1024;    // bytes
 };
-using DecodeForm = Form<1, 4, 1, 1>;
-using FewForm = Form<2, 4, 2, 1>;
+using DecodeForm = Form<1, 4, 1>;
+using FewForm = Form<2, 4, 2>;
 
 // 16-byte chunk c of row r of a granule lies at c ^ rows_key(r): a pass of the K reads takes one
 // chunk of 16 rows, of the transposed V reads 32 bytes of 8 rows.  (Linear in the bits of r.)
@@ -31,7 +30,7 @@ __device__ __forceinline__ constexpr std::uint32_t rows_key(std::uint32_t r, boo
 
 template <class F> struct RowsShared {
   union {
-    alignas(1024) unsigned char rows[F::WAVES][F::ST][2][F::kPlane]; // K, V
+    alignas(1024) unsigned char rows[F::WAVES][2][F::kPlane]; // K, V
     // (the pad puts the 16 columns of a store on banks of their own)
     float acc[F::WAVES][16][kHeadDim + 4];
   };
@@ -65,7 +64,7 @@ template <int kOffset, bool Once> __device__ __forceinline__ void load_rows(cons
 // and the first keys, 2.5 for the queries, 4 for two steps, 4 to join the waves.
 template <class F, bool HeadMajor, bool Once>
 __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a, PagedScratch sc, PagedSplit sp) {
-  constexpr int CB = F::CB, WAVES = F::WAVES, G = F::G, ST = F::ST, L = F::kLoads;
+  constexpr int CB = F::CB, WAVES = F::WAVES, G = F::G, L = F::kLoads;
   __shared__ RowsShared<F> sh;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -105,8 +104,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
   const std::uint32_t row_bytes = HeadMajor ? kRowBytes : a.row_step * kRowBytes, skip = 2 * (row_bytes - kRowBytes);
   const std::uint32_t off_row = (lane >> 5) * row_bytes;
   const std::uint32_t off_k = off_row + 16 * ((lane & 31) ^ rows_key(lane >> 5, false)), off_v = off_row + 16 * ((lane & 31) ^ rows_key(lane >> 5, true));
-  const unsigned slots = lds_address(sh.rows[wave][0][0]);
-  const auto plane_at = [&](std::uint32_t t, bool is_v) { return slots + F::kPlane * (2 * (t % ST) + is_v); };
+  const unsigned k_plane = lds_address(sh.rows[wave][0]), v_plane = k_plane + F::kPlane;
   const auto load = [&](std::uint32_t t, auto is_v) __attribute__((always_inline)) {
     prefill::static_for<L>([&](auto ic) __attribute__((always_inline)) {
       constexpr int g = ic / 8, i = ic % 8;
@@ -114,7 +112,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
       const unsigned char *base = a.pages + static_cast<std::size_t>(row) * kRowBytes + (i >> 2) * 8 * (HeadMajor ? kRowBytes : row_bytes);
       std::uint32_t off = (is_v ? off_v : off_k) ^ (16 * rows_key(2 * i, is_v));
       if constexpr (!HeadMajor && (i & 3) != 0) off += (i & 3) * skip;
-      load_rows<1024 * (i & 3), Once>(base, off, plane_at(t, is_v) + 8192 * g + 4096 * (i >> 2));
+      load_rows<1024 * (i & 3), Once>(base, off, (is_v ? v_plane : k_plane) + 8192 * g + 4096 * (i >> 2));
     });
   };
   constexpr std::false_type kIsK{};
@@ -149,11 +147,6 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
 #pragma unroll
     for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(qb[cb][i]));
   if (steps != 0) load(0, kIsV);
-  if constexpr (ST == 2)
-    if (steps > 1) {
-      load(1, kIsK);
-      load(1, kIsV);
-    }
   // The gates of the columns that this wave writes: every WAVES-th of 16, four dims a lane.
   constexpr int kMine = 16 / WAVES;
   [[maybe_unused]] u32x2 gate[CB][kMine];
@@ -192,13 +185,12 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
 #pragma unroll 1
   for (std::uint32_t t = 0; t < steps; ++t) {
     const std::uint32_t j0 = tile_of(t) * F::kKeys;
-    const bool hide = masked(j0), more = t + ST < steps;
-    if ((t + ST - t0) * G >= 64 && more) load_table(t + ST);
-    // K(t): V(t) and, of two stages, K(t + 1), V(t + 1) are behind it
-    if (ST == 2 && t + 1 < steps) wait_vm<3 * L>(); else wait_vm<L>();
+    const bool hide = masked(j0), more = t + 1 < steps;
+    if ((t + 1 - t0) * G >= 64 && more) load_table(t + 1);
+    wait_vm<L>(); // K(t): V(t) is behind it
     floatx4 s[CB][G]; // keys j0 + 16 g + 4 kq + e
     {
-      const unsigned k_base = plane_at(t, false) + k_lane;
+      const unsigned k_base = k_plane + k_lane;
       const auto read_k = [&](int i) { return lds_operand((k_base ^ (64u * (i / G))) + 8192u * (i % G)); };
       constexpr int kRing = 8;
       bf16x8 op[kRing];
@@ -221,7 +213,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
     }
     __builtin_amdgcn_sched_barrier(0);
     wait_lgkm0(); // the reads are done: their place is free
-    if (more) load(t + ST, kIsK);
+    if (more) load(t + 1, kIsK);
     constexpr float kScale = kLog2e / 16.0f;
     bool grow = false;
     float mx[CB];
@@ -275,13 +267,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
         }
       }
     }
-    // V(t): K(t + 1) is behind it, of two stages V(t + 1) and K(t + 2) too
-    if constexpr (ST == 2) {
-      if (more) wait_vm<3 * L>(); else if (t + 1 < steps) wait_vm<2 * L>(); else wait_vm<0>();
-    } else {
-      if (more) wait_vm<L>(); else wait_vm<0>();
-    }
-    const unsigned v_plane = plane_at(t, true);
+    if (more) wait_vm<L>(); else wait_vm<0>(); // V(t): K(t + 1) is behind it
     if (hide) {
       // A masked key has probability 0, and 0 times an infinite or NaN value is not 0: such
       // values are taken out here and added behind the loop, to the columns that see them.
@@ -328,7 +314,7 @@ __global__ __launch_bounds__(F::kThreads, 1) void paged_rows_kernel(PagedArgs a,
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_lgkm0();
-    if (more) load(t + ST, kIsV);
+    if (more) load(t + 1, kIsV);
   }
   if (odd != 0) {
 #pragma unroll 1
