@@ -688,3 +688,20 @@ def test_graphs_that_share_a_workspace(gpu):
         torch.cuda.synchronize()
         a.check()
         b.check()
+
+
+@pytest.mark.parametrize("sequences,decode", [(700, True), (700, False), (4300, True)])
+def test_sequences_beyond_waves(gpu, sequences, decode):
+    """Several sequences a lane, and beyond 64 of them; some unused, one long."""
+    rng = np.random.default_rng(sequences)
+    each = [(1 if decode else int(rng.integers(0, 4)), int(rng.integers(4, 40))) for i in range(sequences)]
+    each[sequences // 3] = (1, 3000)
+    b = Batch(each, 1, 2, seed=sequences, decode=decode)
+    idle = [i for i in range(sequences) if decode and i % 9 == 4]
+    if idle:
+        b.lengths[torch.tensor(idle, device="cuda")] = 0
+    b.call()
+    torch.cuda.synchronize()
+    b.pages = b.pages.cpu().double()  # (once, not for every sequence)
+    b.check(only=set(range(sequences)) - set(idle))
+    assert all((b.out[i] == 7).all() for i in idle[:50]) and errors() == 0
