@@ -705,3 +705,34 @@ def test_sequences_beyond_waves(gpu, sequences, decode):
     b.pages = b.pages.cpu().double()  # (once, not for every sequence)
     b.check(only=set(range(sequences)) - set(idle))
     assert all((b.out[i] == 7).all() for i in idle[:50]) and errors() == 0
+
+
+@pytest.mark.parametrize("head_major,rotary,interleaved,norm,kv_heads,group", [(True, 64, False, "bf16", 4, 4), (False, 256, True, "f32", 3, 5),
+                                                                               (True, 0, False, "q", 1, 1), (False, 32, False, "k", 1, 16)])
+def test_append_of_long_chunks(gpu, head_major, rotary, interleaved, norm, kv_heads, group):
+    """Rows enough for several a workgroup, sequences that begin and end inside one."""
+    each = [(701, 800), (0, 9), (330, 330), (1, 50), (2, 2), (1, 17), (6, 100)]
+    test_append(gpu, each, 48, kv_heads, group, rotary, interleaved, norm, head_major)
+
+
+def test_append_of_long_chunks_refuses_bad_sequences(gpu):
+    b = Batch([(501, 600), (3, 20), (402, 500), (203, 300), (2, 7)], seed=7)
+    before, out = b.pages.clone(), torch.full_like(b.q, 7.0)
+    b.lengths[1] = 2                              # below its new tokens
+    b.table[2, 499 // 16] = -1                    # the page of the positions 496 .. 499
+    b.starts[5] = b.rows + 9                      # behind the call's rows
+    k, v = (torch.randn(b.rows, 4, 256, generator=b.g, device="cuda").to(BF) for _ in (0, 1))
+    errors()
+    ops.qwen35_paged_cache_append(b.q, k, v, out, b.pages, b.table, b.starts, b.lengths, None, None, None, b.shape,
+                                  ops.Qwen35PagedRotary(0), ops.HEAD_MAJOR)
+    torch.cuda.synchronize()
+    assert errors() >= 3
+    expect = before.clone()
+    for i, skip in ((0, 600), (2, 496), (3, 300)):
+        n, c = b.each[i]
+        for p in range(c - n, min(c, skip)):
+            page, row = int(b.table[i, p // 16]), int(b.starts_host[i]) + p - (c - n)
+            expect[page, 0, :, p % 16], expect[page, 1, :, p % 16] = k[row], v[row]
+    assert torch.equal(b.pages.view(torch.int16), expect.view(torch.int16))
+    assert torch.equal(out[:501], b.q[:501]) and torch.equal(out[504:1109], b.q[504:1109])
+    assert (out[501:504] == 7).all() and (out[1109:] == 7).all()
