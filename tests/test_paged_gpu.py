@@ -736,3 +736,37 @@ def test_append_of_long_chunks_refuses_bad_sequences(gpu):
     assert torch.equal(b.pages.view(torch.int16), expect.view(torch.int16))
     assert torch.equal(out[:501], b.q[:501]) and torch.equal(out[504:1109], b.q[504:1109])
     assert (out[501:504] == 7).all() and (out[1109:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["decode", "few", "much"])
+def test_more_heads_than_places(gpu, kind):
+    """KV heads beyond the workgroups that are dealt out for each."""
+    b = Batch([(1 if kind == "decode" else 12, 600)], 260, 1, seed=2, decode=kind == "decode")
+    if kind == "much":
+        roomy(b)
+    b.call()
+    torch.cuda.synchronize()
+    b.pages = b.pages.cpu().double()
+    b.check()
+    assert errors() == 0
+
+
+@pytest.mark.parametrize("kind", ["decode", "few", "much"])
+def test_infinite_keys(gpu, kind):
+    """A score of +inf makes its row NaN, one of -inf leaves its key out; rows that do not see the key are as ever."""
+    b = Batch([(1, 600), (1, 70)] if kind == "decode" else [(40, 600), (30, 70)], seed=17, decode=kind == "decode")
+    if kind == "much":
+        roomy(b)
+    for i, j in ((0, 590), (0, 3), (1, 60)):
+        b.pages[int(b.table[i, j // 16]), 0, i, j % 16, 5] = float("inf")
+    b.call()
+    torch.cuda.synchronize()
+    got = wide(b.out)
+    some = False
+    for i, (n, c) in enumerate(b.each):
+        rows, want, tol = b.want(i)
+        assert np.array_equal(np.isnan(got[rows]), np.isnan(want)), i
+        some |= np.isnan(want).any() and not np.isnan(want).all()
+    assert some
+    # finite rows of the KV heads that the keys do not belong to, and of the others without the keys
+    b.check()
