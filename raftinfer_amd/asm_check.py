@@ -12,7 +12,10 @@ The build therefore scans the kernels' gfx950 assembly and fails on
 * any vector instruction that writes an operand of an inline-asm MFMA, its
   accumulator among them, within the two wait states before it;
 * in kernels that address the accumulation registers by number (`owned_agprs`),
-  any use of one outside asm: it would overwrite an accumulator.
+  any use of one outside asm: it would overwrite an accumulator;
+* any memory instruction that reads a scalar register within the five wait states
+  behind a vector instruction that writes it, and any load into LDS right behind a
+  write of M0: around inline asm the compiler leaves these waits out too.
 """
 from __future__ import annotations
 
@@ -25,8 +28,14 @@ RESULT_WAIT_STATES = 19
 # Wait states between a VALU write of a register and an MFMA that reads it.
 OPERAND_WAIT_STATES = 2
 
+# Wait states between a VALU write of a scalar register and a memory instruction that
+# reads it, and between a write of M0 and a load into LDS.
+SCALAR_WAIT_STATES = 5
+M0_WAIT_STATES = 1
+
 _INDEX = r"(0x[0-9a-f]+|\d+)"
 _REGISTER = re.compile(rf"\b([av])\[{_INDEX}:{_INDEX}\]|\b([av])\[?{_INDEX}\b")
+_SCALAR = re.compile(rf"\bs\[{_INDEX}:{_INDEX}\]|\bs{_INDEX}\b|\b(vcc|m0)\b")
 _LABEL = re.compile(r"^([\w.$]+):")
 _NOP = re.compile(r"^s_nop\s+(\d+)")
 
@@ -139,4 +148,67 @@ def _one_pass(assembly: str, owned_agprs: bool, arrivals):
         written = [e for e in written if e[1] > 0]
         if not opcode.startswith("v_mfma"):
             written += [[r, OPERAND_WAIT_STATES, number] for r in _vector_writes(opcode, operands)]
+    return hazards, found
+
+
+def _scalars(text: str):
+    """(name, first, last) of every scalar register named; vcc and m0 by their names."""
+    found = []
+    for m in _SCALAR.finditer(text):
+        if m.group(4):
+            found.append((m.group(4), 0, 0))
+        else:
+            first = m.group(1) or m.group(3)
+            found.append(("s", int(first, 0), int(m.group(2) or first, 0)))
+    return found
+
+
+def scalar_wait_hazards(assembly: str) -> list[str]:
+    """The memory instructions that read a scalar register, or M0, too soon after it is
+    written, along every path as above."""
+    arrivals: dict[str, dict] = {}
+    while True:
+        hazards, found = _one_scalar_pass(assembly, arrivals)
+        if found == arrivals:
+            return hazards
+        arrivals = found
+
+
+def _one_scalar_pass(assembly: str, arrivals):
+    found = {label: dict(entries) for label, entries in arrivals.items()}
+    hazards: list[str] = []
+    pending: dict = {}  # (register, line): wait states left
+    for number, raw in enumerate(assembly.splitlines(), 1):
+        text = raw.strip()
+        label = _LABEL.match(text)
+        if label and label.group(1) in arrivals:
+            _merge(pending, [(r, left, line) for (r, line), left in arrivals[label.group(1)].items()])
+        text = text.split(";")[0].strip()
+        if not text or text.startswith(".") or text.endswith(":"):
+            continue
+        opcode, _, rest = text.partition(" ")
+        operands = rest.split(",")
+        if opcode.startswith(("global_", "buffer_", "flat_", "scratch_")):
+            reads = _scalars(rest) + ([("m0", 0, 0)] if "lds" in opcode or rest.endswith(" lds") else [])
+            hazards += [f"line {number}: {text}: reads {r[0]} {left} wait states too soon after line {line}"
+                        for (r, line), left in pending.items() if any(_overlap(r, x) for x in reads)]
+        nop = _NOP.match(text)
+        step = int(nop.group(1)) + 1 if nop else 1
+        pending = {key: left - step for key, left in pending.items() if left > step}
+        if opcode.startswith("v_"):
+            if rest.lstrip().startswith("v") and "s[" not in rest and "vcc" not in rest and not opcode.startswith("v_cmp"):
+                continue  # (most: no scalar result)
+            # a scalar result: the first operand, of carries and scaled divisors the second; vcc unnamed
+            results = _scalars(operands[0]) + (_scalars(operands[1]) if re.search("_co_|div_scale|v_mad_[iu]64", opcode) else [])
+            results += [("vcc", 0, 0)] if opcode.startswith("v_cmp") and opcode.endswith("_e32") else []
+            pending.update({(r, number): SCALAR_WAIT_STATES for r in results})
+        elif opcode.startswith("s_") and not opcode.startswith(("s_cmp", "s_bitcmp")) and rest:
+            written = _scalars(operands[0])
+            pending = {key: left for key, left in pending.items() if not any(key[0][0] == w[0] and w[1] <= key[0][1] and key[0][2] <= w[2] for w in written)}
+            if ("m0", 0, 0) in written:
+                pending[("m0", 0, 0), number] = M0_WAIT_STATES
+        if opcode.startswith(("s_branch", "s_cbranch")):
+            _merge(found.setdefault(rest.strip(), {}), [(r, left, line) for (r, line), left in pending.items()])
+        if opcode.startswith(("s_branch", "s_endpgm", "s_setpc")):
+            pending = {}
     return hazards, found

@@ -43,19 +43,21 @@ def _compile(src: pathlib.Path) -> pathlib.Path:
     return obj
 
 
-# Sources whose kernels issue MFMAs from inline asm; their gfx950 assembly is
-# checked for the hazards that the compiler cannot see (asm_check.py).  The
-# second entry: whether the kernel owns the accumulation registers by number.
+# Sources whose kernels issue MFMAs from inline asm, or loads into LDS whose waits are
+# not all in the asm itself; their gfx950 assembly is checked for the hazards that the
+# compiler cannot see (asm_check.py).  The second entry: whether the kernel owns the
+# accumulation registers by number.
 ASM_CHECKED = {"attention_prefill_mfma.hip": False, "attention_prefill_wide.hip": True,
-               "paged_prefill.hip": True}
+               "paged_prefill.hip": True, "paged_rows.hip": False, "compact_prefill.hip": False,
+               "delta.hip": False}
 
 
 def _check_asm(name: str) -> None:
     try:
-        from .asm_check import asm_mfma_hazards
+        from .asm_check import asm_mfma_hazards, scalar_wait_hazards
     except ImportError:  # run as a script
         sys.path.insert(0, str(PKG))
-        from asm_check import asm_mfma_hazards
+        from asm_check import asm_mfma_hazards, scalar_wait_hazards
 
     src = CSRC / name
     out = BUILD / (name + ".s")
@@ -63,9 +65,10 @@ def _check_asm(name: str) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc -S failed for {name}:\n{res.stderr}")
-    hazards = asm_mfma_hazards(out.read_text(), ASM_CHECKED[name])
+    assembly = out.read_text()
+    hazards = asm_mfma_hazards(assembly, ASM_CHECKED[name]) + scalar_wait_hazards(assembly)
     if hazards:
-        raise RuntimeError(f"{name}: inline-asm MFMA hazards "
+        raise RuntimeError(f"{name}: hazards around inline asm "
                            f"({len(hazards)}):\n" + "\n".join(hazards[:10]))
 
 

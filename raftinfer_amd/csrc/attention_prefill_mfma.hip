@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void prefill_mfma_kernel(
     if (rows_left >= kKTile) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        load_lds_b128(base, voff_half[i & 1] + 8 * (i >> 1) * row_bytes + 256u * hh,
+        load_lds_b128<0>(base, voff_half[i & 1] + 8 * (i >> 1) * row_bytes + 256u * hh,
                       lds + 8192u * hh + 1024u * i);
     } else {
 #pragma unroll
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads) void prefill_mfma_kernel(
         const int r = 4 * i + hrow;
         const int last = static_cast<int>(rows_left) - 1;
         const std::uint32_t rr = r < last ? r : last;
-        load_lds_b128(base, rr * row_bytes + 256u * hh + 16u * (hpc ^ swz(r)), lds + 8192u * hh + 1024u * i);
+        load_lds_b128<0>(base, rr * row_bytes + 256u * hh + 16u * (hpc ^ swz(r)), lds + 8192u * hh + 1024u * i);
       }
     }
   };
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void prefill_mfma_kernel(
       const std::size_t rrow = static_cast<std::size_t>(rt) < q_rows ? rt : q_rows - 1;
       const std::uint32_t voff = static_cast<std::uint32_t>(rrow * kQueryHeads + (r >> 3)) * (q_row_elems * 2) +
                                  16u * (col ^ swz(r));
-      load_lds_b128(query + (t0 * kQueryHeads + kv_head * kGroup) * q_row_elems, voff, lq + 1024u * i);
+      load_lds_b128<0>(query + (t0 * kQueryHeads + kv_head * kGroup) * q_row_elems, voff, lq + 1024u * i);
     }
   }
   [[maybe_unused]] NormQShared *nqs = nullptr;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void prefill_mfma_kernel(
     if (wave_u == 0) {
       const std::uint32_t bytes = nq.weight_f32 ? 1024u : 512u;
       const std::uint32_t off = 16u * lane < bytes ? 16u * lane : bytes - 16u;
-      load_lds_b128(nq.weight, off, lds_address(nq_sh.weight));
+      load_lds_b128<0>(nq.weight, off, lds_address(nq_sh.weight));
     }
   }
   std::size_t t = wave_u;

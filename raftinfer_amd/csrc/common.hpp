@@ -203,8 +203,12 @@ template <typename T> __device__ __forceinline__ unsigned lds_address(T *p) {
 // operands never depend on the compiler proving that uniformity.  Written as
 // asm, with the waits below issued by hand: the compiler cannot tell which
 // LDS region such a load writes and would otherwise wait for every
-// outstanding one before each LDS read.  The kernels that use it issue no
-// other instruction that reads M0.
+// outstanding one before each LDS read.  Nor does it insert wait states around
+// asm: the hardware needs one between a write of M0 and the load, and five between
+// a vector instruction's write of a scalar register (a readfirstlane that stays one)
+// and a memory instruction that reads it.  kNop 3 gives both, 0 the first; then the
+// base must come out of scalar arithmetic, which the build checks (asm_check.py).
+template <int kNop = 3>
 __device__ __forceinline__ void load_lds_b128(const void *base, std::uint32_t voff, unsigned lds) {
   // readfirstlane returns int: each half goes back to uint32 before it is
   // widened, so a low word with bit 31 set is not sign-extended into the
@@ -216,9 +220,9 @@ __device__ __forceinline__ void load_lds_b128(const void *base, std::uint32_t vo
   const auto slds = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(lds));
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop %3\n\tglobal_load_lds_dwordx4 %1, %2"
                :
-               : "s"(slds), "v"(voff), "s"(sbase)
+               : "s"(slds), "v"(voff), "s"(sbase), "n"(kNop)
                : "memory", "m0");
 #pragma clang diagnostic pop
 }
@@ -232,7 +236,7 @@ __device__ __forceinline__ void load_lds_b32(const void *base, std::uint32_t vof
   const auto slds = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(lds));
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
                :
                : "s"(slds), "v"(voff), "s"(sbase)
                : "memory", "m0");

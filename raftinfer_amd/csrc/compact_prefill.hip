@@ -236,12 +236,12 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       const std::uint32_t off = in * row_bytes + 16u * (Fp8 ? chunk : chunk ^ row_key(8 * wave + in));
 #pragma unroll
       for (int i = 0; i < kInst; ++i)
-        load_lds_b128(tile + (8u * wave + kRows * i) * row_bytes, Fp8 ? off : off ^ (16u * (8 * (i & 1) + (i >> 1))), to + 1024u * i);
+        load_lds_b128<0>(tile + (8u * wave + kRows * i) * row_bytes, Fp8 ? off : off ^ (16u * (8 * (i & 1) + (i >> 1))), to + 1024u * i);
     } else {
 #pragma unroll
       for (int i = 0; i < kInst; ++i) {
         const std::uint32_t r = 8 * wave + kRows * i + in;
-        load_lds_b128(tile, (r < last ? r : last) * row_bytes + 16u * (Fp8 ? chunk : chunk ^ row_key(r)), to + 1024u * i);
+        load_lds_b128<0>(tile, (r < last ? r : last) * row_bytes + 16u * (Fp8 ? chunk : chunk ^ row_key(r)), to + 1024u * i);
       }
     }
   };
@@ -548,12 +548,12 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
       const std::uint32_t off = in_row * row_bytes + 16 * (chunk ^ keys_at<Fp8>(in_row, is_v));
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        load_lds_b128(tile + kRows * i * row_bytes, off ^ (16 * keys_at<Fp8>(kRows * i, is_v)), to + 1024 * i);
+        load_lds_b128<0>(tile + kRows * i * row_bytes, off ^ (16 * keys_at<Fp8>(kRows * i, is_v)), to + 1024 * i);
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const std::uint32_t r = kRows * i + in_row;
-        load_lds_b128(tile, (r < last ? r : last) * row_bytes + 16 * (chunk ^ keys_at<Fp8>(r, is_v)), to + 1024 * i);
+        load_lds_b128<0>(tile, (r < last ? r : last) * row_bytes + 16 * (chunk ^ keys_at<Fp8>(r, is_v)), to + 1024 * i);
       }
     }
   };
@@ -596,7 +596,7 @@ __global__ __launch_bounds__(kPThreads, 1) void compact_prefill_keys_kernel(
   if (!part) {
 #pragma unroll
     for (int i = 0; i < kKCols / kPWaves; i += 2)
-      load_lds_b128(a.gate + row0, 2 * row_at(kPWaves * (i + (lane >> 5)) + wave) + 16 * (lane & 31), lds_address(sh.gate[wave][i]));
+      load_lds_b128<0>(a.gate + row0, 2 * row_at(kPWaves * (i + (lane >> 5)) + wave) + 16 * (lane & 31), lds_address(sh.gate[wave][i]));
   }
   if constexpr (!Fp8) {
     if (a.store_inside && (!Split || blockIdx.z == 0)) store_rows(a, c, kvh, col0, col0 + last_x + 1);

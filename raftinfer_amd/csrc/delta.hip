@@ -1330,7 +1330,7 @@ __device__ __forceinline__ void load_rows_lds(const unsigned char *record, std::
     for (int j = 0; j < ROWS / kRpi; ++j) {
       const int row = row0 + j * kRpi + rr;
       const int logical = C == kChunkDim ? p ^ (row & 15) : p ^ ((row >> 1) & 7);
-      load_lds_b128(record, off + static_cast<std::uint32_t>(((hl * R + row) * C + logical * 8) * 2),
+      load_lds_b128<0>(record, off + static_cast<std::uint32_t>(((hl * R + row) * C + logical * 8) * 2),
                     lds_address(&dst[hl][row0 + j * kRpi][0]));
     }
 }
@@ -1362,13 +1362,13 @@ struct ScanLoads {
     load_rows_lds<kChunk, kChunkDim, 16, 2>(record, rec::kW, sh.w, 16 * wave);
     const int lane = threadIdx.x & 63;
     // U rows 16 wave + lane / 4, 16-byte piece lane % 4 of columns c0 ..
-    load_lds_b128(record,
+    load_lds_b128<0>(record,
                   static_cast<std::uint32_t>(rec::kU + ((16 * wave + (lane >> 2)) * kChunkDim + c0) * 4 +
                                              (lane & 3) * 16),
                   lds_address(&sh.u[16 * wave][0]));
     // G[16 wave .. +15]: lanes 0..3 only (every wave issues the instruction).
     if (lane < 4)
-      load_lds_b128(record, static_cast<std::uint32_t>(rec::kG + (16 * wave + 4 * lane) * 4),
+      load_lds_b128<0>(record, static_cast<std::uint32_t>(rec::kG + (16 * wave + 4 * lane) * 4),
                     lds_address(&sh.g[parity][16 * wave]));
   }
   __device__ static void kt(Scan3Shared &sh, const unsigned char *record, int wave) {
@@ -1824,8 +1824,8 @@ __device__ __forceinline__ void tscan_issue(TScanBuf &b, const Src<bf16_bits> &q
     const int row0 = 16 * u + 4 * j, row = row0 + (lane >> 4), p = lane & 15;
     const int src = row < L ? row : L - 1;
     const std::uint32_t chunk = static_cast<std::uint32_t>((p ^ (row & 15)) * 16);
-    load_lds_b128(qb, static_cast<std::uint32_t>(src * qs.row * 2) + chunk, lds_address(&b.q[row0][0]));
-    load_lds_b128(kb, static_cast<std::uint32_t>(src * ks.row * 2) + chunk, lds_address(&b.k[row0][0]));
+    load_lds_b128<0>(qb, static_cast<std::uint32_t>(src * qs.row * 2) + chunk, lds_address(&b.q[row0][0]));
+    load_lds_b128<0>(kb, static_cast<std::uint32_t>(src * ks.row * 2) + chunk, lds_address(&b.k[row0][0]));
   }
   const int half = u >> 1, rows = 32 * (u & 1);
   load_rows_lds<kChunk, kChunk, 32, 1>(record, static_cast<std::uint32_t>(rec2::kTb + half * kChunk * kChunk * 2),
@@ -1835,10 +1835,10 @@ __device__ __forceinline__ void tscan_issue(TScanBuf &b, const Src<bf16_bits> &q
   if (u < 2) {
     const int row = 32 * u + (lane >> 1), src = row < L ? row : L - 1;
     const bf16_bits *vb = vs.base + t0 * vs.row + h * vs.head_stride + c0;
-    load_lds_b128(vb, static_cast<std::uint32_t>(src * vs.row * 2 + (lane & 1) * 16),
+    load_lds_b128<0>(vb, static_cast<std::uint32_t>(src * vs.row * 2 + (lane & 1) * 16),
                   lds_address(&b.v[32 * u][0]));
   } else if (u == 2 && lane < 16) {
-    load_lds_b128(record, static_cast<std::uint32_t>(rec2::kG + 16 * lane), lds_address(&b.g[0]));
+    load_lds_b128<0>(record, static_cast<std::uint32_t>(rec2::kG + 16 * lane), lds_address(&b.g[0]));
   }
 }
 
@@ -2054,7 +2054,7 @@ struct TScanSplitLoads {
     for (int j = 0; j < 4; ++j) {
       const int row0 = 16 * u + 4 * j, r = row0 + (lane >> 4), p = lane & 15;
       const int src = r < L ? r : L - 1;
-      load_lds_b128(base, static_cast<std::uint32_t>(src * row * 2 + (p ^ (r & 15)) * 16),
+      load_lds_b128<0>(base, static_cast<std::uint32_t>(src * row * 2 + (p ^ (r & 15)) * 16),
                     lds_address(&dst[row0][0]));
     }
   }
@@ -2064,7 +2064,7 @@ struct TScanSplitLoads {
     rows128(sh.k[parity][0], kb, ks.row, L, u);
     rows128(sh.k[parity][1], kb + lo_plane, ks.row, L, u);
     if (u == 2 && (threadIdx.x & 63) < 16)
-      load_lds_b128(record, static_cast<std::uint32_t>(rec2::kG + 16 * (threadIdx.x & 63)),
+      load_lds_b128<0>(record, static_cast<std::uint32_t>(rec2::kG + 16 * (threadIdx.x & 63)),
                     lds_address(&sh.g[parity][0]));
   }
   __device__ static void m(TScanSplitShared &sh, const unsigned char *record, int u) {
@@ -2086,7 +2086,7 @@ struct TScanSplitLoads {
     const int lane = threadIdx.x & 63;
     const int row = 32 * (u & 1) + (lane >> 1), src = row < L ? row : L - 1;
     const bf16_bits *vb = vs.base + t0 * vs.row + h * vs.head_stride + c0 + (u >> 1) * lo_plane;
-    load_lds_b128(vb, static_cast<std::uint32_t>(src * vs.row * 2 + (lane & 1) * 16),
+    load_lds_b128<0>(vb, static_cast<std::uint32_t>(src * vs.row * 2 + (lane & 1) * 16),
                   lds_address(&sh.v[u >> 1][32 * (u & 1)][0]));
   }
   // Waits until at most `later` of this wave's loads are outstanding (loads

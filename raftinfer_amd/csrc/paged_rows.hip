@@ -44,14 +44,16 @@ __device__ __forceinline__ float lane_value(float x, int lane) {
 __device__ __forceinline__ std::uint32_t cut_bf16x2(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
-// load_lds_b128 with an instruction offset, which counts for both addresses; Once: the memory is not
-// read again.
+// load_lds_b128_at; Once: the memory is not read again.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int kOffset, bool Once> __device__ __forceinline__ void load_rows(const void *base, std::uint32_t voff, unsigned lds) {
   if constexpr (Once)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3 nt" : : "s"(lds), "v"(voff), "s"(base), "n"(kOffset) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3 nt" : : "s"(lds), "v"(voff), "s"(base), "n"(kOffset) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" : : "s"(lds), "v"(voff), "s"(base), "n"(kOffset) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" : : "s"(lds), "v"(voff), "s"(base), "n"(kOffset) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // A workgroup takes the columns of one block of one KV head and a range of their keys; wave w takes the
 // range's steps w, w + WAVES, ..  S = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16, operands

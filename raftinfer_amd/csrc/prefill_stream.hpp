@@ -29,19 +29,24 @@ template <unsigned kXor, unsigned kAdd> __device__ __forceinline__ std::uint32_t
   return x;
 }
 // load_lds_b128 with an instruction offset, which the hardware adds to both the
-// memory and the LDS address.
+// memory and the LDS address.  Between the write of M0 and the load the hardware
+// needs a wait state; the five in front of it for a base that a vector instruction
+// writes are for the compiler's scalar arithmetic to give (the build checks both).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int kOffset>
 __device__ __forceinline__ void load_lds_b128_at(const void *base, std::uint32_t voff, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
                :
                : "s"(lds), "v"(voff), "s"(base), "n"(kOffset)
-               : "memory");
+               : "memory", "m0");
 }
 
 // 16 bytes from an address of each lane's own into LDS at lds + 16 * lane.
 __device__ __forceinline__ void load_lds_b128_lane(const void *from, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // The O^T accumulators (2 column blocks x 8 dim blocks x 16 registers) fill the
 // 256 accumulation registers, and are addressed by number from asm: block

@@ -110,3 +110,65 @@ def test_built_paged_kernel_has_no_hazard():
         import pytest
         pytest.skip("the library has not been built here")
     assert asm_mfma_hazards(s.read_text(), owned_agprs=True) == []
+
+
+# ------------------------------------------ waits of loads through scalar registers
+
+LOAD = "\tglobal_load_lds_dwordx4 v4, s[10:11] offset:1024\n"
+
+
+def test_a_load_into_lds_waits_for_m0():
+    from raftinfer_amd.asm_check import scalar_wait_hazards
+    assert len(scalar_wait_hazards("\ts_mov_b32 m0, s5\n" + LOAD)) == 1
+    assert len(scalar_wait_hazards("\ts_add_i32 m0, s5, 16\n\tbuffer_load_dword v1, s[4:7], 0 offen lds\n")) == 1
+    assert scalar_wait_hazards("\ts_mov_b32 m0, s5\n\ts_nop 0\n" + LOAD) == []
+    assert scalar_wait_hazards("\ts_mov_b32 m0, s5\n\tglobal_load_dwordx4 v[4:7], v4, s[10:11]\n" + LOAD) == []
+    # over a branch, which is a wait state itself
+    assert scalar_wait_hazards("\ts_mov_b32 m0, s5\n\ts_branch .L1\n\ts_nop 0\n.L1:\n" + LOAD) == []
+
+
+def test_a_memory_instruction_waits_for_a_vector_write_of_its_scalars():
+    from raftinfer_amd.asm_check import scalar_wait_hazards
+    write = "\tv_readfirstlane_b32 s11, v2\n"
+    assert len(scalar_wait_hazards(write + "\ts_nop 3\n" + LOAD)) == 1
+    assert scalar_wait_hazards(write + "\ts_nop 4\n" + LOAD) == []
+    assert scalar_wait_hazards(write.replace("s11", "s12") + LOAD) == []
+    # a scalar instruction's own write has no such wait
+    assert scalar_wait_hazards(write + "\ts_add_u32 s11, s11, s3\n" + LOAD) == []
+    assert len(scalar_wait_hazards(write + "\ts_cmp_eq_u32 s11, s3\n" + LOAD)) == 1
+    assert len(scalar_wait_hazards("\tv_cmp_gt_u32_e64 s[10:11], v1, v2\n" + LOAD)) == 1
+    # back to a loop's head, and over two branches
+    loop = ".L1:\n" + LOAD + "\ts_nop 7\n" + write + "\ts_cbranch_scc0 .L1\n\ts_endpgm\n"
+    assert len(scalar_wait_hazards(loop)) == 1
+    assert len(scalar_wait_hazards(write + "\ts_branch .L2\n.L3:\n" + LOAD + "\ts_endpgm\n.L2:\n\ts_branch .L3\n")) == 1
+    assert scalar_wait_hazards(write + "\ts_endpgm\n.L2:\n" + LOAD) == []
+
+
+def test_asm_loads_into_lds_have_their_waits():
+    """In the sources: behind its write of M0 every asm load waits, and where the wait is too short for a base that a vector
+    instruction may write, the build checks the assembly."""
+    import re
+    from raftinfer_amd.build import ASM_CHECKED
+    sources = pathlib.Path(asm_check.__file__).resolve().parent / "csrc"
+    found = 0
+    for path in sorted(sources.iterdir()):
+        text = path.read_text()
+        for line in text.splitlines():
+            if "s_mov_b32 m0" in line:
+                found += 1
+                assert re.search(r"s_mov_b32 m0, %0\\n\\ts_nop (\d|%3)\\n\\tglobal_load_lds", line), (path.name, line)
+        if path.suffix == ".hip" and re.search(r"load_lds_b128<0>|load_lds_b128_at<|load_rows<", text):
+            assert path.name in ASM_CHECKED, path.name
+    assert found >= 5
+
+
+def test_built_kernels_wait_for_their_scalars():
+    from raftinfer_amd.asm_check import scalar_wait_hazards
+    from raftinfer_amd.build import ASM_CHECKED
+    folder = pathlib.Path(asm_check.__file__).resolve().parent / "_build"
+    for name in ASM_CHECKED:
+        s = folder / (name + ".s")
+        if not s.exists():
+            import pytest
+            pytest.skip("the library has not been built here")
+        assert scalar_wait_hazards(s.read_text()) == [], name
