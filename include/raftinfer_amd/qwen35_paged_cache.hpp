@@ -25,7 +25,7 @@
 //
 // What the host cannot check is checked on the device, before any access: a sequence
 // whose rows fall or end behind the call's, whose context is below its new tokens or
-// above max_context_tokens, or that needs a page number that is not below `pages`.  The
+// above max_context_tokens or the table's positions, or that needs a page number that is not below `pages`.  The
 // attention calls make such a sequence's rows NaN (a bad page: at least the rows that
 // see it; rows behind the call's are not written), the append stores none of it (a bad
 // page: none of the rows that belong there).  Each is counted at least once
@@ -86,7 +86,7 @@ struct Qwen35PagedShape {
   std::size_t pages;       // of the pool
   std::size_t page_tokens; // a multiple of 16
   std::size_t table_pages;
-  std::size_t max_context_tokens; // of this call's sequences, at most table_pages * page_tokens
+  std::size_t max_context_tokens; // of the call's sequences, at most 2^28; above table_pages * page_tokens: that many
   std::size_t window_tokens; // a token at position p sees j <= p with j > p - window_tokens; 0: all j <= p
 };
 

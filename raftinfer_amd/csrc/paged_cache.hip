@@ -5,6 +5,7 @@
 #include "rotary.hpp"
 #include "raftinfer_amd/qwen35_paged_cache.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace raftinfer::amd {
@@ -195,9 +196,8 @@ void validate_shape(const Qwen35PagedShape &s) {
   require<Err>(s.pages > 0 && s.pages <= kMaxPoolRows / 2 / s.kv_heads / s.page_tokens,
                "paged cache pages must be 1 to 2^31 rows of all KV heads");
   require<Err>(s.table_pages > 0 && s.table_pages <= kMaxPositions, "paged cache table_pages must be 1 to 2^28");
-  require<Err>(s.max_context_tokens > 0 && s.max_context_tokens <= kMaxPositions &&
-                   (s.max_context_tokens - 1) / s.page_tokens < s.table_pages,
-               "paged cache max_context_tokens must be 1 to 2^28 and within the page table");
+  require<Err>(s.max_context_tokens > 0 && s.max_context_tokens <= kMaxPositions,
+               "paged cache max_context_tokens must be 1 to 2^28");
 }
 
 std::size_t pool_bytes(const Qwen35PagedShape &s) { return s.pages * 2 * s.kv_heads * s.page_tokens * kRowBytes; }
@@ -217,8 +217,8 @@ PagedArgs to_args(const Qwen35PagedShape &s, Qwen35KvCacheLayout layout) {
   a.page_count = u32(s.pages);
   a.page_tokens = u32(s.page_tokens);
   a.table_pages = u32(s.table_pages);
-  a.max_ctx = u32(s.max_context_tokens);
-  a.window = s.window_tokens < s.max_context_tokens ? u32(s.window_tokens) : 0; // one that holds every position is none
+  a.max_ctx = u32(std::min(s.max_context_tokens, s.table_pages * s.page_tokens)); // (the table names no page for more)
+  a.window = s.window_tokens < a.max_ctx ? u32(s.window_tokens) : 0; // one that holds every position is none
   a.row_step = head_major ? 1 : a.kv_heads;
   a.head_step = head_major ? a.page_tokens : 1;
   a.plane_rows = a.kv_heads * a.page_tokens;

@@ -537,6 +537,14 @@ class Qwen35PagedRotary:
     epsilon: float = 1e-6
 
 
+def _paged(shape: Qwen35PagedShape, page_table) -> PagedShape:
+    """The call's shape.  Its max_context_tokens may be above the positions of a table that is a tensor; of
+    a bare address nothing but the shape tells the size."""
+    if not hasattr(page_table, "shape"):
+        _within_table(shape)
+    return shape.c()
+
+
 def _strides(t) -> tuple:
     """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else must be dense."""
     if t is None:
@@ -591,7 +599,15 @@ def qwen35_rotary(input, weight, output, positions, frequencies, shape: Qwen35Ro
         epsilon, dtype, dtype if weight is None else _dtype_code(weight), _stream_of(stream, input)))
 
 
+def _within_table(shape: Qwen35PagedShape) -> None:
+    """Where no page table is at hand whose size the call could go by, the shape's own numbers have to agree."""
+    positions = shape.table_pages * shape.page_tokens
+    if 0 < positions < shape.max_context_tokens:
+        raise Qwen35PrimitiveError(1, "paged cache max_context_tokens must be within the page table")
+
+
 def qwen35_paged_cache_bytes(shape: Qwen35PagedShape) -> int:
+    _within_table(shape)
     out = ctypes.c_size_t()
     _checked(_lib.load().raftinfer_amd_paged_cache_bytes(shape.c(), ctypes.byref(out)))
     return out.value
@@ -624,7 +640,7 @@ def qwen35_paged_cache_append(query, key, value, query_output, pages, page_table
     _checked(_lib.load().raftinfer_amd_paged_cache_append(
         _raw(query), _raw(key), _raw(value), _raw(query_output), _dense(pages),
         _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
-        _dense(context_lengths), _dense(frequencies), _dense(query_weight), _dense(key_weight), shape.c(),
+        _dense(context_lengths), _dense(frequencies), _dense(query_weight), _dense(key_weight), _paged(shape, page_table),
         PagedRotary(rotary.rotary_dim, rotary.interleaved, rotary.magnitude, rotary.epsilon,
                     *_strides(query), *_strides(key), *_strides(value), *_strides(query_output)),
         activation_dtype, weight_dtype, cache_layout, _stream_of(stream, key)))
@@ -639,7 +655,7 @@ def qwen35_paged_attention_prefill(query, gate, output, pages, page_table, query
         _raw(query), _raw(gate), _raw(output), _dense(pages),
         _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
         _dense(context_lengths), _dense(workspace),
-        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, _paged(shape, page_table),
         PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
         cache_layout, _stream_of(stream, query)))
 
@@ -653,7 +669,7 @@ def qwen35_paged_attention_decode(query, gate, output, pages, page_table, contex
         _raw(query), _raw(gate), _raw(output), _dense(pages),
         _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table),
         _dense(context_lengths), _dense(workspace),
-        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, shape.c(),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, _paged(shape, page_table),
         PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
         cache_layout, _stream_of(stream, query)))
 

@@ -245,3 +245,27 @@ def test_views_that_have_no_strides_to_pass():
     with refused("one type"):
         ops.qwen35_paged_cache_append(rest[0], rest[1], rest[2], rest[3], rest[4], rest[0], rest[1], rest[2], rest[3],
                                       torch.ones(256), torch.ones(256, dtype=torch.bfloat16), STEP, R(64), 1, stream=0x1234)
+
+
+def test_a_bound_above_the_table_is_the_tables():
+    """A program's largest context can be above what a call's page table holds: the sizes are those of the table's positions, and
+    calls refuse what comes behind the shape's checks."""
+    for shape, call in ((MODEL, "prefill"), (STEP, "decode")):
+        table_pages = 600  # 9600 positions
+        tight = dataclasses.replace(shape, pages=10000, table_pages=table_pages, max_context_tokens=table_pages * 16)
+        size = getattr(ops, f"qwen35_paged_{call}_workspace_bytes")
+        assert size(tight) > 0
+        for bound in (table_pages * 16 + 1, 262144, 2 ** 28):
+            for window in (0, 100, table_pages * 16 + 5):
+                loose = dataclasses.replace(tight, max_context_tokens=bound, window_tokens=window)
+                assert size(loose) == size(dataclasses.replace(tight, window_tokens=window))
+            a = spaced(7)
+            table = torch.zeros(3, table_pages, dtype=torch.int32)
+            starts = [a[4]] if call == "prefill" else []
+            with pytest.raises(ops.Qwen35PrimitiveError, match="workspace is too small"):
+                getattr(ops, f"qwen35_paged_attention_{call}")(*a[:4], table, *starts, a[5], a[6], dataclasses.replace(tight, max_context_tokens=bound), 1,
+                                                               stream=0x1234, workspace_bytes=0)
+    a = spaced(9)
+    with pytest.raises(ops.Qwen35PrimitiveError, match="overlap"):
+        ops.qwen35_paged_cache_append(a[0], a[1], a[2], a[0], a[4], torch.zeros(3, 20, dtype=torch.int32), *a[6:9], None, None,
+                                      dataclasses.replace(MODEL, max_context_tokens=6001), R(64), 1, stream=0x1234)

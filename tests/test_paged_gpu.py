@@ -770,3 +770,60 @@ def test_infinite_keys(gpu, kind):
     assert some
     # finite rows of the KV heads that the keys do not belong to, and of the others without the keys
     b.check()
+
+
+# ------------------------------------------------ bounds above the page table
+
+@pytest.mark.parametrize("kind,window", [("decode", 0), ("decode", 30), ("few", 0), ("few", 30), ("much", 0), ("much", 66)])
+def test_a_bound_above_the_table(gpu, kind, window):
+    """It gives the same bits as the table's positions for a bound; a sequence above them is NaN and counted."""
+    n = 1 if kind == "decode" else 20
+    each = [(n, 700), (n, 333), (n, 64), (n, 450)]
+    if kind == "much" and window:
+        each = [(700, 900), (33, 64), (300, 450)]  # (many rows take the kernel for much work, few keys or not)
+    b = Batch(each, window=window, decode=kind == "decode", seed=31)
+    if kind == "much":
+        roomy(b)
+    positions = b.shape.table_pages * b.page
+    b.shape = dataclasses.replace(b.shape, max_context_tokens=positions)
+    tight = b.call().clone()
+    for bound in (positions + 1, 1 << 28):
+        loose = dataclasses.replace(b.shape, max_context_tokens=bound)
+        size = ops.qwen35_paged_decode_workspace_bytes if b.decode else ops.qwen35_paged_prefill_workspace_bytes
+        assert size(loose) == size(b.shape)
+        b.out.fill_(7)
+        assert torch.equal(b.call(shape=loose), tight)
+    b.check()
+    bad = len(each) - 1
+    b.lengths[bad] = positions + 1
+    b.out.fill_(7)
+    errors()
+    b.call(shape=loose)
+    b.check(only=set(range(bad)))
+    assert errors() >= 1 and torch.isnan(b.out[int(b.starts_host[bad]):]).all()
+
+
+@pytest.mark.parametrize("rows", [3, 400])
+def test_append_with_a_bound_above_the_table(gpu, rows):
+    b = Batch([(rows, 500), (rows, 430), (rows, 420)], seed=32)
+    k, v = (torch.randn(b.rows, 4, 256, generator=b.g, device="cuda").to(BF) for _ in (0, 1))
+    positions = b.shape.table_pages * b.page
+    b.lengths[1] = positions + 1
+    before, got = b.pages.clone(), []
+    for bound in (positions, positions + 1, 1 << 28):
+        b.pages, out = before.clone(), torch.full_like(b.q, 7.0)
+        errors()
+        ops.qwen35_paged_cache_append(b.q, k, v, out, b.pages, b.table, b.starts, b.lengths, None, None, None,
+                                      dataclasses.replace(b.shape, max_context_tokens=bound), ops.Qwen35PagedRotary(0), ops.HEAD_MAJOR)
+        torch.cuda.synchronize()
+        assert errors() >= 1
+        got.append((b.pages.view(torch.int16), out))
+    for pages, out in got[1:]:
+        assert torch.equal(pages, got[0][0]) and torch.equal(out, got[0][1])
+    expect = before.clone()
+    for i in (0, 2):
+        for t in range(rows):
+            p, row = b.each[i][1] - rows + t, i * rows + t
+            page = int(b.table[i, p // 16])
+            expect[page, 0, :, p % 16], expect[page, 1, :, p % 16] = k[row], v[row]
+    assert torch.equal(got[0][0], expect.view(torch.int16)) and (got[0][1][rows:2 * rows] == 7).all()
