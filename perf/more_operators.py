@@ -300,9 +300,8 @@ def run(state):
         ops.qwen35_rotary(state["x"], state["weight"], state["out"], state["positions"], state["frequencies"], shape, EPS)
         return {"out": state["out"]}
     layout = ops.HEAD_MAJOR if c["head_major"] else ops.TOKEN_MAJOR
-    entries = state["table"].shape[1]
-    shape = ops.Qwen35PagedShape(state["rows"], c["sequences"], HQ, HKV, D, state["pages"].shape[0], c["page_tokens"], entries,
-                                 min(state["max_context"], entries * c["page_tokens"]), c.get("window", 0))
+    shape = ops.Qwen35PagedShape(state["rows"], c["sequences"], HQ, HKV, D, state["pages"].shape[0], c["page_tokens"], state["table"].shape[1],
+                                 state["max_context"], c.get("window", 0))
     if c["kind"] == "append":
         rotary = ops.Qwen35PagedRotary(c["rotary"], interleaved=c["interleaved"], magnitude=state["magnitude"], epsilon=EPS)
         ops.qwen35_paged_cache_append(state["projection"][:, :, 0], state["k"], state["v"], state["q"], state["pages"], state["table"], state["starts"],
