@@ -2360,10 +2360,11 @@ __global__ __launch_bounds__(1024) void decode_step_fused_kernel(
   // convolution.  Instruction i of a wave moves row r0 + i of both row groups
   // of the wave (lanes 0-31, 32-63).
   __shared__ float4 stage[16][kRows][64];
-  float *sh = state + h * kDim * kDim;
+  const int sw = __builtin_amdgcn_readfirstlane(tid >> 6); // (addresses by scalar arithmetic: 5.65 us a step against 5.80)
+  float *sh = state + (kh + (sw >> 3) * hk) * kDim * kDim;
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
-    load_lds_b128(sh, static_cast<std::uint32_t>(((r0 + i) * kDim + c0) * 4), lds_address(&stage[tid >> 6][i][0]));
+    load_lds_b128<0>(sh, static_cast<std::uint32_t>(((r0 + i) * kDim + c0) * 4), lds_address(&stage[sw][i][0]));
   float nw[4], z[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
