@@ -103,7 +103,12 @@ def _fptr(t):
 
 
 def _nbytes(t) -> int:
-    return 0 if t is None else t.numel() * t.element_size()
+    if t is None:
+        return 0
+    try:
+        return t.nbytes
+    except AttributeError:  # not a tensor
+        return t.numel() * t.element_size()
 
 
 def _stream(stream) -> ctypes.c_void_p:
@@ -402,13 +407,19 @@ def _raw(t):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = None  # of a device, by its index (0.1 us; a Stream object takes 1.8 us to make)
+
+
 def _stream_of(stream, tensor) -> int:
     """The stream's handle; None: the current stream of the tensor's device."""
     if stream is None:
+        global _raw_stream
+        if _raw_stream is None:
+            import torch
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        if tensor.is_cuda:
+            return _raw_stream(tensor.get_device())
         import torch
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (0.1 us; a Stream object takes 1.8 us to make)
-        if raw is not None and tensor.is_cuda:
-            return raw(tensor.get_device())
         return torch.cuda.current_stream(tensor.device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
 
@@ -509,6 +520,11 @@ class Qwen35RotaryShape:
     interleaved: bool = False
     magnitude: float = 1.0
 
+    # (all fields at once: set one by one, as a frozen dataclass does, a call's shape takes twice as long to make)
+    def __init__(self, rows, heads, head_dim, rotary_dim, interleaved=False, magnitude=1.0):
+        self.__dict__.update(rows=rows, heads=heads, head_dim=head_dim, rotary_dim=rotary_dim,
+                             interleaved=interleaved, magnitude=magnitude)
+
 
 @dataclass(frozen=True)
 class Qwen35PagedShape:
@@ -523,10 +539,14 @@ class Qwen35PagedShape:
     max_context_tokens: int
     window_tokens: int = 0
 
+    def __init__(self, rows, sequences, query_heads, kv_heads, head_dim, pages, page_tokens, table_pages,
+                 max_context_tokens, window_tokens=0):
+        self.__dict__.update(rows=rows, sequences=sequences, query_heads=query_heads, kv_heads=kv_heads,
+                             head_dim=head_dim, pages=pages, page_tokens=page_tokens, table_pages=table_pages,
+                             max_context_tokens=max_context_tokens, window_tokens=window_tokens)
+
     def c(self) -> PagedShape:
-        return PagedShape(self.rows, self.sequences, self.query_heads, self.kv_heads, self.head_dim,
-                          self.pages, self.page_tokens, self.table_pages, self.max_context_tokens,
-                          self.window_tokens)
+        return PagedShape(*self.__dict__.values())
 
 
 @dataclass(frozen=True)
@@ -536,19 +556,26 @@ class Qwen35PagedRotary:
     magnitude: float = 1.0
     epsilon: float = 1e-6
 
+    def __init__(self, rotary_dim, interleaved=False, magnitude=1.0, epsilon=1e-6):
+        self.__dict__.update(rotary_dim=rotary_dim, interleaved=interleaved, magnitude=magnitude, epsilon=epsilon)
 
-def _paged(shape: Qwen35PagedShape, page_table) -> PagedShape:
-    """The call's shape.  Its max_context_tokens may be above the positions of a table that is a tensor; of
-    a bare address nothing but the shape tells the size."""
-    if not hasattr(page_table, "shape"):
-        _within_table(shape)
-    return shape.c()
+
+_TYPES = None
+
+
+def _types():
+    """(types of indices, of frequencies, of pages, of activations by their code, of weights)."""
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = ((torch.int32, torch.uint32), (torch.float64,), (torch.bfloat16, torch.uint8, torch.int8),
+                  {DTYPE_F32: torch.float32, DTYPE_F16: torch.float16, DTYPE_BF16: torch.bfloat16},
+                  (torch.float32, torch.float16, torch.bfloat16))
+    return _TYPES
 
 
 def _strides(t) -> tuple:
     """(row, head) strides of a tensor [rows, heads, dim] whose dims are neighbours; anything else must be dense."""
-    if t is None:
-        return 0, 0
     try:
         row, head, dim = t.stride()
     except (AttributeError, ValueError):  # not three dimensions
@@ -575,6 +602,49 @@ def _dense(t):
     return t.data_ptr()
 
 
+def _heads(t, dtype) -> tuple:
+    """(address, row stride, head stride) of an activation; strides of 0: dense."""
+    if t is None:
+        return None, 0, 0
+    try:
+        if t.dtype is not dtype:
+            raise Qwen35PrimitiveError(1, f"activations must be of one type, {dtype}: got {t.dtype}")
+        row, head, one = t.stride()
+        if one == 1 and row > 0 and head > 0:
+            rows, heads, _ = t.shape
+            return t.data_ptr(), (row if rows > 1 else 0), (head if heads > 1 else 0)
+    except (AttributeError, ValueError):  # an address, with strides or without; not three dimensions
+        pass
+    return (t.data_ptr(), *_strides(t))
+
+
+def _listed(t, dtypes, what):
+    """The address of an argument of elements of one of the types that follow each other."""
+    if t is None:
+        return None
+    try:
+        if t.dtype in dtypes and t.is_contiguous():
+            return t.data_ptr()
+        if not t.is_contiguous():
+            raise Qwen35PrimitiveError(1, "indices, pages, weights and workspaces must be contiguous")
+        raise Qwen35PrimitiveError(1, f"{what} must be of type {' or '.join(map(str, dtypes))}: got {t.dtype}")
+    except AttributeError:  # not a tensor: it has an address only
+        pass
+    return t.data_ptr()
+
+
+def _table(t, dtypes, shape) -> tuple:
+    """(address of a page table [sequences, table_pages], the call's shape).  The shape's max_context_tokens may be
+    above the positions of a table that is a tensor; of a bare address nothing but the shape tells the size."""
+    try:
+        if t.dtype in dtypes and t.is_contiguous():
+            return t.data_ptr(), shape.c()
+        return _listed(t, dtypes, "page_table"), shape.c()
+    except AttributeError:  # a bare address, or none
+        _within_table(shape)
+        return (None if t is None else t.data_ptr()), shape.c()
+
+
 def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
                               factor: float = 1.0, trained_tokens: float = 0.0,
                               fast_turns: float = 32.0, slow_turns: float = 1.0) -> tuple:
@@ -591,12 +661,16 @@ def qwen35_rotary(input, weight, output, positions, frequencies, shape: Qwen35Ro
                   epsilon: float, stream=None) -> None:
     """RoPE(input / rms(input) * weight) of every head by the rows' positions (int32/uint32); weight
     None: no norm.  frequencies: float64 [rotary_dim / 2].  output may be input."""
+    index, wide, _, _, floats = _TYPES or _types()
+    rows, heads, dim, kind = shape.rows, shape.heads, shape.head_dim, input.dtype
     dtype = _dtype_code(input)
-    _checked(_lib.load().raftinfer_amd_rotary(
-        input.data_ptr(), _dense(weight), output.data_ptr(), _dense(positions), _dense(frequencies),
-        RotaryShape(shape.rows, shape.heads, shape.head_dim, shape.rotary_dim, shape.interleaved,
-                    shape.magnitude, *_strides(input), *_strides(output)),
-        epsilon, dtype, dtype if weight is None else _dtype_code(weight), _stream_of(stream, input)))
+    src, in_row, in_head = _heads(input, kind)
+    dst, out_row, out_head = _heads(output, kind)
+    _checked((_lib._lib or _lib.load()).raftinfer_amd_rotary(
+        src, _listed(weight, floats, "weight"), dst, _listed(positions, index, "positions"),
+        _listed(frequencies, wide, "frequencies"),
+        RotaryShape(rows, heads, dim, shape.rotary_dim, shape.interleaved, shape.magnitude, in_row, in_head, out_row, out_head),
+        epsilon, dtype, dtype if weight is None or weight.dtype is kind else _dtype_code(weight), _stream_of(stream, input)))
 
 
 def _within_table(shape: Qwen35PagedShape) -> None:
@@ -635,14 +709,26 @@ def qwen35_paged_cache_append(query, key, value, query_output, pages, page_table
     if weight_dtype is None:
         weight = query_weight if query_weight is not None else key_weight
         weight_dtype = DTYPE_BF16 if weight is None else _dtype_code(weight)
-        if key_weight is not None and _dtype_code(key_weight) != weight_dtype:
+        if key_weight is not None and key_weight is not weight and key_weight.dtype is not weight.dtype:
             raise Qwen35PrimitiveError(1, "query_weight and key_weight must be of one type")
-    _checked(_lib.load().raftinfer_amd_paged_cache_append(
-        _raw(query), _raw(key), _raw(value), _raw(query_output), _dense(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
-        _dense(context_lengths), _dense(frequencies), _dense(query_weight), _dense(key_weight), _paged(shape, page_table),
+    index, wide, raw, kinds, _ = _TYPES or _types()
+    act = kinds.get(activation_dtype)
+    weights = (kinds.get(weight_dtype),)
+    q, *q_strides = _heads(query, act)
+    k, *k_strides = _heads(key, act)
+    v, *v_strides = _heads(value, act)
+    out, *out_strides = _heads(query_output, act)
+    table, call = _table(page_table, index, shape)
+    _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_cache_append(
+        q, k, v, out, _listed(pages, raw, "pages"),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, table,
+        _listed(query_starts, index, "query_starts"),
+        _listed(context_lengths, index, "context_lengths"),
+        _listed(frequencies, wide, "frequencies"),
+        _listed(query_weight, weights, "query_weight"), _listed(key_weight, weights, "key_weight"),
+        call,
         PagedRotary(rotary.rotary_dim, rotary.interleaved, rotary.magnitude, rotary.epsilon,
-                    *_strides(query), *_strides(key), *_strides(value), *_strides(query_output)),
+                    *q_strides, *k_strides, *v_strides, *out_strides),
         activation_dtype, weight_dtype, cache_layout, _stream_of(stream, key)))
 
 
@@ -651,13 +737,19 @@ def qwen35_paged_attention_prefill(query, gate, output, pages, page_table, query
                                    cache_layout: int, activation_dtype: int = DTYPE_BF16, stream=None,
                                    pages_bytes=None, workspace_bytes=None) -> None:
     """Attention of every sequence's new tokens over its pages; gate None: no gate."""
-    _checked(_lib.load().raftinfer_amd_paged_attention_prefill(
-        _raw(query), _raw(gate), _raw(output), _dense(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table), _dense(query_starts),
-        _dense(context_lengths), _dense(workspace),
-        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, _paged(shape, page_table),
-        PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
-        cache_layout, _stream_of(stream, query)))
+    index, _, raw, kinds, _ = _TYPES or _types()
+    act = kinds.get(activation_dtype)
+    q, *q_strides = _heads(query, act)
+    g, *g_strides = _heads(gate, act)
+    out, *out_strides = _heads(output, act)
+    table, call = _table(page_table, index, shape)
+    _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_attention_prefill(
+        q, g, out, _listed(pages, raw, "pages"),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, table,
+        _listed(query_starts, index, "query_starts"),
+        _listed(context_lengths, index, "context_lengths"), _dense(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, call,
+        PagedStrides(*q_strides, *g_strides, *out_strides), activation_dtype, cache_layout, _stream_of(stream, query)))
 
 
 def qwen35_paged_attention_decode(query, gate, output, pages, page_table, context_lengths, workspace,
@@ -665,13 +757,18 @@ def qwen35_paged_attention_decode(query, gate, output, pages, page_table, contex
                                   activation_dtype: int = DTYPE_BF16, stream=None, pages_bytes=None,
                                   workspace_bytes=None) -> None:
     """The same for one new token of every sequence; a context length of 0: an unused row."""
-    _checked(_lib.load().raftinfer_amd_paged_attention_decode(
-        _raw(query), _raw(gate), _raw(output), _dense(pages),
-        _nbytes(pages) if pages_bytes is None else pages_bytes, _dense(page_table),
-        _dense(context_lengths), _dense(workspace),
-        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, _paged(shape, page_table),
-        PagedStrides(*_strides(query), *_strides(gate), *_strides(output)), activation_dtype,
-        cache_layout, _stream_of(stream, query)))
+    index, _, raw, kinds, _ = _TYPES or _types()
+    act = kinds.get(activation_dtype)
+    q, *q_strides = _heads(query, act)
+    g, *g_strides = _heads(gate, act)
+    out, *out_strides = _heads(output, act)
+    table, call = _table(page_table, index, shape)
+    _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_attention_decode(
+        q, g, out, _listed(pages, raw, "pages"),
+        _nbytes(pages) if pages_bytes is None else pages_bytes, table,
+        _listed(context_lengths, index, "context_lengths"), _dense(workspace),
+        _nbytes(workspace) if workspace_bytes is None else workspace_bytes, call,
+        PagedStrides(*q_strides, *g_strides, *out_strides), activation_dtype, cache_layout, _stream_of(stream, query)))
 
 
 def qwen35_gated_delta(input, conv_weight, recurrent_a, dt_bias, output_norm_weight, output,

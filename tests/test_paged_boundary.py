@@ -269,3 +269,79 @@ def test_a_bound_above_the_table_is_the_tables():
     with pytest.raises(ops.Qwen35PrimitiveError, match="overlap"):
         ops.qwen35_paged_cache_append(a[0], a[1], a[2], a[0], a[4], torch.zeros(3, 20, dtype=torch.int32), *a[6:9], None, None,
                                       dataclasses.replace(MODEL, max_context_tokens=6001), R(64), 1, stream=0x1234)
+
+
+def real(shape, decode=False):
+    """Arguments of an attention call that are tensors, on the host: a call that is not refused for them is for its null stream."""
+    bf, i32 = torch.bfloat16, torch.int32
+    x = {"query": torch.zeros(shape.rows, 16, 256, dtype=bf), "gate": torch.zeros(shape.rows, 16, 256, dtype=bf),
+         "output": torch.zeros(shape.rows, 16, 256, dtype=bf), "pages": torch.zeros(shape.pages, 2, 4, 16, 256, dtype=bf),
+         "page_table": torch.zeros(shape.sequences, shape.table_pages, dtype=i32), "query_starts": torch.zeros(shape.sequences + 1, dtype=i32),
+         "context_lengths": torch.zeros(shape.sequences, dtype=i32), "workspace": torch.zeros(1 << 20, dtype=torch.uint8)}
+    if decode:
+        del x["query_starts"]
+    return x
+
+
+def append_arguments(shape):
+    x = real(shape)
+    q = {k: x[k] for k in ("pages", "page_table", "query_starts", "context_lengths")}
+    key = torch.zeros(shape.rows, 4, 256, dtype=torch.bfloat16)
+    return {"query": x["query"], "key": key, "value": key.clone(), "query_output": x["output"], **q, "frequencies": torch.zeros(32, dtype=torch.float64),
+            "query_weight": torch.ones(256), "key_weight": torch.ones(256)}
+
+
+CALLS = {"prefill": lambda a, **kw: ops.qwen35_paged_attention_prefill(*a.values(), MODEL, 1, stream=0, **kw),
+         "decode": lambda a, **kw: ops.qwen35_paged_attention_decode(*a.values(), STEP, 1, stream=0, **kw),
+         "append": lambda a, **kw: ops.qwen35_paged_cache_append(*a.values(), MODEL, R(64), 1, stream=0, **kw),
+         "rotary": lambda a, **kw: ops.qwen35_rotary(*a.values(), Q(40, 16, 256, 64), 1e-6, stream=0, **kw)}
+
+
+def arguments(call):
+    if call == "append":
+        return append_arguments(MODEL)
+    if call == "rotary":
+        x = append_arguments(MODEL)
+        return {"input": x["query"], "weight": x["query_weight"], "output": x["query_output"], "positions": torch.zeros(40, dtype=torch.int32),
+                "frequencies": x["frequencies"]}
+    return real(MODEL if call == "prefill" else STEP, call == "decode")
+
+
+def right(call, change={}, **kw):
+    """The call with these arguments is refused for its stream alone."""
+    with pytest.raises(ops.Qwen35PrimitiveError, match="stream is null"):
+        CALLS[call]({**arguments(call), **change}, **kw)
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+def test_element_types(call):
+    """A tensor of another element type than the call reads is refused: its bytes would be taken for that type's."""
+    right(call)
+    a = arguments(call)
+    indices = [k for k in a if k in ("positions", "page_table", "query_starts", "context_lengths")]
+    for name in indices:
+        right(call, {name: a[name].view(torch.uint32)})
+        for other in (torch.int64, torch.float32, torch.int16):
+            with pytest.raises(ops.Qwen35PrimitiveError, match=f"{name} must be of type"):
+                CALLS[call]({**a, name: a[name].to(other)})
+    if "frequencies" in a:
+        with pytest.raises(ops.Qwen35PrimitiveError, match="frequencies must be of type"):
+            CALLS[call]({**a, "frequencies": a["frequencies"].float()})
+    for name in ("query", "key", "value", "query_output", "gate", "output"):
+        if name in a:
+            for other in (torch.float16, torch.float32, torch.int16):
+                with pytest.raises(ops.Qwen35PrimitiveError, match="activations must be of one type"):
+                    CALLS[call]({**a, name: a[name].to(other)})
+    if "pages" in a:
+        right(call, {"pages": a["pages"].view(torch.uint8)})
+        for other in (torch.float16, torch.float32):
+            with pytest.raises(ops.Qwen35PrimitiveError, match="pages must be of type"):
+                CALLS[call]({**a, "pages": a["pages"].to(other)})
+    if call == "append":
+        right(call, {"query_weight": torch.ones(256, dtype=torch.bfloat16), "key_weight": torch.ones(256, dtype=torch.bfloat16)})
+        with pytest.raises(ops.Qwen35PrimitiveError, match="query_weight must be of type"):
+            CALLS[call](a, weight_dtype=ops.DTYPE_BF16)
+    if call == "rotary":
+        right(call, {"weight": None})
+        with pytest.raises(ops.Qwen35PrimitiveError, match="weight must be of type"):
+            CALLS[call]({**a, "weight": torch.ones(256, dtype=torch.float64)})
