@@ -602,32 +602,47 @@ def _dense(t):
     return t.data_ptr()
 
 
-def _heads(t, dtype) -> tuple:
-    """(address, row stride, head stride) of an activation; strides of 0: dense."""
+def _heads(t, dtype, size) -> tuple:
+    """(address, row stride, head stride) of an activation of `size` [rows, heads, dim]; strides of 0: dense."""
     if t is None:
         return None, 0, 0
     try:
         if t.dtype is not dtype:
             raise Qwen35PrimitiveError(1, f"activations must be of one type, {dtype}: got {t.dtype}")
+        if t.shape != size:
+            return _other_heads(t, size)
         row, head, one = t.stride()
         if one == 1 and row > 0 and head > 0:
-            rows, heads, _ = t.shape
-            return t.data_ptr(), (row if rows > 1 else 0), (head if heads > 1 else 0)
+            return t.data_ptr(), (row if size[0] > 1 else 0), (head if size[1] > 1 else 0)
     except (AttributeError, ValueError):  # an address, with strides or without; not three dimensions
         pass
     return (t.data_ptr(), *_strides(t))
 
 
-def _listed(t, dtypes, what):
-    """The address of an argument of elements of one of the types that follow each other."""
+def _other_heads(t, size) -> tuple:
+    """The same of a tensor of another size: part of a larger one, or the same values without gaps in other dimensions."""
+    strides = _strides(t)
+    rows, heads, dim = size
+    shape = tuple(t.shape)
+    if len(shape) == 3 and shape[0] >= rows and shape[1] >= heads and shape[2] >= dim:
+        return (t.data_ptr(), *strides)
+    if not t.is_contiguous() or t.numel() < rows * heads * dim or shape == (heads, rows, dim):
+        raise Qwen35PrimitiveError(1, f"an activation must be [{rows}, {heads}, {dim}]: got {list(shape)}")
+    return t.data_ptr(), 0, 0
+
+
+def _listed(t, dtypes, least, what):
+    """The address of an argument of at least `least` elements of one of the types that follow each other."""
     if t is None:
         return None
     try:
-        if t.dtype in dtypes and t.is_contiguous():
+        if t.dtype in dtypes and t.numel() >= least and t.is_contiguous():
             return t.data_ptr()
         if not t.is_contiguous():
             raise Qwen35PrimitiveError(1, "indices, pages, weights and workspaces must be contiguous")
-        raise Qwen35PrimitiveError(1, f"{what} must be of type {' or '.join(map(str, dtypes))}: got {t.dtype}")
+        if t.dtype not in dtypes:
+            raise Qwen35PrimitiveError(1, f"{what} must be of type {' or '.join(map(str, dtypes))}: got {t.dtype}")
+        raise Qwen35PrimitiveError(1, f"{what} must have {least} elements: got {t.numel()}")
     except AttributeError:  # not a tensor: it has an address only
         pass
     return t.data_ptr()
@@ -637,9 +652,12 @@ def _table(t, dtypes, shape) -> tuple:
     """(address of a page table [sequences, table_pages], the call's shape).  The shape's max_context_tokens may be
     above the positions of a table that is a tensor; of a bare address nothing but the shape tells the size."""
     try:
-        if t.dtype in dtypes and t.is_contiguous():
+        if t.dtype in dtypes and t.shape == (shape.sequences, shape.table_pages) and t.is_contiguous():
             return t.data_ptr(), shape.c()
-        return _listed(t, dtypes, "page_table"), shape.c()
+        at = _listed(t, dtypes, shape.sequences * shape.table_pages, "page_table")
+        if shape.sequences > 1 and len(t.shape) == 2 and t.shape[1] != shape.table_pages:
+            raise Qwen35PrimitiveError(1, f"page_table must have rows of {shape.table_pages} entries: got {t.shape[1]}")
+        return at, shape.c()
     except AttributeError:  # a bare address, or none
         _within_table(shape)
         return (None if t is None else t.data_ptr()), shape.c()
@@ -664,11 +682,11 @@ def qwen35_rotary(input, weight, output, positions, frequencies, shape: Qwen35Ro
     index, wide, _, _, floats = _TYPES or _types()
     rows, heads, dim, kind = shape.rows, shape.heads, shape.head_dim, input.dtype
     dtype = _dtype_code(input)
-    src, in_row, in_head = _heads(input, kind)
-    dst, out_row, out_head = _heads(output, kind)
+    src, in_row, in_head = _heads(input, kind, (rows, heads, dim))
+    dst, out_row, out_head = _heads(output, kind, (rows, heads, dim))
     _checked((_lib._lib or _lib.load()).raftinfer_amd_rotary(
-        src, _listed(weight, floats, "weight"), dst, _listed(positions, index, "positions"),
-        _listed(frequencies, wide, "frequencies"),
+        src, _listed(weight, floats, dim, "weight"), dst, _listed(positions, index, rows, "positions"),
+        _listed(frequencies, wide, shape.rotary_dim // 2, "frequencies"),
         RotaryShape(rows, heads, dim, shape.rotary_dim, shape.interleaved, shape.magnitude, in_row, in_head, out_row, out_head),
         epsilon, dtype, dtype if weight is None or weight.dtype is kind else _dtype_code(weight), _stream_of(stream, input)))
 
@@ -712,23 +730,24 @@ def qwen35_paged_cache_append(query, key, value, query_output, pages, page_table
         if key_weight is not None and key_weight is not weight and key_weight.dtype is not weight.dtype:
             raise Qwen35PrimitiveError(1, "query_weight and key_weight must be of one type")
     index, wide, raw, kinds, _ = _TYPES or _types()
-    act = kinds.get(activation_dtype)
+    act, dim = kinds.get(activation_dtype), shape.head_dim
+    heads, kv_heads = (shape.rows, shape.query_heads, dim), (shape.rows, shape.kv_heads, dim)
     weights = (kinds.get(weight_dtype),)
-    q, *q_strides = _heads(query, act)
-    k, *k_strides = _heads(key, act)
-    v, *v_strides = _heads(value, act)
-    out, *out_strides = _heads(query_output, act)
+    q, q_row, q_head = _heads(query, act, heads)
+    k, k_row, k_head = _heads(key, act, kv_heads)
+    v, v_row, v_head = _heads(value, act, kv_heads)
+    out, out_row, out_head = _heads(query_output, act, heads)
     table, call = _table(page_table, index, shape)
     _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_cache_append(
-        q, k, v, out, _listed(pages, raw, "pages"),
+        q, k, v, out, _listed(pages, raw, 0, "pages"),
         _nbytes(pages) if pages_bytes is None else pages_bytes, table,
-        _listed(query_starts, index, "query_starts"),
-        _listed(context_lengths, index, "context_lengths"),
-        _listed(frequencies, wide, "frequencies"),
-        _listed(query_weight, weights, "query_weight"), _listed(key_weight, weights, "key_weight"),
+        _listed(query_starts, index, shape.sequences + 1, "query_starts"),
+        _listed(context_lengths, index, shape.sequences, "context_lengths"),
+        _listed(frequencies, wide, rotary.rotary_dim // 2, "frequencies"),
+        _listed(query_weight, weights, dim, "query_weight"), _listed(key_weight, weights, dim, "key_weight"),
         call,
         PagedRotary(rotary.rotary_dim, rotary.interleaved, rotary.magnitude, rotary.epsilon,
-                    *q_strides, *k_strides, *v_strides, *out_strides),
+                    q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head),
         activation_dtype, weight_dtype, cache_layout, _stream_of(stream, key)))
 
 
@@ -738,18 +757,18 @@ def qwen35_paged_attention_prefill(query, gate, output, pages, page_table, query
                                    pages_bytes=None, workspace_bytes=None) -> None:
     """Attention of every sequence's new tokens over its pages; gate None: no gate."""
     index, _, raw, kinds, _ = _TYPES or _types()
-    act = kinds.get(activation_dtype)
-    q, *q_strides = _heads(query, act)
-    g, *g_strides = _heads(gate, act)
-    out, *out_strides = _heads(output, act)
+    act, heads = kinds.get(activation_dtype), (shape.rows, shape.query_heads, shape.head_dim)
+    q, q_row, q_head = _heads(query, act, heads)
+    g, g_row, g_head = _heads(gate, act, heads)
+    out, out_row, out_head = _heads(output, act, heads)
     table, call = _table(page_table, index, shape)
     _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_attention_prefill(
-        q, g, out, _listed(pages, raw, "pages"),
+        q, g, out, _listed(pages, raw, 0, "pages"),
         _nbytes(pages) if pages_bytes is None else pages_bytes, table,
-        _listed(query_starts, index, "query_starts"),
-        _listed(context_lengths, index, "context_lengths"), _dense(workspace),
+        _listed(query_starts, index, shape.sequences + 1, "query_starts"),
+        _listed(context_lengths, index, shape.sequences, "context_lengths"), _dense(workspace),
         _nbytes(workspace) if workspace_bytes is None else workspace_bytes, call,
-        PagedStrides(*q_strides, *g_strides, *out_strides), activation_dtype, cache_layout, _stream_of(stream, query)))
+        PagedStrides(q_row, q_head, g_row, g_head, out_row, out_head), activation_dtype, cache_layout, _stream_of(stream, query)))
 
 
 def qwen35_paged_attention_decode(query, gate, output, pages, page_table, context_lengths, workspace,
@@ -758,17 +777,17 @@ def qwen35_paged_attention_decode(query, gate, output, pages, page_table, contex
                                   workspace_bytes=None) -> None:
     """The same for one new token of every sequence; a context length of 0: an unused row."""
     index, _, raw, kinds, _ = _TYPES or _types()
-    act = kinds.get(activation_dtype)
-    q, *q_strides = _heads(query, act)
-    g, *g_strides = _heads(gate, act)
-    out, *out_strides = _heads(output, act)
+    act, heads = kinds.get(activation_dtype), (shape.rows, shape.query_heads, shape.head_dim)
+    q, q_row, q_head = _heads(query, act, heads)
+    g, g_row, g_head = _heads(gate, act, heads)
+    out, out_row, out_head = _heads(output, act, heads)
     table, call = _table(page_table, index, shape)
     _checked((_lib._lib or _lib.load()).raftinfer_amd_paged_attention_decode(
-        q, g, out, _listed(pages, raw, "pages"),
+        q, g, out, _listed(pages, raw, 0, "pages"),
         _nbytes(pages) if pages_bytes is None else pages_bytes, table,
-        _listed(context_lengths, index, "context_lengths"), _dense(workspace),
+        _listed(context_lengths, index, shape.sequences, "context_lengths"), _dense(workspace),
         _nbytes(workspace) if workspace_bytes is None else workspace_bytes, call,
-        PagedStrides(*q_strides, *g_strides, *out_strides), activation_dtype, cache_layout, _stream_of(stream, query)))
+        PagedStrides(q_row, q_head, g_row, g_head, out_row, out_head), activation_dtype, cache_layout, _stream_of(stream, query)))
 
 
 def qwen35_gated_delta(input, conv_weight, recurrent_a, dt_bias, output_norm_weight, output,

@@ -345,3 +345,50 @@ def test_element_types(call):
         right(call, {"weight": None})
         with pytest.raises(ops.Qwen35PrimitiveError, match="weight must be of type"):
             CALLS[call]({**a, "weight": torch.ones(256, dtype=torch.float64)})
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+def test_tensors_too_small(call):
+    """A tensor of fewer elements than the shape says would be read, or written, past its end."""
+    a = arguments(call)
+    for name in [k for k in a if k in ("positions", "page_table", "query_starts", "context_lengths", "frequencies", "weight", "query_weight", "key_weight")]:
+        with pytest.raises(ops.Qwen35PrimitiveError, match=f"{name} must have"):
+            CALLS[call]({**a, name: a[name][:-1].contiguous()})
+    if call != "rotary":
+        more = {k: v for k, v in a.items()}
+        wider = torch.zeros(3, 21, dtype=torch.int32)
+        with pytest.raises(ops.Qwen35PrimitiveError, match="rows of 20 entries"):
+            CALLS[call]({**more, "page_table": wider})
+        right(call, {"page_table": torch.zeros(60, dtype=torch.int32)})
+        right(call, {"page_table": torch.zeros(5, 20, dtype=torch.int32), "context_lengths": torch.zeros(9, dtype=torch.int32)})
+    for name in ("input", "query", "key", "value", "query_output", "gate", "output"):
+        if name in a:
+            with pytest.raises(ops.Qwen35PrimitiveError, match="activation must be"):
+                CALLS[call]({**a, name: a[name][:-1]})
+            with pytest.raises(ops.Qwen35PrimitiveError, match="activation must be"):
+                CALLS[call]({**a, name: a[name][:, :-1]})
+            with pytest.raises(ops.Qwen35PrimitiveError, match="activation must be"):
+                CALLS[call]({**a, name: a[name][..., :-8]})
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+def test_activations_in_other_dimensions(call):
+    """Strides are those of rows and heads only where the dimensions are rows, heads and dim: a tensor [1, rows, heads * dim] had
+    its rows' stride taken for the heads', and was read past its end."""
+    a = arguments(call)
+    for name in ("input", "query", "key", "value", "query_output", "gate", "output"):
+        if name not in a:
+            continue
+        x = a[name]
+        rows, heads, dim = x.shape
+        for same in (x.view(1, rows, heads * dim), x.view(rows, 1, heads * dim), x.view(rows, heads * dim), x.view(rows * heads, dim),
+                     x.view(1, rows * heads, dim), x.view(rows, heads, 2, dim // 2), x.view(-1)):
+            assert ops._heads(same, x.dtype, (rows, heads, dim))[1:] in ((0, 0), (heads * dim, 0)), same.shape
+            right(call, {name: same})
+        # part of a larger tensor, given whole
+        more = torch.zeros(rows + 2, heads + 3, dim + 8, dtype=x.dtype)
+        assert ops._heads(more, x.dtype, (rows, heads, dim))[1:] == ((heads + 3) * (dim + 8), dim + 8)
+        right(call, {name: more})
+        for other in (x.transpose(0, 1).contiguous(), x.view(1, rows, heads * dim).expand(2, rows, heads * dim)):
+            with pytest.raises(ops.Qwen35PrimitiveError):
+                CALLS[call]({**a, name: other})
