@@ -48,6 +48,7 @@ namespace raftinfer::kernels {
 // factor).  by_turns: k = (t_p - slow_turns) / (fast_turns - slow_turns), held to 0 .. 1.
 // by_pair: k falls from 1 to 0 between the pair (rounded down) that turns fast_turns
 // times and the one (rounded up) that turns slow_turns times, held to 0 .. rotary_dim - 1.
+// (Models with by_pair have 32 and 1 for fast_turns and slow_turns, models with by_turns 4 and 1.)
 enum class Qwen35RotaryScaling : std::uint8_t { none = 0, linear = 1, by_pair = 2, by_turns = 3 };
 
 // Writes rotary_dim / 2 frequencies (host) for the calls below, which take them in

@@ -665,8 +665,11 @@ def _table(t, dtypes, shape) -> tuple:
 
 def qwen35_rotary_frequencies(rotary_dim: int, base: float, scaling: int = SCALING_NONE,
                               factor: float = 1.0, trained_tokens: float = 0.0,
-                              fast_turns: float = 32.0, slow_turns: float = 1.0) -> tuple:
-    """(the rotary_dim / 2 angles per position, their magnitude), on the host."""
+                              fast_turns: float | None = None, slow_turns: float = 1.0) -> tuple:
+    """(the rotary_dim / 2 angles per position, their magnitude), on the host.  fast_turns None: 32 by pair, 4 by
+    turns, as models with these scalings have them."""
+    if fast_turns is None:
+        fast_turns = 4.0 if scaling == SCALING_BY_TURNS else 32.0
     out = (ctypes.c_double * max(1, rotary_dim // 2))()
     magnitude = ctypes.c_float()
     _checked(_lib.load().raftinfer_amd_rotary_frequencies(

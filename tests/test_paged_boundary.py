@@ -392,3 +392,13 @@ def test_activations_in_other_dimensions(call):
         for other in (x.transpose(0, 1).contiguous(), x.view(1, rows, heads * dim).expand(2, rows, heads * dim)):
             with pytest.raises(ops.Qwen35PrimitiveError):
                 CALLS[call]({**a, name: other})
+
+
+def test_frequencies_left_at_their_defaults():
+    """By turns from 4 to 1 of them over the trained context, by pair from 32 to 1: what models with these scalings publish."""
+    for scaling, name, fast in ((ops.SCALING_BY_TURNS, "turns", 4.0), (ops.SCALING_BY_PAIR, "pair", 32.0)):
+        got, magnitude = ops.qwen35_rotary_frequencies(128, 5e5, scaling, 8.0, 8192.0)
+        want, m = ref.frequencies(128, 5e5, name, 8.0, 8192.0, fast, 1.0)
+        assert np.allclose(got, want, rtol=1e-13, atol=0) and abs(magnitude - m) <= 2.0 ** -24 * m
+        other, _ = ref.frequencies(128, 5e5, name, 8.0, 8192.0, 36.0 - fast, 1.0)
+        assert not np.allclose(got, other, rtol=1e-3, atol=0)
