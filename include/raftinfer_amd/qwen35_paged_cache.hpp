@@ -73,6 +73,8 @@ struct Qwen35RotaryShape {
 // output = RoPE(input / rms(input) * weight) of every head, by the rows' positions
 // (device uint32 [rows]); weight null: RoPE(input).  frequencies: device double
 // [rotary_dim / 2].  An angle is position * frequency in 64 bits, reduced to one turn.
+// The mean of a head's squares is held in 32 bits: right for sums of squares below 2^128, and
+// with epsilon 0 for a mean of at least 2^-126 (smaller ones lose bits, below 2^-149 it is 0).
 // output may be input, with the same strides.
 void qwen35_rotary(const void *input, const void *weight, void *output, const std::uint32_t *positions,
                    const double *frequencies, Qwen35RotaryShape shape, float epsilon,

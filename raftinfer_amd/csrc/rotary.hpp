@@ -70,6 +70,13 @@ template <int LANES> __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
+// 1 / sqrt(x), off by one step of 32 bits.  (The instruction takes values below 2^-126 for 0: a small
+// mean square, where epsilon does not hold it up, is scaled by 2^96 first.)
+__device__ __forceinline__ float inverse_root(float x) {
+  const bool small = x < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(small ? x * 0x1p96f : x) * (small ? 0x1p48f : 1.0f);
+}
+
 // A head lies in LANES neighbouring lanes, N values in each, in order; lane c has values
 // N c .. (0 behind head_dim).  rot: cos of the pairs, then sin.  Halves: pairs a multiple of
 // N, the partner values are pairs / N lanes away.  Every lane of the wave must call it.
@@ -80,7 +87,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[N], const float (&w)[N], 
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], ss);
-    const float scale = __builtin_amdgcn_rsqf(fmaf(lanes_sum<LANES>(ss), 1.0f / head_dim, epsilon)); // (off by one step of 32 bits)
+    const float scale = inverse_root(fmaf(lanes_sum<LANES>(ss), 1.0f / head_dim, epsilon));
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = x[e] * scale * w[e];
   }

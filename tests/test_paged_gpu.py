@@ -827,3 +827,34 @@ def test_append_with_a_bound_above_the_table(gpu, rows):
             page = int(b.table[i, p // 16])
             expect[page, 0, :, p % 16], expect[page, 1, :, p % 16] = k[row], v[row]
     assert torch.equal(got[0][0], expect.view(torch.int16)) and (got[0][1][rows:2 * rows] == 7).all()
+
+
+# --------------------------------------------------------- norms of small heads
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 256), (torch.float32, 128), (torch.float32, 33)])
+@pytest.mark.parametrize("size", [2.0 ** -66, 2.0 ** -64, 2.0 ** -48])
+def test_norm_of_small_values(gpu, dtype, dim, size):
+    """Without an epsilon a head's size goes out of its norm, also where the mean of the squares is below the smallest normal number."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = (torch.randn(7, 3, dim, generator=g, device="cuda").clamp(-2, 2) * size).to(dtype)
+    w = (1 + 0.1 * torch.randn(dim, generator=g, device="cuda")).to(dtype)
+    out, positions = torch.empty_like(x), torch.arange(7, dtype=torch.int32, device="cuda")
+    freq, _ = ops.qwen35_rotary_frequencies(32, 1e4)
+    ops.qwen35_rotary(x, w, out, positions, torch.tensor(freq, dtype=torch.float64, device="cuda"), ops.Qwen35RotaryShape(7, 3, dim, 32), 0.0)
+    torch.cuda.synchronize()
+    want = ref.rotate(wide(x), wide(w), np.arange(7), freq, 1.0, False, 0.0)
+    # 32 bits: `dim` squares, each off by 2^-150 or half a step, and their mean (a mean of at least 2^-134 is off by 2^-16 of itself,
+    # its root by half of that); two dozen roundings of values up to 1.5 times the pair's; the result is rounded once
+    mean = (wide(x) ** 2).mean(-1, keepdims=True)
+    off = (2 * 2.0 ** -150 / mean) / 2 + 2.0 ** -24 * (dim / 2 + 24)
+    assert (np.abs(wide(out) - want) <= torch.finfo(dtype).eps / 2 * np.abs(want) + 2 * off * np.abs(want).max()).all()
+    if dim == 256:
+        b = Batch([(7, 20)], 3, 1, seed=1)
+        q, one = torch.empty_like(x), torch.ones(256, device="cuda")
+        ops.qwen35_paged_cache_append(x, x, x, q, b.pages, b.table, b.starts, b.lengths, None, one, one, b.shape, ops.Qwen35PagedRotary(0, epsilon=0.0),
+                                      ops.HEAD_MAJOR)
+        torch.cuda.synchronize()
+        y = wide(x) / np.sqrt(mean)
+        assert (np.abs(wide(q) - y) <= ref.HALF_BF16 * np.abs(y) + 2 * off * np.abs(y).max()).all()
+        at = torch.stack([b.pages[int(b.table[0, p // 16]), 0, :, p % 16] for p in range(13, 20)])
+        assert torch.equal(at, q)
