@@ -134,6 +134,9 @@ void qwen35_paged_cache_append(const void *query, const void *key, const void *v
 // summed in f32 with probabilities of at most 1: finite where |probability * value|
 // over a token's keys sums to less than 2^128.  (The sums are held scaled down by up to
 // 2^16, so products below 2^-110 lose bits.)
+// Probabilities enter the product with the values in bf16, 8 bits, and are divided by the
+// sum of what they were rounded to: besides its own rounding an output is off by up to
+// 2^-8 of the probabilities' mean of |value - output|.
 void qwen35_paged_attention_prefill(const void *query, const void *gate, void *output, const void *pages,
                                     std::size_t pages_bytes, const std::int32_t *page_table,
                                     const std::uint32_t *query_starts, const std::uint32_t *context_lengths,
@@ -143,6 +146,8 @@ void qwen35_paged_attention_prefill(const void *query, const void *gate, void *o
 
 // The same with one new token of each sequence: row s belongs to sequence s, rows equals
 // sequences.  A context length of 0 marks an unused row, which is left as it was.
+// Probabilities are held in two bf16 parts, off by 2^-15 + 2^-17 of themselves at most, so
+// that a token's output can differ from the other call's by that call's rounding of them.
 void qwen35_paged_attention_decode(const void *query, const void *gate, void *output, const void *pages,
                                    std::size_t pages_bytes, const std::int32_t *page_table,
                                    const std::uint32_t *context_lengths, void *workspace,

@@ -184,8 +184,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   floatx16 s0[2], s1[2];
   std::uint32_t pk[2][8]; // P^T, bf16 pairs in accumulator order
   float mx[2];            // max of the next S over this lane's keys
-  // Pair u of the probabilities (blocks in turn): registers 2i, 2i + 1 of an S.  The sum takes the
-  // same bf16 probabilities as the product with V.  The empty asm keeps the pair where it is
+  // Pair u of the probabilities (blocks in turn): registers 2i, 2i + 1 of an S.  Rounded to bf16, as the
+  // product with V takes them (in two parts it would be twice as long, half of a step's matrix time more); the
+  // sum takes the same rounded probabilities, so that a row of equal values is theirs.  The empty asm keeps the pair where it is
   // written, among the MFMAs.
   const auto soft_pair = [&](const floatx16(&s)[2], auto uc) __attribute__((always_inline)) {
     constexpr int bq = uc % 2, i = uc / 2;

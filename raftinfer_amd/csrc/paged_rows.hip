@@ -59,8 +59,8 @@ template <int kOffset, bool Once> __device__ __forceinline__ void load_rows(cons
 // range's steps w, w + WAVES, ..  S = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16, operands
 // out of LDS, where LDS-direct loads put the rows as they lie in the pages: whole granules, whose rows
 // behind the last key are masked, and cleaned, like other keys that a column does not see.  A product
-// with V has 32 places: of 16 keys (G = 1) the probabilities in two bf16 parts, 16 bits together, of
-// 32 keys one part.  What bounds it: long caches the memory (32 sequences of up to 32768 tokens 6.05 TB/s, one of 60001 6.3 in
+// with V has 32 places: of 16 keys (G = 1) the probabilities in two bf16 parts, which cost nothing there (off by
+// 2^-15 + 2^-17 of themselves at most), of 32 keys one part, 8 bits: two would double those products.  What bounds it: long caches the memory (32 sequences of up to 32768 tokens 6.05 TB/s, one of 60001 6.3 in
 // the kernel; non-temporal loads where more than 16 MiB are read once: 6.05 against 5.3 TB/s plain, but warm small caches
 // are slower with them), short calls the round trips: of 15 us for 16 tokens of 217, 1.4 to find the work, 2 for the table
 // and the first keys, 2.5 for the queries, 4 for two steps, 4 to join the waves.

@@ -858,3 +858,67 @@ def test_norm_of_small_values(gpu, dtype, dim, size):
         assert (np.abs(wide(q) - y) <= ref.HALF_BF16 * np.abs(y) + 2 * off * np.abs(y).max()).all()
         at = torch.stack([b.pages[int(b.table[0, p // 16]), 0, :, p % 16] for p in range(13, 20)])
         assert torch.equal(at, q)
+
+
+# ------------------------------------------------------ bits of the probabilities
+
+def cancelling(each, decode, much=False):
+    """Values of neighbouring keys cancel as the probabilities weigh them, so that an output shows their roundings and not its own; scores
+    are small.  One query head per KV head."""
+    b = Batch(each, 4, 1, decode=decode, gate=False, seed=41)
+    if much:
+        roomy(b)
+    b.q = (b.q.float() / 8).to(BF)
+    for i, (n, c) in enumerate(each):
+        where = [(int(b.table[i, j // 16]), j % 16) for j in range(c)]
+        k = torch.stack([b.pages[p, 0, :, at] for p, at in where]).double()              # [c, heads, 256]
+        last = b.q[int(b.starts_host[i]) + n - 1].double()                               # the last token cancels
+        w = torch.softmax(torch.einsum("jhd,hd->hj", k.cpu(), last.cpu()) / 16, -1)
+        v = torch.randn(c, 4, 256, generator=b.g, device="cuda").cpu().double()
+        for j in range(0, c - 1, 2):
+            v[j] = v[j].to(BF).double()
+            v[j + 1] = -v[j] * (w[:, j] / w[:, j + 1])[:, None]
+        if c % 2:
+            v[c - 1] = 0
+        for j, (p, at) in enumerate(where):
+            b.pages[p, 1, :, at] = v[j].to(BF).cuda()
+    return b
+
+
+def last_tokens(b):
+    """Of every sequence: its last row's output, the exact one, one of probabilities in 8 bits, the sum of |probability * value|, and how far
+    scores in 32 bits move a probability, relative to it."""
+    for i, (n, c) in enumerate(b.each):
+        row = int(b.starts_host[i]) + n - 1
+        kv = ref.rows_of(wide(b.pages), b.table[i].cpu().numpy(), c, b.page, True)
+        q = wide(b.q[row])
+        for h in range(4):
+            k, v = kv[0, h], kv[1, h]
+            e = np.exp(k @ q[h] / 16 - (k @ q[h] / 16).max())
+            cut = torch.tensor(e).to(BF).double().numpy()
+            off = 2 * 256 * 2.0 ** -24 * (np.abs(k) @ np.abs(q[h])).max() / 16
+            yield wide(b.out[row, h]), e / e.sum() @ v, cut / cut.sum() @ v, e / e.sum() @ np.abs(v), off
+
+
+def test_decode_holds_probabilities_in_two_parts(gpu):
+    """The first part is at most 2^-9 and a truncation (2^-7) below the probability, the rest is rounded (2^-8): off by 2^-15 + 2^-17."""
+    b = cancelling([(1, 2), (1, 8), (1, 33), (1, 64)], True)
+    b.call()
+    torch.cuda.synchronize()
+    shown = []
+    for got, want, cut, size, off in last_tokens(b):
+        # (sums of up to 64 products in 32 bits, exponentials, the division: 100 roundings at most)
+        tol = ref.HALF_BF16 * np.abs(want) + (2.0 ** -15 + 2.0 ** -17 + off + 100 * 2.0 ** -24) * size
+        assert (np.abs(got - want) <= tol).all()
+        shown.append((np.abs(cut - want) > tol).mean())
+    assert np.median(shown) > 0.3  # probabilities in 8 bits would not pass
+
+
+@pytest.mark.parametrize("much", [False, True])
+def test_chunks_hold_probabilities_in_8_bits(gpu, much):
+    """Each is off by 2^-8 of itself at most, and they are divided by the sum of what they were rounded to."""
+    b = cancelling([(5, 8), (3, 33), (40, 64)], False, much)
+    b.call()
+    torch.cuda.synchronize()
+    for got, want, _, size, off in last_tokens(b):
+        assert (np.abs(got - want) <= ref.HALF_BF16 * np.abs(want) + (2.0 ** -8 * 1.01 + off + 100 * 2.0 ** -24) * (size + np.abs(want))).all()
