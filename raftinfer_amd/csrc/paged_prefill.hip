@@ -35,11 +35,6 @@ constexpr unsigned kPart = kSlot / kShare;  // a wave's share of a slot: one gra
 
 constexpr float kSlack = 16.0f; // log2 units
 
-// Of a workgroup's tile at j0 some column (tokens at p_lo .. p_hi) does not see some key.
-__device__ __forceinline__ bool stream_masked(const PagedArgs &a, std::uint32_t j0, std::uint32_t p_lo, std::uint32_t p_hi) {
-  return j0 + kKTile - 1 > p_lo || (a.window != 0 && p_hi - j0 >= a.window);
-}
-
 template <bool HeadMajor>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_stream_kernel(
     PagedArgs a, PagedScratch sc, PagedSplit sp) {
