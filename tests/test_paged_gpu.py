@@ -922,3 +922,124 @@ def test_chunks_hold_probabilities_in_8_bits(gpu, much):
     torch.cuda.synchronize()
     for got, want, _, size, off in last_tokens(b):
         assert (np.abs(got - want) <= ref.HALF_BF16 * np.abs(want) + (2.0 ** -8 * 1.01 + off + 100 * 2.0 ** -24) * (size + np.abs(want))).all()
+
+
+# -------------------------------- ranges longer than the page entries that a wave holds
+
+def check_on_device(b, i):
+    """Batch.check for one sequence with 64-bit sums on the GPU: pools that are too large for the host's reference."""
+    n, c = b.each[i]
+    a, j = int(b.starts_host[i]), torch.arange(c, device="cuda")
+    page, at = b.table[i].long()[j // b.page], j % b.page
+    token = c - n + torch.arange(n, device="cuda")
+    hidden = j > token[:, None]
+    if b.window:
+        hidden |= j <= token[:, None] - b.window
+    for h in range(b.kv_heads):
+        k, v = ((b.pages[page, x, h, at] if b.head_major else b.pages[page, x, at, h]).double().masked_fill(hidden.all(0)[:, None], 0)
+                for x in (0, 1))
+        for g in range(h * b.group, (h + 1) * b.group):
+            q = b.q[a:a + n, g].double()
+            p = torch.softmax((q @ k.T / 16).masked_fill(hidden, -torch.inf), -1)
+            want = p @ v
+            seen, size = ~hidden.all(0), torch.where(hidden.all(0)[:, None], 0, v.abs())
+            spread = p @ size + want.abs()                                      # (at least the mean of |value - output|)
+            off = 256 * 2.0 ** -24 * (q.abs() @ k[seen].abs().T).max() / 16
+            gate = 1 if b.gate is None else torch.sigmoid(b.gate[a:a + n, g].double())
+            tol = ref.HALF_BF16 * (want * gate).abs() + gate * (2.0 ** -8 * 1.01 * spread * (not b.decode) + (2.0 ** -14 + 2 * off) * (p @ size))
+            assert ((b.out[a:a + n, g].double() - want * gate).abs() <= tol).all(), (h, g)
+
+
+@pytest.mark.parametrize("kind,n,c,kv_heads,page,head_major,window", [
+    # a workgroup of the single-token kernel holds the entries of 256 tiles of 16 keys, of short chunks 128 of 32
+    ("decode", 1, 20000, 64, 16, True, 0), ("decode", 1, 10007, 128, 48, False, 0), ("decode", 1, 12001, 128, 32, True, 9000),
+    ("few", 2, 20000, 64, 48, True, 0), ("few", 3, 9999, 128, 16, False, 0),
+    # of long chunks about 120 of 32: met where every column sees all of a tile, and in the last, masked, tiles
+    ("much", 40, 6001, 260, 48, False, 0), ("much", 128, 3968, 260, 16, True, 0), ("much", 120, 3950, 260, 64, False, 0),
+    ("much", 60, 6500, 260, 16, True, 4500)])
+def test_long_ranges(gpu, kind, n, c, kv_heads, page, head_major, window):
+    b = Batch([(n, c)], kv_heads, 1, page, head_major, window, seed=c, decode=kind == "decode", gate=kind != "few")
+    columns, keys = n * kv_heads, min(c, window or c)
+    assert (columns * keys > 40 * 256 * 32 * 32) == (kind == "much") or kind == "decode"
+    errors()
+    b.call()
+    torch.cuda.synchronize()
+    assert errors() == 0
+    b.table[0, :max(0, c - n + 1 - window) // page if window else 0] = 0
+    check_on_device(b, 0)
+    # every entry counts: with any of some neighbours of the refill gone, the sequence is NaN
+    table = b.table.clone()
+    lo = (c - n + 1 - window) // page + 1 if window else 0
+    for entry in sorted({lo, (lo + c // page) // 2, min(c // page - 1, lo + 4096 // page), (c - 1) // page}):
+        b.table = table.clone()
+        b.table[0, entry] = b.shape.pages
+        b.call()
+        torch.cuda.synchronize()
+        assert errors() >= 1 and torch.isnan(b.out).all(-1).any(), entry
+        assert torch.isnan(b.out[-1]).all(), entry  # (the last token sees every one of them)
+
+
+def test_a_sequence_alone_and_among_others(gpu):
+    """In each kernel a sequence's rows meet the reference alone and in a batch; the last token also as a single one; twice the same bits."""
+    n, c = 9, 700
+    others = [(3, 40), (n, c), (70, 300), (1, 900)]
+    alone, among = Batch([(n, c)], seed=51), Batch(others, seed=52)
+    where = [(int(alone.table[0, j]), int(among.table[1, j])) for j in range(-(-c // 16))]
+    for one, other in where:
+        among.pages[other] = alone.pages[one]
+    at = int(among.starts_host[1])
+    among.q[at:at + n], among.gate[at:at + n] = alone.q, alone.gate
+    rows, want, tol = alone.want(0)
+    for kind in ("few", "much"):
+        if kind == "much":
+            roomy(alone)
+            roomy(among)
+        first = [alone.call().clone(), among.call().clone()]
+        for got in (first[0], first[1][at:at + n]):
+            assert (np.abs(wide(got) - want) <= tol).all()
+        assert torch.equal(alone.call(), first[0]) and torch.equal(among.call(), first[1])
+    single = P(1, 1, 16, 4, 256, alone.shape.pages, 16, alone.shape.table_pages, c)
+    out = torch.empty(1, 16, 256, device="cuda", dtype=BF)
+    ws = torch.empty(max(16, ops.qwen35_paged_decode_workspace_bytes(single)), device="cuda", dtype=torch.uint8)
+    ops.qwen35_paged_attention_decode(alone.q[n - 1:], alone.gate[n - 1:], out, alone.pages, alone.table, alone.lengths, ws, single, ops.HEAD_MAJOR)
+    torch.cuda.synchronize()
+    assert (np.abs(wide(out) - want[n - 1:]) <= tol[n - 1:]).all()
+
+
+def test_append_to_its_last_bit(gpu):
+    """Keys and queries of append are off by their rounding and a few dozen steps of 32 bits."""
+    b = Batch([(33, 50), (1, 300)], seed=61)
+    k = torch.randn(b.rows, 4, 256, generator=b.g, device="cuda").to(BF)
+    w = 1 + 0.1 * torch.randn(256, generator=b.g, device="cuda")
+    freq, m = ops.qwen35_rotary_frequencies(64, 1e7)
+    out = torch.empty_like(b.q)
+    ops.qwen35_paged_cache_append(b.q, k, k, out, b.pages, b.table, b.starts, b.lengths, torch.tensor(freq, dtype=torch.float64, device="cuda"), w, w,
+                                  b.shape, ops.Qwen35PagedRotary(64, False, m, 1e-6), ops.HEAD_MAJOR)
+    torch.cuda.synchronize()
+    at = np.concatenate([np.arange(c - n, c) for n, c in b.each])
+    stored = torch.stack([b.pages[int(b.table[i, p // 16]), 0, :, p % 16] for i, (n, c) in enumerate(b.each) for p in range(c - n, c)])
+    for got, x in ((out, b.q), (stored, k)):
+        want = ref.rotate(wide(x), wide(w), at, freq, m, False, 1e-6)
+        # a pair's sizes bound its two results: the norm's sum of 256 squares and its root, the angle (reduced, up to pi: half a step is
+        # pi 2^-24), sine and cosine (2 steps), products and sum
+        pair = np.abs(ref.rotate(np.abs(wide(x)), np.abs(wide(w)), np.zeros(len(at), int), freq, 1.0, False, 1e-6))
+        pair[..., :32] = pair[..., 32:64] = pair[..., :32] + pair[..., 32:64]
+        assert (np.abs(wide(got) - want) <= ref.HALF_BF16 * np.abs(want) + pair * 2.0 ** -24 * (128 + 16)).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 16384), (torch.float32, 16384), (torch.float16, 16382)])
+def test_rotary_of_the_largest_heads(gpu, dtype, dim):
+    """The angles of a row fill 64 KiB of LDS."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn(2, 3, dim, generator=g, device="cuda").to(dtype)
+    out, positions = torch.empty_like(x), torch.tensor([5, 100000], dtype=torch.int32, device="cuda")
+    freq, _ = ops.qwen35_rotary_frequencies(dim, 1e7)
+    ops.qwen35_rotary(x, None, out, positions, torch.tensor(freq, dtype=torch.float64, device="cuda"), ops.Qwen35RotaryShape(2, 3, dim, dim), 0.0)
+    torch.cuda.synchronize()
+    y, half = wide(x), dim // 2
+    turn = np.array([[np.longdouble(p) * np.longdouble(f) % (2 * np.longdouble(np.pi)) for f in freq] for p in (5, 100000)]).astype(np.float64)[:, None]
+    a, c = y[..., :half], y[..., half:]
+    want = np.concatenate([a * np.cos(turn) - c * np.sin(turn), a * np.sin(turn) + c * np.cos(turn)], -1)
+    size = np.tile(np.abs(a) + np.abs(c), 2)
+    tol = torch.finfo(dtype).eps / 2 * np.abs(want) + size * 2.0 ** -24 * 12 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    assert (np.abs(wide(out) - want) <= tol).all()
