@@ -70,9 +70,11 @@ template <int LANES> __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
-// 1 / sqrt(x), off by one step of 32 bits.  (The instruction takes values below 2^-126 for 0: a small
-// mean square, where epsilon does not hold it up, is scaled by 2^96 first.)
-__device__ __forceinline__ float inverse_root(float x) {
+// 1 / sqrt(sum * share + epsilon), off by one step of 32 bits.  (The instruction takes values below 2^-126 for 0: a
+// small mean that no epsilon holds up is scaled by 2^96 first.)
+__device__ __forceinline__ float inverse_rms(float sum, float share, float epsilon) {
+  const float x = fmaf(sum, share, epsilon);
+  if (epsilon >= 0x1p-96f) return __builtin_amdgcn_rsqf(x); // (uniform)
   const bool small = x < 0x1p-96f;
   return __builtin_amdgcn_rsqf(small ? x * 0x1p96f : x) * (small ? 0x1p48f : 1.0f);
 }
@@ -87,7 +89,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[N], const float (&w)[N], 
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], ss);
-    const float scale = inverse_root(fmaf(lanes_sum<LANES>(ss), 1.0f / head_dim, epsilon));
+    const float scale = inverse_rms(lanes_sum<LANES>(ss), 1.0f / head_dim, epsilon);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = x[e] * scale * w[e];
   }
