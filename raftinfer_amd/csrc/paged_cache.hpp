@@ -281,8 +281,8 @@ __device__ __forceinline__ void paged_sort(PagedSeq &q, std::uint32_t &id, std::
 // time.  `first`: the caller is the one wave that counts bad sequences, in `count`, and writes the
 // plan for the kernel that joins the ranges.  With kRounds the items of up to 64 sequences are
 // the longest first and their ranges' length is chosen (16 query and 4 KV heads, against an even
-// share in the batch's order, us: 300 tokens of 30000 284 -> 190, 200 of 60000 359 -> 243, 16 sequences of
-// up to 8192 behind a window of 4096, ten of them single tokens, 222 -> 176; it takes a workgroup 1.6 to 6 us, of 1 to 64
+// share in the batch's order, in a graph, us: 300 tokens of 30000 291 -> 189, 200 of 60000 374 -> 255, 16 sequences of
+// up to 8192 behind a window of 4096, ten of them single tokens, 260 -> 185; it takes a workgroup 1.6 to 6 us, of 1 to 64
 // sequences).
 template <int kCols, int kUnit, bool kRounds = false>
 __device__ __forceinline__ bool paged_find(const PagedArgs &a, const PagedSplit &sp, const PagedScratch &sc, std::uint32_t index, bool first,

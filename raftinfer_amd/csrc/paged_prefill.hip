@@ -16,16 +16,19 @@ __device__ unsigned int g_stream_capacity_errors = 0;
 // S^T = K q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, the probabilities of a tile formed among the matrix instructions of
 // the step before their product.  64 columns of a wave are what lets an operand read from LDS (16 clocks of the unit's 32 for
 // each product of 32 columns) feed two products; their 256 accumulators fill the accumulation registers, one wave a SIMD.
-// Measured (16 query and 4 KV heads): 2048 tokens of 32768 1150 TFLOP/s (a product of 8192^3 in the BLAS library 1300), 500 of
-// 30501 940, 8001 926.  A step of 64 keys takes 3850 clocks for 2048 of matrix time: exponentials and packing among
-// them, LDS reads, one barrier; the matrix units are busy for 49% of a long chunk at 2.0 GHz.  Start and end of a workgroup take
-// 35,000 to 40,000 clocks: 4,000 to find its work, 12,000 until the first tiles and queries are there, 20,000 to join the
-// key groups, for gates and stores.
+// Measured (16 query and 4 KV heads): 2048 tokens of 32768 1094 to 1150 TFLOP/s (a product of 8192^3 in the BLAS library 1300),
+// 500 of 30501 910 to 960, 8001 910 to 940.  By the counters the matrix units are busy for 56%, 48% and 42% of the waves' time in
+// these; at that share 1094 and 1150 TFLOP/s are clocks of 1.87 and 1.97 GHz (1.75, 2.0 and 1.86 under the profiler).  A step of 64
+// keys has 2048 clocks of matrix time and takes about 3,600 in the first: exponentials and packing among them, LDS reads, one
+// barrier.  Start and end of a workgroup take 35,000 to 40,000 clocks: 4,000 to find its work, 12,000 until the first tiles and
+// queries are there, 20,000 to join the key groups, for gates and stores: 2% of the first's, 8% of the
+// second's, a seventh of the third's.
 //
 // Two key groups of two waves; the waves of a group share its tiles, each has 64 columns of its
 // own.  A ring slot holds a tile's K or V: 32 rows of 512 bytes.  (One group of four waves, which
-// halves the bytes that go into LDS for a column, was no faster over long contexts, 1159 against 1151
-// TFLOP/s, and keeps Q operands in scratch.)
+// halves the bytes that go into LDS for a column and has no groups to join, was no faster over long contexts, 1159
+// against 1151 TFLOP/s for 2048 tokens of 32768, and keeps Q operands in scratch; on whole prompts, where the
+// join is a larger share, it was not measured.)
 constexpr int kGroups = 2, kShare = kWaves / kGroups;
 constexpr int kStreamCols = 64 * kShare;
 constexpr unsigned kSlot = 32 * kRowBytes;
@@ -45,7 +48,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int kg = wave % kGroups, cg = wave / kGroups; // key group, column group
   // The hardware deals workgroups to the 8 dies in turn and of a die's to its 4 engines in turn, whatever has
   // become free: every other row of 32 takes the engines the other way round, so that of items that lie
-  // longest first each engine gets about as much.  (16 sequences, 268 workgroups for 256 places: 219 -> 182 us.)
+  // longest first each engine gets about as much.  (16 sequences of up to 8192 behind a window of 4096, ten of
+  // them single tokens, 268 workgroups for 256 places, in a graph: 208 -> 185 us.)
   const std::uint32_t turned = (blockIdx.x & 32) != 0 ? blockIdx.x ^ 24 : blockIdx.x;
   const std::uint32_t index = scalar(turned / a.kv_heads), kvh = turned - index * a.kv_heads;
   PagedItem it;

@@ -593,7 +593,7 @@ Bounds stream_bounds(const PagedArgs &a) { return bounds_of(a, kStreamBlockCols,
 // kernel first: 512 tokens 20.5 / 38.6, 1000 43.7 / 57.4, 500 of 1500 37.5 / 44.2, 64 of 4000 25.3 / 37.6, 16 of
 // 30000 56.7 / 69.6), above it the stream kernel (100 of 8000 68.3 / 51.5, 300 of 4000 78.4 / 56.4, 500 of 30501 and
 // 8001: twice as fast and more).  Several sequences: 4 of up to 500 tokens 41.5 / 42.6, 8 with 7 single tokens up to 8000
-// 105 / 80, 16 with up to 8192 behind a window of 4096 275 / 172.  Where the rows kernel would take a third round of
+// 105 / 80, 16 with up to 8192 behind a window of 4096, in a graph, 289 / 185.  Where the rows kernel would take a third round of
 // workgroups, few keys or not, the stream kernel is the faster too (windows of 32 and 200: 900 tokens 26.7 / 26.6 and 31.4 / 35.3,
 // 1200 38.1 / 22.3 and 46.1 / 36.3), unless its blocks would be half empty (600 sequences of 2 tokens 136 / 195).
 bool streams(const PagedArgs &a) {
