@@ -402,3 +402,15 @@ def test_frequencies_left_at_their_defaults():
         assert np.allclose(got, want, rtol=1e-13, atol=0) and abs(magnitude - m) <= 2.0 ** -24 * m
         other, _ = ref.frequencies(128, 5e5, name, 8.0, 8192.0, 36.0 - fast, 1.0)
         assert not np.allclose(got, other, rtol=1e-3, atol=0)
+
+
+def test_the_library_takes_a_bound_above_the_table_everywhere():
+    """Through the C interface, where nothing but the shape is at hand, the pool's bytes too."""
+    import ctypes
+    from raftinfer_amd import _lib
+    for bound, ok in ((321, True), (2 ** 28, True), (2 ** 28 + 1, False), (0, False)):
+        size = ctypes.c_size_t()
+        shape = dataclasses.replace(MODEL, max_context_tokens=bound).c()
+        status = _lib.load().raftinfer_amd_paged_cache_bytes(shape, ctypes.byref(size))
+        assert (status == 0) == ok, bound
+        assert not ok or size.value == ops.qwen35_paged_cache_bytes(MODEL)
